@@ -15,7 +15,8 @@ DFT_OK, DFT_ERR_INVALID, DFT_ERR_UNSUPPORTED, DFT_ERR_LAUNCH = 0, 1, 2, 3
 DFT_F32, DFT_BF16, DFT_F16, DFT_I32, DFT_I64 = 0, 1, 2, 3, 4
 DFT_VERIFY_AUX_K_PER_KHEAD = 1
 DFT_COMMIT_KV, DFT_COMMIT_CHECK_ANC, DFT_COMMIT_LEN_IS_LAST = 1, 2, 4
-DFT_STATUS_SPAN, DFT_STATUS_PATH, DFT_STATUS_WALK = 1, 2, 4
+DFT_STATUS_SPAN, DFT_STATUS_PATH, DFT_STATUS_WALK, DFT_STATUS_PAGES, DFT_STATUS_TABLE = 1, 2, 4, 8, 16
+DFT_ATTN_CAUSAL = 1
 ABI_VERSION = 5
 
 i32, i64, f32, vp = C.c_int32, C.c_int64, C.c_float, C.c_void_p
@@ -145,11 +146,73 @@ class MaskArgs(C.Structure):
     ]
 
 
+class PagePlanArgs(C.Structure):
+    _fields_ = [
+        ("batch", i32), ("columns", i32), ("page_size", i32), ("trim", i32),
+        ("rows", i64), ("capacity", i64),
+        ("prefix_len", vp), ("prefix_len_dtype", i32),
+        ("new_len", vp), ("new_len_dtype", i32),
+        ("block_table", vp), ("table_row_stride", i64),
+        ("held", vp), ("held_out", vp),
+        ("free_pages", vp), ("free_pos", vp), ("free_pos_out", vp),
+        ("depth", vp), ("depth_dtype", i32),
+        ("slots", vp), ("positions", vp), ("index_dtype", i32),
+        ("cu_seqlens", vp), ("seq_len", vp), ("status", vp),
+    ]
+
+
+class KvAppendArgs(C.Structure):
+    _fields_ = [
+        ("heads", i32), ("head_dim", i32), ("page_size", i32),
+        ("src_dtype", i32), ("cache_dtype", i32), ("slots_dtype", i32), ("rows_dtype", i32),
+        ("n", i64), ("src_rows", i64), ("num_pages", i64),
+        ("k", vp), ("k_row_stride", i64), ("k_h_stride", i64),
+        ("v", vp), ("v_row_stride", i64), ("v_h_stride", i64),
+        ("key_cache", vp), ("kc_page_stride", i64), ("kc_token_stride", i64), ("kc_h_stride", i64),
+        ("value_cache", vp), ("vc_page_stride", i64), ("vc_token_stride", i64), ("vc_h_stride", i64),
+        ("slots", vp), ("rows", vp), ("status", vp),
+    ]
+
+
+class PagedAttentionArgs(C.Structure):
+    _fields_ = [
+        ("batch", i32), ("n_new", i32), ("hq", i32), ("hkv", i32), ("head_dim", i32),
+        ("page_size", i32), ("columns", i32), ("flags", i32), ("scale", f32), ("dtype", i32),
+        ("rows", i64), ("num_pages", i64),
+        ("q", vp), ("q_row_stride", i64), ("q_h_stride", i64),
+        ("key_cache", vp), ("kc_page_stride", i64), ("kc_token_stride", i64), ("kc_h_stride", i64),
+        ("value_cache", vp), ("vc_page_stride", i64), ("vc_token_stride", i64), ("vc_h_stride", i64),
+        ("block_table", vp), ("table_row_stride", i64),
+        ("seq_len", vp), ("seq_len_dtype", i32),
+        ("cu_seqlens", vp), ("anc_bits", vp),
+        ("o", vp), ("o_row_stride", i64), ("o_h_stride", i64), ("o_dtype", i32),
+        ("lse", vp), ("lse_row_stride", i64),
+        ("status", vp), ("workspace", vp), ("workspace_bytes", i64),
+    ]
+
+
+class PromptAttentionArgs(C.Structure):
+    _fields_ = [
+        ("batch", i32), ("max_len", i32), ("hq", i32), ("hkv", i32), ("head_dim", i32),
+        ("flags", i32), ("scale", f32), ("dtype", i32),
+        ("rows", i64),
+        ("q", vp), ("q_row_stride", i64), ("q_h_stride", i64),
+        ("k", vp), ("k_row_stride", i64), ("k_h_stride", i64),
+        ("v", vp), ("v_row_stride", i64), ("v_h_stride", i64),
+        ("cu_seqlens", vp),
+        ("o", vp), ("o_row_stride", i64), ("o_h_stride", i64), ("o_dtype", i32),
+        ("lse", vp), ("lse_row_stride", i64),
+        ("status", vp),
+    ]
+
+
 DFT_BITS_LITTLE, DFT_BITS_BIG = 0, 1
 
 EXPORTS = ("dft_tree_verify", "dft_tree_commit_verify", "dft_tree_conv", "dft_tree_commit", "dft_tree_struct",
            "dft_tree_struct_filled",
            "dft_anc_pack", "dft_block_inverse", "dft_packbits", "dft_tree_mask_pack", "dft_size_order",
+           "dft_page_plan", "dft_kv_append", "dft_paged_attention", "dft_paged_attention_workspace",
+           "dft_prompt_attention",
            "dft_error_string", "dft_abi_version")
 
 
@@ -184,6 +247,11 @@ def load() -> C.CDLL:
                        ("dft_anc_pack", [C.POINTER(AncPackArgs), vp]),
                        ("dft_packbits", [C.POINTER(PackbitsArgs), vp]),
                        ("dft_tree_mask_pack", [C.POINTER(MaskArgs), vp]),
+                       ("dft_page_plan", [C.POINTER(PagePlanArgs), vp]),
+                       ("dft_kv_append", [C.POINTER(KvAppendArgs), vp]),
+                       ("dft_paged_attention", [C.POINTER(PagedAttentionArgs), vp]),
+                       ("dft_paged_attention_workspace", [C.POINTER(PagedAttentionArgs), C.POINTER(i64)]),
+                       ("dft_prompt_attention", [C.POINTER(PromptAttentionArgs), vp]),
                        ("dft_block_inverse", [vp, i32, i32, i64, vp]),
                        ("dft_size_order", [vp, i32, i32, vp, vp])):
         fn = getattr(lib, name)

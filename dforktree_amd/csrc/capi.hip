@@ -15,6 +15,11 @@ int launch_tree_struct(const dft_tree_args* a, int64_t rows, hipStream_t stream)
 int launch_anc_pack(const dft_anc_pack_args* a, hipStream_t stream);
 int launch_packbits(const dft_packbits_args* a, hipStream_t stream);
 int launch_tree_mask(const dft_mask_args* a, hipStream_t stream);
+int launch_page_plan(const dft_page_plan_args* a, hipStream_t stream);
+int launch_kv_append(const dft_kv_append_args* a, hipStream_t stream);
+int launch_paged_attention(const dft_paged_attention_args* a, hipStream_t stream);
+int64_t paged_attention_workspace(const dft_paged_attention_args* a);
+int launch_prompt_attention(const dft_prompt_attention_args* a, hipStream_t stream);
 }  // namespace dft
 
 namespace {
@@ -72,6 +77,40 @@ int tree_status(const dft_tree_args* a) {
   if (a->depth && !index_tag(a->depth_dtype)) return DFT_ERR_INVALID;
   if (a->cidx && (!index_tag(a->cidx_dtype) || a->kc < 1)) return DFT_ERR_INVALID;
   if ((a->nxt || a->sib) && !index_tag(a->link_dtype)) return DFT_ERR_INVALID;
+  return DFT_OK;
+}
+
+// Checks that both attention entry points share: heads, types, the rows'
+// 16-byte pieces and the grid.
+template <class Args>
+int attention_status(const Args* a, int span) {
+  if (!a) return DFT_ERR_INVALID;
+  if (a->batch < 0 || span < 0 || a->rows < 0) return DFT_ERR_INVALID;
+  if (a->hq <= 0 || a->hkv <= 0 || a->hq % a->hkv != 0) return DFT_ERR_INVALID;
+  if (a->head_dim != 64 && a->head_dim != 128 && a->head_dim != 256) return DFT_ERR_UNSUPPORTED;
+  if (a->dtype != DFT_BF16 && a->dtype != DFT_F16) return DFT_ERR_UNSUPPORTED;
+  if (!float_tag(a->o_dtype)) return DFT_ERR_INVALID;
+  if (a->batch == 0 || span == 0 || a->rows == 0) return -1;
+  if (a->batch > 65535 || a->hq > 65535) return DFT_ERR_UNSUPPORTED;
+  if (!a->q || !a->o) return DFT_ERR_INVALID;
+  if (!aligned16(a->q) || a->q_row_stride % 8 || a->q_h_stride % 8) return DFT_ERR_INVALID;
+  return DFT_OK;
+}
+
+int paged_attention_status(const dft_paged_attention_args* a) {
+  const int st = attention_status(a, a ? a->n_new : 0);
+  if (st > 0) return st;
+  if (a->page_size < 1 || a->columns < 0 || a->num_pages < 0) return DFT_ERR_INVALID;
+  if (a->num_pages > 0x7fffffffll) return DFT_ERR_UNSUPPORTED;  // 32-bit page ids
+  if (a->anc_bits && a->n_new > 64) return DFT_ERR_UNSUPPORTED;
+  if (a->anc_bits && (a->flags & DFT_ATTN_CAUSAL)) return DFT_ERR_INVALID;  // one mask or the other
+  if (st < 0) return st;
+  if (!a->seq_len || !index_tag(a->seq_len_dtype)) return DFT_ERR_INVALID;
+  if ((!a->block_table && a->columns) || ((!a->key_cache || !a->value_cache) && a->num_pages)) return DFT_ERR_INVALID;
+  if (!aligned16(a->key_cache) || !aligned16(a->value_cache)) return DFT_ERR_INVALID;
+  if (a->kc_page_stride % 8 || a->kc_token_stride % 8 || a->kc_h_stride % 8 || a->vc_page_stride % 8 ||
+      a->vc_token_stride % 8 || a->vc_h_stride % 8)
+    return DFT_ERR_INVALID;
   return DFT_OK;
 }
 
@@ -227,6 +266,63 @@ int dft_tree_mask_pack(const dft_mask_args* a, void* stream) {
   if (!a->anc_bits || !a->prefix_len || !a->out || !index_tag(a->prefix_len_dtype)) return DFT_ERR_INVALID;
   if (a->out_indptr && !index_tag(a->out_indptr_dtype)) return DFT_ERR_INVALID;
   return dft::launch_tree_mask(a, static_cast<hipStream_t>(stream));
+}
+
+int dft_page_plan(const dft_page_plan_args* a, void* stream) {
+  if (!a) return DFT_ERR_INVALID;
+  if (a->batch < 0 || a->columns < 0 || a->page_size < 1 || a->rows < 0 || a->capacity < 1) return DFT_ERR_INVALID;
+  // the running sums of every request sit in a workgroup's LDS; rows and pages are counted in 32 bits
+  if (a->batch > 8192 || a->rows > 0x7fffffffll || a->capacity > 0x7fffffffll) return DFT_ERR_UNSUPPORTED;
+  if (!a->free_pages || !a->free_pos || !a->free_pos_out || !a->cu_seqlens) return DFT_ERR_INVALID;
+  // every workgroup reads these while one writes the others
+  if (a->free_pos == a->free_pos_out || (a->batch && a->held == a->held_out)) return DFT_ERR_INVALID;
+  if (a->batch && (!a->prefix_len || !a->new_len || !a->held || !a->held_out || !a->seq_len || !a->status))
+    return DFT_ERR_INVALID;
+  if (a->batch && a->columns && !a->block_table) return DFT_ERR_INVALID;
+  if (!index_tag(a->prefix_len_dtype) || !index_tag(a->new_len_dtype) || !index_tag(a->index_dtype))
+    return DFT_ERR_INVALID;
+  if (a->depth && !index_tag(a->depth_dtype)) return DFT_ERR_INVALID;
+  if (a->rows && (!a->slots || !a->positions)) return DFT_ERR_INVALID;
+  return dft::launch_page_plan(a, static_cast<hipStream_t>(stream));
+}
+
+int dft_kv_append(const dft_kv_append_args* a, void* stream) {
+  if (!a) return DFT_ERR_INVALID;
+  if (a->heads < 1 || a->head_dim < 1 || a->page_size < 1 || a->n < 0 || a->src_rows < 0 || a->num_pages < 0)
+    return DFT_ERR_INVALID;
+  if (!float_tag(a->src_dtype) || !float_tag(a->cache_dtype)) return DFT_ERR_INVALID;
+  if (!index_tag(a->slots_dtype) || (a->rows && !index_tag(a->rows_dtype))) return DFT_ERR_INVALID;
+  if (a->n == 0) return DFT_OK;
+  if (!a->slots) return DFT_ERR_INVALID;
+  if (a->src_rows && (!a->k || !a->v)) return DFT_ERR_INVALID;
+  if (a->num_pages && (!a->key_cache || !a->value_cache)) return DFT_ERR_INVALID;
+  return dft::launch_kv_append(a, static_cast<hipStream_t>(stream));
+}
+
+int dft_paged_attention(const dft_paged_attention_args* a, void* stream) {
+  const int st = paged_attention_status(a);
+  if (st != DFT_OK) return st < 0 ? DFT_OK : st;
+  const int64_t need = dft::paged_attention_workspace(a);
+  if (need > 0 && (!a->workspace || !aligned16(a->workspace) || a->workspace_bytes < need)) return DFT_ERR_INVALID;
+  return dft::launch_paged_attention(a, static_cast<hipStream_t>(stream));
+}
+
+int dft_paged_attention_workspace(const dft_paged_attention_args* a, int64_t* bytes) {
+  if (!bytes) return DFT_ERR_INVALID;
+  *bytes = 0;
+  // the sizes decide: what the pointers hold is not looked at
+  const int st = attention_status(a, a ? a->n_new : 0);
+  if (st > DFT_OK) return st;
+  if (st == DFT_OK) *bytes = dft::paged_attention_workspace(a);
+  return DFT_OK;
+}
+
+int dft_prompt_attention(const dft_prompt_attention_args* a, void* stream) {
+  const int st = attention_status(a, a ? a->max_len : 0);
+  if (st != DFT_OK) return st < 0 ? DFT_OK : st;
+  if (!a->k || !a->v || !aligned16(a->k) || !aligned16(a->v)) return DFT_ERR_INVALID;
+  if (a->k_row_stride % 8 || a->k_h_stride % 8 || a->v_row_stride % 8 || a->v_h_stride % 8) return DFT_ERR_INVALID;
+  return dft::launch_prompt_attention(a, static_cast<hipStream_t>(stream));
 }
 
 }  // extern "C"

@@ -21,7 +21,8 @@ import torch
 
 from . import _lib
 from ._lib import (DFT_BF16, DFT_BITS_BIG, DFT_BITS_LITTLE, DFT_F16, DFT_F32, DFT_I32, DFT_I64, AncPackArgs,
-                   CommitArgs, ConvArgs, MaskArgs, PackbitsArgs, PendingArgs, TreeArgs, VerifyArgs, check, load)
+                   CommitArgs, ConvArgs, KvAppendArgs, MaskArgs, PackbitsArgs, PagedAttentionArgs, PagePlanArgs,
+                   PendingArgs, PromptAttentionArgs, TreeArgs, VerifyArgs, check, load)
 
 _FLOAT_TAG = {torch.float32: DFT_F32, torch.bfloat16: DFT_BF16, torch.float16: DFT_F16}
 _INDEX_TAG = {torch.int32: DFT_I32, torch.int64: DFT_I64}
@@ -840,3 +841,305 @@ def tree_mask_pack(anc_bits: torch.Tensor, prefix_len: torch.Tensor, *, batch: O
     if batch:
         check("dft_tree_mask_pack", load().dft_tree_mask_pack(C.byref(a), _stream(dev)))
     return out, out_indptr
+
+
+# ---------------------------------------------------------------------------
+# the full-attention layers: a paged KV cache and the attentions over it
+# ---------------------------------------------------------------------------
+def page_plan(prefix_len: torch.Tensor, new_len: torch.Tensor, block_table: torch.Tensor, held: torch.Tensor,
+              free_pages: torch.Tensor, free_pos: torch.Tensor, *, page_size: int, rows: int, trim: bool = False,
+              depth: Optional[torch.Tensor] = None, index_dtype: torch.dtype = torch.int64) -> dict:
+    """Pages, slots and positions of new_len[b] new tokens after prefix_len[b]
+    committed ones, for every request in one launch (``dft_page_plan``).
+
+    block_table [batch, columns] int32: request b's token t is in page
+    block_table[b, t // page_size]; its first held[b] (int32) entries are its
+    pages.  free_pages [capacity] int32 is a ring of free page ids, those at
+    i % capacity for free_pos[0] <= i < free_pos[1] (int64 [2]).  Requests
+    that need pages take them from the ring's front in request order (their
+    new cells of block_table are written); with ``trim`` a request that holds
+    more than it needs puts the others at the ring's end, all of them when
+    its lengths are 0.  ``rows``: the new tokens there is room for (their
+    total, or more).  ``depth`` [rows]: a draft tree's node depths, for
+    positions prefix_len + depth instead of prefix_len + index.
+
+    Returns slots [rows] (page * page_size + offset; -1 past the tokens and
+    for requests without pages), positions [rows], cu_seqlens int32
+    [batch + 1], seq_len int32 [batch] (prefix and new; 0 without pages),
+    held int32 [batch] and free_pos int64 [2] for the next call, and status
+    int32 [batch] (DFT_STATUS_PAGES: the ring ran out; DFT_STATUS_TABLE: too
+    few columns; DFT_STATUS_SPAN: lengths cut to ``rows``, or negative).
+    Calling it again with the same arguments gives the same result.
+    """
+    dev = _device_of(prefix_len, new_len, block_table, held, free_pages, free_pos, depth)
+    pl, pl_tag = _idx_vec(prefix_len, "prefix_len")
+    nl, nl_tag = _idx_vec(new_len, "new_len")
+    batch = pl.numel()
+    if nl.numel() != batch or held.numel() != batch:
+        raise ValueError(f"prefix_len, new_len and held have {batch}, {nl.numel()} and {held.numel()} entries")
+    if block_table.dtype != torch.int32 or held.dtype != torch.int32 or free_pages.dtype != torch.int32:
+        raise TypeError("block_table, held and free_pages must be int32")
+    if block_table.dim() != 2 or block_table.shape[0] != batch:
+        raise ValueError(f"block_table must be [{batch}, columns], got {tuple(block_table.shape)}")
+    if block_table.stride(1) != 1 and block_table.shape[1] > 1:
+        raise ValueError("block_table must have column stride 1 (it is updated in place)")
+    if batch > 1 and block_table.stride(0) < block_table.shape[1]:
+        raise ValueError("block_table's rows overlap (it is updated in place)")
+    if not free_pages.is_contiguous() or not free_pages.numel():
+        raise ValueError("free_pages must be a contiguous ring of at least one entry (it is updated in place)")
+    if free_pos.dtype != torch.int64 or free_pos.numel() != 2 or not free_pos.is_contiguous():
+        raise ValueError("free_pos must be a contiguous int64 tensor of 2 entries")
+    if not held.is_contiguous():
+        held = held.contiguous()
+    if page_size < 1 or rows < 0:
+        raise ValueError("page_size must be at least 1 and rows at least 0")
+    dep, dep_tag = _idx_vec(depth, "depth")
+    if dep is not None and dep.numel() < rows:
+        raise ValueError(f"depth has {dep.numel()} entries for {rows} rows")
+    a = PagePlanArgs()
+    out = {"slots": torch.empty(rows, device=dev, dtype=index_dtype),
+           "positions": torch.empty(rows, device=dev, dtype=index_dtype)}
+    try:
+        a.index_dtype = _INDEX_TAG[index_dtype]
+    except KeyError:
+        raise TypeError(f"index_dtype must be int32 or int64, got {index_dtype}") from None
+    words = torch.empty(4 * batch + 1, device=dev, dtype=torch.int32)
+    out["cu_seqlens"], out["seq_len"], out["held"], out["status"] = words.split([batch + 1, batch, batch, batch])
+    out["free_pos"] = torch.empty(2, device=dev, dtype=torch.int64)
+    a.batch, a.columns, a.page_size, a.trim = batch, block_table.shape[1], page_size, int(bool(trim))
+    a.rows, a.capacity = rows, free_pages.numel()
+    a.prefix_len, a.prefix_len_dtype = pl.data_ptr(), pl_tag
+    a.new_len, a.new_len_dtype = nl.data_ptr(), nl_tag
+    a.block_table, a.table_row_stride = block_table.data_ptr(), block_table.stride(0)
+    a.held, a.held_out = held.data_ptr(), out["held"].data_ptr()
+    a.free_pages, a.free_pos, a.free_pos_out = free_pages.data_ptr(), free_pos.data_ptr(), out["free_pos"].data_ptr()
+    a.depth, a.depth_dtype = _ptr(dep), dep_tag
+    a.slots, a.positions = out["slots"].data_ptr(), out["positions"].data_ptr()
+    a.cu_seqlens, a.seq_len, a.status = words.data_ptr(), out["seq_len"].data_ptr(), out["status"].data_ptr()
+    check("dft_page_plan", load().dft_page_plan(C.byref(a), _stream(dev)))
+    return out
+
+
+def _check_cache(key_cache, value_cache):
+    """A pair of caches [pages, page_size, heads, head_dim] of one shape and type."""
+    if key_cache.dim() != 4 or key_cache.shape != value_cache.shape:
+        raise ValueError("key_cache and value_cache must be [pages, page_size, heads, head_dim] of one shape (pass "
+                         f"pages of [heads, page_size, head_dim] as .transpose(1, 2)), got {tuple(key_cache.shape)} "
+                         f"and {tuple(value_cache.shape)}")
+    if key_cache.dtype != value_cache.dtype:
+        raise TypeError(f"key_cache is {key_cache.dtype}, value_cache {value_cache.dtype}")
+    if key_cache.stride(3) != 1 or value_cache.stride(3) != 1:
+        raise ValueError("the caches need stride 1 along the head dim")
+    if key_cache.shape[1] < 1:
+        raise ValueError("a page holds at least one token")
+
+
+def kv_append(k: torch.Tensor, v: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
+              slots: torch.Tensor, *, rows: Optional[torch.Tensor] = None,
+              status: Optional[torch.Tensor] = None) -> None:
+    """Writes K/V rows into the slots of a paged cache (``dft_kv_append``).
+
+    k, v [T, heads, head_dim] (unit stride along head_dim, e.g. slices of one
+    projection); caches [pages, page_size, heads, head_dim], any strides but
+    the last (``.transpose(1, 2)`` of pages kept heads first).  Row i, or
+    rows[i], goes to slot slots[i] (``page_plan``'s), cast to the cache's
+    type; a negative slot or row is skipped.  One past the cache or past T is
+    skipped as well and sets ``status`` (int32, one entry, never cleared) to
+    1.  No slot may occur twice.  With ``rows`` = the nodes of the accepted
+    paths (-1 padded) and ``slots`` = the places after their prefixes this
+    commits a draft tree's keys and values.
+    """
+    dev = _device_of(k, v, key_cache, value_cache, slots, rows, status)
+    _check_cache(key_cache, value_cache)
+    if k.dim() != 3 or k.shape != v.shape or tuple(k.shape[1:]) != tuple(key_cache.shape[2:]):
+        raise ValueError(f"k and v must be [T, {key_cache.shape[2]}, {key_cache.shape[3]}], got {tuple(k.shape)} and "
+                         f"{tuple(v.shape)}")
+    if k.dtype != v.dtype:
+        raise TypeError(f"k is {k.dtype}, v {v.dtype}")
+    if k.stride(2) != 1 or v.stride(2) != 1:
+        raise ValueError("k and v need stride 1 along the head dim")
+    a = KvAppendArgs()
+    sl, a.slots_dtype = _idx_vec(slots, "slots")
+    ri, a.rows_dtype = _idx_vec(rows, "rows")
+    n = sl.numel()
+    if ri is not None and ri.numel() != n:
+        raise ValueError(f"rows has {ri.numel()} entries, slots {n}")
+    if ri is None and n > k.shape[0]:
+        raise ValueError(f"slots has {n} entries for {k.shape[0]} rows")
+    if status is not None and (status.dtype != torch.int32 or status.numel() < 1):
+        raise ValueError("status must be an int32 tensor of one entry")
+    if not k.numel() or not n:
+        return
+    a.heads, a.head_dim, a.page_size = k.shape[1], k.shape[2], key_cache.shape[1]
+    a.src_dtype, a.cache_dtype = _ftag(k, "k"), _ftag(key_cache, "key_cache")
+    a.n, a.src_rows, a.num_pages = n, k.shape[0], key_cache.shape[0]
+    a.k, a.k_row_stride, a.k_h_stride = k.data_ptr(), k.stride(0), k.stride(1)
+    a.v, a.v_row_stride, a.v_h_stride = v.data_ptr(), v.stride(0), v.stride(1)
+    a.key_cache, a.kc_page_stride, a.kc_token_stride, a.kc_h_stride = key_cache.data_ptr(), *key_cache.stride()[:3]
+    a.value_cache, a.vc_page_stride, a.vc_token_stride, a.vc_h_stride = (value_cache.data_ptr(),
+                                                                        *value_cache.stride()[:3])
+    a.slots, a.rows, a.status = sl.data_ptr(), _ptr(ri), _ptr(status)
+    check("dft_kv_append", load().dft_kv_append(C.byref(a), _stream(dev)))
+
+
+def _aligned_rows(t, name):
+    """A [rows, heads, d] view whose rows the kernels read as 16-byte pieces:
+    itself, or a copy when its address or strides do not allow it."""
+    if t.dim() != 3:
+        raise ValueError(f"{name} must be [rows, heads, head_dim], got {tuple(t.shape)}")
+    if t.stride(2) != 1 or t.stride(0) % 8 or t.stride(1) % 8 or t.data_ptr() % 16:
+        t = torch.empty(t.shape, device=t.device, dtype=t.dtype).copy_(t)
+    return t
+
+
+def _attention_out(q, o, lse, dev):
+    """The output (allocated unless given) and the checked lse."""
+    if o is None:
+        o = torch.empty(q.shape, device=dev, dtype=q.dtype)
+    elif o.shape != q.shape or o.stride(2) != 1:
+        raise ValueError(f"o must be {tuple(q.shape)} with stride 1 along the head dim")
+    if lse is not None:
+        if lse.dtype != torch.float32:
+            raise TypeError("lse must be float32")
+        if lse.shape != q.shape[:2] or (lse.stride(1) != 1 and q.shape[1] > 1):
+            raise ValueError(f"lse must be {tuple(q.shape[:2])} with stride 1 along heads")
+    return o
+
+
+def _packed_rows(cu_seqlens, rows, limit, name, batch):
+    """(cu_seqlens, batch, rows of the longest request) of packed or uniform rows."""
+    if cu_seqlens is not None:
+        if cu_seqlens.dtype != torch.int32:
+            raise TypeError("cu_seqlens must be int32")
+        if limit is None:
+            raise ValueError(f"packed input needs {name} (the largest request) on the host")
+        if cu_seqlens.numel() < 1:
+            raise ValueError("cu_seqlens needs at least one entry")
+        if batch is not None and cu_seqlens.numel() != batch + 1:
+            raise ValueError(f"cu_seqlens has {cu_seqlens.numel()} entries for {batch} requests")
+        return cu_seqlens.contiguous(), cu_seqlens.numel() - 1, limit
+    if batch is None:
+        batch = 1 if limit is None else rows // max(limit, 1)
+    if limit is None:
+        limit = rows // max(batch, 1)
+    if batch * limit > rows:
+        raise ValueError(f"{batch} requests of {limit} rows exceed the {rows} rows of q")
+    return None, batch, limit
+
+
+def paged_attention(q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor, block_table: torch.Tensor,
+                    seq_len: torch.Tensor, *, cu_seqlens: Optional[torch.Tensor] = None,
+                    n_new: Optional[int] = None, causal: bool = True, anc_bits: Optional[torch.Tensor] = None,
+                    scale: Optional[float] = None, o: Optional[torch.Tensor] = None,
+                    lse: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of every request's new tokens over its pages
+    (``dft_paged_attention``): decode (one row each), a draft tree's verify,
+    a chunk of a long prompt.
+
+    q [rows, hq, d] bf16 or fp16, d 64, 128 or 256, any unit-stride view;
+    caches [pages, page_size, hkv, d] as in ``kv_append``, of q's type, hq a
+    multiple of hkv; block_table [batch, columns] int32 and seq_len [batch]
+    (``page_plan``'s), the new tokens included: ``kv_append`` them first.
+    Request b's rows start at cu_seqlens[b] (then n_new is the most rows of
+    one request) or at b * n_new.  They are the last of its keys: row i sees
+    the keys up to its own (``causal``), with ``anc_bits`` (int64 [rows],
+    ``tree_struct``'s; n_new <= 64) the prefix and its ancestors, which takes
+    the place of ``causal``, with neither every key.  A row that sees no key
+    gets o = 0 and lse = -inf.  ``scale`` defaults to d ** -0.5.  ``lse``
+    (float32 [rows, hq]) receives the logarithm of each softmax's sum, with
+    which outputs over parts of the keys are joined; ``status`` (int32
+    [batch]) DFT_STATUS_SPAN and DFT_STATUS_TABLE bits.  Returns o.
+    """
+    dev = _device_of(q, key_cache, value_cache, block_table, seq_len, cu_seqlens, anc_bits, o, lse)
+    _check_cache(key_cache, value_cache)
+    q = _aligned_rows(q, "q")
+    rows, hq, d = q.shape
+    pages, page_size, hkv, dc = key_cache.shape
+    if q.dtype not in (torch.bfloat16, torch.float16) or key_cache.dtype != q.dtype:
+        raise TypeError(f"q and the caches must be both bfloat16 or both float16, got {q.dtype} and {key_cache.dtype}")
+    if d != dc or hkv < 1 or hq % hkv:
+        raise ValueError(f"q has {hq} heads of {d}, the caches {hkv} of {dc}")
+    if block_table.dtype != torch.int32:
+        raise TypeError("block_table must be int32")
+    sl, sl_tag = _idx_vec(seq_len, "seq_len")
+    if block_table.dim() != 2 or block_table.shape[0] != sl.numel():
+        raise ValueError(f"block_table must be [{sl.numel()}, columns], got {tuple(block_table.shape)}")
+    if block_table.stride(1) != 1:
+        block_table = block_table.contiguous()
+    cu, batch, n_new = _packed_rows(cu_seqlens, rows, n_new, "n_new", sl.numel())
+    if anc_bits is not None:
+        if anc_bits.dtype != torch.int64:
+            raise TypeError("anc_bits must be int64 (uint64 bit masks)")
+        if n_new > MAX_NODES:
+            raise ValueError(f"at most {MAX_NODES} nodes per request, got {n_new}")
+        if anc_bits.numel() < rows:
+            raise ValueError(f"anc_bits has {anc_bits.numel()} entries for {rows} rows")
+        anc_bits = anc_bits.contiguous()
+    o = _attention_out(q, o, lse, dev)
+    a = PagedAttentionArgs()
+    a.batch, a.n_new, a.hq, a.hkv, a.head_dim = batch, n_new, hq, hkv, d
+    a.page_size, a.columns = page_size, block_table.shape[1]
+    a.flags = _lib.DFT_ATTN_CAUSAL if causal and anc_bits is None else 0
+    a.scale = d ** -0.5 if scale is None else scale
+    a.dtype, a.rows, a.num_pages = _FLOAT_TAG[q.dtype], rows, pages
+    a.q, a.q_row_stride, a.q_h_stride = q.data_ptr(), q.stride(0), q.stride(1)
+    a.key_cache, a.kc_page_stride, a.kc_token_stride, a.kc_h_stride = key_cache.data_ptr(), *key_cache.stride()[:3]
+    a.value_cache, a.vc_page_stride, a.vc_token_stride, a.vc_h_stride = (value_cache.data_ptr(),
+                                                                        *value_cache.stride()[:3])
+    a.block_table, a.table_row_stride = block_table.data_ptr(), block_table.stride(0)
+    a.seq_len, a.seq_len_dtype = sl.data_ptr(), sl_tag
+    a.cu_seqlens, a.anc_bits = _ptr(cu), _ptr(anc_bits)
+    a.o, a.o_row_stride, a.o_h_stride, a.o_dtype = o.data_ptr(), o.stride(0), o.stride(1), _ftag(o, "o")
+    if lse is not None:
+        a.lse, a.lse_row_stride = lse.data_ptr(), lse.stride(0)
+    a.status = _status_ptr(status, batch, dev)
+    lib = load()
+    need = C.c_int64()
+    check("dft_paged_attention_workspace", lib.dft_paged_attention_workspace(C.byref(a), C.byref(need)))
+    if need.value:
+        work = torch.empty(need.value, device=dev, dtype=torch.uint8)
+        a.workspace, a.workspace_bytes = work.data_ptr(), need.value
+    check("dft_paged_attention", lib.dft_paged_attention(C.byref(a), _stream(dev)))
+    return o
+
+
+def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: Optional[torch.Tensor] = None, *,
+                     max_len: Optional[int] = None, batch: Optional[int] = None, causal: bool = True,
+                     scale: Optional[float] = None, o: Optional[torch.Tensor] = None,
+                     lse: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention over whole prompts, packed (``dft_prompt_attention``).
+
+    q [rows, hq, d], k, v [rows, hkv, d], bf16 or fp16, d 64, 128 or 256, any
+    unit-stride views (slices of one projection), hq a multiple of hkv.
+    Request b's tokens are rows cu_seqlens[b] .. cu_seqlens[b + 1] (max_len:
+    the longest's, on the host) or b * max_len ...; each sees the ones up to
+    itself (``causal``) or all.  ``scale``, ``o``, ``lse`` and ``status`` as in
+    ``paged_attention``.  Returns o.
+    """
+    dev = _device_of(q, k, v, cu_seqlens, o, lse)
+    q, k, v = _aligned_rows(q, "q"), _aligned_rows(k, "k"), _aligned_rows(v, "v")
+    rows, hq, d = q.shape
+    if k.shape != v.shape or k.shape[0] != rows or k.shape[2] != d:
+        raise ValueError(f"k and v must be [{rows}, hkv, {d}], got {tuple(k.shape)} and {tuple(v.shape)}")
+    if q.dtype not in (torch.bfloat16, torch.float16) or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError(f"q, k and v must be all bfloat16 or all float16, got {q.dtype}, {k.dtype} and {v.dtype}")
+    hkv = k.shape[1]
+    if hkv < 1 or hq % hkv:
+        raise ValueError(f"q has {hq} heads, k and v {hkv}")
+    cu, batch, max_len = _packed_rows(cu_seqlens, rows, max_len, "max_len", batch)
+    o = _attention_out(q, o, lse, dev)
+    a = PromptAttentionArgs()
+    a.batch, a.max_len, a.hq, a.hkv, a.head_dim = batch, max_len, hq, hkv, d
+    a.flags = _lib.DFT_ATTN_CAUSAL if causal else 0
+    a.scale = d ** -0.5 if scale is None else scale
+    a.dtype, a.rows = _FLOAT_TAG[q.dtype], rows
+    a.q, a.q_row_stride, a.q_h_stride = q.data_ptr(), q.stride(0), q.stride(1)
+    a.k, a.k_row_stride, a.k_h_stride = k.data_ptr(), k.stride(0), k.stride(1)
+    a.v, a.v_row_stride, a.v_h_stride = v.data_ptr(), v.stride(0), v.stride(1)
+    a.cu_seqlens = _ptr(cu)
+    a.o, a.o_row_stride, a.o_h_stride, a.o_dtype = o.data_ptr(), o.stride(0), o.stride(1), _ftag(o, "o")
+    if lse is not None:
+        a.lse, a.lse_row_stride = lse.data_ptr(), lse.stride(0)
+    a.status = _status_ptr(status, batch, dev)
+    check("dft_prompt_attention", load().dft_prompt_attention(C.byref(a), _stream(dev)))
+    return o

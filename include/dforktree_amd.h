@@ -76,7 +76,14 @@ enum dft_request_status {
    * (an ancestor missing or out of order, a non-ancestor, a repeat).  The
    * path was not committed: the slot keeps its state, and the verify ran on
    * it. */
-  DFT_STATUS_WALK = 4
+  DFT_STATUS_WALK = 4,
+  /* (dft_page_plan) the free pages ran out before this request, or its
+   * returned pages found no room in the ring: it neither took nor gave any */
+  DFT_STATUS_PAGES = 8,
+  /* the request's tokens need more pages than its row of the block table has
+   * columns: dft_page_plan gave it none, dft_paged_attention reads what the
+   * row holds */
+  DFT_STATUS_TABLE = 16
 };
 
 /* ---------------------------------------------------------------------------
@@ -480,6 +487,170 @@ DFT_API int dft_tree_mask_pack(const dft_mask_args* args, void* stream);
  * The upper triangle of the result is zeroed.
  * ------------------------------------------------------------------------- */
 DFT_API int dft_block_inverse(float* x, int32_t n_mats, int32_t n, int64_t mat_stride, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * The full-attention layers' paged KV cache and the attentions that fill and
+ * read it.  No counterpart in the reference, whose attention layers run in
+ * SGLang's backend (fc1_plan.py packs the mask that backend takes).
+ *
+ * A cache is an array of pages of page_size token slots; slot s is token
+ * s % page_size of page s / page_size.  Request b's token t lives in page
+ * block_table[b][t / page_size].  Free pages wait in a ring of `capacity`
+ * page ids: those at free_pages[i % capacity] for free_pos[0] <= i <
+ * free_pos[1].
+ *
+ * Page plan: pages, slots and positions for new_len[b] new tokens after
+ * prefix_len[b] committed ones, for every request in one launch.
+ *   n_b    = new_len[b], cut so that the rows so far stay within `rows`
+ *            (DFT_STATUS_SPAN)
+ *   want_b = ceil((prefix_len[b] + n_b) / page_size)
+ * A request that holds fewer pages than want_b takes the next ones of the
+ * ring, in request order; with `trim` one that holds more returns those past
+ * want_b to the ring's end (a finished request: prefix 0, new 0).  One that
+ * cannot be served (DFT_STATUS_PAGES: so many pages are not free, counting
+ * those of every request before it; DFT_STATUS_TABLE) keeps what it holds,
+ * gets slots of -1 and a seq_len of 0, which an attention launch takes as no
+ * keys at all.  Pages returned by this launch are not taken by it.
+ * Everything but block_table's new cells and the ring's returned pages is
+ * written to outputs of its own, so the same launch again writes the same.
+ * Negative lengths count as 0.
+ * ------------------------------------------------------------------------- */
+typedef struct dft_page_plan_args {
+  int32_t batch;     /* <= 8192 */
+  int32_t columns;   /* of the block table */
+  int32_t page_size; /* >= 1 */
+  int32_t trim;
+  int64_t rows;     /* new tokens that slots / positions have room for */
+  int64_t capacity; /* of the ring, 1 <= capacity < 2^31 */
+  const void* prefix_len; /* [batch] */
+  int32_t prefix_len_dtype;
+  const void* new_len; /* [batch] */
+  int32_t new_len_dtype;
+  int32_t* block_table; /* [batch][columns], column stride 1 */
+  int64_t table_row_stride;
+  const int32_t* held; /* [batch] pages each row of the table holds */
+  int32_t* held_out;   /* [batch], not the same array as held */
+  int32_t* free_pages; /* [capacity] */
+  const int64_t* free_pos; /* {first, past the last} */
+  int64_t* free_pos_out;   /* not the same array as free_pos */
+  const void* depth; /* optional [rows]: a draft tree's node depths */
+  int32_t depth_dtype;
+  void* slots;     /* [rows]: the slot of every new token, -1 past them */
+  void* positions; /* [rows]: prefix_len + index, or + depth when given; 0 past them */
+  int32_t index_dtype;
+  int32_t* cu_seqlens; /* [batch + 1] */
+  int32_t* seq_len;    /* [batch]: prefix_len + n_b */
+  int32_t* status;     /* [batch] */
+} dft_page_plan_args;
+
+DFT_API int dft_page_plan(const dft_page_plan_args* args, void* stream);
+
+/* New K/V rows into their slots: row rows[i] (or i) of k and v to slot
+ * slots[i], cast to the cache's type.  A negative slot or row is skipped; one
+ * past the cache or past src_rows is skipped too and sets *status, when
+ * given, to 1 (never cleared).  No two entries may name one slot.  The rows
+ * of an accepted path (rows = its nodes, slots = the places after the
+ * prefix) make this the KV side of a commit. */
+typedef struct dft_kv_append_args {
+  int32_t heads, head_dim; /* of k, v and the caches */
+  int32_t page_size;
+  int32_t src_dtype, cache_dtype; /* DFT_F32 / DFT_BF16 / DFT_F16 */
+  int32_t slots_dtype, rows_dtype;
+  int64_t n;        /* entries of slots */
+  int64_t src_rows; /* rows of k and v */
+  int64_t num_pages;
+  const void* k; /* [src_rows][heads][head_dim], unit stride along head_dim, as for every array here */
+  int64_t k_row_stride, k_h_stride;
+  const void* v;
+  int64_t v_row_stride, v_h_stride;
+  void* key_cache;
+  int64_t kc_page_stride, kc_token_stride, kc_h_stride;
+  void* value_cache;
+  int64_t vc_page_stride, vc_token_stride, vc_h_stride;
+  const void* slots; /* [n] */
+  const void* rows;  /* optional [n] */
+  int32_t* status;   /* optional, one word */
+} dft_kv_append_args;
+
+DFT_API int dft_kv_append(const dft_kv_append_args* args, void* stream);
+
+/* Attention.  Row i of request b and query head h:
+ *   o = sum_j p_j v_j,  p = softmax over the keys j it sees of scale q . k_j,
+ * with kv head h / (hq / hkv).  lse (optional) is the natural logarithm of
+ * the softmax's sum.  A row that sees no key: o = 0, lse = -inf.  Keys that
+ * a row does not see do not touch it, whatever they hold.
+ * Types: q, k, v all bf16 or all fp16, head_dim 64, 128 or 256, unit stride
+ * along it; 16-byte aligned q, k and v, their other strides multiples of 8
+ * elements.  The outputs' strides are free. */
+enum dft_attention_flags { DFT_ATTN_CAUSAL = 1 };
+
+/* Over a paged cache, which holds the new tokens already: request b's n_b
+ * rows (row0 as in dft_verify_args) are the last n_b of its seq_len[b] keys.
+ * Row i sees, with DFT_ATTN_CAUSAL, keys j <= seq_len - n_b + i; with
+ * anc_bits (n_new <= 64) the keys before seq_len - n_b and new token j where
+ * bit j of its word is set; with neither every key.  A page id outside
+ * [0, num_pages) is a page of no keys. */
+typedef struct dft_paged_attention_args {
+  int32_t batch, n_new; /* n_new: rows per request, with cu_seqlens the most of them (more are cut: DFT_STATUS_SPAN) */
+  int32_t hq, hkv, head_dim;
+  int32_t page_size, columns;
+  int32_t flags; /* dft_attention_flags */
+  float scale;
+  int32_t dtype; /* of q and the caches */
+  int64_t rows;  /* of q and o: a span that ends past them is cut */
+  int64_t num_pages;
+  const void* q;
+  int64_t q_row_stride, q_h_stride;
+  const void* key_cache;
+  int64_t kc_page_stride, kc_token_stride, kc_h_stride;
+  const void* value_cache;
+  int64_t vc_page_stride, vc_token_stride, vc_h_stride;
+  const int32_t* block_table; /* column stride 1 */
+  int64_t table_row_stride;
+  const void* seq_len; /* [batch] */
+  int32_t seq_len_dtype;
+  const int32_t* cu_seqlens; /* [batch + 1] or NULL */
+  const uint64_t* anc_bits;  /* [rows] or NULL */
+  void* o;
+  int64_t o_row_stride, o_h_stride;
+  int32_t o_dtype;
+  float* lse; /* optional, head stride 1 */
+  int64_t lse_row_stride;
+  int32_t* status; /* optional [batch] */
+  void* workspace; /* dft_paged_attention_workspace bytes, 16-byte aligned; used by this launch alone until it is done */
+  int64_t workspace_bytes;
+} dft_paged_attention_args;
+
+DFT_API int dft_paged_attention(const dft_paged_attention_args* args, void* stream);
+/* *bytes = what `workspace` must hold for these sizes (pointers are not read) */
+DFT_API int dft_paged_attention_workspace(const dft_paged_attention_args* args, int64_t* bytes);
+
+/* Over whole packed prompts: rows cu_seqlens[b] .. cu_seqlens[b+1] of q, k
+ * and v are request b's tokens; row i sees key j <= i (DFT_ATTN_CAUSAL) or
+ * every one.  A request of more than max_len tokens is cut to max_len. */
+typedef struct dft_prompt_attention_args {
+  int32_t batch, max_len;
+  int32_t hq, hkv, head_dim;
+  int32_t flags;
+  float scale;
+  int32_t dtype;
+  int64_t rows; /* of q, k, v and o */
+  const void* q;
+  int64_t q_row_stride, q_h_stride;
+  const void* k;
+  int64_t k_row_stride, k_h_stride;
+  const void* v;
+  int64_t v_row_stride, v_h_stride;
+  const int32_t* cu_seqlens; /* [batch + 1], or NULL: batch x max_len */
+  void* o;
+  int64_t o_row_stride, o_h_stride;
+  int32_t o_dtype;
+  float* lse;
+  int64_t lse_row_stride;
+  int32_t* status; /* optional [batch]: DFT_STATUS_SPAN */
+} dft_prompt_attention_args;
+
+DFT_API int dft_prompt_attention(const dft_prompt_attention_args* args, void* stream);
 
 DFT_API const char* dft_error_string(int status);
 DFT_API int dft_abi_version(void);

@@ -29,6 +29,10 @@ PyTorch fp32 CPU ops (the CPU baseline bench.py times), pinned against
 segment, as flashinfer packs the custom mask for fc1_plan.py:26) and
 ``tree_mask`` / ``tree_mask_packed`` (the mask of fc1_branch64.py:39).
 
+``oracle.paged``: the full-attention layers' page tables (a loop over
+requests), cache writes and attention (row by row, fp64).
+
 Pinning status of every function is listed in the module docstrings of
-``oracle.gdn_tree`` and ``oracle.mask``.
+``oracle.gdn_tree`` and ``oracle.mask``; ``oracle.paged`` is pinned by
+tests/test_paged_oracle.py.
 """
