@@ -99,8 +99,5 @@ int64_t paged_attention_workspace(const dft_paged_attention_args* a) { return 0;
 int launch_paged_attention(const dft_paged_attention_args* a, hipStream_t stream) {
   return launch<true>(*a, a->n_new, stream);
 }
-int launch_prompt_attention(const dft_prompt_attention_args* a, hipStream_t stream) {
-  return launch<false>(*a, a->max_len, stream);
-}
 
 }  // namespace dft
