@@ -73,7 +73,7 @@ __device__ __forceinline__ void dma16(uint64_t base, uint32_t off, uint32_t lds)
       "s_mov_b32 m0, %0\n\t"
       "s_nop 0"
       : "=&s"(keep)
-      : "v"(off), "s"(base), "s"(lds)
+      : "v"(off), "s"(base), "s"(__builtin_amdgcn_readfirstlane(lds))
       : "memory");
 }
 // the same from an address of each lane's own
@@ -87,7 +87,7 @@ __device__ __forceinline__ void dma16_at(uint64_t at, uint32_t lds) {
       "s_mov_b32 m0, %0\n\t"
       "s_nop 0"
       : "=&s"(keep)
-      : "v"(at), "s"(lds)
+      : "v"(at), "s"(__builtin_amdgcn_readfirstlane(lds))
       : "memory");
 }
 // and of 4 bytes a lane
@@ -101,7 +101,7 @@ __device__ __forceinline__ void dma4_at(uint64_t at, uint32_t lds) {
       "s_mov_b32 m0, %0\n\t"
       "s_nop 0"
       : "=&s"(keep)
-      : "v"(at), "s"(lds)
+      : "v"(at), "s"(__builtin_amdgcn_readfirstlane(lds))
       : "memory");
 }
 
@@ -122,6 +122,13 @@ __device__ __forceinline__ int value_swizzle(int row) {
 
 // Bits [0, n) of a word, none for n <= 0.
 __device__ __forceinline__ uint64_t first_bits(int n) { return n <= 0 ? 0 : n >= 64 ? ~0ull : (1ull << n) - 1; }
+
+// a where the bit is set, b elsewhere, without a comparison (whose results
+// would wait in scalar registers, a pair for each)
+__device__ __forceinline__ uint32_t select(uint32_t a, uint32_t b, uint32_t bits, int bit) {
+  const uint32_t m = (uint32_t)__builtin_amdgcn_sbfe((int)bits, bit, 1);
+  return (a & m) | (b & ~m);
+}
 
 // What of a scale goes where: |scale| log2(e) multiplies the scores, its sign
 // goes into the queries (a rounding-free change), and a scale of 0 clears them
@@ -189,7 +196,7 @@ struct Rows {
       for (int t = 0; t < ST; ++t)
 #pragma unroll
         for (int r = 0; r < 16; ++r)
-          if (!((mine >> (32 * t + acc_row(r, 0))) & 1)) s[t][r] = -INFINITY;
+          s[t][r] = __uint_as_float(select(__float_as_uint(s[t][r]), 0xff800000u, (uint32_t)(mine >> (32 * t)), acc_row(r, 0)));
     }
 
     float high = s[0][0];
@@ -223,17 +230,17 @@ struct Rows {
     }
     sum += part[0] + part[1];
 
-    const int r4 = (lane & 15) >> 2;
-    const uint32_t va = v + (4 * half + r4) * kRow + (((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ value_swizzle<D>(r4)) << 4) +
-                        ((lane & 1) << 3);
-    if (partial && !finite_values(v)) {
-      spoiled(va, p, vis);
-      return;
-    }
+    const uint32_t va = value_address(v);
 #pragma unroll
     for (int j = 0; j < PK; ++j)
 #pragma unroll
       for (int t = 0; t < DT; ++t) o[t] = T::mfma(value(va, j, t), p[j], o[t]);
+  }
+
+  __device__ __forceinline__ static uint32_t value_address(uint32_t v) {
+    const int lane = threadIdx.x & 63, r4 = (lane & 15) >> 2;
+    return v + (4 * (lane >> 5) + r4) * kRow +
+           (((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ value_swizzle<D>(r4)) << 4) + ((lane & 1) << 3);
   }
 
   // V^T fragment (16 keys j, 32 columns t) in the key order of the weights
@@ -244,31 +251,17 @@ struct Rows {
     return __builtin_bit_cast(x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
   }
 
-  // Whether the wave's values of this tile are all finite.  An unseen value
-  // has weight 0, which keeps a finite one out of the sum but no other.
-  __device__ __forceinline__ bool finite_values(uint32_t v) {
-    const int lane = threadIdx.x & 63;
-    bool bad = false;
-#pragma unroll 4
-    for (int i = 0; i < KW * kRow / 1024; ++i) {
-      const u32x4 w = *(const DFT_LDS u32x4*)(uintptr_t)(v + 1024 * i + 16 * lane);
-#pragma unroll
-      for (int x = 0; x < 4; ++x)
-        bad |= (w[x] & T::kExp) == T::kExp || ((w[x] >> 16) & T::kExp) == T::kExp;
-    }
-    return !__any(bad);
-  }
-
-  // The second product where some rows must not see a value that is not
-  // finite: those values are left out of it, and which outputs get an
-  // infinity (a NaN is both) is noted in the wave's `notes` by products of
-  // 0 / 1 matrices, for finish().  Rare, so written to need few registers.
-  __device__ __forceinline__ void spoiled(uint32_t va, const x8 (&p)[PK], uint64_t vis) {
+  // Which of the lane's outputs see a value of this tile that is an infinity
+  // or a NaN (which counts as both), by products of 0 / 1 matrices.  Kept in
+  // the wave's `notes`, for finish(); the tile's values are then cleared of
+  // them.  Rare, so written to need few registers.
+  __device__ __forceinline__ void note(uint32_t v, uint64_t vis) {
     const int lane = threadIdx.x & 63;
     DFT_LDS uint32_t* note = (DFT_LDS uint32_t*)(uintptr_t)(notes + 4 * lane);
     if (!noted)
       for (int t = 0; t < DT; ++t) note[64 * t] = 0;
     noted = true;
+    const uint32_t va = value_address(v);
     uint64_t mine = vis >> (4 * (lane >> 5));
 #pragma unroll 1
     for (int j = 0; j < PK; ++j, mine >>= 16) {
@@ -289,24 +282,11 @@ struct Rows {
           for (int x = 0; x < 4; ++x) flag[x] = infinite(w[x], sign) + (infinite(w[x] >> 16, sign) << 16);
           const f32x16 n = T::mfma(__builtin_bit_cast(x8, flag), __builtin_bit_cast(x8, seen), f32x16{});
 #pragma unroll
-          for (int r = 0; r < 16; ++r) word |= n[r] > 0 ? 1u << (r + 16 * sign) : 0u;
+          for (int r = 0; r < 16; ++r) word |= min(__float_as_uint(n[r]), 1u) << (r + 16 * sign);  // counts
         }
         note[64 * t] |= word;
       }
     }
-#pragma unroll
-    for (int j = 0; j < PK; ++j)
-#pragma unroll
-      for (int t = 0; t < DT; ++t) {
-        __builtin_amdgcn_sched_barrier(0);
-        u32x4 w = __builtin_bit_cast(u32x4, value(va, j, t));
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          if ((w[x] & T::kExp) == T::kExp) w[x] &= 0xffff0000u;
-          if ((w[x] >> 16 & T::kExp) == T::kExp) w[x] &= 0xffffu;
-        }
-        o[t] = T::mfma(__builtin_bit_cast(x8, w), p[j], o[t]);
-      }
   }
 
   // 1.0 for an infinity of that sign or a NaN in the low half, 0 otherwise
@@ -324,8 +304,8 @@ struct Rows {
       const uint32_t word = note[64 * t];
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        if (word >> r & 1) o[t][r] += INFINITY;
-        if (word >> (r + 16) & 1) o[t][r] -= INFINITY;
+        o[t][r] += __uint_as_float(select(0x7f800000u, 0, word, r));
+        o[t][r] += __uint_as_float(select(0xff800000u, 0, word, r + 16));
       }
     }
   }
@@ -333,6 +313,36 @@ struct Rows {
   // The whole row's sum, in both of its lanes.
   __device__ __forceinline__ float whole_sum() const { return sum + __shfl_xor(sum, 32); }
 };
+
+// An unseen value has weight 0, which keeps a finite one out of a row's sum but
+// no other.  Where some row of the workgroup does not see some key of a tile,
+// these look at a wave's share of the tile's values (BYTES of them), and
+// clear what is not finite.
+template <class T, int BYTES>
+__device__ __forceinline__ bool finite(uint32_t share) {
+  bool bad = false;
+#pragma unroll 4
+  for (int i = 0; i < BYTES / 1024; ++i) {
+    const u32x4 w = *(const DFT_LDS u32x4*)(uintptr_t)(share + 1024 * i + 16 * (threadIdx.x & 63));
+#pragma unroll
+    for (int x = 0; x < 4; ++x) bad |= (w[x] & T::kExp) == T::kExp || (w[x] >> 16 & T::kExp) == T::kExp;
+  }
+  return !__any(bad);
+}
+template <class T, int BYTES>
+__device__ __forceinline__ void clear_infinite(uint32_t share) {
+#pragma unroll 1
+  for (int i = 0; i < BYTES / 1024; ++i) {
+    DFT_LDS u32x4* at = (DFT_LDS u32x4*)(uintptr_t)(share + 1024 * i + 16 * (threadIdx.x & 63));
+    u32x4 w = *at;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      if ((w[x] & T::kExp) == T::kExp) w[x] &= 0xffff0000u;
+      if ((w[x] >> 16 & T::kExp) == T::kExp) w[x] &= 0xffffu;
+    }
+    *at = w;
+  }
+}
 
 // 1 / sum, 0 where a row saw no key, NaN kept
 __device__ __forceinline__ float weight_of(float sum) { return sum > 0 ? 1.f / sum : sum == 0 ? 0.f : sum; }

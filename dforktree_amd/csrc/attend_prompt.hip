@@ -18,6 +18,7 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) prompt_kernel(dft_p
   typedef Rows<D, kTile, T> Wave;
   __shared__ __attribute__((aligned(1024))) char lds[2][2][kBytes];
   __shared__ char notes[NW][Wave::kNotes];
+  __shared__ int spoiled;  // the last tile found to hold a value that is not finite
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
   const int group = a.hq / a.hkv;
   const int pairs = a.batch * a.hkv, turn = blockIdx.x / pairs, pair = blockIdx.x - turn * pairs;
@@ -43,6 +44,7 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) prompt_kernel(dft_p
   const int limit = causal ? i + 1 : n;  // keys this lane's row sees
   const int least = __builtin_amdgcn_readlane(limit, 0), most = __builtin_amdgcn_readlane(limit, 31);
   const bool works = pw < rows;
+  const int fewest = causal ? (int)(p0 / group) + 1 : n;  // keys that the workgroup's first row sees
 
   // Copy i of a wave: rows (i NW + wave) kRows ..., the first of them through
   // the scalar base, the lane's through its offset.
@@ -71,6 +73,7 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) prompt_kernel(dft_p
   Wave w;
   w.clear();
   w.notes = lds_address(notes[wave]);
+  if (threadIdx.x == 0) spoiled = -1;
   copy(0, 0);
   w.load_q(static_cast<const uint16_t*>(a.q) + (r0 + i) * a.q_row_stride + h * a.q_h_stride, sc);
   for (int t = 0; t < tiles; ++t) {
@@ -78,10 +81,20 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) prompt_kernel(dft_p
     __syncthreads();
     if (t + 1 < tiles) copy(t + 1, (t + 1) & 1);
     const int j0 = t * kTile;
-    if (!works || j0 >= most) continue;
-    const uint32_t at = lds0 + (t & 1) * 2 * kBytes;
-    const bool partial = j0 + kTile > least;
-    w.tile(at, at + kBytes, sc.c, partial, partial ? first_bits(limit - j0) : 0);
+    const uint32_t at = lds0 + (t & 1) * 2 * kBytes, mine = at + kBytes + wave * (kBytes / NW);
+    const bool acts = works && j0 < most, partial = j0 + kTile > least;
+    const uint64_t vis = partial ? first_bits(limit - j0) : ~0ull;
+    if (j0 + kTile > fewest) {
+      if (!finite<T, kBytes / NW>(mine)) spoiled = t;
+      __syncthreads();
+      if (spoiled == t) {
+        if (acts) w.note(at + kBytes, vis);
+        __syncthreads();
+        clear_infinite<T, kBytes / NW>(mine);
+        __syncthreads();
+      }
+    }
+    if (acts) w.tile(at, at + kBytes, sc.c, partial, vis);
   }
   if (!works) return;
   w.finish();
