@@ -38,12 +38,18 @@ struct Bf16 {
   static __device__ __forceinline__ f32x16 mfma(x8 a, x8 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
+  static __device__ __forceinline__ f32x4 mfma16(x8 a, x8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
 };
 struct F16 {
   typedef f16x8 x8;
   static constexpr uint32_t kExp = 0x7c00, kOne = 0x3c00;
   static __device__ __forceinline__ f32x16 mfma(x8 a, x8 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ f32x4 mfma16(x8 a, x8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
   }
 };
 
@@ -140,6 +146,13 @@ struct Scale {
 inline Scale split_scale(float scale) {
   if (scale == 0) return {kLog2e, 0, 0};
   return {fabsf(scale) * kLog2e, ~0u, scale < 0 ? 0x80008000u : 0};
+}
+
+// 1.0 for an infinity of that sign or a NaN in the low half, 0 otherwise
+template <class T>
+__device__ __forceinline__ uint32_t infinite(uint32_t w, int sign) {
+  const uint32_t e = w & 0x7fffu;
+  return e > T::kExp || (e == T::kExp && (w >> 15 & 1) == (uint32_t)sign) ? T::kOne : 0;
 }
 
 // The state of a wave's 32 rows over KW keys of each tile.
@@ -279,7 +292,7 @@ struct Rows {
         for (int sign = 0; sign < 2; ++sign) {  // +inf and NaN, -inf and NaN
           u32x4 flag;
 #pragma unroll
-          for (int x = 0; x < 4; ++x) flag[x] = infinite(w[x], sign) + (infinite(w[x] >> 16, sign) << 16);
+          for (int x = 0; x < 4; ++x) flag[x] = infinite<T>(w[x], sign) + (infinite<T>(w[x] >> 16, sign) << 16);
           const f32x16 n = T::mfma(__builtin_bit_cast(x8, flag), __builtin_bit_cast(x8, seen), f32x16{});
 #pragma unroll
           for (int r = 0; r < 16; ++r) word |= min(__float_as_uint(n[r]), 1u) << (r + 16 * sign);  // counts
@@ -287,12 +300,6 @@ struct Rows {
         note[64 * t] |= word;
       }
     }
-  }
-
-  // 1.0 for an infinity of that sign or a NaN in the low half, 0 otherwise
-  static __device__ __forceinline__ uint32_t infinite(uint32_t w, int sign) {
-    const uint32_t e = w & 0x7fffu;
-    return e > T::kExp || (e == T::kExp && (w >> 15 & 1) == (uint32_t)sign) ? T::kOne : 0;
   }
 
   // The noted infinities go into the accumulators.

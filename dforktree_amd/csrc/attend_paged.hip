@@ -1,15 +1,18 @@
 // dft_paged_attention: attention of new tokens over a paged cache.
 //
-// An item is 32 WM packed rows of one request and kv head over the keys they
-// see, in tiles of 64.  The items' tiles form one line, cut into equal shares,
-// one a workgroup: the requests' lengths, which only the device knows, neither
-// leave workgroups idle nor set the grid.  A workgroup whose share holds an
-// item whole writes its rows; one that holds a part writes the part's
-// accumulators to the workspace, at most two parts a share, and a second
-// launch joins them.  Where the block table is short the items are not cut.
+// An item is a tile of packed rows of one request (row p: token p / group,
+// head p % group of a kv head) over the keys they see, in tiles.  A kv head's
+// items stand in one line of key tiles, cut into equal shares, one a
+// workgroup: the requests' lengths, which only the device knows, neither leave
+// workgroups idle nor set the grid.  The kv heads' lines are cut alike, and
+// their workgroups run side by side: one token's heads, which lie together,
+// are read at about the same time.  A workgroup whose share holds an item
+// whole writes its rows; one that holds a part writes the part's accumulators
+// to the workspace, at most two parts a share, and a second launch joins them.
+// Where the block table is short the items are not cut.
 //
-// With few rows (decode: a token's group of heads) two waves take the halves
-// of every tile, with more each wave takes rows of its own over whole tiles.
+// few_kernel: up to 32 rows in all (decode: a token's group of heads), bound
+// by the cache's bytes.  many_kernel: more rows, 32 a wave.
 #include "attend.h"
 
 namespace dft {
@@ -17,15 +20,14 @@ namespace {
 
 using namespace attend;
 
-constexpr int kCus = 256;
-constexpr int kLeast = 4;      // tiles in a share
-constexpr int kUncut = 8;      // an item of at most so many tiles is never cut
-constexpr int kJoinWaves = 4;  // of the joining launch's workgroups
+constexpr int kCus = 256, kXcds = 8;
+constexpr int kLeastKeys = 256;  // of a share
+constexpr int kUncutKeys = 512;  // an item of at most so many keys is never cut
 
 // What a share that begins inside an item leaves for the join.
 struct Head {
   int64_t first, last, share;  // the item's tiles on the line, tiles per share
-  int32_t b, g, tile, inside;
+  int32_t b, tile, inside, pad;
 };
 
 struct Plan {
@@ -33,13 +35,15 @@ struct Plan {
   float* parts;
   uint32_t magic;  // j / page_size = j * magic >> shift for j < 2^31
   int shift;
-  int row_tiles;   // of the largest request there may be
+  int shares;      // of a kv head's line
   bool vec, uncut;
 };
 
-template <int D>
-constexpr int part_floats() {  // of a wave's 32 rows: accumulators, reference, sum
-  return 32 * D + 128;
+// A part in the workspace: units of 64 lanes x 4 accumulators, then every
+// row's reference and sum.
+template <int D, int BM>
+constexpr int part_floats() {
+  return BM * (D + 2);
 }
 
 struct Request {
@@ -63,15 +67,24 @@ __device__ __forceinline__ Request request(const dft_paged_attention_args& a, in
   return q;
 }
 
+__device__ __forceinline__ Request uniform_request(const dft_paged_attention_args& a, int b) {
+  Request q = request(a, b);
+  q.r0 = uniform64(q.r0);
+  q.n = __builtin_amdgcn_readfirstlane(q.n);
+  q.keys = __builtin_amdgcn_readfirstlane(q.keys);
+  q.before = __builtin_amdgcn_readfirstlane(q.before);
+  return q;
+}
+
 // Tiles of the row tile's keys; one where it has none, so that its rows are written.
-template <int BM>
+template <int BM, int KT>
 __device__ __forceinline__ int tiles_of(const dft_paged_attention_args& a, const Request& q, int group, int tile) {
   int keys = q.keys;
   if (a.flags & DFT_ATTN_CAUSAL) {
     const int64_t end = min((int64_t)(tile + 1) * BM, (int64_t)q.n * group);
     keys = min(keys, q.before + (int)((end - 1) / group) + 1);
   }
-  return max((keys + kTile - 1) / kTile, 1);
+  return max((keys + KT - 1) / KT, 1);
 }
 
 template <int BM>
@@ -99,119 +112,468 @@ __device__ __forceinline__ int64_t scan(int64_t x, int64_t* red, int64_t& total)
   return s - x;
 }
 
-// The rows of lane l's outputs
+// One of the rows of an item
 struct Place {
   int64_t row;
   int h;
   bool there;
 };
-__device__ __forceinline__ Place place_of(const Request& q, int group, int g, int64_t first) {
-  const int64_t rows = (int64_t)q.n * group, p = min(first + (threadIdx.x & 31), rows - 1);
-  const int64_t i = p / group;
-  return {q.r0 + i, g * group + (int)(p - i * group), first + (threadIdx.x & 31) < rows};
+__device__ __forceinline__ Place place_of(const Request& q, int group, int g, int64_t p) {
+  const int64_t rows = (int64_t)q.n * group, r = min(p, rows - 1), i = r / group;
+  return {q.r0 + i, g * group + (int)(r - i * group), p < rows};
 }
 
-template <int D, int WM, int WK, class T>
-__global__ void __launch_bounds__(64 * WM * WK, D == 256 ? 1 : 2)
-    paged_kernel(dft_paged_attention_args a, Scale sc, Plan pl) {
-  constexpr int kRow = 2 * D, kBytes = kTile * kRow, NW = WM * WK, NT = 64 * NW, BM = 32 * WM, KW = kTile / WK;
+// A workgroup's walk over its share.
+template <int BM, int KT, int NT>
+struct Walk {
+  int64_t left;  // tiles of the share not begun
+  int g, share;  // kv head, number of the share on its line
+  int b, tile, off;
+
+  __device__ __forceinline__ bool begin(const dft_paged_attention_args& a, const Plan& pl, int group) {
+    __shared__ int64_t red[NT / 64];
+    __shared__ int at[3];
+    if (pl.uncut) {
+      const int pairs = a.batch * a.hkv;
+      tile = blockIdx.x / pairs;
+      const int pair = blockIdx.x - tile * pairs;
+      b = pair / a.hkv;
+      g = pair - b * a.hkv;
+      share = 0;
+      off = 0;
+      const Request q = request(a, b);
+      if (a.status && tile == 0 && g == 0 && threadIdx.x == 0) a.status[b] = q.status;
+      if (tile >= row_tiles_of<BM>(q, group)) return false;
+      left = tiles_of<BM, KT>(a, q, group, tile);
+      return true;
+    }
+    // consecutive shares of a line on one XCD
+    const int x = (blockIdx.x % kXcds) * (gridDim.x / kXcds) + blockIdx.x / kXcds;
+    g = x / pl.shares;
+    share = x - g * pl.shares;
+    if (g >= a.hkv) return false;
+    const int per = (a.batch + NT - 1) / NT;
+    const int b0 = min((int)threadIdx.x * per, a.batch), b1 = min(b0 + per, a.batch);
+    auto weight = [&](int r) -> int64_t {
+      const Request q = request(a, r);
+      if (a.status && x == 0) a.status[r] = q.status;
+      int64_t sum = 0;
+      const int n = row_tiles_of<BM>(q, group);
+      for (int t = 0; t < n; ++t) sum += tiles_of<BM, KT>(a, q, group, t);
+      return sum;
+    };
+    int64_t mine = 0, total;
+    for (int r = b0; r < b1; ++r) mine += weight(r);
+    const int64_t ahead = scan<NT>(mine, red, total);
+    const int64_t size = max((total + pl.shares - 1) / pl.shares, (int64_t)(kLeastKeys / KT)), pos = share * size;
+    left = min(size, total - pos);
+    if (pos >= ahead && pos < ahead + mine) {
+      int64_t rest = pos - ahead;
+      int r = b0;
+      for (int64_t w; rest >= (w = weight(r)); ++r) rest -= w;
+      const Request q = request(a, r);
+      int t = 0;
+      for (int n; rest >= (n = tiles_of<BM, KT>(a, q, group, t)); ++t) rest -= n;
+      at[0] = r, at[1] = t, at[2] = (int)rest;
+    }
+    __syncthreads();
+    Head* head = reinterpret_cast<Head*>(pl.heads) + x;
+    if (left <= 0) {
+      if (threadIdx.x == 0) head->inside = 0;
+      return false;
+    }
+    b = __builtin_amdgcn_readfirstlane(at[0]);
+    tile = __builtin_amdgcn_readfirstlane(at[1]);
+    off = __builtin_amdgcn_readfirstlane(at[2]);
+    if (threadIdx.x == 0) {
+      Head h;
+      h.first = pos - off;
+      h.last = h.first + tiles_of<BM, KT>(a, request(a, b), group, tile);
+      h.share = size;
+      h.b = b, h.tile = tile, h.inside = off > 0, h.pad = 0;
+      *head = h;
+    }
+    return true;
+  }
+
+  // behind `done` tiles of the item of request q; false past the share's end
+  __device__ __forceinline__ bool next(const dft_paged_attention_args& a, const Request& q, int group, int done) {
+    left -= done;
+    if (left <= 0) return false;
+    off = 0;
+    if (++tile < row_tiles_of<BM>(q, group)) return true;
+    tile = 0;
+    do {
+      if (++b >= a.batch) return false;
+    } while (__builtin_amdgcn_readfirstlane(request(a, b).n) == 0);
+    return true;
+  }
+
+  template <int D>
+  __device__ __forceinline__ float* part(const Plan& pl, bool begins) const {
+    return pl.parts + (((int64_t)g * pl.shares + share) * 2 + begins) * part_floats<D, BM>();
+  }
+};
+
+// Where a tile's keys are: a lane's own key's address, and whether there is one.
+struct Source {
+  uint64_t at;
+  bool there;
+};
+__device__ __forceinline__ Source source(const dft_paged_attention_args& a, const Plan& pl, uint64_t base,
+                                         int64_t page_stride, int64_t token_stride, int keys, int j, int id) {
+  const uint32_t jj = (uint32_t)min(j, keys - 1), col = (uint32_t)((uint64_t)jj * pl.magic >> pl.shift);
+  const bool ok = j < keys && id >= 0 && id < a.num_pages;
+  const int64_t page = ok ? id : 0, token = ok ? (int)(jj - col * a.page_size) : 0;
+  return {base + 2 * (uint64_t)(page * page_stride + token * token_stride), ok};
+}
+__device__ __forceinline__ uint64_t id_address(const int32_t* table, const Plan& pl, int keys, int j) {
+  const uint32_t jj = (uint32_t)min(j, keys - 1);
+  return (uint64_t)(uintptr_t)(table + (uint32_t)((uint64_t)jj * pl.magic >> pl.shift));
+}
+
+// A tree row's visible keys of the 64 from j0 on.
+__device__ __forceinline__ uint64_t tree_bits(uint64_t bits, int before, int j0) {
+  const int up = before - j0;
+  return first_bits(up) | (up >= 64 || up <= -64 ? 0 : up >= 0 ? bits << up : bits >> -up);
+}
+
+// ---- up to 32 rows ---------------------------------------------------------
+// All four waves work on the same 32-key tiles: each forms the scores of all
+// rows and takes a quarter of the output's columns, so nothing is exchanged
+// between them.  Four tiles' room in the LDS keeps three on their way, 48 D x
+// 8 bytes a workgroup; page ids come three tiles ahead of their use.
+constexpr int kFewTile = 32, kFewStages = 4;
+
+// Where the value pieces lie: read by 16 lanes of 4 consecutive rows each over
+// 2 pieces.
+template <int D>
+__device__ __forceinline__ int few_value_swizzle(int row) {
+  return D == 64 ? ((row >> 1) & 3) << 1 : (row & 7) << 1;
+}
+
+// s_waitcnt: until at most n vector-memory operations are outstanding
+constexpr unsigned wait_loads(int n) { return (unsigned)((n & 15) | ((n >> 4) << 14) | (7 << 4) | (15 << 8)); }
+
+// V^T fragment: 16 columns, the tile's 32 keys in the order of the weights
+template <int D, class T>
+__device__ __forceinline__ typename T::x8 few_value(uint32_t v, int columns) {
+  const int lane = threadIdx.x & 63, row = 4 * (lane >> 4) + ((lane & 15) >> 2);
+  const uint32_t at = v + row * 2 * D + (((((lane & 3) >> 1) ^ few_value_swizzle<D>(row)) << 4) ^ (columns << 5)) + ((lane & 1) << 3);
+  const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((DFT_LDS s16x4*)(uintptr_t)at);
+  const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((DFT_LDS s16x4*)(uintptr_t)(at + 16 * 2 * D));
+  return __builtin_bit_cast(typename T::x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+// One tile for NQ x 16 rows (lane l: row l % 16) and the wave's DT x 16
+// columns.  As Rows::tile, on 16 x 16 products.
+template <int D, int NQ, int DT, class T>
+__device__ __forceinline__ void few_tile(uint32_t k, uint32_t v, int wave, const typename T::x8 (&q)[NQ][D / 32],
+                                         f32x4 (&o)[NQ][DT], float (&top)[NQ], float (&sum)[NQ], float c, bool partial,
+                                         const uint32_t (&vis)[NQ]) {
+  typedef typename T::x8 x8;
+  const int lane = threadIdx.x & 63, quad = lane >> 4, row = lane & 15;
+  const uint32_t ka = k + row * 2 * D + ((quad ^ key_swizzle<D>(row)) << 4);
+  f32x4 s[NQ][2];
+#pragma unroll
+  for (int y = 0; y < NQ; ++y) s[y][0] = s[y][1] = f32x4{};
+#pragma unroll
+  for (int j = 0; j < D / 32; ++j)
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const x8 kf = *(const DFT_LDS x8*)(uintptr_t)((ka ^ (j << 6)) + t * 16 * 2 * D);
+#pragma unroll
+      for (int y = 0; y < NQ; ++y) s[y][t] = T::mfma16(kf, q[y][j], s[y][t]);
+    }
+  x8 p[NQ];
+#pragma unroll
+  for (int y = 0; y < NQ; ++y) {
+    if (partial) {
+      const uint32_t mine = vis[y] >> (4 * quad);
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          s[y][t][r] = __uint_as_float(select(__float_as_uint(s[y][t][r]), 0xff800000u, mine, 16 * t + r));
+    }
+    float high = s[y][0][0];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) high = fmaxf(high, s[y][t][r]);
+    if (__any(high * c > top[y] + kSlack)) {
+      high = fmaxf(high, __shfl_xor(high, 16));
+      const float new_top = fmaxf(high, __shfl_xor(high, 32)) * c;
+      const bool move = new_top > top[y] + kSlack;
+      const float next = move ? new_top : top[y], by = move ? __builtin_amdgcn_exp2f(top[y] - next) : 1.f;
+      top[y] = next;
+      sum[y] *= by;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) o[y][d] *= by;
+    }
+    const float sub = top[y] == -INFINITY ? 0.f : top[y];
+    f32x8 e;
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+      e[x] = __builtin_amdgcn_exp2f(fmaf(s[y][x / 4][x % 4], c, -sub));
+      sum[y] += e[x];
+    }
+    p[y] = __builtin_convertvector(e, x8);
+  }
+#pragma unroll
+  for (int d = 0; d < DT; ++d) {
+    const x8 vf = few_value<D, T>(v, wave * DT + d);
+#pragma unroll
+    for (int y = 0; y < NQ; ++y) o[y][d] = T::mfma16(vf, p[y], o[y][d]);
+  }
+}
+
+// As Rows::note: 2 words a lane and row block, 4 bits a column block.
+template <int D, int NQ, int DT, class T>
+__device__ __forceinline__ void note_few(uint32_t v, int wave, const uint32_t (&vis)[NQ], uint32_t notes, bool noted) {
+  typedef typename T::x8 x8;
+  const int lane = threadIdx.x & 63;
+  DFT_LDS uint32_t* note = (DFT_LDS uint32_t*)(uintptr_t)(notes + 4 * lane);
+#pragma unroll
+  for (int y = 0; y < NQ; ++y) {
+    const uint32_t mine = vis[y] >> (4 * (lane >> 4));
+    u32x4 seen;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const uint32_t bits = mine >> (16 * (x / 2) + 2 * (x % 2));
+      seen[x] = (bits & 1) * T::kOne + (bits >> 1 & 1) * (T::kOne << 16);
+    }
+#pragma unroll
+    for (int sign = 0; sign < 2; ++sign) {
+      uint32_t word = noted ? note[64 * (2 * y + sign)] : 0;
+#pragma unroll 1
+      for (int d = 0; d < DT; ++d) {
+        const u32x4 w = __builtin_bit_cast(u32x4, few_value<D, T>(v, wave * DT + d));
+        u32x4 flag;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) flag[x] = infinite<T>(w[x], sign) + (infinite<T>(w[x] >> 16, sign) << 16);
+        const f32x4 n = T::mfma16(__builtin_bit_cast(x8, flag), __builtin_bit_cast(x8, seen), f32x4{});
+#pragma unroll
+        for (int r = 0; r < 4; ++r) word |= min(__float_as_uint(n[r]), 1u) << (4 * d + r);
+      }
+      note[64 * (2 * y + sign)] = word;
+    }
+  }
+}
+
+template <int D, int NQ, class T>
+__global__ void __launch_bounds__(256) few_kernel(dft_paged_attention_args a, Scale sc, Plan pl) {
+  constexpr int kRow = 2 * D, kBytes = kFewTile * kRow, BM = 16 * NQ, KT = kFewTile, kStages = kFewStages, NW = 4;
+  constexpr int kRows = 1024 / kRow, kCopies = KT / (kRows * NW), kPieces = D / 8, QK = D / 32, DT = D / 16 / NW;
+  constexpr int kLoads = 2 * kCopies + 1;  // of a wave for one tile
+  typedef typename T::x8 x8;
+  __shared__ __attribute__((aligned(1024))) char lds[kStages][2][kBytes];
+  __shared__ int ids[NW][8][64];          // page ids of a tile's keys (twice: for the values too)
+  __shared__ uint64_t from[NW][64];       // addresses of its keys, of its values
+  __shared__ uint32_t notes[NW][NQ * 2][64];
+  __shared__ int spoiled;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), quad = lane >> 4;
+  const int group = a.hq / a.hkv;
+  const bool causal = a.flags & DFT_ATTN_CAUSAL;
+  Walk<BM, KT, 256> walk;
+  if (!walk.begin(a, pl, group)) return;
+
+  const uint32_t lds0 = lds_address(lds), ids0 = lds_address(ids[wave]);
+  const int lrow = lane / kPieces, piece = lane % kPieces, g = walk.g;
+  // lanes 0 .. 31 look up the keys, the others the values
+  const bool upper = lane >= 32;
+  const uint64_t base = upper ? (uint64_t)(uintptr_t)a.value_cache + 2 * (g * a.vc_h_stride)
+                              : (uint64_t)(uintptr_t)a.key_cache + 2 * (g * a.kc_h_stride);
+  const int64_t page_stride = upper ? a.vc_page_stride : a.kc_page_stride;
+  const int64_t token_stride = upper ? a.vc_token_stride : a.kc_token_stride;
+
+  bool more = true;
+  while (more) {
+    const Request q = uniform_request(a, walk.b);
+    const int all = tiles_of<BM, KT>(a, q, group, walk.tile);
+    const int begin = walk.off, stop = (int)min((int64_t)all, begin + walk.left);
+    Place to[NQ];
+    uint64_t bits[NQ];
+    int limit[NQ], fewest = q.keys;
+#pragma unroll
+    for (int y = 0; y < NQ; ++y) {
+      to[y] = place_of(q, group, g, (int64_t)walk.tile * BM + 16 * y + (lane & 15));
+      limit[y] = q.keys;
+      bits[y] = a.anc_bits ? a.anc_bits[to[y].row] : 0;
+      if (causal) limit[y] = min(q.before + (int)(to[y].row - q.r0) + 1, q.keys);
+    }
+    if (a.anc_bits)
+      fewest = q.before;
+    else if (causal)
+      fewest = __builtin_amdgcn_readlane(limit[0], 0);
+    const int32_t* table = a.block_table + walk.b * a.table_row_stride;
+
+    auto fetch_ids = [&](int t) {
+      dma4_at(id_address(table, pl, q.keys, t * KT + (lane & 31)), ids0 + (t & 7) * 256);
+    };
+    auto copy = [&](int t) {
+      const Source s = source(a, pl, base, page_stride, token_stride, q.keys, t * KT + (lane & 31), ids[wave][t & 7][lane]);
+      from[wave][lane] = s.at;
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int x = 0; x < kCopies; ++x) {
+        const int first = (x * NW + wave) * kRows, row = first + lrow;
+        const uint32_t at = lds0 + (t & (kStages - 1)) * 2 * kBytes + first * kRow;
+        dma16_at(from[wave][row] + ((piece ^ key_swizzle<D>(row)) << 4), at);
+        dma16_at(from[wave][32 + row] + ((piece ^ few_value_swizzle<D>(row)) << 4), at + kBytes);
+      }
+    };
+    // which of the tile's keys there are
+    auto there_of = [&](int t) -> uint32_t {
+      const int j = t * KT + (lane & 31), id = ids[wave][t & 7][lane];
+      return (uint32_t)__ballot(j < q.keys && id >= 0 && id < a.num_pages);
+    };
+
+    x8 qf[NQ][QK];
+    f32x4 o[NQ][DT];
+    float top[NQ], sum[NQ];
+    bool noted = false;
+#pragma unroll
+    for (int y = 0; y < NQ; ++y) {
+      top[y] = -INFINITY;
+      sum[y] = 0;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) o[y][d] = f32x4{};
+    }
+    if (q.keys > 0 && begin * KT < q.keys) {
+      if (threadIdx.x == 0) spoiled = -1;
+      const int ahead = kStages - 1;
+      for (int t = begin; t < begin + 2 * ahead; ++t) fetch_ids(t);
+#pragma unroll
+      for (int y = 0; y < NQ; ++y) {
+        const uint16_t* row = static_cast<const uint16_t*>(a.q) + to[y].row * a.q_row_stride + to[y].h * a.q_h_stride;
+#pragma unroll
+        for (int k = 0; k < QK; ++k) {
+          u32x4 w = *reinterpret_cast<const u32x4*>(row + 32 * k + 8 * quad);
+          w = (w & sc.keep) ^ sc.flip;
+          qf[y][k] = __builtin_bit_cast(x8, w);
+        }
+      }
+      __builtin_amdgcn_s_waitcnt(kWaitDma);
+      asm volatile("" ::: "memory");
+      for (int t = begin; t < min(begin + ahead, stop); ++t) {
+        fetch_ids(t + ahead);  // again: as many loads to a tile as in the loop, which counts them
+        copy(t);
+      }
+      for (int t = begin; t < stop; ++t) {
+        // tile t's copies have landed when only those of the tiles behind it are out
+        const int behind = stop - 1 - t;
+        if (behind >= 2)
+          __builtin_amdgcn_s_waitcnt(wait_loads(2 * kLoads));
+        else if (behind == 1)
+          __builtin_amdgcn_s_waitcnt(wait_loads(kLoads));
+        else
+          __builtin_amdgcn_s_waitcnt(kWaitDma);
+        __syncthreads();
+        if (t + ahead < stop) {
+          fetch_ids(t + 2 * ahead);
+          copy(t + ahead);
+        }
+        const uint32_t kt = lds0 + (t & (kStages - 1)) * 2 * kBytes, vt = kt + kBytes;
+        const uint32_t there = there_of(t);
+        const int j0 = t * KT;
+        const bool partial = there != ~0u || j0 + KT > fewest;
+        uint32_t vis[NQ];
+        if (partial) {
+#pragma unroll
+          for (int y = 0; y < NQ; ++y)
+            vis[y] = there & (uint32_t)(a.anc_bits ? tree_bits(bits[y], q.before, j0) : first_bits(limit[y] - j0));
+          const uint32_t slice = vt + wave * (kBytes / NW);
+          if (!finite<T, kBytes / NW>(slice)) spoiled = t;
+          __syncthreads();
+          if (spoiled == t) {
+            note_few<D, NQ, DT, T>(vt, wave, vis, lds_address(notes[wave]), noted);
+            noted = true;
+            __syncthreads();
+            clear_infinite<T, kBytes / NW>(slice);
+            __syncthreads();
+          }
+        }
+        few_tile<D, NQ, DT, T>(kt, vt, wave, qf, o, top, sum, sc.c, partial, vis);
+      }
+      __syncthreads();
+    }
+
+    const bool whole = begin == 0 && stop == all;
+    float* part = walk.template part<D>(pl, begin == 0);
+#pragma unroll
+    for (int y = 0; y < NQ; ++y) {
+      sum[y] += __shfl_xor(sum[y], 16);
+      sum[y] += __shfl_xor(sum[y], 32);
+      const float by = whole ? weight_of(sum[y]) : 1.f;
+      if (noted) {
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+          const uint32_t up = notes[wave][2 * y][lane] >> (4 * d), down = notes[wave][2 * y + 1][lane] >> (4 * d);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            o[y][d][r] += __uint_as_float(select(0x7f800000u, 0, up, r));
+            o[y][d][r] += __uint_as_float(select(0xff800000u, 0, down, r));
+          }
+        }
+      }
+      if (!to[y].there) continue;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        if (whole)
+          store4(a.o, to[y].row * a.o_row_stride + to[y].h * a.o_h_stride + 16 * (wave * DT + d) + 4 * quad, a.o_dtype,
+                 pl.vec, o[y][d] * by);
+        else
+          *reinterpret_cast<f32x4*>(part + ((y * (D / 16) + wave * DT + d) * 64 + lane) * 4) = o[y][d];
+      }
+      if (wave || quad) continue;
+      if (!whole) {
+        part[BM * D + 16 * y + lane] = top[y];
+        part[BM * D + BM + 16 * y + lane] = sum[y];
+      } else if (a.lse) {
+        a.lse[to[y].row * a.lse_row_stride + to[y].h] = lse_of(top[y], sum[y]);
+      }
+    }
+    more = walk.next(a, q, group, stop - begin);
+  }
+}
+
+// ---- more rows -------------------------------------------------------------
+template <int D, int NW, class T>
+__global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) many_kernel(dft_paged_attention_args a, Scale sc, Plan pl) {
+  constexpr int kRow = 2 * D, kBytes = kTile * kRow, BM = 32 * NW;
   constexpr int kRows = 1024 / kRow, kCopies = kTile / (kRows * NW), kPieces = D / 8;
-  typedef Rows<D, KW, T> Wave;
+  typedef Rows<D, kTile, T> Wave;
   typedef uint64_t u64x2 __attribute__((ext_vector_type(2)));
   __shared__ __attribute__((aligned(1024))) char lds[2][2][kBytes];
   __shared__ char notes[NW][Wave::kNotes];
   __shared__ int ids[NW][2][kTile];                  // page ids of a tile's keys
   __shared__ u64x2 from[NW][kTile];                  // addresses of its keys and values
-  __shared__ int64_t red[NW];
   __shared__ int spoiled;                            // the last tile found to hold a value that is not finite
-  __shared__ int at_b, at_g, at_tile, at_off;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
-  const int wm = wave % WM, wk = wave / WM;
   const int group = a.hq / a.hkv;
   const bool causal = a.flags & DFT_ATTN_CAUSAL;
-
-  // ---- this workgroup's share of the line
-  int64_t pos, end, share = 0;
-  int b, g, tile, off;
-  if (pl.uncut) {
-    const int64_t x = blockIdx.x;
-    tile = (int)(x / ((int64_t)a.batch * a.hkv));
-    const int pair = (int)(x - (int64_t)tile * a.batch * a.hkv);
-    b = pair / a.hkv;
-    g = pair - b * a.hkv;
-    const Request q = request(a, b);
-    if (a.status && tile == 0 && g == 0 && threadIdx.x == 0) a.status[b] = q.status;
-    if (tile >= row_tiles_of<BM>(q, group)) return;
-    pos = off = 0;
-    end = tiles_of<BM>(a, q, group, tile);
-  } else {
-    const int per = (a.batch + NT - 1) / NT;
-    const int b0 = min((int)threadIdx.x * per, a.batch), b1 = min(b0 + per, a.batch);
-    auto weight = [&](int x) -> int64_t {  // of one kv head of request x
-      const Request q = request(a, x);
-      if (a.status && blockIdx.x == 0) a.status[x] = q.status;
-      int64_t sum = 0;
-      const int n = row_tiles_of<BM>(q, group);
-      for (int t = 0; t < n; ++t) sum += tiles_of<BM>(a, q, group, t);
-      return sum;
-    };
-    int64_t mine = 0, total;
-    for (int x = b0; x < b1; ++x) mine += weight(x) * a.hkv;
-    const int64_t ahead = scan<NT>(mine, red, total);
-    share = max((total + gridDim.x - 1) / gridDim.x, (int64_t)kLeast);
-    pos = blockIdx.x * share;
-    end = min(pos + share, total);
-    if (pos >= ahead && pos < ahead + mine) {
-      int64_t rest = pos - ahead, w = 0;
-      int x = b0;
-      for (; rest >= (w = weight(x)) * a.hkv; ++x) rest -= w * a.hkv;
-      at_b = x;
-      at_g = (int)(rest / w);
-      rest -= at_g * w;
-      const Request q = request(a, x);
-      int t = 0;
-      for (int n; rest >= (n = tiles_of<BM>(a, q, group, t)); ++t) rest -= n;
-      at_tile = t;
-      at_off = (int)rest;
-    }
-    __syncthreads();
-    if (pos >= end) {
-      if (threadIdx.x == 0) reinterpret_cast<Head*>(pl.heads)[blockIdx.x].inside = 0;
-      return;
-    }
-    b = __builtin_amdgcn_readfirstlane(at_b);
-    g = __builtin_amdgcn_readfirstlane(at_g);
-    tile = __builtin_amdgcn_readfirstlane(at_tile);
-    off = __builtin_amdgcn_readfirstlane(at_off);
-    if (threadIdx.x == 0) {
-      Head h;
-      h.first = pos - off;
-      h.last = h.first + tiles_of<BM>(a, request(a, b), group, tile);
-      h.share = share;
-      h.b = b, h.g = g, h.tile = tile, h.inside = off > 0;
-      reinterpret_cast<Head*>(pl.heads)[blockIdx.x] = h;
-    }
-  }
+  Walk<BM, kTile, 64 * NW> walk;
+  if (!walk.begin(a, pl, group)) return;
 
   const uint32_t lds0 = lds_address(lds), ids0 = lds_address(ids[wave]);
-  const int lrow = lane / kPieces, piece = lane % kPieces;
+  const int lrow = lane / kPieces, piece = lane % kPieces, g = walk.g;
+  const uint64_t kbase = (uint64_t)(uintptr_t)a.key_cache + 2 * (g * a.kc_h_stride);
+  const uint64_t vbase = (uint64_t)(uintptr_t)a.value_cache + 2 * (g * a.vc_h_stride);
   Wave w;
   w.notes = lds_address(notes[wave]);
 
-  while (true) {
-    Request q = request(a, b);
-    q.r0 = uniform64(q.r0);
-    q.n = __builtin_amdgcn_readfirstlane(q.n);
-    q.keys = __builtin_amdgcn_readfirstlane(q.keys);
-    q.before = __builtin_amdgcn_readfirstlane(q.before);
-    const int all = tiles_of<BM>(a, q, group, tile);
-    const int begin = off, stop = (int)min((int64_t)all, off + (end - pos));
-    const int64_t rows = (int64_t)q.n * group, pw = (int64_t)tile * BM + 32 * wm;
+  bool more = true;
+  while (more) {
+    const Request q = uniform_request(a, walk.b);
+    const int all = tiles_of<BM, kTile>(a, q, group, walk.tile);
+    const int begin = walk.off, stop = (int)min((int64_t)all, begin + walk.left);
+    const int64_t rows = (int64_t)q.n * group, pw = (int64_t)walk.tile * BM + 32 * wave;
     const bool works = pw < rows;
-    const Place to = place_of(q, group, g, min(pw, rows - 1));
-    const int i = (int)(to.row - q.r0);
+    const Place to = place_of(q, group, g, pw + (lane & 31));
     const int fewest = a.anc_bits ? q.before  // keys that every row of the workgroup sees
-                       : causal   ? min(q.before + (int)((int64_t)tile * BM / group) + 1, q.keys)
+                       : causal   ? min(q.before + (int)((int64_t)walk.tile * BM / group) + 1, q.keys)
                                   : q.keys;
     uint64_t bits = 0;
     int limit = q.keys, least = q.keys, most = q.keys;  // keys the lane's row sees, all rows do, any does
@@ -219,40 +581,32 @@ __global__ void __launch_bounds__(64 * WM * WK, D == 256 ? 1 : 2)
       bits = a.anc_bits[to.row];
       least = q.before;
     } else if (causal) {
-      limit = min(q.before + i + 1, q.keys);
+      limit = min(q.before + (int)(to.row - q.r0) + 1, q.keys);
       least = __builtin_amdgcn_readlane(limit, 0), most = __builtin_amdgcn_readlane(limit, 31);
     }
-    const int32_t* table = a.block_table + b * a.table_row_stride;
-    const uint64_t kbase = (uint64_t)(uintptr_t)a.key_cache + 2 * (g * a.kc_h_stride);
-    const uint64_t vbase = (uint64_t)(uintptr_t)a.value_cache + 2 * (g * a.vc_h_stride);
+    const int32_t* table = a.block_table + walk.b * a.table_row_stride;
 
     // a key's page id, for every lane of this wave's own copy of the list
     auto fetch_ids = [&](int t) {
-      const uint32_t j = (uint32_t)min(t * kTile + lane, q.keys - 1);
-      const uint32_t col = (uint32_t)((uint64_t)j * pl.magic >> pl.shift);
-      dma4_at((uint64_t)(uintptr_t)(table + col), ids0 + (t & 1) * 4 * kTile);
+      dma4_at(id_address(table, pl, q.keys, t * kTile + lane), ids0 + (t & 1) * 4 * kTile);
     };
     // the tile's keys and values; returns which of its keys there are
     auto copy = [&](int t, int stage) -> uint64_t {
-      const int j = t * kTile + lane;
-      const uint32_t jj = (uint32_t)min(j, q.keys - 1), col = (uint32_t)((uint64_t)jj * pl.magic >> pl.shift);
-      const int id = ids[wave][t & 1][lane];
-      const bool ok = j < q.keys && id >= 0 && id < a.num_pages;
-      const int64_t page = ok ? id : 0, token = ok ? (int)(jj - col * a.page_size) : 0;
-      u64x2 src = {kbase + 2 * (uint64_t)(page * a.kc_page_stride + token * a.kc_token_stride),
-                   vbase + 2 * (uint64_t)(page * a.vc_page_stride + token * a.vc_token_stride)};
-      from[wave][lane] = src;
+      const int j = t * kTile + lane, id = ids[wave][t & 1][lane];
+      const Source k = source(a, pl, kbase, a.kc_page_stride, a.kc_token_stride, q.keys, j, id);
+      const Source v = source(a, pl, vbase, a.vc_page_stride, a.vc_token_stride, q.keys, j, id);
+      from[wave][lane] = u64x2{k.at, v.at};
       asm volatile("" ::: "memory");
       __builtin_amdgcn_wave_barrier();
 #pragma unroll
       for (int x = 0; x < kCopies; ++x) {
         const int first = (x * NW + wave) * kRows, row = first + lrow;
-        src = from[wave][row];
+        const u64x2 src = from[wave][row];
         const uint32_t at = lds0 + stage * 2 * kBytes + first * kRow;
         dma16_at(src[0] + ((piece ^ key_swizzle<D>(row)) << 4), at);
         dma16_at(src[1] + ((piece ^ value_swizzle<D>(row)) << 4), at + kBytes);
       }
-      return __ballot(ok);
+      return __ballot(k.there);
     };
 
     w.clear();
@@ -271,22 +625,12 @@ __global__ void __launch_bounds__(64 * WM * WK, D == 256 ? 1 : 2)
           next = copy(t + 1, (t + 1) & 1);
           if (t + 2 < stop) fetch_ids(t + 2);
         }
-        const int j0 = t * kTile + wk * KW;
-        const uint32_t tile_at = lds0 + (t & 1) * 2 * kBytes, at = tile_at + wk * KW * kRow;
-        const uint32_t slice = tile_at + kBytes + wave * (kBytes / NW);
-        const uint64_t every = KW == 64 ? ~0ull : (1ull << KW) - 1, valid = there >> (wk * KW) & every;
-        const bool acts = works && j0 < most, partial = valid != every || j0 + KW > least;
-        uint64_t vis = every;
-        if (partial) {
-          if (a.anc_bits) {
-            const int up = q.before - j0;
-            vis = first_bits(up) | (up >= 64 || up <= -64 ? 0 : up >= 0 ? bits << up : bits >> -up);
-          } else {
-            vis = first_bits(limit - j0);
-          }
-          vis &= valid;
-        }
-        if (there != ~0ull || (t + 1) * kTile > fewest) {
+        const int j0 = t * kTile;
+        const uint32_t at = lds0 + (t & 1) * 2 * kBytes, slice = at + kBytes + wave * (kBytes / NW);
+        const bool acts = works && j0 < most, partial = there != ~0ull || j0 + kTile > least;
+        uint64_t vis = ~0ull;
+        if (partial) vis = there & (a.anc_bits ? tree_bits(bits, q.before, j0) : first_bits(limit - j0));
+        if (there != ~0ull || j0 + kTile > fewest) {
           if (!finite<T, kBytes / NW>(slice)) spoiled = t;
           __syncthreads();
           if (spoiled == t) {
@@ -302,181 +646,152 @@ __global__ void __launch_bounds__(64 * WM * WK, D == 256 ? 1 : 2)
     }
     w.finish();
 
-    if constexpr (WK == 2) {  // the halves of the tiles
-      float* other = reinterpret_cast<float*>(&lds[0][0][0]);
-      if (wk == 1) {
-#pragma unroll
-        for (int t = 0; t < Wave::DT; ++t)
-#pragma unroll
-          for (int x = 0; x < 4; ++x)
-            *reinterpret_cast<f32x4*>(other + ((t * 4 + x) * 64 + lane) * 4) =
-                f32x4{w.o[t][4 * x], w.o[t][4 * x + 1], w.o[t][4 * x + 2], w.o[t][4 * x + 3]};
-        other[32 * D + lane] = w.top;
-        other[32 * D + 64 + lane] = w.sum;
-      }
-      __syncthreads();
-      if (wk == 0) {
-        const float top = other[32 * D + lane], high = fmaxf(w.top, top);
-        const float by = w.top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(w.top - high);
-        const float his = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - high);
-        w.top = high;
-        w.sum = w.sum * by + other[32 * D + 64 + lane] * his;
+    if (works) {
+      const bool whole = begin == 0 && stop == all;
+      const float sum = w.whole_sum(), by = weight_of(sum);
+      if (to.there) {
+        float* part = walk.template part<D>(pl, begin == 0);
+        const int64_t out = to.row * a.o_row_stride + to.h * a.o_h_stride + 4 * half;
 #pragma unroll
         for (int t = 0; t < Wave::DT; ++t)
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
-            const f32x4 y = *reinterpret_cast<f32x4*>(other + ((t * 4 + x) * 64 + lane) * 4);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) w.o[t][4 * x + e] = w.o[t][4 * x + e] * by + y[e] * his;
+            f32x4 y = {w.o[t][4 * x], w.o[t][4 * x + 1], w.o[t][4 * x + 2], w.o[t][4 * x + 3]};
+            if (whole)
+              store4(a.o, out + 32 * t + 8 * x, a.o_dtype, pl.vec, y * by);
+            else
+              *reinterpret_cast<f32x4*>(part + (((wave * Wave::DT + t) * 4 + x) * 64 + lane) * 4) = y;
           }
-      }
-      __syncthreads();
-    }
-
-    if (works && wk == 0) {
-      if (begin == 0 && stop == all) {
-        const float sum = w.whole_sum(), by = weight_of(sum);
-        if (to.there) {
-          const int64_t out = to.row * a.o_row_stride + to.h * a.o_h_stride + 4 * half;
-#pragma unroll
-          for (int t = 0; t < Wave::DT; ++t)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              f32x4 y;
-#pragma unroll
-              for (int e = 0; e < 4; ++e) y[e] = w.o[t][4 * x + e] * by;
-              store4(a.o, out + 32 * t + 8 * x, a.o_dtype, pl.vec, y);
-            }
-          if (a.lse && half == 0) a.lse[to.row * a.lse_row_stride + to.h] = lse_of(w.top, sum);
+        if (half == 0) {
+          if (!whole) {
+            part[BM * D + 32 * wave + lane] = w.top;
+            part[BM * D + BM + 32 * wave + lane] = sum;
+          } else if (a.lse) {
+            a.lse[to.row * a.lse_row_stride + to.h] = lse_of(w.top, sum);
+          }
         }
-      } else if (to.there) {
-        float* part = pl.parts + (((int64_t)blockIdx.x * 2 + (begin == 0)) * WM + wm) * part_floats<D>();
-#pragma unroll
-        for (int t = 0; t < Wave::DT; ++t)
-#pragma unroll
-          for (int x = 0; x < 4; ++x)
-            *reinterpret_cast<f32x4*>(part + ((t * 4 + x) * 64 + lane) * 4) =
-                f32x4{w.o[t][4 * x], w.o[t][4 * x + 1], w.o[t][4 * x + 2], w.o[t][4 * x + 3]};
-        part[32 * D + lane] = w.top;
-        part[32 * D + 64 + lane] = w.sum;
       }
     }
-
-    // the next item of the share
-    pos += stop - begin;
-    if (pos >= end) return;
-    off = 0;
-    if (++tile < row_tiles_of<BM>(q, group)) continue;
-    tile = 0;
-    if (++g < a.hkv) continue;
-    g = 0;
-    do {
-      if (++b == a.batch) return;
-    } while (__builtin_amdgcn_readfirstlane(request(a, b).n) == 0);
+    more = walk.next(a, q, group, stop - begin);
   }
 }
 
-// Joins the parts of the item that the share boundary in front of workgroup
-// blockIdx.x cuts first: 32 columns of 32 rows, the parts dealt to the waves.
-template <int D, int WM>
-__global__ void __launch_bounds__(64 * kJoinWaves) join_kernel(dft_paged_attention_args a, Plan pl) {
-  constexpr int BM = 32 * WM;
-  const Head h = reinterpret_cast<const Head*>(pl.heads)[blockIdx.x];
-  // cut elsewhere, or before: that boundary's workgroup joins it
-  if (!h.inside || h.first < (int64_t)(blockIdx.x - 1) * h.share) return;
-  __shared__ f32x4 sums[kJoinWaves][4][64];
-  __shared__ float tops[kJoinWaves][64], totals[kJoinWaves][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
-  const int t = blockIdx.y % (D / 32), wm = blockIdx.y / (D / 32), group = a.hq / a.hkv;
-  const Request q = request(a, h.b);
-  const int64_t first = (int64_t)h.tile * BM + 32 * wm;
-  if (first >= (int64_t)q.n * group) return;
-  const Place to = place_of(q, group, h.g, first);
-  const int64_t past = (h.last - 1) / h.share;  // the item's last share
+// ---- the join --------------------------------------------------------------
+// Joins the parts of the items that share boundaries cut.  The workgroups of
+// an item's boundaries deal its units out among them: as many workgroups as
+// there are parts to read.  With few parts a wave takes a unit, with many the
+// waves divide a unit's parts.
+constexpr int kJoinWaves = 8;
 
-  float top = -INFINITY, sum = 0;
-  f32x4 o[4] = {};
-  if (to.there)
-    for (int64_t s = (int64_t)blockIdx.x - 1 + wave; s <= past; s += kJoinWaves) {
-      const float* part = pl.parts + ((s * 2 + (s < blockIdx.x)) * WM + wm) * part_floats<D>();
-      const float his = part[32 * D + lane], high = fmaxf(top, his);
-      const float by = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - high);
-      const float with = his == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(his - high);
-      top = high;
-      sum = sum * by + part[32 * D + 64 + lane] * with;
-#pragma unroll
-      for (int x = 0; x < 4; ++x)
-        o[x] = o[x] * by + *reinterpret_cast<const f32x4*>(part + ((t * 4 + x) * 64 + lane) * 4) * with;
+template <int D, int BM>
+__global__ void __launch_bounds__(64 * kJoinWaves) join_kernel(dft_paged_attention_args a, Plan pl) {
+  // rows of a block of units, units of it, of all
+  constexpr int kLane = BM <= 32 ? 16 : 32, kOf = kLane == 16 ? D / 16 : D / 8, kUnits = BM / kLane * kOf;
+  const int x = blockIdx.x, g = x / pl.shares, share = x - g * pl.shares;
+  const Head h = reinterpret_cast<const Head*>(pl.heads)[x];
+  if (!h.inside) return;
+  __shared__ f32x4 sums[kJoinWaves][64];
+  __shared__ float tops[kJoinWaves][64], totals[kJoinWaves][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, group = a.hq / a.hkv;
+  const int64_t begin = h.first / h.share, past = (h.last - 1) / h.share;  // the item's first and last share
+  const int parts = (int)(past - begin) + 1, split = parts > 8 ? kJoinWaves : 1;
+  const int units = kJoinWaves / split, turn = wave % split;  // units at a time; which of the parts
+  const float* first = pl.parts + ((int64_t)g * pl.shares + begin) * 2 * part_floats<D, BM>();
+  const Request q = request(a, h.b);
+  for (int u0 = (share - 1 - (int)begin) * units; u0 < kUnits; u0 += (parts - 1) * units) {
+    const int unit = min(u0 + wave / split, kUnits - 1), block = unit / kOf, in = unit % kOf;
+    const int row = block * kLane + lane % kLane;
+    const int d = kLane == 16 ? 16 * in + 4 * (lane / 16) : 8 * in + 4 * (lane / 32);
+    const Place to = place_of(q, group, g, (int64_t)h.tile * BM + row);
+    float top = -INFINITY, sum = 0;
+    f32x4 o = {};
+    if (to.there) {
+#pragma unroll 4
+      for (int s = turn; s < parts; s += split) {
+        const float* part = first + (int64_t)(2 * s + (s == 0)) * part_floats<D, BM>();
+        const float his = part[BM * D + row], high = fmaxf(top, his), add = part[BM * D + BM + row];
+        const f32x4 y = *reinterpret_cast<const f32x4*>(part + (unit * 64 + lane) * 4);
+        const float by = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - high);
+        const float with = his == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(his - high);
+        top = high;
+        sum = sum * by + add * with;
+        o = o * by + y * with;
+      }
     }
-  tops[wave][lane] = top;
-  totals[wave][lane] = sum;
+    if (split > 1) {
+      tops[wave][lane] = top;
+      totals[wave][lane] = sum;
+      sums[wave][lane] = o;
+      __syncthreads();
 #pragma unroll
-  for (int x = 0; x < 4; ++x) sums[wave][x][lane] = o[x];
-  __syncthreads();
-  if (wave) return;
-  float high = top;
-  for (int s = 1; s < kJoinWaves; ++s) high = fmaxf(high, tops[s][lane]);
-  sum = 0;
+      for (int s = 0; s < kJoinWaves; ++s) top = fmaxf(top, tops[s][lane]);
+      sum = 0;
+      o = f32x4{};
 #pragma unroll
-  for (int x = 0; x < 4; ++x) o[x] = f32x4{};
-  for (int s = 0; s < kJoinWaves; ++s) {
-    const float by = tops[s][lane] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(tops[s][lane] - high);
-    sum += totals[s][lane] * by;
-#pragma unroll
-    for (int x = 0; x < 4; ++x) o[x] += sums[s][x][lane] * by;
+      for (int s = 0; s < kJoinWaves; ++s) {
+        const float his = tops[s][lane], by = his == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(his - top);
+        sum += totals[s][lane] * by;
+        o += sums[s][lane] * by;
+      }
+      __syncthreads();
+    }
+    if (turn || !to.there || u0 + wave / split >= kUnits) continue;
+    store4(a.o, to.row * a.o_row_stride + to.h * a.o_h_stride + d, a.o_dtype, pl.vec, o * weight_of(sum));
+    if (a.lse && d == 0) a.lse[to.row * a.lse_row_stride + to.h] = lse_of(top, sum);
   }
-  sum += __shfl_xor(sum, 32);
-  if (!to.there) return;
-  const float by = weight_of(sum);
-  const int64_t out = to.row * a.o_row_stride + to.h * a.o_h_stride + 32 * t + 4 * half;
-#pragma unroll
-  for (int x = 0; x < 4; ++x) store4(a.o, out + 8 * x, a.o_dtype, pl.vec, o[x] * by);
-  if (a.lse && t == 0 && half == 0) a.lse[to.row * a.lse_row_stride + to.h] = lse_of(high, sum);
 }
 
 // The launch's sizes.
 struct Shape {
-  int wm;
+  int rows;  // of an item: 16, 32 (few_kernel), 128 (many_kernel)
   bool uncut;
-  int64_t grid, heads_bytes, parts_bytes;
+  int64_t grid, shares, heads_bytes, parts_bytes;
 };
 Shape shape_of(const dft_paged_attention_args& a) {
-  Shape s;
+  Shape s = {};
   const int64_t rows = (int64_t)a.n_new * (a.hq / a.hkv);
-  s.wm = rows <= 32 ? 1 : 4;
-  s.uncut = (int64_t)a.columns * a.page_size <= kUncut * kTile;
+  s.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : 128;
+  s.uncut = (int64_t)a.columns * a.page_size <= kUncutKeys;
   if (s.uncut) {
-    s.grid = (int64_t)a.batch * a.hkv * ((rows + 32 * s.wm - 1) / (32 * s.wm));
-    s.heads_bytes = s.parts_bytes = 0;
+    s.grid = (int64_t)a.batch * a.hkv * ((rows + s.rows - 1) / s.rows);
     return s;
   }
   // as many workgroups as the LDS holds: 512 D bytes of tiles each, and a little
-  s.grid = kCus * (a.head_dim == 256 ? 1 : a.head_dim == 128 ? 2 : 4);
+  const int room = kCus * (a.head_dim == 256 ? 1 : a.head_dim == 128 ? 2 : 3);
+  s.shares = a.hkv < room ? room / a.hkv : 1;
+  s.grid = (s.shares * a.hkv + kXcds - 1) / kXcds * kXcds;
   s.heads_bytes = s.grid * sizeof(Head);
-  s.parts_bytes = s.grid * 2 * s.wm * (32 * a.head_dim + 128) * sizeof(float);
+  s.parts_bytes = s.shares * a.hkv * 2 * s.rows * (a.head_dim + 2) * sizeof(float);
   return s;
 }
 
-template <int D, int WM, int WK, class T>
+template <int D, class T>
 int launch(const dft_paged_attention_args& a, const Shape& s, const Plan& pl, hipStream_t stream) {
-  paged_kernel<D, WM, WK, T><<<(unsigned)s.grid, 64 * WM * WK, 0, stream>>>(a, split_scale(a.scale), pl);
+  const Scale sc = split_scale(a.scale);
+  const unsigned grid = (unsigned)s.grid, lines = (unsigned)(s.shares * a.hkv);
+  if (s.rows == 16)
+    few_kernel<D, 1, T><<<grid, 256, 0, stream>>>(a, sc, pl);
+  else if (s.rows == 32)
+    few_kernel<D, 2, T><<<grid, 256, 0, stream>>>(a, sc, pl);
+  else
+    many_kernel<D, 4, T><<<grid, 256, 0, stream>>>(a, sc, pl);
   if (hipGetLastError() != hipSuccess) return DFT_ERR_LAUNCH;
   if (s.uncut) return DFT_OK;
-  join_kernel<D, WM><<<dim3((unsigned)s.grid, WM * D / 32), 64 * kJoinWaves, 0, stream>>>(a, pl);
+  if (s.rows == 16)
+    join_kernel<D, 16><<<lines, 64 * kJoinWaves, 0, stream>>>(a, pl);
+  else if (s.rows == 32)
+    join_kernel<D, 32><<<lines, 64 * kJoinWaves, 0, stream>>>(a, pl);
+  else
+    join_kernel<D, 128><<<lines, 64 * kJoinWaves, 0, stream>>>(a, pl);
   return hipGetLastError() == hipSuccess ? DFT_OK : DFT_ERR_LAUNCH;
-}
-
-template <int D, class T>
-int launch_rows(const dft_paged_attention_args& a, const Shape& s, const Plan& pl, hipStream_t stream) {
-  return s.wm == 1 ? launch<D, 1, 2, T>(a, s, pl, stream) : launch<D, 4, 1, T>(a, s, pl, stream);
 }
 
 template <class T>
 int launch_type(const dft_paged_attention_args& a, const Shape& s, const Plan& pl, hipStream_t stream) {
   switch (a.head_dim) {
-    case 64: return launch_rows<64, T>(a, s, pl, stream);
-    case 128: return launch_rows<128, T>(a, s, pl, stream);
-    default: return launch_rows<256, T>(a, s, pl, stream);
+    case 64: return launch<64, T>(a, s, pl, stream);
+    case 128: return launch<128, T>(a, s, pl, stream);
+    default: return launch<256, T>(a, s, pl, stream);
   }
 }
 
@@ -489,7 +804,7 @@ int64_t paged_attention_workspace(const dft_paged_attention_args* a) {
 
 int launch_paged_attention(const dft_paged_attention_args* a, hipStream_t stream) {
   const Shape s = shape_of(*a);
-  if (s.grid > 0xffffffffll / 256) return DFT_ERR_UNSUPPORTED;  // a grid counts work-items in 32 bits
+  if (s.grid > 0xffffffffll / 512) return DFT_ERR_UNSUPPORTED;  // a grid counts work-items in 32 bits
   Plan pl = {};
   pl.heads = static_cast<char*>(a->workspace);
   pl.parts = reinterpret_cast<float*>(pl.heads + s.heads_bytes);
@@ -497,7 +812,7 @@ int launch_paged_attention(const dft_paged_attention_args* a, hipStream_t stream
   while ((1ll << log) < a->page_size) ++log;
   pl.shift = 31 + log;
   pl.magic = (uint32_t)(((1ull << pl.shift) + a->page_size - 1) / a->page_size);
-  pl.row_tiles = 0;
+  pl.shares = (int)s.shares;
   pl.vec = vector_out(*a);
   pl.uncut = s.uncut;
   return a->dtype == DFT_BF16 ? launch_type<Bf16>(*a, s, pl, stream) : launch_type<F16>(*a, s, pl, stream);
