@@ -82,19 +82,33 @@ __device__ __forceinline__ void dma16(uint64_t base, uint32_t off, uint32_t lds)
       : "v"(off), "s"(base), "s"(__builtin_amdgcn_readfirstlane(lds))
       : "memory");
 }
-// the same from an address of each lane's own
+// the same from an address of each lane's own; once: of data read once, which
+// then does not displace what the caches hold
+template <bool ONCE>
 __device__ __forceinline__ void dma16_at(uint64_t at, uint32_t lds) {
   uint32_t keep;
-  asm volatile(
-      "s_mov_b32 %0, m0\n\t"
-      "s_mov_b32 m0, %2\n\t"
-      "s_nop 0\n\t"
-      "global_load_lds_dwordx4 %1, off\n\t"
-      "s_mov_b32 m0, %0\n\t"
-      "s_nop 0"
-      : "=&s"(keep)
-      : "v"(at), "s"(__builtin_amdgcn_readfirstlane(lds))
-      : "memory");
+  if constexpr (ONCE)
+    asm volatile(
+        "s_mov_b32 %0, m0\n\t"
+        "s_mov_b32 m0, %2\n\t"
+        "s_nop 0\n\t"
+        "global_load_lds_dwordx4 %1, off nt\n\t"
+        "s_mov_b32 m0, %0\n\t"
+        "s_nop 0"
+        : "=&s"(keep)
+        : "v"(at), "s"(__builtin_amdgcn_readfirstlane(lds))
+        : "memory");
+  else
+    asm volatile(
+        "s_mov_b32 %0, m0\n\t"
+        "s_mov_b32 m0, %2\n\t"
+        "s_nop 0\n\t"
+        "global_load_lds_dwordx4 %1, off\n\t"
+        "s_mov_b32 m0, %0\n\t"
+        "s_nop 0"
+        : "=&s"(keep)
+        : "v"(at), "s"(__builtin_amdgcn_readfirstlane(lds))
+        : "memory");
 }
 // and of 4 bytes a lane
 __device__ __forceinline__ void dma4_at(uint64_t at, uint32_t lds) {

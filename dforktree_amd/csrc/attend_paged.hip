@@ -48,7 +48,7 @@ constexpr int part_floats() {
 
 struct Request {
   int64_t r0;
-  int n, keys, before;  // rows, keys, keys in front of the rows' own (negative: some rows have none)
+  int n, keys, before;  // rows (times the group within 31 bits), keys, keys in front of the rows' own (negative: some rows have none)
   int status;
 };
 
@@ -81,15 +81,15 @@ template <int BM, int KT>
 __device__ __forceinline__ int tiles_of(const dft_paged_attention_args& a, const Request& q, int group, int tile) {
   int keys = q.keys;
   if (a.flags & DFT_ATTN_CAUSAL) {
-    const int64_t end = min((int64_t)(tile + 1) * BM, (int64_t)q.n * group);
-    keys = min(keys, q.before + (int)((end - 1) / group) + 1);
+    const uint32_t end = (uint32_t)min((tile + 1) * BM, q.n * group);
+    keys = min(keys, q.before + (int)((end - 1) / (uint32_t)group) + 1);
   }
   return max((keys + KT - 1) / KT, 1);
 }
 
 template <int BM>
 __device__ __forceinline__ int row_tiles_of(const Request& q, int group) {
-  return (int)(((int64_t)q.n * group + BM - 1) / BM);
+  return (q.n * group + BM - 1) / BM;
 }
 
 // Sum of the threads' values in front of this thread's, and of all.
@@ -118,9 +118,10 @@ struct Place {
   int h;
   bool there;
 };
-__device__ __forceinline__ Place place_of(const Request& q, int group, int g, int64_t p) {
-  const int64_t rows = (int64_t)q.n * group, r = min(p, rows - 1), i = r / group;
-  return {q.r0 + i, g * group + (int)(r - i * group), p < rows};
+__device__ __forceinline__ Place place_of(const Request& q, int group, int g, int p) {
+  const int rows = q.n * group, r = min(p, rows - 1);
+  const int i = (int)((uint32_t)r / (uint32_t)group);
+  return {q.r0 + i, g * group + (r - i * group), p < rows};
 }
 
 // A workgroup's walk over its share.
@@ -215,22 +216,121 @@ struct Walk {
   }
 };
 
-// Where a tile's keys are: a lane's own key's address, and whether there is one.
-struct Source {
-  uint64_t at;
-  bool there;
+// Where the value pieces lie: few_kernel reads them by 16 lanes of 4 consecutive rows each over
+// 2 pieces.
+template <int D>
+__device__ __forceinline__ int few_value_swizzle(int row) {
+  return D == 64 ? ((row >> 1) & 3) << 1 : (row & 7) << 1;
+}
+
+// s_waitcnt: until at most n vector-memory operations are outstanding
+constexpr unsigned wait_loads(int n) { return (unsigned)((n & 15) | ((n >> 4) << 14) | (7 << 4) | (15 << 8)); }
+
+// The copies of an item's tiles into STAGES places of the LDS, STAGES - 1
+// tiles ahead of their use, and of their keys' page ids, as many tiles ahead
+// of the copies.  Every wave fetches the same ids to the same place (it then
+// only waits for itself) and copies its share of the rows; a wave's loads are
+// the same number for every tile, so that a counted wait ends with a tile's.
+// FEW: the values' places are those of few_value_swizzle.
+template <int D, int KT, int NW, int STAGES, bool ONCE, bool FEW>
+struct Feed {
+  static constexpr int kRow = 2 * D, kBytes = KT * kRow, kAhead = STAGES - 1, kSlots = STAGES > 2 ? 8 : 4;
+  static constexpr int kRows = 1024 / kRow, kCopies = KT / (kRows * NW), kPieces = D / 8, kLoads = 2 * kCopies + 1;
+  static constexpr int kMine = kCopies * kRows;  // rows of a tile that a wave copies
+  struct Room {
+    char tiles[STAGES][2][kBytes];
+    uint64_t from[NW][2 * kMine];  // addresses of a wave's keys of a tile, and of its values
+    int ids[kSlots][64];           // page ids of a tile's keys; with 32 of them twice
+  };
+
+  const dft_paged_attention_args& a;
+  const Plan& pl;
+  Room& room;
+  const int32_t* table;
+  uint64_t base;  // of what the lane looks up: keys or values
+  int64_t page_stride, token_stride;
+  int keys, wave, lane;
+
+  __device__ __forceinline__ Feed(const dft_paged_attention_args& a, const Plan& pl, Room& room, int g, int wave)
+      : a(a), pl(pl), room(room), wave(wave), lane(threadIdx.x & 63) {
+    const bool value = lane & kMine;
+    base = value ? (uint64_t)(uintptr_t)a.value_cache + 2 * (g * a.vc_h_stride)
+                 : (uint64_t)(uintptr_t)a.key_cache + 2 * (g * a.kc_h_stride);
+    page_stride = value ? a.vc_page_stride : a.kc_page_stride;
+    token_stride = value ? a.vc_token_stride : a.kc_token_stride;
+  }
+  __device__ __forceinline__ uint32_t tile(int t) const {
+    return lds_address(&room) + (STAGES == 3 ? t % 3 : t & (STAGES - 1)) * 2 * kBytes;
+  }
+  __device__ __forceinline__ uint32_t column(uint32_t j) const { return (uint32_t)((uint64_t)j * pl.magic >> pl.shift); }
+
+  __device__ __forceinline__ void fetch_ids(int t) {
+    const uint32_t j = (uint32_t)min(t * KT + lane % KT, keys - 1);
+    dma4_at((uint64_t)(uintptr_t)(table + column(j)), lds_address(room.ids[t & (kSlots - 1)]));
+  }
+  // -1 for a key that there is, 0 for none.  Arithmetic, as what follows in
+  // copy(): a branch of some lanes only among so many live registers let the
+  // compiler put register copies in front of the rejoin, where they left out
+  // the other lanes (a memory fault at 256 columns in fp16).
+  __device__ __forceinline__ int there(int j, int id) const {
+    return -(int)((j < keys) & ((uint32_t)id < (uint32_t)a.num_pages));
+  }
+  __device__ __forceinline__ void copy(int t) {
+    // a lane looks up one of the wave's rows, for the keys or for the values
+    const int mine = lane % kMine, row = (mine / kRows * NW + wave) * kRows + mine % kRows, j = t * KT + row;
+    const int id = room.ids[t & (kSlots - 1)][row];
+    const uint32_t jj = (uint32_t)min(j, keys - 1);
+    const int ok = there(j, id);
+    const uint64_t page = (uint32_t)(id & ok), token = (jj - column(jj) * a.page_size) & ok;
+    room.from[wave][lane & (2 * kMine - 1)] = base + 2 * (page * page_stride + token * token_stride);
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int x = 0; x < kCopies; ++x) {
+      const int first = (x * NW + wave) * kRows, row = first + lane / kPieces, piece = lane % kPieces;
+      const uint32_t at = tile(t) + first * kRow;
+      const uint64_t* from = room.from[wave] + x * kRows + lane / kPieces;
+      dma16_at<ONCE>(from[0] + ((piece ^ key_swizzle<D>(row)) << 4), at);
+      dma16_at<ONCE>(from[kMine] + ((piece ^ (FEW ? few_value_swizzle<D>(row) : value_swizzle<D>(row))) << 4),
+                     at + kBytes);
+    }
+  }
+  // which of the tile's keys there are
+  __device__ __forceinline__ uint64_t present(int t) const {
+    return __ballot(there(t * KT + lane % KT, room.ids[t & (kSlots - 1)][lane]));
+  }
+
+  // the first tiles of an item: `between` runs while their ids are on the way
+  template <class F>
+  __device__ __forceinline__ void begin(const int32_t* row, int n, int first, int stop, F between) {
+    table = row;
+    keys = n;
+    for (int t = first; t < first + 2 * kAhead; ++t) fetch_ids(t);
+    between();
+    __builtin_amdgcn_s_waitcnt(kWaitDma);
+    asm volatile("" ::: "memory");
+    for (int t = first; t < min(first + kAhead, stop); ++t) {
+      fetch_ids(t + kAhead);  // again, for the count
+      copy(t);
+    }
+  }
+  // until this wave's copies of tile t have landed, with those of the tiles behind it out
+  __device__ __forceinline__ void wait(int t, int stop) const {
+    const int behind = min(stop - 1 - t, kAhead - 1);
+    static_assert(kAhead <= 3);
+    if (behind == 2)
+      __builtin_amdgcn_s_waitcnt(wait_loads(2 * kLoads));
+    else if (behind == 1)
+      __builtin_amdgcn_s_waitcnt(wait_loads(kLoads));
+    else
+      __builtin_amdgcn_s_waitcnt(kWaitDma);
+  }
+  __device__ __forceinline__ void advance(int t, int stop) {
+    if (t + kAhead >= stop) return;
+    fetch_ids(t + 2 * kAhead);
+    copy(t + kAhead);
+  }
 };
-__device__ __forceinline__ Source source(const dft_paged_attention_args& a, const Plan& pl, uint64_t base,
-                                         int64_t page_stride, int64_t token_stride, int keys, int j, int id) {
-  const uint32_t jj = (uint32_t)min(j, keys - 1), col = (uint32_t)((uint64_t)jj * pl.magic >> pl.shift);
-  const bool ok = j < keys && id >= 0 && id < a.num_pages;
-  const int64_t page = ok ? id : 0, token = ok ? (int)(jj - col * a.page_size) : 0;
-  return {base + 2 * (uint64_t)(page * page_stride + token * token_stride), ok};
-}
-__device__ __forceinline__ uint64_t id_address(const int32_t* table, const Plan& pl, int keys, int j) {
-  const uint32_t jj = (uint32_t)min(j, keys - 1);
-  return (uint64_t)(uintptr_t)(table + (uint32_t)((uint64_t)jj * pl.magic >> pl.shift));
-}
 
 // A tree row's visible keys of the 64 from j0 on.
 __device__ __forceinline__ uint64_t tree_bits(uint64_t bits, int before, int j0) {
@@ -244,16 +344,6 @@ __device__ __forceinline__ uint64_t tree_bits(uint64_t bits, int before, int j0)
 // between them.  Four tiles' room in the LDS keeps three on their way, 48 D x
 // 8 bytes a workgroup; page ids come three tiles ahead of their use.
 constexpr int kFewTile = 32, kFewStages = 4;
-
-// Where the value pieces lie: read by 16 lanes of 4 consecutive rows each over
-// 2 pieces.
-template <int D>
-__device__ __forceinline__ int few_value_swizzle(int row) {
-  return D == 64 ? ((row >> 1) & 3) << 1 : (row & 7) << 1;
-}
-
-// s_waitcnt: until at most n vector-memory operations are outstanding
-constexpr unsigned wait_loads(int n) { return (unsigned)((n & 15) | ((n >> 4) << 14) | (7 << 4) | (15 << 8)); }
 
 // V^T fragment: 16 columns, the tile's 32 keys in the order of the weights
 template <int D, class T>
@@ -363,13 +453,10 @@ __device__ __forceinline__ void note_few(uint32_t v, int wave, const uint32_t (&
 
 template <int D, int NQ, class T>
 __global__ void __launch_bounds__(256) few_kernel(dft_paged_attention_args a, Scale sc, Plan pl) {
-  constexpr int kRow = 2 * D, kBytes = kFewTile * kRow, BM = 16 * NQ, KT = kFewTile, kStages = kFewStages, NW = 4;
-  constexpr int kRows = 1024 / kRow, kCopies = KT / (kRows * NW), kPieces = D / 8, QK = D / 32, DT = D / 16 / NW;
-  constexpr int kLoads = 2 * kCopies + 1;  // of a wave for one tile
+  constexpr int BM = 16 * NQ, KT = kFewTile, NW = 4, QK = D / 32, DT = D / 16 / NW;
+  typedef Feed<D, KT, NW, kFewStages, true, true> Tiles;
   typedef typename T::x8 x8;
-  __shared__ __attribute__((aligned(1024))) char lds[kStages][2][kBytes];
-  __shared__ int ids[NW][8][64];          // page ids of a tile's keys (twice: for the values too)
-  __shared__ uint64_t from[NW][64];       // addresses of its keys, of its values
+  __shared__ __attribute__((aligned(1024))) typename Tiles::Room room;
   __shared__ uint32_t notes[NW][NQ * 2][64];
   __shared__ int spoiled;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), quad = lane >> 4;
@@ -378,14 +465,8 @@ __global__ void __launch_bounds__(256) few_kernel(dft_paged_attention_args a, Sc
   Walk<BM, KT, 256> walk;
   if (!walk.begin(a, pl, group)) return;
 
-  const uint32_t lds0 = lds_address(lds), ids0 = lds_address(ids[wave]);
-  const int lrow = lane / kPieces, piece = lane % kPieces, g = walk.g;
-  // lanes 0 .. 31 look up the keys, the others the values
-  const bool upper = lane >= 32;
-  const uint64_t base = upper ? (uint64_t)(uintptr_t)a.value_cache + 2 * (g * a.vc_h_stride)
-                              : (uint64_t)(uintptr_t)a.key_cache + 2 * (g * a.kc_h_stride);
-  const int64_t page_stride = upper ? a.vc_page_stride : a.kc_page_stride;
-  const int64_t token_stride = upper ? a.vc_token_stride : a.kc_token_stride;
+  const int g = walk.g;
+  Tiles feed(a, pl, room, g, wave);
 
   bool more = true;
   while (more) {
@@ -397,7 +478,7 @@ __global__ void __launch_bounds__(256) few_kernel(dft_paged_attention_args a, Sc
     int limit[NQ], fewest = q.keys;
 #pragma unroll
     for (int y = 0; y < NQ; ++y) {
-      to[y] = place_of(q, group, g, (int64_t)walk.tile * BM + 16 * y + (lane & 15));
+      to[y] = place_of(q, group, g, walk.tile * BM + 16 * y + (lane & 15));
       limit[y] = q.keys;
       bits[y] = a.anc_bits ? a.anc_bits[to[y].row] : 0;
       if (causal) limit[y] = min(q.before + (int)(to[y].row - q.r0) + 1, q.keys);
@@ -406,30 +487,6 @@ __global__ void __launch_bounds__(256) few_kernel(dft_paged_attention_args a, Sc
       fewest = q.before;
     else if (causal)
       fewest = __builtin_amdgcn_readlane(limit[0], 0);
-    const int32_t* table = a.block_table + walk.b * a.table_row_stride;
-
-    auto fetch_ids = [&](int t) {
-      dma4_at(id_address(table, pl, q.keys, t * KT + (lane & 31)), ids0 + (t & 7) * 256);
-    };
-    auto copy = [&](int t) {
-      const Source s = source(a, pl, base, page_stride, token_stride, q.keys, t * KT + (lane & 31), ids[wave][t & 7][lane]);
-      from[wave][lane] = s.at;
-      asm volatile("" ::: "memory");
-      __builtin_amdgcn_wave_barrier();
-#pragma unroll
-      for (int x = 0; x < kCopies; ++x) {
-        const int first = (x * NW + wave) * kRows, row = first + lrow;
-        const uint32_t at = lds0 + (t & (kStages - 1)) * 2 * kBytes + first * kRow;
-        dma16_at(from[wave][row] + ((piece ^ key_swizzle<D>(row)) << 4), at);
-        dma16_at(from[wave][32 + row] + ((piece ^ few_value_swizzle<D>(row)) << 4), at + kBytes);
-      }
-    };
-    // which of the tile's keys there are
-    auto there_of = [&](int t) -> uint32_t {
-      const int j = t * KT + (lane & 31), id = ids[wave][t & 7][lane];
-      return (uint32_t)__ballot(j < q.keys && id >= 0 && id < a.num_pages);
-    };
-
     x8 qf[NQ][QK];
     f32x4 o[NQ][DT];
     float top[NQ], sum[NQ];
@@ -443,8 +500,7 @@ __global__ void __launch_bounds__(256) few_kernel(dft_paged_attention_args a, Sc
     }
     if (q.keys > 0 && begin * KT < q.keys) {
       if (threadIdx.x == 0) spoiled = -1;
-      const int ahead = kStages - 1;
-      for (int t = begin; t < begin + 2 * ahead; ++t) fetch_ids(t);
+      feed.begin(a.block_table + walk.b * a.table_row_stride, q.keys, begin, stop, [&] {
 #pragma unroll
       for (int y = 0; y < NQ; ++y) {
         const uint16_t* row = static_cast<const uint16_t*>(a.q) + to[y].row * a.q_row_stride + to[y].h * a.q_h_stride;
@@ -455,28 +511,13 @@ __global__ void __launch_bounds__(256) few_kernel(dft_paged_attention_args a, Sc
           qf[y][k] = __builtin_bit_cast(x8, w);
         }
       }
-      __builtin_amdgcn_s_waitcnt(kWaitDma);
-      asm volatile("" ::: "memory");
-      for (int t = begin; t < min(begin + ahead, stop); ++t) {
-        fetch_ids(t + ahead);  // again: as many loads to a tile as in the loop, which counts them
-        copy(t);
-      }
+      });
       for (int t = begin; t < stop; ++t) {
-        // tile t's copies have landed when only those of the tiles behind it are out
-        const int behind = stop - 1 - t;
-        if (behind >= 2)
-          __builtin_amdgcn_s_waitcnt(wait_loads(2 * kLoads));
-        else if (behind == 1)
-          __builtin_amdgcn_s_waitcnt(wait_loads(kLoads));
-        else
-          __builtin_amdgcn_s_waitcnt(kWaitDma);
+        feed.wait(t, stop);
         __syncthreads();
-        if (t + ahead < stop) {
-          fetch_ids(t + 2 * ahead);
-          copy(t + ahead);
-        }
-        const uint32_t kt = lds0 + (t & (kStages - 1)) * 2 * kBytes, vt = kt + kBytes;
-        const uint32_t there = there_of(t);
+        feed.advance(t, stop);
+        const uint32_t kt = feed.tile(t), vt = kt + Tiles::kBytes;
+        const uint32_t there = (uint32_t)feed.present(t);
         const int j0 = t * KT;
         const bool partial = there != ~0u || j0 + KT > fewest;
         uint32_t vis[NQ];
@@ -484,14 +525,14 @@ __global__ void __launch_bounds__(256) few_kernel(dft_paged_attention_args a, Sc
 #pragma unroll
           for (int y = 0; y < NQ; ++y)
             vis[y] = there & (uint32_t)(a.anc_bits ? tree_bits(bits[y], q.before, j0) : first_bits(limit[y] - j0));
-          const uint32_t slice = vt + wave * (kBytes / NW);
-          if (!finite<T, kBytes / NW>(slice)) spoiled = t;
+          const uint32_t slice = vt + wave * (Tiles::kBytes / NW);
+          if (!finite<T, Tiles::kBytes / NW>(slice)) spoiled = t;
           __syncthreads();
           if (spoiled == t) {
             note_few<D, NQ, DT, T>(vt, wave, vis, lds_address(notes[wave]), noted);
             noted = true;
             __syncthreads();
-            clear_infinite<T, kBytes / NW>(slice);
+            clear_infinite<T, Tiles::kBytes / NW>(slice);
             __syncthreads();
           }
         }
@@ -540,40 +581,41 @@ __global__ void __launch_bounds__(256) few_kernel(dft_paged_attention_args a, Sc
 }
 
 // ---- more rows -------------------------------------------------------------
-template <int D, int NW, class T>
-__global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) many_kernel(dft_paged_attention_args a, Scale sc, Plan pl) {
-  constexpr int kRow = 2 * D, kBytes = kTile * kRow, BM = 32 * NW;
-  constexpr int kRows = 1024 / kRow, kCopies = kTile / (kRows * NW), kPieces = D / 8;
-  typedef Rows<D, kTile, T> Wave;
-  typedef uint64_t u64x2 __attribute__((ext_vector_type(2)));
-  __shared__ __attribute__((aligned(1024))) char lds[2][2][kBytes];
+// WM waves of 32 rows each, times WK that take a part of every tile's keys
+// and are joined through the LDS at an item's end.
+template <int D, int WM, int WK, int KT, int STAGES, bool ONCE, class T>
+__global__ void __launch_bounds__(64 * WM * WK, D == 256 ? 1 : 2)
+    many_kernel(dft_paged_attention_args a, Scale sc, Plan pl) {
+  constexpr int NW = WM * WK, BM = 32 * WM, KW = KT / WK, kRow = 2 * D;
+  typedef Feed<D, KT, NW, STAGES, ONCE, false> Tiles;
+  typedef Rows<D, KW, T> Wave;
+  constexpr int kBytes = Tiles::kBytes;
+  constexpr uint64_t kEvery = KW == 64 ? ~0ull : (1ull << KW) - 1, kAll = KT == 64 ? ~0ull : (1ull << KT) - 1;
+  __shared__ __attribute__((aligned(1024))) typename Tiles::Room room;
   __shared__ char notes[NW][Wave::kNotes];
-  __shared__ int ids[NW][2][kTile];                  // page ids of a tile's keys
-  __shared__ u64x2 from[NW][kTile];                  // addresses of its keys and values
-  __shared__ int spoiled;                            // the last tile found to hold a value that is not finite
+  __shared__ int spoiled;  // the last tile found to hold a value that is not finite
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
+  const int wm = wave % WM, wk = wave / WM;
   const int group = a.hq / a.hkv;
   const bool causal = a.flags & DFT_ATTN_CAUSAL;
-  Walk<BM, kTile, 64 * NW> walk;
+  Walk<BM, KT, 64 * NW> walk;
   if (!walk.begin(a, pl, group)) return;
 
-  const uint32_t lds0 = lds_address(lds), ids0 = lds_address(ids[wave]);
-  const int lrow = lane / kPieces, piece = lane % kPieces, g = walk.g;
-  const uint64_t kbase = (uint64_t)(uintptr_t)a.key_cache + 2 * (g * a.kc_h_stride);
-  const uint64_t vbase = (uint64_t)(uintptr_t)a.value_cache + 2 * (g * a.vc_h_stride);
+  const int g = walk.g;
+  Tiles feed(a, pl, room, g, wave);
   Wave w;
   w.notes = lds_address(notes[wave]);
 
   bool more = true;
   while (more) {
     const Request q = uniform_request(a, walk.b);
-    const int all = tiles_of<BM, kTile>(a, q, group, walk.tile);
+    const int all = tiles_of<BM, KT>(a, q, group, walk.tile);
     const int begin = walk.off, stop = (int)min((int64_t)all, begin + walk.left);
-    const int64_t rows = (int64_t)q.n * group, pw = (int64_t)walk.tile * BM + 32 * wave;
+    const int rows = q.n * group, pw = walk.tile * BM + 32 * wm;
     const bool works = pw < rows;
     const Place to = place_of(q, group, g, pw + (lane & 31));
     const int fewest = a.anc_bits ? q.before  // keys that every row of the workgroup sees
-                       : causal   ? min(q.before + (int)((int64_t)walk.tile * BM / group) + 1, q.keys)
+                       : causal   ? min(q.before + (int)((uint32_t)(walk.tile * BM) / (uint32_t)group) + 1, q.keys)
                                   : q.keys;
     uint64_t bits = 0;
     int limit = q.keys, least = q.keys, most = q.keys;  // keys the lane's row sees, all rows do, any does
@@ -584,69 +626,72 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) many_kernel(dft_pag
       limit = min(q.before + (int)(to.row - q.r0) + 1, q.keys);
       least = __builtin_amdgcn_readlane(limit, 0), most = __builtin_amdgcn_readlane(limit, 31);
     }
-    const int32_t* table = a.block_table + walk.b * a.table_row_stride;
-
-    // a key's page id, for every lane of this wave's own copy of the list
-    auto fetch_ids = [&](int t) {
-      dma4_at(id_address(table, pl, q.keys, t * kTile + lane), ids0 + (t & 1) * 4 * kTile);
-    };
-    // the tile's keys and values; returns which of its keys there are
-    auto copy = [&](int t, int stage) -> uint64_t {
-      const int j = t * kTile + lane, id = ids[wave][t & 1][lane];
-      const Source k = source(a, pl, kbase, a.kc_page_stride, a.kc_token_stride, q.keys, j, id);
-      const Source v = source(a, pl, vbase, a.vc_page_stride, a.vc_token_stride, q.keys, j, id);
-      from[wave][lane] = u64x2{k.at, v.at};
-      asm volatile("" ::: "memory");
-      __builtin_amdgcn_wave_barrier();
-#pragma unroll
-      for (int x = 0; x < kCopies; ++x) {
-        const int first = (x * NW + wave) * kRows, row = first + lrow;
-        const u64x2 src = from[wave][row];
-        const uint32_t at = lds0 + stage * 2 * kBytes + first * kRow;
-        dma16_at(src[0] + ((piece ^ key_swizzle<D>(row)) << 4), at);
-        dma16_at(src[1] + ((piece ^ value_swizzle<D>(row)) << 4), at + kBytes);
-      }
-      return __ballot(k.there);
-    };
 
     w.clear();
-    if (q.keys > 0 && begin * kTile < q.keys) {
+    if (q.keys > 0 && begin * KT < q.keys) {
       if (threadIdx.x == 0) spoiled = -1;
-      fetch_ids(begin);
-      __builtin_amdgcn_s_waitcnt(kWaitDma);
-      asm volatile("" ::: "memory");
-      uint64_t there = copy(begin, begin & 1), next = 0;
-      if (begin + 1 < stop) fetch_ids(begin + 1);
-      w.load_q(static_cast<const uint16_t*>(a.q) + to.row * a.q_row_stride + to.h * a.q_h_stride, sc);
-      for (int t = begin; t < stop; ++t, there = next) {
-        __builtin_amdgcn_s_waitcnt(kWaitDma);
+      feed.begin(a.block_table + walk.b * a.table_row_stride, q.keys, begin, stop, [&] {
+        w.load_q(static_cast<const uint16_t*>(a.q) + to.row * a.q_row_stride + to.h * a.q_h_stride, sc);
+      });
+      for (int t = begin; t < stop; ++t) {
+        feed.wait(t, stop);
         __syncthreads();
-        if (t + 1 < stop) {
-          next = copy(t + 1, (t + 1) & 1);
-          if (t + 2 < stop) fetch_ids(t + 2);
-        }
-        const int j0 = t * kTile;
-        const uint32_t at = lds0 + (t & 1) * 2 * kBytes, slice = at + kBytes + wave * (kBytes / NW);
-        const bool acts = works && j0 < most, partial = there != ~0ull || j0 + kTile > least;
-        uint64_t vis = ~0ull;
-        if (partial) vis = there & (a.anc_bits ? tree_bits(bits, q.before, j0) : first_bits(limit - j0));
-        if (there != ~0ull || j0 + kTile > fewest) {
+        feed.advance(t, stop);
+        const uint32_t kt = feed.tile(t), vt = kt + kBytes, slice = vt + wave * (kBytes / NW);
+        const uint64_t there = feed.present(t) & kAll, mine = there >> (wk * KW) & kEvery;
+        const int j0 = t * KT + wk * KW;
+        const bool acts = works && j0 < most, partial = mine != kEvery || j0 + KW > least;
+        uint64_t vis = kEvery;
+        if (partial) vis = mine & (a.anc_bits ? tree_bits(bits, q.before, j0) : first_bits(limit - j0));
+        if (there != kAll || (t + 1) * KT > fewest) {
           if (!finite<T, kBytes / NW>(slice)) spoiled = t;
           __syncthreads();
           if (spoiled == t) {
-            if (acts) w.note(at + kBytes, vis);
+            if (acts) w.note(vt + wk * KW * kRow, vis);
             __syncthreads();
             clear_infinite<T, kBytes / NW>(slice);
             __syncthreads();
           }
         }
-        if (acts) w.tile(at, at + kBytes, sc.c, partial, vis);
+        if (acts) w.tile(kt + wk * KW * kRow, vt + wk * KW * kRow, sc.c, partial, vis);
       }
       __syncthreads();
     }
     w.finish();
 
-    if (works) {
+    if constexpr (WK == 2) {
+      static_assert(sizeof(room.tiles) >= WM * (32 * D + 128) * sizeof(float));
+      float* his = reinterpret_cast<float*>(room.tiles) + wm * (32 * D + 128);
+      if (wk == 1) {
+#pragma unroll
+        for (int t = 0; t < Wave::DT; ++t)
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+            *reinterpret_cast<f32x4*>(his + ((t * 4 + x) * 64 + lane) * 4) =
+                f32x4{w.o[t][4 * x], w.o[t][4 * x + 1], w.o[t][4 * x + 2], w.o[t][4 * x + 3]};
+        his[32 * D + lane] = w.top;
+        his[32 * D + 64 + lane] = w.sum;
+      }
+      __syncthreads();
+      if (wk == 0) {
+        const float top = his[32 * D + lane], high = fmaxf(w.top, top);
+        const float by = w.top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(w.top - high);
+        const float with = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - high);
+        w.top = high;
+        w.sum = w.sum * by + his[32 * D + 64 + lane] * with;
+#pragma unroll
+        for (int t = 0; t < Wave::DT; ++t)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const f32x4 y = *reinterpret_cast<f32x4*>(his + ((t * 4 + x) * 64 + lane) * 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w.o[t][4 * x + e] = w.o[t][4 * x + e] * by + y[e] * with;
+          }
+      }
+      __syncthreads();
+    }
+
+    if (works && wk == 0) {
       const bool whole = begin == 0 && stop == all;
       const float sum = w.whole_sum(), by = weight_of(sum);
       if (to.there) {
@@ -660,12 +705,12 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) many_kernel(dft_pag
             if (whole)
               store4(a.o, out + 32 * t + 8 * x, a.o_dtype, pl.vec, y * by);
             else
-              *reinterpret_cast<f32x4*>(part + (((wave * Wave::DT + t) * 4 + x) * 64 + lane) * 4) = y;
+              *reinterpret_cast<f32x4*>(part + (((wm * Wave::DT + t) * 4 + x) * 64 + lane) * 4) = y;
           }
         if (half == 0) {
           if (!whole) {
-            part[BM * D + 32 * wave + lane] = w.top;
-            part[BM * D + BM + 32 * wave + lane] = sum;
+            part[BM * D + 32 * wm + lane] = w.top;
+            part[BM * D + BM + 32 * wm + lane] = sum;
           } else if (a.lse) {
             a.lse[to.row * a.lse_row_stride + to.h] = lse_of(w.top, sum);
           }
@@ -702,7 +747,7 @@ __global__ void __launch_bounds__(64 * kJoinWaves) join_kernel(dft_paged_attenti
     const int unit = min(u0 + wave / split, kUnits - 1), block = unit / kOf, in = unit % kOf;
     const int row = block * kLane + lane % kLane;
     const int d = kLane == 16 ? 16 * in + 4 * (lane / 16) : 8 * in + 4 * (lane / 32);
-    const Place to = place_of(q, group, g, (int64_t)h.tile * BM + row);
+    const Place to = place_of(q, group, g, h.tile * BM + row);
     float top = -INFINITY, sum = 0;
     f32x4 o = {};
     if (to.there) {
@@ -744,20 +789,21 @@ __global__ void __launch_bounds__(64 * kJoinWaves) join_kernel(dft_paged_attenti
 // The launch's sizes.
 struct Shape {
   int rows;  // of an item: 16, 32 (few_kernel), 128 (many_kernel)
-  bool uncut;
+  bool once, uncut;
   int64_t grid, shares, heads_bytes, parts_bytes;
 };
 Shape shape_of(const dft_paged_attention_args& a) {
   Shape s = {};
   const int64_t rows = (int64_t)a.n_new * (a.hq / a.hkv);
   s.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : 128;
+  s.once = rows <= s.rows;  // a key is read for one item only
   s.uncut = (int64_t)a.columns * a.page_size <= kUncutKeys;
   if (s.uncut) {
     s.grid = (int64_t)a.batch * a.hkv * ((rows + s.rows - 1) / s.rows);
     return s;
   }
   // as many workgroups as the LDS holds: 512 D bytes of tiles each, and a little
-  const int room = kCus * (a.head_dim == 256 ? 1 : a.head_dim == 128 ? 2 : 3);
+  const int room = kCus * (a.head_dim == 256 ? 1 : a.head_dim == 128 ? s.rows == 128 && s.once ? 1 : 2 : 3);
   s.shares = a.hkv < room ? room / a.hkv : 1;
   s.grid = (s.shares * a.hkv + kXcds - 1) / kXcds * kXcds;
   s.heads_bytes = s.grid * sizeof(Head);
@@ -773,8 +819,12 @@ int launch(const dft_paged_attention_args& a, const Shape& s, const Plan& pl, hi
     few_kernel<D, 1, T><<<grid, 256, 0, stream>>>(a, sc, pl);
   else if (s.rows == 32)
     few_kernel<D, 2, T><<<grid, 256, 0, stream>>>(a, sc, pl);
+  else if (!s.once)
+    many_kernel<D, 4, 1, 64, 2, false, T><<<grid, 256, 0, stream>>>(a, sc, pl);
+  else if constexpr (D == 128)
+    many_kernel<D, 4, 2, 64, 4, true, T><<<grid, 512, 0, stream>>>(a, sc, pl);
   else
-    many_kernel<D, 4, T><<<grid, 256, 0, stream>>>(a, sc, pl);
+    many_kernel<D, 4, 1, 32, 4, true, T><<<grid, 256, 0, stream>>>(a, sc, pl);
   if (hipGetLastError() != hipSuccess) return DFT_ERR_LAUNCH;
   if (s.uncut) return DFT_OK;
   if (s.rows == 16)

@@ -32,19 +32,19 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) prompt_kernel(dft_p
   if (a.status && turn == 0 && g == 0 && threadIdx.x == 0) a.status[b] = cut ? DFT_STATUS_SPAN : 0;
 
   // the longest rows first: they see the most keys
-  const int64_t p0 = (int64_t)(gridDim.x / pairs - 1 - turn) * 32 * NW, rows = (int64_t)n * group;
+  const int p0 = (int)(gridDim.x / pairs - 1 - turn) * 32 * NW, rows = n * group;
   if (p0 >= rows) return;
   const bool causal = a.flags & DFT_ATTN_CAUSAL;
-  const int last = (int)((min(p0 + 32 * NW, rows) - 1) / group);  // token of the workgroup's last row
+  const int last = (int)((uint32_t)(min(p0 + 32 * NW, rows) - 1) / (uint32_t)group);  // token of the workgroup's last row
   const int keys = causal ? last + 1 : n, tiles = (keys + kTile - 1) / kTile;
 
-  const int64_t pw = p0 + 32 * wave;  // the wave's first row
-  const int64_t p = min(pw + (lane & 31), rows - 1);
-  const int i = (int)(p / group), h = g * group + (int)(p - (int64_t)i * group);
+  const int pw = p0 + 32 * wave;  // the wave's first row
+  const int p = min(pw + (lane & 31), rows - 1);
+  const int i = (int)((uint32_t)p / (uint32_t)group), h = g * group + (p - i * group);
   const int limit = causal ? i + 1 : n;  // keys this lane's row sees
   const int least = __builtin_amdgcn_readlane(limit, 0), most = __builtin_amdgcn_readlane(limit, 31);
   const bool works = pw < rows;
-  const int fewest = causal ? (int)(p0 / group) + 1 : n;  // keys that the workgroup's first row sees
+  const int fewest = causal ? (int)((uint32_t)p0 / (uint32_t)group) + 1 : n;  // keys that the workgroup's first row sees
 
   // Copy i of a wave: rows (i NW + wave) kRows ..., the first of them through
   // the scalar base, the lane's through its offset.

@@ -92,6 +92,8 @@ int attention_status(const Args* a, int span) {
   if (!float_tag(a->o_dtype)) return DFT_ERR_INVALID;
   if (a->batch == 0 || span == 0 || a->rows == 0) return -1;
   if (a->batch > 65535 || a->hq > 65535) return DFT_ERR_UNSUPPORTED;
+  // a request's rows times the heads of a group are counted in 31 bits
+  if ((int64_t)span * (a->hq / a->hkv) > 0x7fff0000ll) return DFT_ERR_UNSUPPORTED;
   if (!a->q || !a->o) return DFT_ERR_INVALID;
   if (!aligned16(a->q) || a->q_row_stride % 8 || a->q_h_stride % 8) return DFT_ERR_INVALID;
   return DFT_OK;
