@@ -64,51 +64,167 @@ __device__ __forceinline__ uint32_t lds_address(const void* p) {
   return (uint32_t)(uintptr_t)(const DFT_LDS void*)p;
 }
 
-// global -> LDS, 16 bytes a lane to lds + 16 * lane, from base + off bytes.
+// global -> LDS, N copies of 16 bytes a lane: copy i from base + from[i] bytes
+// to lds + i STEP + 16 * lane.
 // Issued from inline assembly, which the backend's wait analysis does not see:
 // it would wait for the copy ahead of the next LDS read of any tile.  The
 // caller waits for vmcnt before the tile is read.  m0 is reserved to the
-// backend: its value is kept, with the wait state that a write of m0 needs.
-__device__ __forceinline__ void dma16(uint64_t base, uint32_t off, uint32_t lds) {
+// backend: its value is kept.  A copy needs a wait state after a write of m0,
+// and five after a vector write of its scalar base.
+template <int N, int STEP>
+__device__ __forceinline__ void dma16(uint64_t base, const uint32_t* from, uint32_t lds) {
   uint32_t keep;
-  asm volatile(
-      "s_mov_b32 %0, m0\n\t"
-      "s_mov_b32 m0, %3\n\t"
-      "s_nop 0\n\t"
-      "global_load_lds_dwordx4 %1, %2\n\t"
-      "s_mov_b32 m0, %0\n\t"
-      "s_nop 0"
-      : "=&s"(keep)
-      : "v"(off), "s"(base), "s"(__builtin_amdgcn_readfirstlane(lds))
-      : "memory");
+  static_assert(N == 1 || N == 2 || N == 4 || N == 8);
+  if constexpr (N == 8) {
+    dma16<4, STEP>(base, from, lds);
+    dma16<4, STEP>(base, from + 4, lds + 4 * STEP);
+  } else if constexpr (N == 4) {
+    asm volatile(
+        "s_mov_b32 %0, m0\n\t"
+        "s_mov_b32 m0, %6\n\t"
+        "s_nop 2\n\t"
+        "global_load_lds_dwordx4 %1, %5\n\t"
+        "s_add_u32 m0, m0, %7\n\t"
+        "s_nop 0\n\t"
+        "global_load_lds_dwordx4 %2, %5\n\t"
+        "s_add_u32 m0, m0, %7\n\t"
+        "s_nop 0\n\t"
+        "global_load_lds_dwordx4 %3, %5\n\t"
+        "s_add_u32 m0, m0, %7\n\t"
+        "s_nop 0\n\t"
+        "global_load_lds_dwordx4 %4, %5\n\t"
+        "s_mov_b32 m0, %0\n\t"
+        "s_nop 0"
+        : "=&s"(keep)
+        : "v"(from[0]), "v"(from[1]), "v"(from[2]), "v"(from[3]), "s"(base), "s"(__builtin_amdgcn_readfirstlane(lds)), "i"(STEP)
+        : "memory", "scc");
+  } else if constexpr (N == 2) {
+    asm volatile(
+        "s_mov_b32 %0, m0\n\t"
+        "s_mov_b32 m0, %4\n\t"
+        "s_nop 2\n\t"
+        "global_load_lds_dwordx4 %1, %3\n\t"
+        "s_add_u32 m0, m0, %5\n\t"
+        "s_nop 0\n\t"
+        "global_load_lds_dwordx4 %2, %3\n\t"
+        "s_mov_b32 m0, %0\n\t"
+        "s_nop 0"
+        : "=&s"(keep)
+        : "v"(from[0]), "v"(from[1]), "s"(base), "s"(__builtin_amdgcn_readfirstlane(lds)), "i"(STEP)
+        : "memory", "scc");
+  } else if constexpr (N == 1) {
+    asm volatile(
+        "s_mov_b32 %0, m0\n\t"
+        "s_mov_b32 m0, %3\n\t"
+        "s_nop 2\n\t"
+        "global_load_lds_dwordx4 %1, %2\n\t"
+        "s_mov_b32 m0, %0\n\t"
+        "s_nop 0"
+        : "=&s"(keep)
+        : "v"(from[0]), "s"(base), "s"(__builtin_amdgcn_readfirstlane(lds)), "i"(STEP)
+        : "memory", "scc");
+  }
 }
-// the same from an address of each lane's own; once: of data read once, which
+// the same from addresses of each lane's own; ONCE: of data read once, which
 // then does not displace what the caches hold
-template <bool ONCE>
-__device__ __forceinline__ void dma16_at(uint64_t at, uint32_t lds) {
+template <int N, int STEP, bool ONCE>
+__device__ __forceinline__ void dma16_at(const uint64_t* from, uint32_t lds) {
   uint32_t keep;
-  if constexpr (ONCE)
+  static_assert(N == 1 || N == 2 || N == 4 || N == 8);
+  if constexpr (N == 8) {
+    dma16_at<4, STEP, ONCE>(from, lds);
+    dma16_at<4, STEP, ONCE>(from + 4, lds + 4 * STEP);
+  } else if constexpr (N == 4 && ONCE) {
+    asm volatile(
+        "s_mov_b32 %0, m0\n\t"
+        "s_mov_b32 m0, %5\n\t"
+        "s_nop 2\n\t"
+        "global_load_lds_dwordx4 %1, off nt\n\t"
+        "s_add_u32 m0, m0, %6\n\t"
+        "s_nop 0\n\t"
+        "global_load_lds_dwordx4 %2, off nt\n\t"
+        "s_add_u32 m0, m0, %6\n\t"
+        "s_nop 0\n\t"
+        "global_load_lds_dwordx4 %3, off nt\n\t"
+        "s_add_u32 m0, m0, %6\n\t"
+        "s_nop 0\n\t"
+        "global_load_lds_dwordx4 %4, off nt\n\t"
+        "s_mov_b32 m0, %0\n\t"
+        "s_nop 0"
+        : "=&s"(keep)
+        : "v"(from[0]), "v"(from[1]), "v"(from[2]), "v"(from[3]), "s"(__builtin_amdgcn_readfirstlane(lds)), "i"(STEP)
+        : "memory", "scc");
+  } else if constexpr (N == 4) {
+    asm volatile(
+        "s_mov_b32 %0, m0\n\t"
+        "s_mov_b32 m0, %5\n\t"
+        "s_nop 2\n\t"
+        "global_load_lds_dwordx4 %1, off\n\t"
+        "s_add_u32 m0, m0, %6\n\t"
+        "s_nop 0\n\t"
+        "global_load_lds_dwordx4 %2, off\n\t"
+        "s_add_u32 m0, m0, %6\n\t"
+        "s_nop 0\n\t"
+        "global_load_lds_dwordx4 %3, off\n\t"
+        "s_add_u32 m0, m0, %6\n\t"
+        "s_nop 0\n\t"
+        "global_load_lds_dwordx4 %4, off\n\t"
+        "s_mov_b32 m0, %0\n\t"
+        "s_nop 0"
+        : "=&s"(keep)
+        : "v"(from[0]), "v"(from[1]), "v"(from[2]), "v"(from[3]), "s"(__builtin_amdgcn_readfirstlane(lds)), "i"(STEP)
+        : "memory", "scc");
+  } else if constexpr (N == 2 && ONCE) {
+    asm volatile(
+        "s_mov_b32 %0, m0\n\t"
+        "s_mov_b32 m0, %3\n\t"
+        "s_nop 2\n\t"
+        "global_load_lds_dwordx4 %1, off nt\n\t"
+        "s_add_u32 m0, m0, %4\n\t"
+        "s_nop 0\n\t"
+        "global_load_lds_dwordx4 %2, off nt\n\t"
+        "s_mov_b32 m0, %0\n\t"
+        "s_nop 0"
+        : "=&s"(keep)
+        : "v"(from[0]), "v"(from[1]), "s"(__builtin_amdgcn_readfirstlane(lds)), "i"(STEP)
+        : "memory", "scc");
+  } else if constexpr (N == 2) {
+    asm volatile(
+        "s_mov_b32 %0, m0\n\t"
+        "s_mov_b32 m0, %3\n\t"
+        "s_nop 2\n\t"
+        "global_load_lds_dwordx4 %1, off\n\t"
+        "s_add_u32 m0, m0, %4\n\t"
+        "s_nop 0\n\t"
+        "global_load_lds_dwordx4 %2, off\n\t"
+        "s_mov_b32 m0, %0\n\t"
+        "s_nop 0"
+        : "=&s"(keep)
+        : "v"(from[0]), "v"(from[1]), "s"(__builtin_amdgcn_readfirstlane(lds)), "i"(STEP)
+        : "memory", "scc");
+  } else if constexpr (N == 1 && ONCE) {
     asm volatile(
         "s_mov_b32 %0, m0\n\t"
         "s_mov_b32 m0, %2\n\t"
-        "s_nop 0\n\t"
+        "s_nop 2\n\t"
         "global_load_lds_dwordx4 %1, off nt\n\t"
         "s_mov_b32 m0, %0\n\t"
         "s_nop 0"
         : "=&s"(keep)
-        : "v"(at), "s"(__builtin_amdgcn_readfirstlane(lds))
-        : "memory");
-  else
+        : "v"(from[0]), "s"(__builtin_amdgcn_readfirstlane(lds)), "i"(STEP)
+        : "memory", "scc");
+  } else if constexpr (N == 1) {
     asm volatile(
         "s_mov_b32 %0, m0\n\t"
         "s_mov_b32 m0, %2\n\t"
-        "s_nop 0\n\t"
+        "s_nop 2\n\t"
         "global_load_lds_dwordx4 %1, off\n\t"
         "s_mov_b32 m0, %0\n\t"
         "s_nop 0"
         : "=&s"(keep)
-        : "v"(at), "s"(__builtin_amdgcn_readfirstlane(lds))
-        : "memory");
+        : "v"(from[0]), "s"(__builtin_amdgcn_readfirstlane(lds)), "i"(STEP)
+        : "memory", "scc");
+  }
 }
 // and of 4 bytes a lane
 __device__ __forceinline__ void dma4_at(uint64_t at, uint32_t lds) {
@@ -169,6 +285,48 @@ __device__ __forceinline__ uint32_t infinite(uint32_t w, int sign) {
   return e > T::kExp || (e == T::kExp && (w >> 15 & 1) == (uint32_t)sign) ? T::kOne : 0;
 }
 
+// N times four outputs in a row: value(i) to o[at + offset(i)].  `vec`: in whole pieces
+template <int N, class Value, class Offset>
+__device__ __forceinline__ void store_all(void* o, int64_t at, int dtype, bool vec, Value value, Offset offset) {
+  typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+  typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+  typedef uint16_t u16x4 __attribute__((ext_vector_type(4)));
+  if (dtype == DFT_F32) {
+    float* to = static_cast<float*>(o) + at;
+    if (vec) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) *reinterpret_cast<f32x4*>(to + offset(i)) = value(i);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const f32x4 x = value(i);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) to[offset(i) + e] = x[e];
+      }
+    }
+    return;
+  }
+  uint16_t* to = static_cast<uint16_t*>(o) + at;
+  const bool bf16 = dtype == DFT_BF16;
+  auto narrow = [&](int i) {
+    const f32x4 x = value(i);
+    const u16x4 b = __builtin_bit_cast(u16x4, __builtin_convertvector(x, bf16x4));
+    const u16x4 h = __builtin_bit_cast(u16x4, __builtin_convertvector(x, f16x4));
+    return bf16 ? b : h;
+  };
+  if (vec) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) *reinterpret_cast<u16x4*>(to + offset(i)) = narrow(i);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const u16x4 y = narrow(i);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) to[offset(i) + e] = y[e];
+    }
+  }
+}
+
 // The state of a wave's 32 rows over KW keys of each tile.
 template <int D, int KW, class T>
 struct Rows {
@@ -180,6 +338,7 @@ struct Rows {
   f32x16 o[DT];  // lane: d = 32 t + acc_row(r, lane / 32) of its row
   float top;     // the reference that the weights are taken against, in log2 units (-inf: none yet)
   float sum;     // of the weights of this lane's keys
+  float high;    // of the lane's scores of the tile at hand
   bool noted;    // whether `notes` holds infinities that the accumulators lack
   uint32_t notes;  // LDS address of kNotes bytes of the wave's own
   static constexpr int kNotes = 256 * DT;
@@ -203,67 +362,125 @@ struct Rows {
     }
   }
 
-  // One tile: keys and values at the LDS addresses k and v (rows of kRow
-  // bytes, kRow-aligned).  With `partial`, vis holds the lane's visible keys.
-  __device__ __forceinline__ void tile(uint32_t k, uint32_t v, float c, bool partial, uint64_t vis) {
-    const int lane = threadIdx.x & 63, half = lane >> 5, row = lane & 31;
-    const uint32_t ka = k + row * kRow + ((half ^ key_swizzle<D>(row)) << 4);
-    f32x16 s[ST];
+  typedef f32x16 Scores[ST];
+
+  // A tile's scores, from its keys at LDS address k (rows of kRow bytes,
+  // kRow-aligned).
+  __device__ __forceinline__ void scores(uint32_t k, Scores& s) {
 #pragma unroll
     for (int t = 0; t < ST; ++t) s[t] = f32x16{};
 #pragma unroll
     for (int j = 0; j < QK; ++j)
 #pragma unroll
-      for (int t = 0; t < ST; ++t)
-        s[t] = T::mfma(*(const DFT_LDS x8*)(uintptr_t)((ka ^ (j << 5)) + t * 32 * kRow), q[j], s[t]);
+      for (int t = 0; t < ST; ++t) s[t] = T::mfma(key(key_address(k), j, t), q[j], s[t]);
+    high = peak(s);
+  }
 
-    if (partial) {
-      const uint64_t mine = vis >> (4 * half);
-#pragma unroll
-      for (int t = 0; t < ST; ++t)
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          s[t][r] = __uint_as_float(select(__float_as_uint(s[t][r]), 0xff800000u, (uint32_t)(mine >> (32 * t)), acc_row(r, 0)));
-    }
-
-    float high = s[0][0];
+  // Leaves the lane's visible keys, the bits of vis.
+  __device__ __forceinline__ void mask(Scores& s, uint64_t vis) {
+    const uint64_t mine = vis >> (4 * ((threadIdx.x & 63) >> 5));
 #pragma unroll
     for (int t = 0; t < ST; ++t)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) high = fmaxf(high, s[t][r]);
-    if (__any(high * c > top + kSlack)) {
-      // row by row: what a row gets does not depend on the others of the wave
-      const float new_top = fmaxf(high, __shfl_xor(high, 32)) * c;
-      const bool move = new_top > top + kSlack;
-      const float next = move ? new_top : top, by = move ? __builtin_amdgcn_exp2f(top - next) : 1.f;
-      top = next;
-      sum *= by;
-#pragma unroll
-      for (int t = 0; t < DT; ++t) o[t] *= by;
-    }
-    const float sub = top == -INFINITY ? 0.f : top;
-    x8 p[PK];
-    float part[2] = {0, 0};
-#pragma unroll
-    for (int j = 0; j < PK; ++j) {
-      f32x8 e;
-#pragma unroll
-      for (int x = 0; x < 8; ++x) {
-        e[x] = __builtin_amdgcn_exp2f(fmaf(s[j / 2][8 * (j % 2) + x], c, -sub));
-        part[x & 1] += e[x];
-      }
-      // the weights are rounded to the inputs' type, half a step each, for the second product
-      p[j] = __builtin_convertvector(e, x8);
-    }
-    sum += part[0] + part[1];
-
-    const uint32_t va = value_address(v);
-#pragma unroll
-    for (int j = 0; j < PK; ++j)
-#pragma unroll
-      for (int t = 0; t < DT; ++t) o[t] = T::mfma(value(va, j, t), p[j], o[t]);
+      for (int r = 0; r < 16; ++r)
+        s[t][r] = __uint_as_float(select(__float_as_uint(s[t][r]), 0xff800000u, (uint32_t)(mine >> (32 * t)), acc_row(r, 0)));
+    high = peak(s);
   }
 
+  // Moves the reference of the rows whose scores (high: their maximum so far)
+  // exceed it by too much.
+  __device__ __forceinline__ void settle(float c) {
+    if (!__any(high * c > top + kSlack)) return;
+    // row by row: what a row gets does not depend on the others of the wave
+    const float new_top = fmaxf(high, __shfl_xor(high, 32)) * c;
+    const bool move = new_top > top + kSlack;
+    const float next = move ? new_top : top, by = move ? __builtin_amdgcn_exp2f(top - next) : 1.f;
+    top = next;
+    sum *= by;
+#pragma unroll
+    for (int t = 0; t < DT; ++t) o[t] *= by;
+  }
+
+  // The rest of a tile whose scores are s, with its values at v: the weights
+  // and the second product.  With NEXT also the next tile's scores, from its
+  // keys at k: the matrix unit forms them while the weights are taken.  The
+  // order is pinned product by product, each with the fragment read ahead by
+  // kReach products and its share of the weights: left to itself the compiler
+  // reads a fragment right in front of its product and waits for the LDS.
+  static constexpr int kReach = 4;
+
+  template <bool NEXT>
+  __device__ __forceinline__ void step(uint32_t k, uint32_t v, float c, Scores& s) {
+    settle(c);
+    const float sub = top == -INFINITY ? 0.f : top;
+    const uint32_t ka = key_address(k), va = value_address(v);
+    x8 p[PK], ring[kReach];
+    float part[2] = {0, 0};
+    // weight pair i of the tile: scores 2 i and 2 i + 1 of the lane, rounded
+    // to the inputs' type, half a step each, for the second product
+    f32x8 e;
+    auto weigh = [&](int i) {
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        const int x = 2 * i + y;
+        e[x % 8] = __builtin_amdgcn_exp2f(fmaf(s[x / 16][x % 16], c, -sub));
+        part[y] += e[x % 8];
+        asm volatile("" : "+v"(part[y]));  // here, not when the tile is done with every weight kept until then
+      }
+      if (i % 4 == 3) p[i / 4] = __builtin_convertvector(e, x8);
+    };
+    constexpr int kFirst = NEXT ? ST * QK : 0, kSecond = PK * DT, kPairs = 8 * ST;
+    auto fragment = [&](int m) {  // of product m of both lists
+      return m < kFirst ? key(ka, m % QK, m / QK) : value(va, (m - kFirst) / DT, (m - kFirst) % DT);
+    };
+    Scores n;
+#pragma unroll
+    for (int t = 0; t < ST; ++t) n[t] = f32x16{};
+#pragma unroll
+    for (int m = 0; m < kReach; ++m) ring[m] = fragment(m);
+    if constexpr (!NEXT) {
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) weigh(i);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int m = 0; m < kFirst + kSecond; ++m) {
+      const x8 f = ring[m % kReach];
+      if (m < kFirst)
+        n[m / QK] = T::mfma(f, q[m % QK], n[m / QK]);
+      else
+        o[(m - kFirst) % DT] = T::mfma(f, p[(m - kFirst) / DT], o[(m - kFirst) % DT]);
+      if (m + kReach < kFirst + kSecond) ring[m % kReach] = fragment(m + kReach);
+      if (m < kFirst) {
+#pragma unroll
+        for (int i = m * kPairs / (ST * QK); i < (m + 1) * kPairs / (ST * QK); ++i) weigh(i);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    sum += part[0] + part[1];
+    if constexpr (NEXT) {
+#pragma unroll
+      for (int t = 0; t < ST; ++t) s[t] = n[t];
+      high = peak(s);
+    }
+  }
+
+  static __device__ __forceinline__ float peak(const Scores& s) {
+    float m = s[0][0];
+#pragma unroll
+    for (int t = 0; t < ST; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) m = __builtin_elementwise_maximum(m, s[t][r]);
+    return m;
+  }
+  static __device__ __forceinline__ uint32_t key_address(uint32_t k) {
+    const int lane = threadIdx.x & 63, row = lane & 31;
+    return k + row * kRow + (((lane >> 5) ^ key_swizzle<D>(row)) << 4);
+  }
+  // K fragment (16 columns j, 32 keys t)
+  static __device__ __forceinline__ x8 key(uint32_t ka, int j, int t) {
+    return *(const DFT_LDS x8*)(uintptr_t)((ka ^ (j << 5)) + t * 32 * kRow);
+  }
   __device__ __forceinline__ static uint32_t value_address(uint32_t v) {
     const int lane = threadIdx.x & 63, r4 = (lane & 15) >> 2;
     return v + (4 * (lane >> 5) + r4) * kRow +
@@ -331,6 +548,15 @@ struct Rows {
     }
   }
 
+  __device__ __forceinline__ f32x4 four(int t, int x) const {
+    return {o[t][4 * x], o[t][4 * x + 1], o[t][4 * x + 2], o[t][4 * x + 3]};
+  }
+  // The lane's outputs, scaled, to the row at element `at`
+  __device__ __forceinline__ void store(void* out, int64_t at, int dtype, bool vec, float by) const {
+    store_all<4 * DT>(out, at + 4 * ((threadIdx.x & 63) >> 5), dtype, vec, [&](int i) { return four(i / 4, i % 4) * by; },
+                      [](int i) { return 32 * (i / 4) + 8 * (i % 4); });
+  }
+
   // The whole row's sum, in both of its lanes.
   __device__ __forceinline__ float whole_sum() const { return sum + __shfl_xor(sum, 32); }
 };
@@ -371,27 +597,7 @@ __device__ __forceinline__ float lse_of(float top, float sum) {
   return sum == 0 ? -INFINITY : (top + __log2f(sum)) * kLn2;
 }
 
-// Four outputs in a row, x scaled by w.
-__device__ __forceinline__ void store4(void* o, int64_t at, int dtype, bool vec, f32x4 x) {
-  if (vec && dtype == DFT_BF16) {
-    typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
-    *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(o) + at) = __builtin_bit_cast(u32x2, __builtin_convertvector(x, bf16x4));
-  } else if (vec && dtype == DFT_F16) {
-    typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
-    *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(o) + at) = __builtin_bit_cast(u32x2, __builtin_convertvector(x, f16x4));
-  } else if (vec) {
-    *reinterpret_cast<f32x4*>(static_cast<float*>(o) + at) = x;
-  } else {
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (dtype == DFT_BF16)
-        static_cast<__bf16*>(o)[at + e] = (__bf16)x[e];
-      else
-        st_f(o, at + e, dtype, x[e]);
-  }
-}
-
-// Whether store4 may write whole pieces: 8 bytes, 16 of fp32.
+// Whether store_all may write whole pieces: 8 bytes, 16 of fp32.
 template <class Args>
 bool vector_out(const Args& a) {
   const uintptr_t piece = a.o_dtype == DFT_F32 ? 16 : 8;

@@ -52,27 +52,36 @@ struct Request {
   int status;
 };
 
+// How a request's lengths are read: by each lane for itself, or once for the
+// wave, from arrays that this launch does not write.
+struct ByLane {
+  static __device__ __forceinline__ int i32(const int32_t* p) { return *p; }
+  static __device__ __forceinline__ int64_t index(const void* p, int64_t i, int dt) { return ld_i(p, i, dt); }
+};
+struct ByWave {
+  typedef const __attribute__((address_space(4))) int32_t* Words;
+  static __device__ __forceinline__ int i32(const int32_t* p) { return *(Words)(uintptr_t)p; }
+  static __device__ __forceinline__ int64_t index(const void* p, int64_t i, int dt) {
+    const Words w = (Words)(uintptr_t)p;
+    const bool wide = dt == DFT_I64;
+    const int lo = w[wide ? 2 * i : i], hi = w[wide ? 2 * i + 1 : i];
+    return wide ? (int64_t)(((uint64_t)(uint32_t)hi << 32) | (uint32_t)lo) : (int64_t)lo;
+  }
+};
+
+template <class By>
 __device__ __forceinline__ Request request(const dft_paged_attention_args& a, int b) {
   Request q;
-  q.r0 = a.cu_seqlens ? a.cu_seqlens[b] : (int64_t)b * a.n_new;
-  int64_t n = a.cu_seqlens ? (int64_t)a.cu_seqlens[b + 1] - q.r0 : a.n_new;
+  q.r0 = a.cu_seqlens ? By::i32(a.cu_seqlens + b) : (int64_t)b * a.n_new;
+  int64_t n = a.cu_seqlens ? (int64_t)By::i32(a.cu_seqlens + b + 1) - q.r0 : a.n_new;
   q.status = n < 0 || n > a.n_new || q.r0 < 0 || q.r0 + n > a.rows ? DFT_STATUS_SPAN : 0;
   n = q.r0 < 0 ? 0 : min(min(n, (int64_t)a.n_new), a.rows - q.r0);
   q.n = (int)max(n, (int64_t)0);
   const int64_t top = 0x7fffffff - kTile, room = (int64_t)a.columns * a.page_size;
-  const int64_t seq = max(ld_i(a.seq_len, b, a.seq_len_dtype), (int64_t)0);
+  const int64_t seq = max(By::index(a.seq_len, b, a.seq_len_dtype), (int64_t)0);
   if (seq > room) q.status |= DFT_STATUS_TABLE;
   q.before = (int)(min(seq, top) - q.n);
   q.keys = a.num_pages ? (int)min(min(seq, room), top) : 0;
-  return q;
-}
-
-__device__ __forceinline__ Request uniform_request(const dft_paged_attention_args& a, int b) {
-  Request q = request(a, b);
-  q.r0 = uniform64(q.r0);
-  q.n = __builtin_amdgcn_readfirstlane(q.n);
-  q.keys = __builtin_amdgcn_readfirstlane(q.keys);
-  q.before = __builtin_amdgcn_readfirstlane(q.before);
   return q;
 }
 
@@ -129,7 +138,8 @@ template <int BM, int KT, int NT>
 struct Walk {
   int64_t left;  // tiles of the share not begun
   int g, share;  // kv head, number of the share on its line
-  int b, tile, off;
+  int b, tile, off, all;  // the item, the tiles of it that are done, all of them
+  Request q;
 
   __device__ __forceinline__ bool begin(const dft_paged_attention_args& a, const Plan& pl, int group) {
     __shared__ int64_t red[NT / 64];
@@ -142,10 +152,10 @@ struct Walk {
       g = pair - b * a.hkv;
       share = 0;
       off = 0;
-      const Request q = request(a, b);
+      q = request<ByWave>(a, b);
       if (a.status && tile == 0 && g == 0 && threadIdx.x == 0) a.status[b] = q.status;
       if (tile >= row_tiles_of<BM>(q, group)) return false;
-      left = tiles_of<BM, KT>(a, q, group, tile);
+      left = all = tiles_of<BM, KT>(a, q, group, tile);
       return true;
     }
     // consecutive shares of a line on one XCD
@@ -156,7 +166,7 @@ struct Walk {
     const int per = (a.batch + NT - 1) / NT;
     const int b0 = min((int)threadIdx.x * per, a.batch), b1 = min(b0 + per, a.batch);
     auto weight = [&](int r) -> int64_t {
-      const Request q = request(a, r);
+      const Request q = request<ByLane>(a, r);
       if (a.status && x == 0) a.status[r] = q.status;
       int64_t sum = 0;
       const int n = row_tiles_of<BM>(q, group);
@@ -172,7 +182,7 @@ struct Walk {
       int64_t rest = pos - ahead;
       int r = b0;
       for (int64_t w; rest >= (w = weight(r)); ++r) rest -= w;
-      const Request q = request(a, r);
+      const Request q = request<ByLane>(a, r);
       int t = 0;
       for (int n; rest >= (n = tiles_of<BM, KT>(a, q, group, t)); ++t) rest -= n;
       at[0] = r, at[1] = t, at[2] = (int)rest;
@@ -186,10 +196,13 @@ struct Walk {
     b = __builtin_amdgcn_readfirstlane(at[0]);
     tile = __builtin_amdgcn_readfirstlane(at[1]);
     off = __builtin_amdgcn_readfirstlane(at[2]);
+    left = uniform64(left);
+    q = request<ByWave>(a, b);
+    all = tiles_of<BM, KT>(a, q, group, tile);
     if (threadIdx.x == 0) {
       Head h;
       h.first = pos - off;
-      h.last = h.first + tiles_of<BM, KT>(a, request(a, b), group, tile);
+      h.last = h.first + all;
       h.share = size;
       h.b = b, h.tile = tile, h.inside = off > 0, h.pad = 0;
       *head = h;
@@ -197,16 +210,24 @@ struct Walk {
     return true;
   }
 
-  // behind `done` tiles of the item of request q; false past the share's end
-  __device__ __forceinline__ bool next(const dft_paged_attention_args& a, const Request& q, int group, int done) {
+  // behind `done` tiles of the item; false past the share's end
+  __device__ __forceinline__ bool next(const dft_paged_attention_args& a, int group, int done) {
     left -= done;
+    off += done;
     if (left <= 0) return false;
+    if (off < all) return true;
     off = 0;
-    if (++tile < row_tiles_of<BM>(q, group)) return true;
-    tile = 0;
-    do {
-      if (++b >= a.batch) return false;
-    } while (__builtin_amdgcn_readfirstlane(request(a, b).n) == 0);
+    if (++tile >= row_tiles_of<BM>(q, group)) {
+      tile = 0;
+      do {
+        if (++b >= a.batch) {
+          left = 0;
+          return false;
+        }
+        q = request<ByWave>(a, b);
+      } while (q.n == 0);
+    }
+    all = tiles_of<BM, KT>(a, q, group, tile);
     return true;
   }
 
@@ -226,13 +247,13 @@ __device__ __forceinline__ int few_value_swizzle(int row) {
 // s_waitcnt: until at most n vector-memory operations are outstanding
 constexpr unsigned wait_loads(int n) { return (unsigned)((n & 15) | ((n >> 4) << 14) | (7 << 4) | (15 << 8)); }
 
-// The copies of an item's tiles into STAGES places of the LDS, STAGES - 1
-// tiles ahead of their use, and of their keys' page ids, as many tiles ahead
-// of the copies.  Every wave fetches the same ids to the same place (it then
-// only waits for itself) and copies its share of the rows; a wave's loads are
-// the same number for every tile, so that a counted wait ends with a tile's.
-// FEW: the values' places are those of few_value_swizzle.
-template <int D, int KT, int NW, int STAGES, bool ONCE, bool FEW>
+// The copies of a share's tiles, item after item, into STAGES places of the
+// LDS, STAGES - 1 tiles ahead of their use, and of their keys' page ids, as
+// many tiles ahead of the copies.  Every wave fetches the same ids to the same
+// place (it then only waits for itself) and copies its share of the rows; a
+// wave's loads are the same number for every tile, so that a counted wait ends
+// with a tile's.  FEW: the values' places are those of few_value_swizzle.
+template <int D, int KT, int NW, int STAGES, bool ONCE, bool FEW, class Walk>
 struct Feed {
   static constexpr int kRow = 2 * D, kBytes = KT * kRow, kAhead = STAGES - 1, kSlots = STAGES > 2 ? 8 : 4;
   static constexpr int kRows = 1024 / kRow, kCopies = KT / (kRows * NW), kPieces = D / 8, kLoads = 2 * kCopies + 1;
@@ -241,94 +262,109 @@ struct Feed {
     char tiles[STAGES][2][kBytes];
     uint64_t from[NW][2 * kMine];  // addresses of a wave's keys of a tile, and of its values
     int ids[kSlots][64];           // page ids of a tile's keys; with 32 of them twice
+    int2 tile[kSlots];             // its first key and its item's number of keys
   };
 
   const dft_paged_attention_args& a;
   const Plan& pl;
   Room& room;
-  const int32_t* table;
-  uint64_t base;  // of what the lane looks up: keys or values
+  Walk lead;      // the walk as far as the ids
+  int group;
+  uint64_t id_at;  // the last ids fetched
+  int id_slot;
+  int64_t ids, count, used;  // tiles whose ids are fetched; of the share; behind us
+  uint64_t base;             // of what the lane looks up: keys or values
   int64_t page_stride, token_stride;
-  int keys, wave, lane;
+  int wave, lane;
 
-  __device__ __forceinline__ Feed(const dft_paged_attention_args& a, const Plan& pl, Room& room, int g, int wave)
-      : a(a), pl(pl), room(room), wave(wave), lane(threadIdx.x & 63) {
+  __device__ __forceinline__ Feed(const dft_paged_attention_args& a, const Plan& pl, Room& room, const Walk& walk, int group,
+                                  int wave)
+      : a(a), pl(pl), room(room), lead(walk), group(group), id_at(0), id_slot(0), ids(0), count(walk.left), used(0),
+        wave(wave), lane(threadIdx.x & 63) {
     const bool value = lane & kMine;
-    base = value ? (uint64_t)(uintptr_t)a.value_cache + 2 * (g * a.vc_h_stride)
-                 : (uint64_t)(uintptr_t)a.key_cache + 2 * (g * a.kc_h_stride);
+    base = value ? (uint64_t)(uintptr_t)a.value_cache + 2 * (walk.g * a.vc_h_stride)
+                 : (uint64_t)(uintptr_t)a.key_cache + 2 * (walk.g * a.kc_h_stride);
     page_stride = value ? a.vc_page_stride : a.kc_page_stride;
     token_stride = value ? a.vc_token_stride : a.kc_token_stride;
   }
-  __device__ __forceinline__ uint32_t tile(int t) const {
-    return lds_address(&room) + (STAGES == 3 ? t % 3 : t & (STAGES - 1)) * 2 * kBytes;
+  __device__ __forceinline__ uint32_t tile() const {
+    return lds_address(&room) + ((int)used & (STAGES - 1)) * 2 * kBytes;
   }
   __device__ __forceinline__ uint32_t column(uint32_t j) const { return (uint32_t)((uint64_t)j * pl.magic >> pl.shift); }
 
-  __device__ __forceinline__ void fetch_ids(int t) {
-    const uint32_t j = (uint32_t)min(t * KT + lane % KT, keys - 1);
-    dma4_at((uint64_t)(uintptr_t)(table + column(j)), lds_address(room.ids[t & (kSlots - 1)]));
+  // the next tile's ids; past the share's end the last ones again, for the count
+  __device__ __forceinline__ void fetch_ids() {
+    if (ids < count) {
+      id_slot = (int)ids & (kSlots - 1);
+      const int j0 = lead.off * KT;
+      const uint32_t j = (uint32_t)max(min(j0 + lane % KT, lead.q.keys - 1), 0);
+      id_at = (uint64_t)(uintptr_t)(a.block_table + lead.b * a.table_row_stride + column(j));
+      room.tile[id_slot] = int2{j0, lead.q.keys};
+      ++ids;
+      lead.next(a, group, 1);
+    }
+    dma4_at(id_at, lds_address(room.ids[id_slot]));
   }
   // -1 for a key that there is, 0 for none.  Arithmetic, as what follows in
   // copy(): a branch of some lanes only among so many live registers let the
   // compiler put register copies in front of the rejoin, where they left out
   // the other lanes (a memory fault at 256 columns in fp16).
-  __device__ __forceinline__ int there(int j, int id) const {
+  __device__ __forceinline__ int there(int j, int keys, int id) const {
     return -(int)((j < keys) & ((uint32_t)id < (uint32_t)a.num_pages));
   }
-  __device__ __forceinline__ void copy(int t) {
+  __device__ __forceinline__ void copy(int64_t n) {
     // a lane looks up one of the wave's rows, for the keys or for the values
-    const int mine = lane % kMine, row = (mine / kRows * NW + wave) * kRows + mine % kRows, j = t * KT + row;
-    const int id = room.ids[t & (kSlots - 1)][row];
-    const uint32_t jj = (uint32_t)min(j, keys - 1);
-    const int ok = there(j, id);
-    const uint64_t page = (uint32_t)(id & ok), token = (jj - column(jj) * a.page_size) & ok;
+    const int slot = (int)n & (kSlots - 1), mine = lane % kMine;
+    const int row = (mine / kRows * NW + wave) * kRows + mine % kRows;
+    const int2 tile = room.tile[slot];
+    const int j = tile.x + row, id = room.ids[slot][row], ok = there(j, tile.y, id);
+    const uint64_t page = (uint32_t)(id & ok), token = (j - column(j) * a.page_size) & ok;
     room.from[wave][lane & (2 * kMine - 1)] = base + 2 * (page * page_stride + token * token_stride);
     asm volatile("" ::: "memory");
     __builtin_amdgcn_wave_barrier();
+    uint64_t k[kCopies], v[kCopies];
 #pragma unroll
     for (int x = 0; x < kCopies; ++x) {
-      const int first = (x * NW + wave) * kRows, row = first + lane / kPieces, piece = lane % kPieces;
-      const uint32_t at = tile(t) + first * kRow;
+      const int to = (x * NW + wave) * kRows + lane / kPieces, piece = lane % kPieces;
       const uint64_t* from = room.from[wave] + x * kRows + lane / kPieces;
-      dma16_at<ONCE>(from[0] + ((piece ^ key_swizzle<D>(row)) << 4), at);
-      dma16_at<ONCE>(from[kMine] + ((piece ^ (FEW ? few_value_swizzle<D>(row) : value_swizzle<D>(row))) << 4),
-                     at + kBytes);
+      k[x] = from[0] + ((piece ^ key_swizzle<D>(to)) << 4);
+      v[x] = from[kMine] + ((piece ^ (FEW ? few_value_swizzle<D>(to) : value_swizzle<D>(to))) << 4);
     }
+    const uint32_t at = lds_address(&room) + ((int)n & (STAGES - 1)) * 2 * kBytes + 1024 * wave;
+    dma16_at<kCopies, 1024 * NW, ONCE>(k, at);
+    dma16_at<kCopies, 1024 * NW, ONCE>(v, at + kBytes);
   }
-  // which of the tile's keys there are
-  __device__ __forceinline__ uint64_t present(int t) const {
-    return __ballot(there(t * KT + lane % KT, room.ids[t & (kSlots - 1)][lane]));
+  // which of the current tile's keys, from j0 on, there are
+  __device__ __forceinline__ uint64_t present(int j0, int keys) const {
+    return __ballot(there(j0 + lane % KT, keys, room.ids[(int)used & (kSlots - 1)][lane]));
   }
 
-  // the first tiles of an item: `between` runs while their ids are on the way
-  template <class F>
-  __device__ __forceinline__ void begin(const int32_t* row, int n, int first, int stop, F between) {
-    table = row;
-    keys = n;
-    for (int t = first; t < first + 2 * kAhead; ++t) fetch_ids(t);
-    between();
+  // the share's first tiles
+  __device__ __forceinline__ void begin() {
+#pragma unroll 1
+    for (int t = 0; t < 2 * kAhead; ++t) fetch_ids();
     __builtin_amdgcn_s_waitcnt(kWaitDma);
     asm volatile("" ::: "memory");
-    for (int t = first; t < min(first + kAhead, stop); ++t) {
-      fetch_ids(t + kAhead);  // again, for the count
+#pragma unroll 1
+    for (int t = 0; t < min((int64_t)kAhead, count); ++t) {
+      dma4_at(id_at, lds_address(room.ids[id_slot]));
       copy(t);
     }
   }
-  // until this wave's copies of tile t have landed, with those of the tiles behind it out
-  __device__ __forceinline__ void wait(int t, int stop) const {
-    const int behind = min(stop - 1 - t, kAhead - 1);
-    static_assert(kAhead <= 3);
-    if (behind == 2)
+  // the current tile, for all waves, with those behind it on their way
+  __device__ __forceinline__ void ready() {
+    const int64_t behind = count - 1 - used;
+    static_assert(kAhead == 1 || kAhead == 3);
+    if (kAhead == 3 && behind >= 2)
       __builtin_amdgcn_s_waitcnt(wait_loads(2 * kLoads));
-    else if (behind == 1)
+    else if (kAhead == 3 && behind == 1)
       __builtin_amdgcn_s_waitcnt(wait_loads(kLoads));
     else
       __builtin_amdgcn_s_waitcnt(kWaitDma);
-  }
-  __device__ __forceinline__ void advance(int t, int stop) {
-    if (t + kAhead >= stop) return;
-    fetch_ids(t + 2 * kAhead);
-    copy(t + kAhead);
+    __syncthreads();
+    if (used + kAhead >= count) return;
+    fetch_ids();
+    copy(used + kAhead);
   }
 };
 
@@ -454,31 +490,31 @@ __device__ __forceinline__ void note_few(uint32_t v, int wave, const uint32_t (&
 template <int D, int NQ, class T>
 __global__ void __launch_bounds__(256) few_kernel(dft_paged_attention_args a, Scale sc, Plan pl) {
   constexpr int BM = 16 * NQ, KT = kFewTile, NW = 4, QK = D / 32, DT = D / 16 / NW;
-  typedef Feed<D, KT, NW, kFewStages, true, true> Tiles;
+  typedef Walk<BM, KT, 64 * NW> Share;
+  typedef Feed<D, KT, NW, kFewStages, true, true, Share> Tiles;
   typedef typename T::x8 x8;
   __shared__ __attribute__((aligned(1024))) typename Tiles::Room room;
   __shared__ uint32_t notes[NW][NQ * 2][64];
-  __shared__ int spoiled;
+  __shared__ int64_t spoiled;  // the last tile found to hold a value that is not finite
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), quad = lane >> 4;
   const int group = a.hq / a.hkv;
   const bool causal = a.flags & DFT_ATTN_CAUSAL;
-  Walk<BM, KT, 256> walk;
+  Share walk;
   if (!walk.begin(a, pl, group)) return;
-
-  const int g = walk.g;
-  Tiles feed(a, pl, room, g, wave);
+  Tiles feed(a, pl, room, walk, group, wave);
+  if (threadIdx.x == 0) spoiled = -1;
+  feed.begin();
 
   bool more = true;
   while (more) {
-    const Request q = uniform_request(a, walk.b);
-    const int all = tiles_of<BM, KT>(a, q, group, walk.tile);
-    const int begin = walk.off, stop = (int)min((int64_t)all, begin + walk.left);
+    const Request q = walk.q;
+    const int begin = walk.off, stop = (int)min((int64_t)walk.all, begin + walk.left);
     Place to[NQ];
     uint64_t bits[NQ];
     int limit[NQ], fewest = q.keys;
 #pragma unroll
     for (int y = 0; y < NQ; ++y) {
-      to[y] = place_of(q, group, g, walk.tile * BM + 16 * y + (lane & 15));
+      to[y] = place_of(q, group, walk.g, walk.tile * BM + 16 * y + (lane & 15));
       limit[y] = q.keys;
       bits[y] = a.anc_bits ? a.anc_bits[to[y].row] : 0;
       if (causal) limit[y] = min(q.before + (int)(to[y].row - q.r0) + 1, q.keys);
@@ -487,6 +523,7 @@ __global__ void __launch_bounds__(256) few_kernel(dft_paged_attention_args a, Sc
       fewest = q.before;
     else if (causal)
       fewest = __builtin_amdgcn_readlane(limit[0], 0);
+
     x8 qf[NQ][QK];
     f32x4 o[NQ][DT];
     float top[NQ], sum[NQ];
@@ -498,50 +535,42 @@ __global__ void __launch_bounds__(256) few_kernel(dft_paged_attention_args a, Sc
 #pragma unroll
       for (int d = 0; d < DT; ++d) o[y][d] = f32x4{};
     }
-    if (q.keys > 0 && begin * KT < q.keys) {
-      if (threadIdx.x == 0) spoiled = -1;
-      feed.begin(a.block_table + walk.b * a.table_row_stride, q.keys, begin, stop, [&] {
 #pragma unroll
-      for (int y = 0; y < NQ; ++y) {
-        const uint16_t* row = static_cast<const uint16_t*>(a.q) + to[y].row * a.q_row_stride + to[y].h * a.q_h_stride;
+    for (int y = 0; y < NQ; ++y) {
+      const uint16_t* row = static_cast<const uint16_t*>(a.q) + to[y].row * a.q_row_stride + to[y].h * a.q_h_stride;
 #pragma unroll
-        for (int k = 0; k < QK; ++k) {
-          u32x4 w = *reinterpret_cast<const u32x4*>(row + 32 * k + 8 * quad);
-          w = (w & sc.keep) ^ sc.flip;
-          qf[y][k] = __builtin_bit_cast(x8, w);
-        }
+      for (int k = 0; k < QK; ++k) {
+        u32x4 w = *reinterpret_cast<const u32x4*>(row + 32 * k + 8 * quad);
+        w = (w & sc.keep) ^ sc.flip;
+        qf[y][k] = __builtin_bit_cast(x8, w);
       }
-      });
-      for (int t = begin; t < stop; ++t) {
-        feed.wait(t, stop);
+    }
+    for (int t = begin; t < stop; ++t, ++feed.used) {
+      feed.ready();
+      const uint32_t kt = feed.tile(), vt = kt + Tiles::kBytes;
+      const int j0 = t * KT;
+      const uint32_t there = (uint32_t)feed.present(j0, q.keys);
+      const bool partial = there != ~0u || j0 + KT > fewest;
+      uint32_t vis[NQ];
+      if (partial) {
+#pragma unroll
+        for (int y = 0; y < NQ; ++y)
+          vis[y] = there & (uint32_t)(a.anc_bits ? tree_bits(bits[y], q.before, j0) : first_bits(limit[y] - j0));
+        const uint32_t slice = vt + wave * (Tiles::kBytes / NW);
+        if (!finite<T, Tiles::kBytes / NW>(slice)) spoiled = feed.used;
         __syncthreads();
-        feed.advance(t, stop);
-        const uint32_t kt = feed.tile(t), vt = kt + Tiles::kBytes;
-        const uint32_t there = (uint32_t)feed.present(t);
-        const int j0 = t * KT;
-        const bool partial = there != ~0u || j0 + KT > fewest;
-        uint32_t vis[NQ];
-        if (partial) {
-#pragma unroll
-          for (int y = 0; y < NQ; ++y)
-            vis[y] = there & (uint32_t)(a.anc_bits ? tree_bits(bits[y], q.before, j0) : first_bits(limit[y] - j0));
-          const uint32_t slice = vt + wave * (Tiles::kBytes / NW);
-          if (!finite<T, Tiles::kBytes / NW>(slice)) spoiled = t;
+        if (spoiled == feed.used) {
+          note_few<D, NQ, DT, T>(vt, wave, vis, lds_address(notes[wave]), noted);
+          noted = true;
           __syncthreads();
-          if (spoiled == t) {
-            note_few<D, NQ, DT, T>(vt, wave, vis, lds_address(notes[wave]), noted);
-            noted = true;
-            __syncthreads();
-            clear_infinite<T, Tiles::kBytes / NW>(slice);
-            __syncthreads();
-          }
+          clear_infinite<T, Tiles::kBytes / NW>(slice);
+          __syncthreads();
         }
-        few_tile<D, NQ, DT, T>(kt, vt, wave, qf, o, top, sum, sc.c, partial, vis);
       }
-      __syncthreads();
+      few_tile<D, NQ, DT, T>(kt, vt, wave, qf, o, top, sum, sc.c, partial, vis);
     }
 
-    const bool whole = begin == 0 && stop == all;
+    const bool whole = begin == 0 && stop == walk.all;
     float* part = walk.template part<D>(pl, begin == 0);
 #pragma unroll
     for (int y = 0; y < NQ; ++y) {
@@ -560,14 +589,13 @@ __global__ void __launch_bounds__(256) few_kernel(dft_paged_attention_args a, Sc
         }
       }
       if (!to[y].there) continue;
+      if (whole)
+        store_all<DT>(a.o, to[y].row * a.o_row_stride + to[y].h * a.o_h_stride + 16 * wave * DT + 4 * quad, a.o_dtype, pl.vec,
+                      [&](int d) { return o[y][d] * by; }, [](int d) { return 16 * d; });
+      else
 #pragma unroll
-      for (int d = 0; d < DT; ++d) {
-        if (whole)
-          store4(a.o, to[y].row * a.o_row_stride + to[y].h * a.o_h_stride + 16 * (wave * DT + d) + 4 * quad, a.o_dtype,
-                 pl.vec, o[y][d] * by);
-        else
+        for (int d = 0; d < DT; ++d)
           *reinterpret_cast<f32x4*>(part + ((y * (D / 16) + wave * DT + d) * 64 + lane) * 4) = o[y][d];
-      }
       if (wave || quad) continue;
       if (!whole) {
         part[BM * D + 16 * y + lane] = top[y];
@@ -576,44 +604,41 @@ __global__ void __launch_bounds__(256) few_kernel(dft_paged_attention_args a, Sc
         a.lse[to[y].row * a.lse_row_stride + to[y].h] = lse_of(top[y], sum[y]);
       }
     }
-    more = walk.next(a, q, group, stop - begin);
+    more = walk.next(a, group, stop - begin);
   }
 }
 
 // ---- more rows -------------------------------------------------------------
-// WM waves of 32 rows each, times WK that take a part of every tile's keys
-// and are joined through the LDS at an item's end.
-template <int D, int WM, int WK, int KT, int STAGES, bool ONCE, class T>
-__global__ void __launch_bounds__(64 * WM * WK, D == 256 ? 1 : 2)
-    many_kernel(dft_paged_attention_args a, Scale sc, Plan pl) {
-  constexpr int NW = WM * WK, BM = 32 * WM, KW = KT / WK, kRow = 2 * D;
-  typedef Feed<D, KT, NW, STAGES, ONCE, false> Tiles;
-  typedef Rows<D, KW, T> Wave;
+// NW waves of 32 rows each.
+template <int D, int NW, int KT, int STAGES, bool ONCE, class T>
+__global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) many_kernel(dft_paged_attention_args a, Scale sc, Plan pl) {
+  constexpr int BM = 32 * NW;
+  typedef Walk<BM, KT, 64 * NW> Share;
+  typedef Feed<D, KT, NW, STAGES, ONCE, false, Share> Tiles;
+  typedef Rows<D, KT, T> Wave;
   constexpr int kBytes = Tiles::kBytes;
-  constexpr uint64_t kEvery = KW == 64 ? ~0ull : (1ull << KW) - 1, kAll = KT == 64 ? ~0ull : (1ull << KT) - 1;
+  constexpr uint64_t kEvery = KT == 64 ? ~0ull : (1ull << KT) - 1;
   __shared__ __attribute__((aligned(1024))) typename Tiles::Room room;
   __shared__ char notes[NW][Wave::kNotes];
-  __shared__ int spoiled;  // the last tile found to hold a value that is not finite
+  __shared__ int64_t spoiled;  // the last tile found to hold a value that is not finite
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
-  const int wm = wave % WM, wk = wave / WM;
   const int group = a.hq / a.hkv;
   const bool causal = a.flags & DFT_ATTN_CAUSAL;
-  Walk<BM, KT, 64 * NW> walk;
+  Share walk;
   if (!walk.begin(a, pl, group)) return;
-
-  const int g = walk.g;
-  Tiles feed(a, pl, room, g, wave);
+  Tiles feed(a, pl, room, walk, group, wave);
+  if (threadIdx.x == 0) spoiled = -1;
+  feed.begin();
   Wave w;
   w.notes = lds_address(notes[wave]);
 
   bool more = true;
   while (more) {
-    const Request q = uniform_request(a, walk.b);
-    const int all = tiles_of<BM, KT>(a, q, group, walk.tile);
-    const int begin = walk.off, stop = (int)min((int64_t)all, begin + walk.left);
-    const int rows = q.n * group, pw = walk.tile * BM + 32 * wm;
+    const Request q = walk.q;
+    const int begin = walk.off, stop = (int)min((int64_t)walk.all, begin + walk.left);
+    const int rows = q.n * group, pw = walk.tile * BM + 32 * wave;
     const bool works = pw < rows;
-    const Place to = place_of(q, group, g, pw + (lane & 31));
+    const Place to = place_of(q, group, walk.g, pw + (lane & 31));
     const int fewest = a.anc_bits ? q.before  // keys that every row of the workgroup sees
                        : causal   ? min(q.before + (int)((uint32_t)(walk.tile * BM) / (uint32_t)group) + 1, q.keys)
                                   : q.keys;
@@ -628,96 +653,58 @@ __global__ void __launch_bounds__(64 * WM * WK, D == 256 ? 1 : 2)
     }
 
     w.clear();
-    if (q.keys > 0 && begin * KT < q.keys) {
-      if (threadIdx.x == 0) spoiled = -1;
-      feed.begin(a.block_table + walk.b * a.table_row_stride, q.keys, begin, stop, [&] {
-        w.load_q(static_cast<const uint16_t*>(a.q) + to.row * a.q_row_stride + to.h * a.q_h_stride, sc);
-      });
-      for (int t = begin; t < stop; ++t) {
-        feed.wait(t, stop);
+    w.load_q(static_cast<const uint16_t*>(a.q) + to.row * a.q_row_stride + to.h * a.q_h_stride, sc);
+    for (int t = begin; t < stop; ++t, ++feed.used) {
+      feed.ready();
+      const int j0 = t * KT;
+      const uint32_t kt = feed.tile(), vt = kt + kBytes, slice = vt + wave * (kBytes / NW);
+      const uint64_t there = feed.present(j0, q.keys) & kEvery;
+      const bool acts = works && j0 < most, partial = there != kEvery || j0 + KT > least;
+      uint64_t vis = kEvery;
+      if (partial) vis = there & (a.anc_bits ? tree_bits(bits, q.before, j0) : first_bits(limit - j0));
+      if (there != kEvery || j0 + KT > fewest) {
+        if (!finite<T, kBytes / NW>(slice)) spoiled = feed.used;
         __syncthreads();
-        feed.advance(t, stop);
-        const uint32_t kt = feed.tile(t), vt = kt + kBytes, slice = vt + wave * (kBytes / NW);
-        const uint64_t there = feed.present(t) & kAll, mine = there >> (wk * KW) & kEvery;
-        const int j0 = t * KT + wk * KW;
-        const bool acts = works && j0 < most, partial = mine != kEvery || j0 + KW > least;
-        uint64_t vis = kEvery;
-        if (partial) vis = mine & (a.anc_bits ? tree_bits(bits, q.before, j0) : first_bits(limit - j0));
-        if (there != kAll || (t + 1) * KT > fewest) {
-          if (!finite<T, kBytes / NW>(slice)) spoiled = t;
+        if (spoiled == feed.used) {
+          if (acts) w.note(vt, vis);
           __syncthreads();
-          if (spoiled == t) {
-            if (acts) w.note(vt + wk * KW * kRow, vis);
-            __syncthreads();
-            clear_infinite<T, kBytes / NW>(slice);
-            __syncthreads();
-          }
+          clear_infinite<T, kBytes / NW>(slice);
+          __syncthreads();
         }
-        if (acts) w.tile(kt + wk * KW * kRow, vt + wk * KW * kRow, sc.c, partial, vis);
       }
-      __syncthreads();
+      if (!acts) continue;
+      typename Wave::Scores s;
+      w.scores(kt, s);
+      if (partial) w.mask(s, vis);
+      w.template step<false>(0, vt, sc.c, s);
     }
     w.finish();
 
-    if constexpr (WK == 2) {
-      static_assert(sizeof(room.tiles) >= WM * (32 * D + 128) * sizeof(float));
-      float* his = reinterpret_cast<float*>(room.tiles) + wm * (32 * D + 128);
-      if (wk == 1) {
-#pragma unroll
-        for (int t = 0; t < Wave::DT; ++t)
-#pragma unroll
-          for (int x = 0; x < 4; ++x)
-            *reinterpret_cast<f32x4*>(his + ((t * 4 + x) * 64 + lane) * 4) =
-                f32x4{w.o[t][4 * x], w.o[t][4 * x + 1], w.o[t][4 * x + 2], w.o[t][4 * x + 3]};
-        his[32 * D + lane] = w.top;
-        his[32 * D + 64 + lane] = w.sum;
-      }
-      __syncthreads();
-      if (wk == 0) {
-        const float top = his[32 * D + lane], high = fmaxf(w.top, top);
-        const float by = w.top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(w.top - high);
-        const float with = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - high);
-        w.top = high;
-        w.sum = w.sum * by + his[32 * D + 64 + lane] * with;
-#pragma unroll
-        for (int t = 0; t < Wave::DT; ++t)
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const f32x4 y = *reinterpret_cast<f32x4*>(his + ((t * 4 + x) * 64 + lane) * 4);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) w.o[t][4 * x + e] = w.o[t][4 * x + e] * by + y[e] * with;
-          }
-      }
-      __syncthreads();
-    }
-
-    if (works && wk == 0) {
-      const bool whole = begin == 0 && stop == all;
+    if (works) {
+      const bool whole = begin == 0 && stop == walk.all;
       const float sum = w.whole_sum(), by = weight_of(sum);
       if (to.there) {
         float* part = walk.template part<D>(pl, begin == 0);
-        const int64_t out = to.row * a.o_row_stride + to.h * a.o_h_stride + 4 * half;
+        if (whole) {
+          w.store(a.o, to.row * a.o_row_stride + to.h * a.o_h_stride, a.o_dtype, pl.vec, by);
+        } else {
 #pragma unroll
-        for (int t = 0; t < Wave::DT; ++t)
+          for (int t = 0; t < Wave::DT; ++t)
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            f32x4 y = {w.o[t][4 * x], w.o[t][4 * x + 1], w.o[t][4 * x + 2], w.o[t][4 * x + 3]};
-            if (whole)
-              store4(a.o, out + 32 * t + 8 * x, a.o_dtype, pl.vec, y * by);
-            else
-              *reinterpret_cast<f32x4*>(part + (((wm * Wave::DT + t) * 4 + x) * 64 + lane) * 4) = y;
-          }
+            for (int x = 0; x < 4; ++x)
+              *reinterpret_cast<f32x4*>(part + (((wave * Wave::DT + t) * 4 + x) * 64 + lane) * 4) = w.four(t, x);
+        }
         if (half == 0) {
           if (!whole) {
-            part[BM * D + 32 * wm + lane] = w.top;
-            part[BM * D + BM + 32 * wm + lane] = sum;
+            part[BM * D + 32 * wave + lane] = w.top;
+            part[BM * D + BM + 32 * wave + lane] = sum;
           } else if (a.lse) {
             a.lse[to.row * a.lse_row_stride + to.h] = lse_of(w.top, sum);
           }
         }
       }
     }
-    more = walk.next(a, q, group, stop - begin);
+    more = walk.next(a, group, stop - begin);
   }
 }
 
@@ -742,7 +729,7 @@ __global__ void __launch_bounds__(64 * kJoinWaves) join_kernel(dft_paged_attenti
   const int parts = (int)(past - begin) + 1, split = parts > 8 ? kJoinWaves : 1;
   const int units = kJoinWaves / split, turn = wave % split;  // units at a time; which of the parts
   const float* first = pl.parts + ((int64_t)g * pl.shares + begin) * 2 * part_floats<D, BM>();
-  const Request q = request(a, h.b);
+  const Request q = request<ByWave>(a, h.b);
   for (int u0 = (share - 1 - (int)begin) * units; u0 < kUnits; u0 += (parts - 1) * units) {
     const int unit = min(u0 + wave / split, kUnits - 1), block = unit / kOf, in = unit % kOf;
     const int row = block * kLane + lane % kLane;
@@ -781,7 +768,8 @@ __global__ void __launch_bounds__(64 * kJoinWaves) join_kernel(dft_paged_attenti
       __syncthreads();
     }
     if (turn || !to.there || u0 + wave / split >= kUnits) continue;
-    store4(a.o, to.row * a.o_row_stride + to.h * a.o_h_stride + d, a.o_dtype, pl.vec, o * weight_of(sum));
+    store_all<1>(a.o, to.row * a.o_row_stride + to.h * a.o_h_stride + d, a.o_dtype, pl.vec,
+                 [&](int) { return o * weight_of(sum); }, [](int) { return 0; });
     if (a.lse && d == 0) a.lse[to.row * a.lse_row_stride + to.h] = lse_of(top, sum);
   }
 }
@@ -803,7 +791,7 @@ Shape shape_of(const dft_paged_attention_args& a) {
     return s;
   }
   // as many workgroups as the LDS holds: 512 D bytes of tiles each, and a little
-  const int room = kCus * (a.head_dim == 256 ? 1 : a.head_dim == 128 ? s.rows == 128 && s.once ? 1 : 2 : 3);
+  const int room = kCus * (a.head_dim == 256 ? 1 : a.head_dim == 128 ? 2 : 3);
   s.shares = a.hkv < room ? room / a.hkv : 1;
   s.grid = (s.shares * a.hkv + kXcds - 1) / kXcds * kXcds;
   s.heads_bytes = s.grid * sizeof(Head);
@@ -819,12 +807,10 @@ int launch(const dft_paged_attention_args& a, const Shape& s, const Plan& pl, hi
     few_kernel<D, 1, T><<<grid, 256, 0, stream>>>(a, sc, pl);
   else if (s.rows == 32)
     few_kernel<D, 2, T><<<grid, 256, 0, stream>>>(a, sc, pl);
-  else if (!s.once)
-    many_kernel<D, 4, 1, 64, 2, false, T><<<grid, 256, 0, stream>>>(a, sc, pl);
-  else if constexpr (D == 128)
-    many_kernel<D, 4, 2, 64, 4, true, T><<<grid, 512, 0, stream>>>(a, sc, pl);
+  else if (s.once)
+    many_kernel<D, 4, 32, 4, true, T><<<grid, 256, 0, stream>>>(a, sc, pl);
   else
-    many_kernel<D, 4, 1, 32, 4, true, T><<<grid, 256, 0, stream>>>(a, sc, pl);
+    many_kernel<D, 4, 64, 2, false, T><<<grid, 256, 0, stream>>>(a, sc, pl);
   if (hipGetLastError() != hipSuccess) return DFT_ERR_LAUNCH;
   if (s.uncut) return DFT_OK;
   if (s.rows == 16)
@@ -852,7 +838,15 @@ int64_t paged_attention_workspace(const dft_paged_attention_args* a) {
   return s.heads_bytes + s.parts_bytes;
 }
 
-int launch_paged_attention(const dft_paged_attention_args* a, hipStream_t stream) {
+int launch_paged_attention(const dft_paged_attention_args* args, hipStream_t stream) {
+  dft_paged_attention_args copy = *args, *a = &copy;
+  // requests without keys pass through the tiles as well, all masked: where
+  // there is no table or no page they read something that is there
+  if (!a->columns) a->block_table = static_cast<const int32_t*>(a->q), a->table_row_stride = 0;
+  if (!a->num_pages) {
+    a->key_cache = a->value_cache = a->q;
+    a->kc_page_stride = a->kc_token_stride = a->kc_h_stride = a->vc_page_stride = a->vc_token_stride = a->vc_h_stride = 0;
+  }
   const Shape s = shape_of(*a);
   if (s.grid > 0xffffffffll / 512) return DFT_ERR_UNSUPPORTED;  // a grid counts work-items in 32 bits
   Plan pl = {};

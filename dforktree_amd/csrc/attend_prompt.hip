@@ -2,8 +2,9 @@
 //
 // A workgroup takes 32 NW packed rows (row p: token p / group, head p % group
 // of one kv head) of one prompt and walks over the keys they see in tiles of
-// 64, which its waves share.  While a tile is worked on the next one is
-// copied to the other half of the LDS.
+// 64, which its waves share.  A tile's scores are formed beside the tile
+// before's weights, so its keys come a tile earlier than its values; the LDS
+// holds two tiles of either, one in use, one on its way.
 #include "attend.h"
 
 namespace dft {
@@ -16,7 +17,7 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) prompt_kernel(dft_p
   constexpr int kRow = 2 * D, kBytes = kTile * kRow;  // of a tile's keys, and of its values
   constexpr int kRows = 1024 / kRow, kCopies = kTile / (kRows * NW), kPieces = D / 8;
   typedef Rows<D, kTile, T> Wave;
-  __shared__ __attribute__((aligned(1024))) char lds[2][2][kBytes];
+  __shared__ __attribute__((aligned(1024))) char keys_at[2][kBytes], values_at[2][kBytes];
   __shared__ char notes[NW][Wave::kNotes];
   __shared__ int spoiled;  // the last tile found to hold a value that is not finite
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
@@ -42,74 +43,82 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) prompt_kernel(dft_p
   const int p = min(pw + (lane & 31), rows - 1);
   const int i = (int)((uint32_t)p / (uint32_t)group), h = g * group + (p - i * group);
   const int limit = causal ? i + 1 : n;  // keys this lane's row sees
-  const int least = __builtin_amdgcn_readlane(limit, 0), most = __builtin_amdgcn_readlane(limit, 31);
+  const int least = __builtin_amdgcn_readlane(limit, 0);
   const bool works = pw < rows;
   const int fewest = causal ? (int)((uint32_t)p0 / (uint32_t)group) + 1 : n;  // keys that the workgroup's first row sees
 
-  // Copy i of a wave: rows (i NW + wave) kRows ..., the first of them through
-  // the scalar base, the lane's through its offset.
-  const int lrow = lane / kPieces, piece = lane % kPieces;
+  // Copy x of a wave: the kRows rows of the tile from (x NW + wave) kRows on,
+  // the first of them through the scalar base, the lane's through its offset.
+  const int piece = lane % kPieces;
   const uint64_t kbase = (uint64_t)(uintptr_t)a.k + 2 * (r0 * a.k_row_stride + g * a.k_h_stride);
   const uint64_t vbase = (uint64_t)(uintptr_t)a.v + 2 * (r0 * a.v_row_stride + g * a.v_h_stride);
-  const uint32_t lds0 = lds_address(lds);
-  auto copy = [&](int t, int stage) {
-    const int j0 = t * kTile;
+  auto ktile = [&](int t) { return lds_address(keys_at) + (t & 1) * kBytes; };
+  auto vtile = [&](int t) { return lds_address(values_at) + (t & 1) * kBytes; };
+  uint32_t koff[kCopies], voff[kCopies];
+  auto offsets = [&](int last) {  // rows past `last` become it
 #pragma unroll
     for (int x = 0; x < kCopies; ++x) {
-      const int first = (x * NW + wave) * kRows, row = first + lrow;
-      int there = lrow, from = j0 + first;
-      if (j0 + kTile > n) {  // the last tile: rows past the prompt become its last row
-        from = min(from, n - 1);
-        there = min(lrow, n - 1 - from);
-      }
-      const uint32_t at = lds0 + stage * 2 * kBytes + first * kRow;
-      dma16(uniform(kbase + 2 * ((uint64_t)from * a.k_row_stride)),
-            (uint32_t)(there * (int)a.k_row_stride * 2 + ((piece ^ key_swizzle<D>(row)) << 4)), at);
-      dma16(uniform(vbase + 2 * ((uint64_t)from * a.v_row_stride)),
-            (uint32_t)(there * (int)a.v_row_stride * 2 + ((piece ^ value_swizzle<D>(row)) << 4)), at + kBytes);
+      const int row = (x * NW + wave) * kRows + lane / kPieces, there = min(row, last);
+      koff[x] = (uint32_t)(there * (int)a.k_row_stride * 2 + ((piece ^ key_swizzle<D>(row)) << 4));
+      voff[x] = (uint32_t)(there * (int)a.v_row_stride * 2 + ((piece ^ value_swizzle<D>(row)) << 4));
     }
+  };
+  // keys of tile t, or values; the last tile's rows end with the prompt
+  auto copy_keys = [&](int t) {
+    if ((t + 1) * kTile > n) offsets(n - 1 - t * kTile);
+    dma16<kCopies, 1024 * NW>(kbase + (uint64_t)t * (2 * kTile * a.k_row_stride), koff, ktile(t) + 1024 * wave);
+  };
+  auto copy_values = [&](int t) {
+    dma16<kCopies, 1024 * NW>(vbase + (uint64_t)t * (2 * kTile * a.v_row_stride), voff, vtile(t) + 1024 * wave);
   };
 
   Wave w;
   w.clear();
   w.notes = lds_address(notes[wave]);
   if (threadIdx.x == 0) spoiled = -1;
-  copy(0, 0);
+  offsets(kTile - 1);
+  copy_keys(0);
+  copy_values(0);
+  if (tiles > 1) copy_keys(1);
   w.load_q(static_cast<const uint16_t*>(a.q) + (r0 + i) * a.q_row_stride + h * a.q_h_stride, sc);
-  for (int t = 0; t < tiles; ++t) {
+  __builtin_amdgcn_s_waitcnt(kWaitDma);
+  __syncthreads();
+  // of tile t: the keys that the lane's row sees, whether some row of the wave misses some
+  auto seen = [&](int t) { return first_bits(limit - t * kTile); };
+  auto partial = [&](int t) { return (t + 1) * kTile > least; };
+  // what of its values is not finite must not reach a row that does not see it
+  auto look = [&](int t) {
+    if ((t + 1) * kTile <= fewest) return;
+    const uint32_t v = vtile(t), mine = v + wave * (kBytes / NW);
+    if (!finite<T, kBytes / NW>(mine)) spoiled = t;
+    __syncthreads();
+    if (spoiled == t) {
+      w.note(v, seen(t));
+      __syncthreads();
+      clear_infinite<T, kBytes / NW>(mine);
+      __syncthreads();
+    }
+  };
+  typename Wave::Scores s;
+  w.scores(ktile(0), s);
+  if (partial(0)) w.mask(s, seen(0));
+  __syncthreads();  // tile 2's keys take the place of tile 0's
+  for (int t = 0; t + 1 < tiles; ++t) {
+    copy_values(t + 1);
+    if (t + 2 < tiles) copy_keys(t + 2);
+    look(t);
+    w.template step<true>(ktile(t + 1), vtile(t), sc.c, s);
+    if (partial(t + 1)) w.mask(s, seen(t + 1));
     __builtin_amdgcn_s_waitcnt(kWaitDma);
     __syncthreads();
-    if (t + 1 < tiles) copy(t + 1, (t + 1) & 1);
-    const int j0 = t * kTile;
-    const uint32_t at = lds0 + (t & 1) * 2 * kBytes, mine = at + kBytes + wave * (kBytes / NW);
-    const bool acts = works && j0 < most, partial = j0 + kTile > least;
-    const uint64_t vis = partial ? first_bits(limit - j0) : ~0ull;
-    if (j0 + kTile > fewest) {
-      if (!finite<T, kBytes / NW>(mine)) spoiled = t;
-      __syncthreads();
-      if (spoiled == t) {
-        if (acts) w.note(at + kBytes, vis);
-        __syncthreads();
-        clear_infinite<T, kBytes / NW>(mine);
-        __syncthreads();
-      }
-    }
-    if (acts) w.tile(at, at + kBytes, sc.c, partial, vis);
   }
+  look(tiles - 1);
+  w.template step<false>(0, vtile(tiles - 1), sc.c, s);
   if (!works) return;
   w.finish();
   const float sum = w.whole_sum(), by = weight_of(sum);
   if (pw + (lane & 31) >= rows) return;
-  const int64_t to = (r0 + i) * a.o_row_stride + h * a.o_h_stride + 4 * half;
-#pragma unroll
-  for (int t = 0; t < D / 32; ++t)
-#pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      f32x4 y;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] = w.o[t][4 * x + e] * by;
-      store4(a.o, to + 32 * t + 8 * x, a.o_dtype, vec, y);
-    }
+  w.store(a.o, (r0 + i) * a.o_row_stride + h * a.o_h_stride, a.o_dtype, vec, by);
   if (a.lse && half == 0) a.lse[(r0 + i) * a.lse_row_stride + h] = lse_of(w.top, sum);
 }
 
