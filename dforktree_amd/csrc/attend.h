@@ -445,6 +445,7 @@ struct Rows {
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int m = 0; m < kFirst + kSecond; ++m) {
+      if (NEXT && m == kFirst) __builtin_amdgcn_s_setprio(0);
       const x8 f = ring[m % kReach];
       if (m < kFirst)
         n[m / QK] = T::mfma(f, q[m % QK], n[m / QK]);
@@ -457,6 +458,7 @@ struct Rows {
       }
       __builtin_amdgcn_sched_barrier(0);
     }
+    if (NEXT) __builtin_amdgcn_s_setprio(1);
     sum += part[0] + part[1];
     if constexpr (NEXT) {
 #pragma unroll

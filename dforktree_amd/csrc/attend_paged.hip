@@ -255,11 +255,14 @@ constexpr unsigned wait_loads(int n) { return (unsigned)((n & 15) | ((n >> 4) <<
 // with a tile's.  FEW: the values' places are those of few_value_swizzle.
 template <int D, int KT, int NW, int STAGES, bool ONCE, bool FEW, class Walk>
 struct Feed {
+  // many_kernel forms a tile's scores beside the second product of the tile
+  // before it: its keys are fed a tile ahead of its values
+  static constexpr int kSkew = FEW ? 0 : 1;
   static constexpr int kRow = 2 * D, kBytes = KT * kRow, kAhead = STAGES - 1, kSlots = STAGES > 2 ? 8 : 4;
   static constexpr int kRows = 1024 / kRow, kCopies = KT / (kRows * NW), kPieces = D / 8, kLoads = 2 * kCopies + 1;
   static constexpr int kMine = kCopies * kRows;  // rows of a tile that a wave copies
   struct Room {
-    char tiles[STAGES][2][kBytes];
+    char keys[STAGES][kBytes], values[STAGES][kBytes];
     uint64_t from[NW][2 * kMine];  // addresses of a wave's keys of a tile, and of its values
     int ids[kSlots][64];           // page ids of a tile's keys; with 32 of them twice
     int2 tile[kSlots];             // its first key and its item's number of keys
@@ -287,8 +290,12 @@ struct Feed {
     page_stride = value ? a.vc_page_stride : a.kc_page_stride;
     token_stride = value ? a.vc_token_stride : a.kc_token_stride;
   }
-  __device__ __forceinline__ uint32_t tile() const {
-    return lds_address(&room) + ((int)used & (STAGES - 1)) * 2 * kBytes;
+  // where the keys and the values of tile n are
+  __device__ __forceinline__ uint32_t keys_at(int64_t n) const {
+    return lds_address(room.keys) + ((int)n & (STAGES - 1)) * kBytes;
+  }
+  __device__ __forceinline__ uint32_t values_at(int64_t n) const {
+    return lds_address(room.values) + ((int)n & (STAGES - 1)) * kBytes;
   }
   __device__ __forceinline__ uint32_t column(uint32_t j) const { return (uint32_t)((uint64_t)j * pl.magic >> pl.shift); }
 
@@ -312,9 +319,13 @@ struct Feed {
   __device__ __forceinline__ int there(int j, int keys, int id) const {
     return -(int)((j < keys) & ((uint32_t)id < (uint32_t)a.num_pages));
   }
+  // the values of tile n and the keys of tile n + kSkew (past the share's end
+  // the last tile's again); KEYS alone for the share's first
+  template <bool VALUES = true>
   __device__ __forceinline__ void copy(int64_t n) {
     // a lane looks up one of the wave's rows, for the keys or for the values
-    const int slot = (int)n & (kSlots - 1), mine = lane % kMine;
+    const int64_t of_keys = min(n + kSkew, count - 1);
+    const int slot = (int)(lane & kMine ? n : of_keys) & (kSlots - 1), mine = lane % kMine;
     const int row = (mine / kRows * NW + wave) * kRows + mine % kRows;
     const int2 tile = room.tile[slot];
     const int j = tile.x + row, id = room.ids[slot][row], ok = there(j, tile.y, id);
@@ -330,37 +341,46 @@ struct Feed {
       k[x] = from[0] + ((piece ^ key_swizzle<D>(to)) << 4);
       v[x] = from[kMine] + ((piece ^ (FEW ? few_value_swizzle<D>(to) : value_swizzle<D>(to))) << 4);
     }
-    const uint32_t at = lds_address(&room) + ((int)n & (STAGES - 1)) * 2 * kBytes + 1024 * wave;
-    dma16_at<kCopies, 1024 * NW, ONCE>(k, at);
-    dma16_at<kCopies, 1024 * NW, ONCE>(v, at + kBytes);
+    dma16_at<kCopies, 1024 * NW, ONCE>(k, keys_at(n + kSkew) + 1024 * wave);
+    if constexpr (VALUES) dma16_at<kCopies, 1024 * NW, ONCE>(v, values_at(n) + 1024 * wave);
   }
-  // which of the current tile's keys, from j0 on, there are
-  __device__ __forceinline__ uint64_t present(int j0, int keys) const {
-    return __ballot(there(j0 + lane % KT, keys, room.ids[(int)used & (kSlots - 1)][lane]));
+  // which of tile n's keys, from j0 on, there are
+  __device__ __forceinline__ uint64_t present(int64_t n, int j0, int keys) const {
+    return __ballot(there(j0 + lane % KT, keys, room.ids[(int)n & (kSlots - 1)][lane]));
   }
 
   // the share's first tiles
   __device__ __forceinline__ void begin() {
 #pragma unroll 1
-    for (int t = 0; t < 2 * kAhead; ++t) fetch_ids();
+    for (int t = 0; t < 2 * kAhead + kSkew; ++t) fetch_ids();
     __builtin_amdgcn_s_waitcnt(kWaitDma);
     asm volatile("" ::: "memory");
+    if constexpr (kSkew) copy<false>(-1);
 #pragma unroll 1
     for (int t = 0; t < min((int64_t)kAhead, count); ++t) {
       dma4_at(id_at, lds_address(room.ids[id_slot]));
       copy(t);
     }
+    if constexpr (kSkew) {  // the first tile's keys, for all waves
+      wait(min((int64_t)kAhead, count));
+      __syncthreads();
+    }
   }
-  // the current tile, for all waves, with those behind it on their way
-  __device__ __forceinline__ void ready() {
-    const int64_t behind = count - 1 - used;
-    static_assert(kAhead == 1 || kAhead == 3);
-    if (kAhead == 3 && behind >= 2)
+  // until this wave's copies are done, but for those of `behind` tiles
+  __device__ __forceinline__ void wait(int64_t behind) const {
+    if (kAhead == 3 && behind >= 3)
+      __builtin_amdgcn_s_waitcnt(wait_loads(3 * kLoads));
+    else if (kAhead == 3 && behind == 2)
       __builtin_amdgcn_s_waitcnt(wait_loads(2 * kLoads));
-    else if (kAhead == 3 && behind == 1)
+    else if (behind == 1)
       __builtin_amdgcn_s_waitcnt(wait_loads(kLoads));
     else
       __builtin_amdgcn_s_waitcnt(kWaitDma);
+  }
+  // the current tile, for all waves, with those behind it on their way
+  __device__ __forceinline__ void ready() {
+    static_assert(kAhead == 1 || kAhead == 3);
+    wait(min(count - 1 - used, (int64_t)kAhead - 1));
     __syncthreads();
     if (used + kAhead >= count) return;
     fetch_ids();
@@ -547,9 +567,9 @@ __global__ void __launch_bounds__(256) few_kernel(dft_paged_attention_args a, Sc
     }
     for (int t = begin; t < stop; ++t, ++feed.used) {
       feed.ready();
-      const uint32_t kt = feed.tile(), vt = kt + Tiles::kBytes;
+      const uint32_t kt = feed.keys_at(feed.used), vt = feed.values_at(feed.used);
       const int j0 = t * KT;
-      const uint32_t there = (uint32_t)feed.present(j0, q.keys);
+      const uint32_t there = (uint32_t)feed.present(feed.used, j0, q.keys);
       const bool partial = there != ~0u || j0 + KT > fewest;
       uint32_t vis[NQ];
       if (partial) {
@@ -643,41 +663,52 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) many_kernel(dft_pag
                        : causal   ? min(q.before + (int)((uint32_t)(walk.tile * BM) / (uint32_t)group) + 1, q.keys)
                                   : q.keys;
     uint64_t bits = 0;
-    int limit = q.keys, least = q.keys, most = q.keys;  // keys the lane's row sees, all rows do, any does
+    int limit = q.keys, least = q.keys;  // keys the lane's row sees, all rows of the wave do
     if (a.anc_bits) {
       bits = a.anc_bits[to.row];
       least = q.before;
     } else if (causal) {
       limit = min(q.before + (int)(to.row - q.r0) + 1, q.keys);
-      least = __builtin_amdgcn_readlane(limit, 0), most = __builtin_amdgcn_readlane(limit, 31);
+      least = __builtin_amdgcn_readlane(limit, 0);
     }
 
     w.clear();
     w.load_q(static_cast<const uint16_t*>(a.q) + to.row * a.q_row_stride + to.h * a.q_h_stride, sc);
-    for (int t = begin; t < stop; ++t, ++feed.used) {
-      feed.ready();
-      const int j0 = t * KT;
-      const uint32_t kt = feed.tile(), vt = kt + kBytes, slice = vt + wave * (kBytes / NW);
-      const uint64_t there = feed.present(j0, q.keys) & kEvery;
-      const bool acts = works && j0 < most, partial = there != kEvery || j0 + KT > least;
-      uint64_t vis = kEvery;
-      if (partial) vis = there & (a.anc_bits ? tree_bits(bits, q.before, j0) : first_bits(limit - j0));
-      if (there != kEvery || j0 + KT > fewest) {
-        if (!finite<T, kBytes / NW>(slice)) spoiled = feed.used;
+    // the keys there are of the tile at hand, from j0 on, and of the next one
+    int j0 = begin * KT;
+    uint64_t there = feed.present(feed.used, j0, q.keys) & kEvery;
+    auto seen = [&](uint64_t here, int from) {
+      return here & (a.anc_bits ? tree_bits(bits, q.before, from) : first_bits(limit - from));
+    };
+    typename Wave::Scores s;
+    w.scores(feed.keys_at(feed.used), s);
+    if (there != kEvery || j0 + KT > least) w.mask(s, seen(there, j0));
+    // what of a tile's values is not finite must not reach a row that does not see it
+    auto look = [&](uint32_t vt) {
+      if (there == kEvery && j0 + KT <= fewest) return;
+      const uint32_t slice = vt + wave * (kBytes / NW);
+      if (!finite<T, kBytes / NW>(slice)) spoiled = feed.used;
+      __syncthreads();
+      if (spoiled == feed.used) {
+        w.note(vt, seen(there, j0));
         __syncthreads();
-        if (spoiled == feed.used) {
-          if (acts) w.note(vt, vis);
-          __syncthreads();
-          clear_infinite<T, kBytes / NW>(slice);
-          __syncthreads();
-        }
+        clear_infinite<T, kBytes / NW>(slice);
+        __syncthreads();
       }
-      if (!acts) continue;
-      typename Wave::Scores s;
-      w.scores(kt, s);
-      if (partial) w.mask(s, vis);
-      w.template step<false>(0, vt, sc.c, s);
+    };
+    for (int t = begin; t + 1 < stop; ++t) {
+      feed.ready();
+      look(feed.values_at(feed.used));
+      w.template step<true>(feed.keys_at(feed.used + 1), feed.values_at(feed.used), sc.c, s);
+      ++feed.used;
+      j0 += KT;
+      there = feed.present(feed.used, j0, q.keys) & kEvery;
+      if (there != kEvery || j0 + KT > least) w.mask(s, seen(there, j0));
     }
+    feed.ready();
+    look(feed.values_at(feed.used));
+    w.template step<false>(0, feed.values_at(feed.used), sc.c, s);
+    ++feed.used;
     w.finish();
 
     if (works) {
