@@ -839,7 +839,7 @@ int launch(const dft_paged_attention_args& a, const Shape& s, const Plan& pl, hi
   else if (s.rows == 32)
     few_kernel<D, 2, T><<<grid, 256, 0, stream>>>(a, sc, pl);
   else if (s.once)
-    many_kernel<D, 4, 32, 4, true, T><<<grid, 256, 0, stream>>>(a, sc, pl);
+    many_kernel<D, 4, 64, 2, true, T><<<grid, 256, 0, stream>>>(a, sc, pl);
   else
     many_kernel<D, 4, 64, 2, false, T><<<grid, 256, 0, stream>>>(a, sc, pl);
   if (hipGetLastError() != hipSuccess) return DFT_ERR_LAUNCH;

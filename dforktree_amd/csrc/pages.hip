@@ -186,13 +186,20 @@ __global__ void __launch_bounds__(kThreads) page_plan_kernel(dft_page_plan_args 
 }
 
 // ---- KV append -------------------------------------------------------------
-// One entry's place; false when it is skipped.
-__device__ __forceinline__ bool append_place(const dft_kv_append_args& a, int64_t i, int64_t& row, int64_t& page,
-                                             int64_t& token) {
+struct Append {
+  uint32_t magic;     // slot / page_size = slot * magic >> shift for slot < 2^31
+  int shift;
+  int pieces, log;    // of an entry; log2 of the threads on an entry
+  int per_head;       // pieces of a head
+};
+
+// An entry's place; false when it is skipped.
+__device__ __forceinline__ bool append_place(const dft_kv_append_args& a, const Append& p, int64_t i, int64_t& row,
+                                             int64_t& page, int64_t& token) {
   const int64_t slot = ld_i(a.slots, i, a.slots_dtype);
   row = a.rows ? ld_i(a.rows, i, a.rows_dtype) : i;
   if (slot < 0 || row < 0) return false;
-  page = slot / a.page_size;
+  page = slot <= 0x7fffffffll ? (int64_t)((uint64_t)(uint32_t)slot * p.magic >> p.shift) : slot / a.page_size;
   token = slot - page * a.page_size;
   if (page >= a.num_pages || row >= a.src_rows) {
     if (a.status) *a.status = 1;
@@ -201,17 +208,85 @@ __device__ __forceinline__ bool append_place(const dft_kv_append_args& a, int64_
   return true;
 }
 
-__global__ void __launch_bounds__(kThreads) kv_append_kernel(dft_kv_append_args a) {
+// Eight elements, cast; of one type they keep their bits.
+template <int SRC, int DST>
+__device__ __forceinline__ void append_piece(const void* src, int64_t from, void* dst, int64_t to) {
+  if constexpr (SRC == DST && SRC != DFT_F32) {
+    *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(dst) + to) =
+        *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(src) + from);
+  } else if constexpr (SRC == DST) {
+    const u32x4* s = reinterpret_cast<const u32x4*>(static_cast<const float*>(src) + from);
+    u32x4* d = reinterpret_cast<u32x4*>(static_cast<float*>(dst) + to);
+    const u32x4 lo = s[0], hi = s[1];
+    d[0] = lo;
+    d[1] = hi;
+  } else {
+    typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+    typedef float f32x8 __attribute__((ext_vector_type(8)));
+    f32x8 x;
+    if constexpr (SRC == DFT_BF16)
+      x = __builtin_convertvector(*reinterpret_cast<const bf16x8*>(static_cast<const uint16_t*>(src) + from), f32x8);
+    else if constexpr (SRC == DFT_F16)
+      x = __builtin_convertvector(*reinterpret_cast<const f16x8*>(static_cast<const uint16_t*>(src) + from), f32x8);
+    else
+      x = *reinterpret_cast<const f32x8*>(static_cast<const float*>(src) + from);
+    if constexpr (DST == DFT_BF16)
+      *reinterpret_cast<bf16x8*>(static_cast<uint16_t*>(dst) + to) = __builtin_convertvector(x, bf16x8);
+    else if constexpr (DST == DFT_F16)
+      *reinterpret_cast<f16x8*>(static_cast<uint16_t*>(dst) + to) = __builtin_convertvector(x, f16x8);
+    else
+      *reinterpret_cast<f32x8*>(static_cast<float*>(dst) + to) = x;
+  }
+}
+
+// 2^log threads take an entry, each a piece of eight elements (or several) of
+// its key and its value; a thread's head and column are the same for every
+// entry.
+template <int SRC, int DST>
+__global__ void __launch_bounds__(kThreads) kv_append_kernel(dft_kv_append_args a, Append p) {
+  const int lane = threadIdx.x & ((1 << p.log) - 1), per = kThreads >> p.log;
+  for (int piece = lane; piece < p.pieces; piece += 1 << p.log) {
+    const int h = piece / p.per_head, x = 8 * (piece - h * p.per_head);
+    const int64_t ks = h * a.k_h_stride + x, vs = h * a.v_h_stride + x, kd = h * a.kc_h_stride + x, vd = h * a.vc_h_stride + x;
+#pragma unroll 4
+    for (int64_t i = (int64_t)blockIdx.x * per + (threadIdx.x >> p.log); i < a.n; i += (int64_t)gridDim.x * per) {
+      int64_t row, page, token;
+      if (!append_place(a, p, i, row, page, token)) continue;
+      append_piece<SRC, DST>(a.k, row * a.k_row_stride + ks, a.key_cache,
+                             page * a.kc_page_stride + token * a.kc_token_stride + kd);
+      append_piece<SRC, DST>(a.v, row * a.v_row_stride + vs, a.value_cache,
+                             page * a.vc_page_stride + token * a.vc_token_stride + vd);
+    }
+  }
+}
+
+// Rows without 16-byte pieces: element by element.
+__global__ void __launch_bounds__(kThreads) kv_append_elements_kernel(dft_kv_append_args a, Append p) {
   const int64_t width = (int64_t)a.heads * a.head_dim, total = a.n * width;
   for (int64_t e = (int64_t)blockIdx.x * kThreads + threadIdx.x; e < total; e += (int64_t)gridDim.x * kThreads) {
     const int64_t i = e / width;
     const int c = (int)(e - i * width), h = c / a.head_dim, x = c - h * a.head_dim;
     int64_t row, page, token;
-    if (!append_place(a, i, row, page, token)) continue;
-    const float k = ld_f(a.k, row * a.k_row_stride + h * a.k_h_stride + x, a.src_dtype);
-    const float v = ld_f(a.v, row * a.v_row_stride + h * a.v_h_stride + x, a.src_dtype);
-    st_f(a.key_cache, page * a.kc_page_stride + token * a.kc_token_stride + h * a.kc_h_stride + x, a.cache_dtype, k);
-    st_f(a.value_cache, page * a.vc_page_stride + token * a.vc_token_stride + h * a.vc_h_stride + x, a.cache_dtype, v);
+    if (!append_place(a, p, i, row, page, token)) continue;
+    const int64_t ks = row * a.k_row_stride + h * a.k_h_stride + x, vs = row * a.v_row_stride + h * a.v_h_stride + x;
+    const int64_t kd = page * a.kc_page_stride + token * a.kc_token_stride + h * a.kc_h_stride + x;
+    const int64_t vd = page * a.vc_page_stride + token * a.vc_token_stride + h * a.vc_h_stride + x;
+    if (a.src_dtype == a.cache_dtype && a.src_dtype != DFT_F32) {  // of one type: the bits
+      static_cast<uint16_t*>(a.key_cache)[kd] = static_cast<const uint16_t*>(a.k)[ks];
+      static_cast<uint16_t*>(a.value_cache)[vd] = static_cast<const uint16_t*>(a.v)[vs];
+    } else {
+      st_f(a.key_cache, kd, a.cache_dtype, ld_f(a.k, ks, a.src_dtype));
+      st_f(a.value_cache, vd, a.cache_dtype, ld_f(a.v, vs, a.src_dtype));
+    }
+  }
+}
+
+template <int SRC>
+void launch_append(const dft_kv_append_args& a, const Append& p, int grid, hipStream_t stream) {
+  switch (a.cache_dtype) {
+    case DFT_BF16: kv_append_kernel<SRC, DFT_BF16><<<grid, kThreads, 0, stream>>>(a, p); break;
+    case DFT_F16: kv_append_kernel<SRC, DFT_F16><<<grid, kThreads, 0, stream>>>(a, p); break;
+    default: kv_append_kernel<SRC, DFT_F32><<<grid, kThreads, 0, stream>>>(a, p); break;
   }
 }
 
@@ -230,8 +305,37 @@ int launch_page_plan(const dft_page_plan_args* a, hipStream_t stream) {
 }
 
 int launch_kv_append(const dft_kv_append_args* a, hipStream_t stream) {
-  const int64_t total = a->n * a->heads * a->head_dim, blocks = (total + kThreads - 1) / kThreads;
-  kv_append_kernel<<<(int)(blocks > 65536 ? 65536 : blocks), kThreads, 0, stream>>>(*a);
+  Append p = {};
+  int log = 0;
+  while ((1ll << log) < a->page_size) ++log;
+  p.shift = 31 + log;
+  p.magic = (uint32_t)(((1ull << p.shift) + a->page_size - 1) / a->page_size);
+  // pieces of eight elements: 16-byte aligned addresses and strides (32 for fp32, which only a vector of its own needs)
+  auto aligned = [](const void* q, int dt, int64_t s0, int64_t s1, int64_t s2) {
+    return reinterpret_cast<uintptr_t>(q) % (dt == DFT_F32 ? 32 : 16) == 0 && s0 % 8 == 0 && s1 % 8 == 0 && s2 % 8 == 0;
+  };
+  const bool pieces = a->head_dim % 8 == 0 && aligned(a->k, a->src_dtype, a->k_row_stride, a->k_h_stride, 0) &&
+                      aligned(a->v, a->src_dtype, a->v_row_stride, a->v_h_stride, 0) &&
+                      aligned(a->key_cache, a->cache_dtype, a->kc_page_stride, a->kc_token_stride, a->kc_h_stride) &&
+                      aligned(a->value_cache, a->cache_dtype, a->vc_page_stride, a->vc_token_stride, a->vc_h_stride) &&
+                      (int64_t)a->heads * a->head_dim < 0x7fffffff;
+  if (!pieces) {
+    const int64_t total = a->n * a->heads * a->head_dim, blocks = (total + kThreads - 1) / kThreads;
+    kv_append_elements_kernel<<<(int)(blocks > 65536 ? 65536 : blocks), kThreads, 0, stream>>>(*a, p);
+    return hipGetLastError() == hipSuccess ? DFT_OK : DFT_ERR_LAUNCH;
+  }
+  p.per_head = a->head_dim / 8;
+  p.pieces = a->heads * p.per_head;
+  while ((1 << p.log) < p.pieces && (1 << p.log) < kThreads) ++p.log;
+  // up to four entries a thread where that still leaves sixteen workgroups a CU
+  const int64_t entries = kThreads >> p.log, all = (a->n + entries - 1) / entries;
+  const int64_t blocks = all <= 4096 ? all : all / 4 > 4096 ? all / 4 : 4096;
+  const int grid = (int)(blocks > (1 << 20) ? (1 << 20) : blocks);
+  switch (a->src_dtype) {
+    case DFT_BF16: launch_append<DFT_BF16>(*a, p, grid, stream); break;
+    case DFT_F16: launch_append<DFT_F16>(*a, p, grid, stream); break;
+    default: launch_append<DFT_F32>(*a, p, grid, stream); break;
+  }
   return hipGetLastError() == hipSuccess ? DFT_OK : DFT_ERR_LAUNCH;
 }
 
