@@ -883,10 +883,7 @@ int launch_paged_attention(const dft_paged_attention_args* args, hipStream_t str
   Plan pl = {};
   pl.heads = static_cast<char*>(a->workspace);
   pl.parts = reinterpret_cast<float*>(pl.heads + s.heads_bytes);
-  int log = 0;
-  while ((1ll << log) < a->page_size) ++log;
-  pl.shift = 31 + log;
-  pl.magic = (uint32_t)(((1ull << pl.shift) + a->page_size - 1) / a->page_size);
+  page_magic(a->page_size, pl.magic, pl.shift);
   pl.shares = (int)s.shares;
   pl.vec = vector_out(*a);
   pl.uncut = s.uncut;

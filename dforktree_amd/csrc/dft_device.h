@@ -54,6 +54,16 @@ __device__ __forceinline__ void st_i(void* p, int64_t i, int dt, int64_t v) {
   else ((int32_t*)p)[i] = (int32_t)v;
 }
 
+// What x / page_size = x * magic >> shift takes, exact for x < 2^31: with
+// 2^(log - 1) < page_size <= 2^log, magic is at most 1 / 2^31 relative above
+// 2^(31 + log) / page_size and fits 32 bits.
+inline void page_magic(int page_size, uint32_t& magic, int& shift) {
+  int log = 0;
+  while ((1ll << log) < page_size) ++log;
+  shift = 31 + log;
+  magic = (uint32_t)(((1ull << shift) + page_size - 1) / page_size);
+}
+
 // bits 0..i set (the ancestor-or-self mask of a topologically ordered node i)
 // a value the workgroup agrees on, as a scalar
 __device__ __forceinline__ int64_t uniform64(int64_t v) {

@@ -15,15 +15,24 @@ namespace {
 constexpr int kThreads = 256;
 
 // ---- page plan -------------------------------------------------------------
-// Every workgroup scans the batch's lengths itself (three running sums over
-// at most 8192 requests: rows, pages taken, pages returned), so one launch
-// suffices; what is per row and per page is then dealt out over the grid.
+// Every workgroup scans the batch's lengths itself (running sums over at most
+// 8192 requests: rows, then pages taken and returned), so one launch suffices;
+// what is per row and per page is then dealt out over the grid, a row a
+// thread: a row's look-ups (its request, its page) follow each other, so the
+// time is their latency and the rows that a thread takes.  Divisions are by
+// multiplication while they fit 31 bits.
+struct PagePlan {
+  uint32_t magic, ring_magic;  // x / page_size = x * magic >> shift for x < 2^31; the same by capacity
+  int shift, ring_shift;
+};
+
 struct Sums {
   int64_t v[2];
 };
 
 // Exclusive scan over the block of two sums per thread.
-__device__ __forceinline__ Sums block_scan(Sums x, int64_t (*red)[kThreads / 64]) {
+template <int THREADS>
+__device__ __forceinline__ Sums block_scan(Sums x, int64_t (*red)[THREADS / 64]) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   Sums s = x;
 #pragma unroll
@@ -61,9 +70,11 @@ __device__ __forceinline__ int find(const int32_t* end, int batch, int64_t i) {
   return lo;
 }
 
-__global__ void __launch_bounds__(kThreads) page_plan_kernel(dft_page_plan_args a) {
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) page_plan_kernel(dft_page_plan_args a, PagePlan p) {
   extern __shared__ int32_t shared[];
-  __shared__ int64_t red[2][kThreads / 64];
+  __shared__ int64_t red[2][THREADS / 64];
+  __shared__ int32_t within[2];  // the sums served: of pages taken, of pages returned
   const int B = a.batch, ps = a.page_size;
   int32_t* end = shared;            // rows up to and with each request
   int32_t* take = shared + B;       // pages taken up to and with it
@@ -71,13 +82,17 @@ __global__ void __launch_bounds__(kThreads) page_plan_kernel(dft_page_plan_args 
   int32_t* state = shared + 3 * B;  // its status word
   const int64_t head = a.free_pos[0], tail = a.free_pos[1];
   const int64_t free_now = min(max(tail - head, (int64_t)0), a.capacity);
-  const int per = (B + kThreads - 1) / kThreads;
+  const int per = (B + THREADS - 1) / THREADS;
   const int b0 = min((int)threadIdx.x * per, B), b1 = min(b0 + per, B);
+  auto over = [&](int64_t x) -> int64_t {  // x / page_size
+    return x <= 0x7fffffffll ? (int64_t)((uint64_t)(uint32_t)x * p.magic >> p.shift) : x / ps;
+  };
 
   // rows
+  if (threadIdx.x < 2) within[threadIdx.x] = 0;
   Sums s = {{0, 0}};
   for (int b = b0; b < b1; ++b) s.v[0] += max(ld_i(a.new_len, b, a.new_len_dtype), (int64_t)0);
-  s = block_scan(s, red);
+  s = block_scan<THREADS>(s, red);
   for (int b = b0; b < b1; ++b) {
     s.v[0] += max(ld_i(a.new_len, b, a.new_len_dtype), (int64_t)0);
     end[b] = (int32_t)min(s.v[0], a.rows);
@@ -89,7 +104,7 @@ __global__ void __launch_bounds__(kThreads) page_plan_kernel(dft_page_plan_args 
     n = end[b] - (b ? end[b - 1] : 0);
     prefix = max(pre, (int64_t)0);
     status = n != len || pre < 0 ? DFT_STATUS_SPAN : 0;
-    const int64_t want = (prefix + n + ps - 1) / ps;
+    const int64_t want = over(prefix + n + ps - 1);
     if (want > a.columns) status |= DFT_STATUS_TABLE;
     return want - min(max(a.held[b], 0), a.columns);
   };
@@ -103,14 +118,14 @@ __global__ void __launch_bounds__(kThreads) page_plan_kernel(dft_page_plan_args 
       if (a.trim) s.v[1] += max(-d, (int64_t)0);
     }
   }
-  s = block_scan(s, red);
+  s = block_scan<THREADS>(s, red);
+  const int64_t room = a.capacity - free_now;
   for (int b = b0; b < b1; ++b) {
     const int64_t d = pages(b, status, prefix, n);
     if (!(status & DFT_STATUS_TABLE)) {
       s.v[0] += max(d, (int64_t)0);
       if (a.trim) s.v[1] += max(-d, (int64_t)0);
-      if ((d > 0 && s.v[0] > free_now) || (a.trim && d < 0 && s.v[1] > a.capacity - free_now))
-        status |= DFT_STATUS_PAGES;
+      if ((d > 0 && s.v[0] > free_now) || (a.trim && d < 0 && s.v[1] > room)) status |= DFT_STATUS_PAGES;
     }
     take[b] = clip32(s.v[0]);
     give[b] = clip32(s.v[1]);
@@ -120,25 +135,19 @@ __global__ void __launch_bounds__(kThreads) page_plan_kernel(dft_page_plan_args 
       const int held = min(max(a.held[b], 0), a.columns);
       a.status[b] = status;
       a.cu_seqlens[b + 1] = end[b];
-      a.seq_len[b] = served ? (int32_t)(prefix + n) : 0;
+      a.seq_len[b] = served ? clip32(prefix + n) : 0;
       a.held_out[b] = served && (d > 0 || a.trim) ? (int32_t)(held + d) : held;
     }
   }
   __syncthreads();
   // What is served of a running sum with an upper bound are its first
-  // entries, those without a refused one in front: `served` of it.
-  auto served_of = [&](const int32_t* sum, int64_t limit) -> int64_t {
-    int lo = 0, hi = B;  // requests whose sum is within the limit
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if ((int64_t)sum[mid] > limit)
-        hi = mid;
-      else
-        lo = mid + 1;
-    }
-    return lo ? sum[lo - 1] : 0;
-  };
-  const int64_t taken = B ? served_of(take, free_now) : 0, given = B ? served_of(give, a.capacity - free_now) : 0;
+  // entries, those without a refused one in front: the last within it.
+  for (int b = b0; b < b1; ++b) {
+    if (take[b] <= free_now && (b + 1 == B || take[b + 1] > free_now)) within[0] = take[b];
+    if (give[b] <= room && (b + 1 == B || give[b + 1] > room)) within[1] = give[b];
+  }
+  __syncthreads();
+  const int64_t taken = within[0], given = within[1];
   const int64_t rows = B ? end[B - 1] : 0;
   if (blockIdx.x == 0 && threadIdx.x == 0) {
     a.cu_seqlens[0] = 0;
@@ -146,23 +155,28 @@ __global__ void __launch_bounds__(kThreads) page_plan_kernel(dft_page_plan_args 
     a.free_pos_out[1] = tail + given;
   }
 
-  const int64_t step = (int64_t)gridDim.x * kThreads, first = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  auto ring = [&](int64_t i) -> int64_t {  // i >= 0 in a valid ring; any i stays inside
+  // cells of the ring, `ahead` (at most its capacity) behind its first or its last
+  auto wrap = [&](int64_t i) { return i >= a.capacity ? i - a.capacity : i; };
+  auto cell = [&](int64_t i) -> int64_t {
+    if (i >= 0 && i <= 0x7fffffffll) return i - (int64_t)((uint64_t)i * p.ring_magic >> p.ring_shift) * a.capacity;
     const int64_t r = i % a.capacity;
     return r < 0 ? r + a.capacity : r;
   };
-  for (int64_t p = first; p < taken; p += step) {
-    const int b = find(take, B, p);
+  const int64_t front = cell(head), back = cell(tail);
+  const int64_t step = (int64_t)gridDim.x * THREADS, first = (int64_t)blockIdx.x * THREADS + threadIdx.x;
+  // pages from the grid's other end: the last threads have the fewest rows
+  const int64_t turned = step - 1 - first;
+  for (int64_t x = turned; x < taken; x += step) {
+    const int b = find(take, B, x);
     const int held = min(max(a.held[b], 0), a.columns);
-    const int64_t col = held + p - (b ? take[b - 1] : 0);
-    a.block_table[b * a.table_row_stride + col] = a.free_pages[ring(head + p)];
+    const int64_t col = held + x - (b ? take[b - 1] : 0);
+    a.block_table[b * a.table_row_stride + col] = a.free_pages[wrap(front + x)];
   }
-  for (int64_t p = first; p < given; p += step) {
-    const int b = find(give, B, p);
-    const int64_t want = (max(ld_i(a.prefix_len, b, a.prefix_len_dtype), (int64_t)0) + end[b] -
-                          (b ? end[b - 1] : 0) + ps - 1) / ps;
-    const int64_t col = want + p - (b ? give[b - 1] : 0);
-    a.free_pages[ring(tail + p)] = a.block_table[b * a.table_row_stride + col];
+  for (int64_t x = turned; x < given; x += step) {
+    const int b = find(give, B, x);
+    const int64_t want = over(max(ld_i(a.prefix_len, b, a.prefix_len_dtype), (int64_t)0) + end[b] - (b ? end[b - 1] : 0) + ps - 1);
+    const int64_t col = want + x - (b ? give[b - 1] : 0);
+    a.free_pages[wrap(back + x)] = a.block_table[b * a.table_row_stride + col];
   }
   for (int64_t r = first; r < a.rows; r += step) {
     int64_t slot = -1, at = 0;
@@ -173,11 +187,11 @@ __global__ void __launch_bounds__(kThreads) page_plan_kernel(dft_page_plan_args 
       at = a.depth ? pre + ld_i(a.depth, r, a.depth_dtype) : place;
       if (!(state[b] & (DFT_STATUS_TABLE | DFT_STATUS_PAGES))) {
         const int held = min(max(a.held[b], 0), a.columns);
-        const int64_t col = place / ps;
+        const int64_t col = over(place);
         // a new page's id comes from the ring: another workgroup writes its cell
         const int32_t page = col < held ? a.block_table[b * a.table_row_stride + col]
-                                        : a.free_pages[ring(head + (b ? take[b - 1] : 0) + col - held)];
-        if (page >= 0) slot = (int64_t)page * ps + place % ps;
+                                        : a.free_pages[wrap(front + (b ? take[b - 1] : 0) + col - held)];
+        if (page >= 0) slot = (int64_t)page * ps + (place - col * ps);
       }
     }
     st_i(a.slots, r, a.index_dtype, slot);
@@ -293,23 +307,29 @@ void launch_append(const dft_kv_append_args& a, const Append& p, int grid, hipSt
 }  // namespace
 
 int launch_page_plan(const dft_page_plan_args* a, hipStream_t stream) {
-  const int64_t blocks = (a->rows + 1023) / 1024;
-  const int grid = (int)(blocks < 1 ? 1 : blocks > 512 ? 512 : blocks);
+  PagePlan p;
+  page_magic(a->page_size, p.magic, p.shift);
+  page_magic((int)a->capacity, p.ring_magic, p.ring_shift);
+  // a request a thread as far as a workgroup goes
+  const bool wide = a->batch > 256;
+  const int threads = wide ? 1024 : 256;
+  const int64_t blocks = (a->rows + a->rows / a->page_size + a->batch + threads - 1) / threads;
+  const int most = wide ? 256 : 1024;  // all at work at once
+  const int grid = (int)(blocks < 1 ? 1 : blocks > most ? most : blocks);
   const size_t lds = 4 * sizeof(int32_t) * (size_t)a->batch;
-  if (lds > 48 * 1024 &&
-      hipFuncSetAttribute(reinterpret_cast<const void*>(page_plan_kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
-                          (int)lds) != hipSuccess)
+  if (lds > 48 * 1024 && hipFuncSetAttribute(reinterpret_cast<const void*>(page_plan_kernel<1024>),
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess)
     return DFT_ERR_LAUNCH;
-  page_plan_kernel<<<grid, kThreads, lds, stream>>>(*a);
+  if (wide)
+    page_plan_kernel<1024><<<grid, 1024, lds, stream>>>(*a, p);
+  else
+    page_plan_kernel<256><<<grid, 256, lds, stream>>>(*a, p);
   return hipGetLastError() == hipSuccess ? DFT_OK : DFT_ERR_LAUNCH;
 }
 
 int launch_kv_append(const dft_kv_append_args* a, hipStream_t stream) {
   Append p = {};
-  int log = 0;
-  while ((1ll << log) < a->page_size) ++log;
-  p.shift = 31 + log;
-  p.magic = (uint32_t)(((1ull << p.shift) + a->page_size - 1) / a->page_size);
+  page_magic(a->page_size, p.magic, p.shift);
   // pieces of eight elements: 16-byte aligned addresses and strides (32 for fp32, which only a vector of its own needs)
   auto aligned = [](const void* q, int dt, int64_t s0, int64_t s1, int64_t s2) {
     return reinterpret_cast<uintptr_t>(q) % (dt == DFT_F32 ? 32 : 16) == 0 && s0 % 8 == 0 && s1 % 8 == 0 && s2 % 8 == 0;
