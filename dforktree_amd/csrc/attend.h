@@ -327,6 +327,11 @@ __device__ __forceinline__ void store_all(void* o, int64_t at, int dtype, bool v
   }
 }
 
+template <int I>
+struct At {
+  constexpr operator int() const { return I; }
+};
+
 // The state of a wave's 32 rows over KW keys of each tile.
 template <int D, int KW, class T>
 struct Rows {
@@ -398,7 +403,16 @@ struct Rows {
     top = next;
     sum *= by;
 #pragma unroll
-    for (int t = 0; t < DT; ++t) o[t] *= by;
+    for (int t = 0; t < DT; ++t) {
+      // With 256 columns the accumulators do not fit beside the rest into the
+      // registers that vector instructions read, and outside of this branch
+      // only the matrix unit needs them: they come into the branch and leave
+      // it in the matrix unit's registers.  Else the compiler moves them over
+      // and back for every tile.
+      if constexpr (D == 256) asm volatile("" : "+a"(o[t]));
+      o[t] *= by;
+      if constexpr (D == 256) asm volatile("" : "+a"(o[t]));
+    }
   }
 
   // The rest of a tile whose scores are s, with its values at v: the weights
@@ -409,8 +423,10 @@ struct Rows {
   // reads a fragment right in front of its product and waits for the LDS.
   static constexpr int kReach = 4;
 
-  template <bool NEXT>
-  __device__ __forceinline__ void step(uint32_t k, uint32_t v, float c, Scores& s) {
+  // Between the products run the four parts of `copy`, which send for tiles
+  // to come: in front of the products each would be waited for.
+  template <bool NEXT, class Copy>
+  __device__ __forceinline__ void step(uint32_t k, uint32_t v, float c, Scores& s, Copy copy) {
     settle(c);
     const float sub = top == -INFINITY ? 0.f : top;
     const uint32_t ka = key_address(k), va = value_address(v);
@@ -443,21 +459,33 @@ struct Rows {
       for (int i = 0; i < kPairs; ++i) weigh(i);
     }
     __builtin_amdgcn_sched_barrier(0);
+    auto products = [&](auto from, auto to) {
 #pragma unroll
-    for (int m = 0; m < kFirst + kSecond; ++m) {
-      if (NEXT && m == kFirst) __builtin_amdgcn_s_setprio(0);
-      const x8 f = ring[m % kReach];
-      if (m < kFirst)
-        n[m / QK] = T::mfma(f, q[m % QK], n[m / QK]);
-      else
-        o[(m - kFirst) % DT] = T::mfma(f, p[(m - kFirst) / DT], o[(m - kFirst) % DT]);
-      if (m + kReach < kFirst + kSecond) ring[m % kReach] = fragment(m + kReach);
-      if (m < kFirst) {
+      for (int m = from; m < to; ++m) {
+        if (NEXT && m == kFirst) __builtin_amdgcn_s_setprio(0);
+        const x8 f = ring[m % kReach];
+        if (m < kFirst)
+          n[m / QK] = T::mfma(f, q[m % QK], n[m / QK]);
+        else
+          o[(m - kFirst) % DT] = T::mfma(f, p[(m - kFirst) / DT], o[(m - kFirst) % DT]);
+        if (m + kReach < kFirst + kSecond) ring[m % kReach] = fragment(m + kReach);
+        if (m < kFirst) {
 #pragma unroll
-        for (int i = m * kPairs / (ST * QK); i < (m + 1) * kPairs / (ST * QK); ++i) weigh(i);
+          for (int i = m * kPairs / (ST * QK); i < (m + 1) * kPairs / (ST * QK); ++i) weigh(i);
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
-      __builtin_amdgcn_sched_barrier(0);
-    }
+    };
+    constexpr int kPart = (NEXT ? kFirst : kSecond) / 4;
+    products(At<0>(), At<kPart>());
+    copy(0);
+    products(At<kPart>(), At<2 * kPart>());
+    copy(1);
+    products(At<2 * kPart>(), At<3 * kPart>());
+    copy(2);
+    products(At<3 * kPart>(), At<4 * kPart>());
+    copy(3);
+    products(At<4 * kPart>(), At<kFirst + kSecond>());
     if (NEXT) __builtin_amdgcn_s_setprio(1);
     sum += part[0] + part[1];
     if constexpr (NEXT) {

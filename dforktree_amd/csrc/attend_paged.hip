@@ -319,30 +319,41 @@ struct Feed {
   __device__ __forceinline__ int there(int j, int keys, int id) const {
     return -(int)((j < keys) & ((uint32_t)id < (uint32_t)a.num_pages));
   }
-  // the values of tile n and the keys of tile n + kSkew (past the share's end
-  // the last tile's again); KEYS alone for the share's first
-  template <bool VALUES = true>
-  __device__ __forceinline__ void copy(int64_t n) {
-    // a lane looks up one of the wave's rows, for the keys or for the values
+  // The values of tile n and the keys of tile n + kSkew (past the share's end
+  // the last tile's again), in parts that many_kernel spreads over its
+  // products: look up, place, send the keys, send the values.
+  int looked_j, looked_id, looked_keys;  // of the row that the lane looks up, for the keys or for the values
+  __device__ __forceinline__ void look_up(int64_t n) {
     const int64_t of_keys = min(n + kSkew, count - 1);
     const int slot = (int)(lane & kMine ? n : of_keys) & (kSlots - 1), mine = lane % kMine;
     const int row = (mine / kRows * NW + wave) * kRows + mine % kRows;
     const int2 tile = room.tile[slot];
-    const int j = tile.x + row, id = room.ids[slot][row], ok = there(j, tile.y, id);
-    const uint64_t page = (uint32_t)(id & ok), token = (j - column(j) * a.page_size) & ok;
+    looked_j = tile.x + row;
+    looked_keys = tile.y;
+    looked_id = room.ids[slot][row];
+  }
+  __device__ __forceinline__ void place() {
+    const int j = looked_j, ok = there(j, looked_keys, looked_id);
+    const uint64_t page = (uint32_t)(looked_id & ok), token = (j - column(j) * a.page_size) & ok;
     room.from[wave][lane & (2 * kMine - 1)] = base + 2 * (page * page_stride + token * token_stride);
     asm volatile("" ::: "memory");
     __builtin_amdgcn_wave_barrier();
-    uint64_t k[kCopies], v[kCopies];
+  }
+  __device__ __forceinline__ void send(int64_t n, bool values) {
+    uint64_t at[kCopies];
 #pragma unroll
     for (int x = 0; x < kCopies; ++x) {
       const int to = (x * NW + wave) * kRows + lane / kPieces, piece = lane % kPieces;
-      const uint64_t* from = room.from[wave] + x * kRows + lane / kPieces;
-      k[x] = from[0] + ((piece ^ key_swizzle<D>(to)) << 4);
-      v[x] = from[kMine] + ((piece ^ (FEW ? few_value_swizzle<D>(to) : value_swizzle<D>(to))) << 4);
+      const int swizzle = !values ? key_swizzle<D>(to) : FEW ? few_value_swizzle<D>(to) : value_swizzle<D>(to);
+      at[x] = room.from[wave][x * kRows + lane / kPieces + (values ? kMine : 0)] + ((piece ^ swizzle) << 4);
     }
-    dma16_at<kCopies, 1024 * NW, ONCE>(k, keys_at(n + kSkew) + 1024 * wave);
-    if constexpr (VALUES) dma16_at<kCopies, 1024 * NW, ONCE>(v, values_at(n) + 1024 * wave);
+    dma16_at<kCopies, 1024 * NW, ONCE>(at, (values ? values_at(n) : keys_at(n + kSkew)) + 1024 * wave);
+  }
+  __device__ __forceinline__ void copy(int64_t n) {
+    look_up(n);
+    place();
+    send(n, false);
+    send(n, true);
   }
   // which of tile n's keys, from j0 on, there are
   __device__ __forceinline__ uint64_t present(int64_t n, int j0, int keys) const {
@@ -355,7 +366,11 @@ struct Feed {
     for (int t = 0; t < 2 * kAhead + kSkew; ++t) fetch_ids();
     __builtin_amdgcn_s_waitcnt(kWaitDma);
     asm volatile("" ::: "memory");
-    if constexpr (kSkew) copy<false>(-1);
+    if constexpr (kSkew) {
+      look_up(-1);
+      place();
+      send(-1, false);
+    }
 #pragma unroll 1
     for (int t = 0; t < min((int64_t)kAhead, count); ++t) {
       dma4_at(id_at, lds_address(room.ids[id_slot]));
@@ -377,14 +392,23 @@ struct Feed {
     else
       __builtin_amdgcn_s_waitcnt(kWaitDma);
   }
-  // the current tile, for all waves, with those behind it on their way
+  // the current tile, for all waves
   __device__ __forceinline__ void ready() {
     static_assert(kAhead == 1 || kAhead == 3);
     wait(min(count - 1 - used, (int64_t)kAhead - 1));
     __syncthreads();
+  }
+  // part 0 .. 3 of sending for the tile kAhead from here
+  __device__ __forceinline__ void advance(int part) {
     if (used + kAhead >= count) return;
-    fetch_ids();
-    copy(used + kAhead);
+    if (part == 0) {
+      fetch_ids();
+      look_up(used + kAhead);
+    } else if (part == 1) {
+      place();
+    } else {
+      send(used + kAhead, part == 3);
+    }
   }
 };
 
@@ -567,6 +591,7 @@ __global__ void __launch_bounds__(256) few_kernel(dft_paged_attention_args a, Sc
     }
     for (int t = begin; t < stop; ++t, ++feed.used) {
       feed.ready();
+      for (int part = 0; part < 4; ++part) feed.advance(part);
       const uint32_t kt = feed.keys_at(feed.used), vt = feed.values_at(feed.used);
       const int j0 = t * KT;
       const uint32_t there = (uint32_t)feed.present(feed.used, j0, q.keys);
@@ -699,7 +724,8 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) many_kernel(dft_pag
     for (int t = begin; t + 1 < stop; ++t) {
       feed.ready();
       look(feed.values_at(feed.used));
-      w.template step<true>(feed.keys_at(feed.used + 1), feed.values_at(feed.used), sc.c, s);
+      w.template step<true>(feed.keys_at(feed.used + 1), feed.values_at(feed.used), sc.c, s,
+                            [&](int part) { feed.advance(part); });
       ++feed.used;
       j0 += KT;
       there = feed.present(feed.used, j0, q.keys) & kEvery;
@@ -707,7 +733,7 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) many_kernel(dft_pag
     }
     feed.ready();
     look(feed.values_at(feed.used));
-    w.template step<false>(0, feed.values_at(feed.used), sc.c, s);
+    w.template step<false>(0, feed.values_at(feed.used), sc.c, s, [&](int part) { feed.advance(part); });
     ++feed.used;
     w.finish();
 

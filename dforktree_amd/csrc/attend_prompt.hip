@@ -107,13 +107,13 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) prompt_kernel(dft_p
     copy_values(t + 1);
     if (t + 2 < tiles) copy_keys(t + 2);
     look(t);
-    w.template step<true>(ktile(t + 1), vtile(t), sc.c, s);
+    w.template step<true>(ktile(t + 1), vtile(t), sc.c, s, [](int) {});
     if (partial(t + 1)) w.mask(s, seen(t + 1));
     __builtin_amdgcn_s_waitcnt(kWaitDma);
     __syncthreads();
   }
   look(tiles - 1);
-  w.template step<false>(0, vtile(tiles - 1), sc.c, s);
+  w.template step<false>(0, vtile(tiles - 1), sc.c, s, [](int) {});
   if (!works) return;
   w.finish();
   const float sum = w.whole_sum(), by = weight_of(sum);
