@@ -275,14 +275,14 @@ struct Feed {
   int group;
   uint64_t id_at;  // the last ids fetched
   int id_slot;
-  int64_t ids, count, used;  // tiles whose ids are fetched; of the share; behind us
+  int ids, count, used;      // tiles whose ids are fetched; of the share; behind us
   uint64_t base;             // of what the lane looks up: keys or values
   int64_t page_stride, token_stride;
   int wave, lane;
 
   __device__ __forceinline__ Feed(const dft_paged_attention_args& a, const Plan& pl, Room& room, const Walk& walk, int group,
                                   int wave)
-      : a(a), pl(pl), room(room), lead(walk), group(group), id_at(0), id_slot(0), ids(0), count(walk.left), used(0),
+      : a(a), pl(pl), room(room), lead(walk), group(group), id_at(0), id_slot(0), ids(0), count((int)min(walk.left, (int64_t)0x7fffffff)), used(0),
         wave(wave), lane(threadIdx.x & 63) {
     const bool value = lane & kMine;
     base = value ? (uint64_t)(uintptr_t)a.value_cache + 2 * (walk.g * a.vc_h_stride)
@@ -291,18 +291,18 @@ struct Feed {
     token_stride = value ? a.vc_token_stride : a.kc_token_stride;
   }
   // where the keys and the values of tile n are
-  __device__ __forceinline__ uint32_t keys_at(int64_t n) const {
-    return lds_address(room.keys) + ((int)n & (STAGES - 1)) * kBytes;
+  __device__ __forceinline__ uint32_t keys_at(int n) const {
+    return lds_address(room.keys) + (n & (STAGES - 1)) * kBytes;
   }
-  __device__ __forceinline__ uint32_t values_at(int64_t n) const {
-    return lds_address(room.values) + ((int)n & (STAGES - 1)) * kBytes;
+  __device__ __forceinline__ uint32_t values_at(int n) const {
+    return lds_address(room.values) + (n & (STAGES - 1)) * kBytes;
   }
   __device__ __forceinline__ uint32_t column(uint32_t j) const { return (uint32_t)((uint64_t)j * pl.magic >> pl.shift); }
 
   // the next tile's ids; past the share's end the last ones again, for the count
   __device__ __forceinline__ void fetch_ids() {
     if (ids < count) {
-      id_slot = (int)ids & (kSlots - 1);
+      id_slot = ids & (kSlots - 1);
       const int j0 = lead.off * KT;
       const uint32_t j = (uint32_t)max(min(j0 + lane % KT, lead.q.keys - 1), 0);
       id_at = (uint64_t)(uintptr_t)(a.block_table + lead.b * a.table_row_stride + column(j));
@@ -323,9 +323,9 @@ struct Feed {
   // the last tile's again), in parts that many_kernel spreads over its
   // products: look up, place, send the keys, send the values.
   int looked_j, looked_id, looked_keys;  // of the row that the lane looks up, for the keys or for the values
-  __device__ __forceinline__ void look_up(int64_t n) {
-    const int64_t of_keys = min(n + kSkew, count - 1);
-    const int slot = (int)(lane & kMine ? n : of_keys) & (kSlots - 1), mine = lane % kMine;
+  __device__ __forceinline__ void look_up(int n) {
+    const int of_keys = min(n + kSkew, count - 1);
+    const int slot = (lane & kMine ? n : of_keys) & (kSlots - 1), mine = lane % kMine;
     const int row = (mine / kRows * NW + wave) * kRows + mine % kRows;
     const int2 tile = room.tile[slot];
     looked_j = tile.x + row;
@@ -339,7 +339,7 @@ struct Feed {
     asm volatile("" ::: "memory");
     __builtin_amdgcn_wave_barrier();
   }
-  __device__ __forceinline__ void send(int64_t n, bool values) {
+  __device__ __forceinline__ void send(int n, bool values) {
     uint64_t at[kCopies];
 #pragma unroll
     for (int x = 0; x < kCopies; ++x) {
@@ -349,15 +349,15 @@ struct Feed {
     }
     dma16_at<kCopies, 1024 * NW, ONCE>(at, (values ? values_at(n) : keys_at(n + kSkew)) + 1024 * wave);
   }
-  __device__ __forceinline__ void copy(int64_t n) {
+  __device__ __forceinline__ void copy(int n) {
     look_up(n);
     place();
     send(n, false);
     send(n, true);
   }
   // which of tile n's keys, from j0 on, there are
-  __device__ __forceinline__ uint64_t present(int64_t n, int j0, int keys) const {
-    return __ballot(there(j0 + lane % KT, keys, room.ids[(int)n & (kSlots - 1)][lane]));
+  __device__ __forceinline__ uint64_t present(int n, int j0, int keys) const {
+    return __ballot(there(j0 + lane % KT, keys, room.ids[n & (kSlots - 1)][lane]));
   }
 
   // the share's first tiles
@@ -372,17 +372,17 @@ struct Feed {
       send(-1, false);
     }
 #pragma unroll 1
-    for (int t = 0; t < min((int64_t)kAhead, count); ++t) {
+    for (int t = 0; t < min(kAhead, count); ++t) {
       dma4_at(id_at, lds_address(room.ids[id_slot]));
       copy(t);
     }
     if constexpr (kSkew) {  // the first tile's keys, for all waves
-      wait(min((int64_t)kAhead, count));
+      wait(min(kAhead, count));
       __syncthreads();
     }
   }
   // until this wave's copies are done, but for those of `behind` tiles
-  __device__ __forceinline__ void wait(int64_t behind) const {
+  __device__ __forceinline__ void wait(int behind) const {
     if (kAhead == 3 && behind >= 3)
       __builtin_amdgcn_s_waitcnt(wait_loads(3 * kLoads));
     else if (kAhead == 3 && behind == 2)
@@ -395,10 +395,16 @@ struct Feed {
   // the current tile, for all waves
   __device__ __forceinline__ void ready() {
     static_assert(kAhead == 1 || kAhead == 3);
-    wait(min(count - 1 - used, (int64_t)kAhead - 1));
+    wait(min(count - 1 - used, kAhead - 1));
     __syncthreads();
   }
-  // part 0 .. 3 of sending for the tile kAhead from here
+  // sends for the tile kAhead from here
+  __device__ __forceinline__ void advance() {
+    if (used + kAhead >= count) return;
+    fetch_ids();
+    copy(used + kAhead);
+  }
+  // the same in parts, 0 .. 3
   __device__ __forceinline__ void advance(int part) {
     if (used + kAhead >= count) return;
     if (part == 0) {
@@ -539,7 +545,7 @@ __global__ void __launch_bounds__(256) few_kernel(dft_paged_attention_args a, Sc
   typedef typename T::x8 x8;
   __shared__ __attribute__((aligned(1024))) typename Tiles::Room room;
   __shared__ uint32_t notes[NW][NQ * 2][64];
-  __shared__ int64_t spoiled;  // the last tile found to hold a value that is not finite
+  __shared__ int spoiled;  // the last tile found to hold a value that is not finite
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), quad = lane >> 4;
   const int group = a.hq / a.hkv;
   const bool causal = a.flags & DFT_ATTN_CAUSAL;
@@ -591,7 +597,7 @@ __global__ void __launch_bounds__(256) few_kernel(dft_paged_attention_args a, Sc
     }
     for (int t = begin; t < stop; ++t, ++feed.used) {
       feed.ready();
-      for (int part = 0; part < 4; ++part) feed.advance(part);
+      feed.advance();
       const uint32_t kt = feed.keys_at(feed.used), vt = feed.values_at(feed.used);
       const int j0 = t * KT;
       const uint32_t there = (uint32_t)feed.present(feed.used, j0, q.keys);
@@ -665,7 +671,7 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) many_kernel(dft_pag
   constexpr uint64_t kEvery = KT == 64 ? ~0ull : (1ull << KT) - 1;
   __shared__ __attribute__((aligned(1024))) typename Tiles::Room room;
   __shared__ char notes[NW][Wave::kNotes];
-  __shared__ int64_t spoiled;  // the last tile found to hold a value that is not finite
+  __shared__ int spoiled;  // the last tile found to hold a value that is not finite
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
   const int group = a.hq / a.hkv;
   const bool causal = a.flags & DFT_ATTN_CAUSAL;

@@ -324,6 +324,9 @@ int dft_prompt_attention(const dft_prompt_attention_args* a, void* stream) {
   if (st != DFT_OK) return st < 0 ? DFT_OK : st;
   if (!a->k || !a->v || !aligned16(a->k) || !aligned16(a->v)) return DFT_ERR_INVALID;
   if (a->k_row_stride % 8 || a->k_h_stride % 8 || a->v_row_stride % 8 || a->v_h_stride % 8) return DFT_ERR_INVALID;
+  // a tile's 64 rows are reached by 32-bit byte offsets from its first
+  if (a->k_row_stride < 0 || a->v_row_stride < 0) return DFT_ERR_INVALID;
+  if (a->k_row_stride >= 1 << 24 || a->v_row_stride >= 1 << 24) return DFT_ERR_UNSUPPORTED;
   return dft::launch_prompt_attention(a, static_cast<hipStream_t>(stream));
 }
 

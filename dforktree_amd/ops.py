@@ -984,10 +984,12 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, key_cache: torch.Tensor, value_c
 
 def _aligned_rows(t, name):
     """A [rows, heads, d] view whose rows the kernels read as 16-byte pieces:
-    itself, or a copy when its address or strides do not allow it."""
+    itself, or a copy when its address or strides (a row stride of 2^24
+    elements or more) do not allow it."""
     if t.dim() != 3:
         raise ValueError(f"{name} must be [rows, heads, head_dim], got {tuple(t.shape)}")
-    if t.stride(2) != 1 or t.stride(0) % 8 or t.stride(1) % 8 or t.data_ptr() % 16:
+    s0, s1, s2 = t.stride()
+    if s2 != 1 or s0 % 8 or s1 % 8 or s0 >= 1 << 24 or t.data_ptr() % 16:
         t = torch.empty(t.shape, device=t.device, dtype=t.dtype).copy_(t)
     return t
 

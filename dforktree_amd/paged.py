@@ -1,0 +1,78 @@
+"""A paged KV cache for the full-attention layers beside the GDN layers.
+
+``PagedKV`` keeps what a serving loop would keep: the layers' pages, one
+block table, the ring of free pages and the requests' committed lengths, all
+on the device.  A step is
+
+    plan = kv.plan(new_len, rows=..., n_new=...)  # pages, slots, positions
+    for layer ...:
+        kv.append(layer, k, v, plan)              # before the attention
+        o = kv.attend(layer, q, plan)
+    kv.commit(new_len)                            # all of them, or for a draft tree:
+    kv.accept(layer, k, v, plan, path)            # each layer's accepted path, then
+    kv.commit(path_len)
+
+The kernels run on the current stream and nothing here waits for the device,
+so a step of fixed sizes can be captured in a HIP graph (over ``held``,
+``free_pos`` and ``prefix``, which every step replaces or updates in place).
+"""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+
+from . import ops
+
+
+class PagedKV:
+    """Pages of ``page_size`` tokens for ``layers`` layers and ``batch``
+    requests of at most ``columns`` pages each.  Every layer's keys and
+    values [pages, page_size, heads, head_dim] share one block table."""
+
+    def __init__(self, layers: int, batch: int, columns: int, pages: int, page_size: int, heads: int, head_dim: int, *,
+                 dtype: torch.dtype = torch.bfloat16, device="cuda"):
+        shape = (layers, pages, page_size, heads, head_dim)
+        self.keys, self.values = (torch.zeros(shape, dtype=dtype, device=device) for _ in range(2))
+        self.page_size = page_size
+        i32 = dict(dtype=torch.int32, device=device)
+        self.block_table = torch.full((batch, columns), -1, **i32)
+        self.held, self.prefix = torch.zeros(batch, **i32), torch.zeros(batch, **i32)
+        self.free_pages = torch.arange(pages, **i32)
+        self.free_pos = torch.tensor([0, pages], dtype=torch.int64, device=device)
+
+    def plan(self, new_len: torch.Tensor, *, rows: int, n_new: int, trim: bool = False,
+             depth: Optional[torch.Tensor] = None, anc_bits: Optional[torch.Tensor] = None) -> dict:
+        """Room for new_len[b] tokens behind every request's prefix
+        (``ops.page_plan``): rows, their total or more, and n_new, the most of
+        one request, are known on the host.  ``trim`` first returns the pages
+        that a rejected draft left; ``depth`` and ``anc_bits`` are a draft
+        tree's (``ops.tree_struct``)."""
+        p = ops.page_plan(self.prefix, new_len, self.block_table, self.held, self.free_pages, self.free_pos,
+                          page_size=self.page_size, rows=rows, trim=trim, depth=depth)
+        self.held, self.free_pos = p["held"], p["free_pos"]
+        return p | {"n_new": n_new, "anc_bits": anc_bits}
+
+    def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, plan: dict) -> None:
+        """The new rows' keys and values [rows, heads, head_dim] into their pages."""
+        ops.kv_append(k, v, self.keys[layer], self.values[layer], plan["slots"])
+
+    def attend(self, layer: int, q: torch.Tensor, plan: dict, **kw) -> torch.Tensor:
+        """The new rows' attention over their request's tokens, the new ones
+        included: causal, or a tree's where the plan has its anc_bits."""
+        return ops.paged_attention(q, self.keys[layer], self.values[layer], self.block_table, plan["seq_len"],
+                                   cu_seqlens=plan["cu_seqlens"], n_new=plan["n_new"], anc_bits=plan["anc_bits"], **kw)
+
+    def accept(self, layer: int, k: torch.Tensor, v: torch.Tensor, plan: dict, path: torch.Tensor) -> None:
+        """The keys and values of an accepted path to the places right behind
+        the prefix.  path [batch, columns]: rows of k and v (the step's), -1
+        past a request's last one; a request has at least as many rows as its
+        path columns that are not -1."""
+        batch, columns = path.shape
+        at = plan["cu_seqlens"][:-1, None].long() + torch.arange(columns, device=path.device)
+        slots = plan["slots"][at.clamp_max(plan["slots"].numel() - 1)]
+        ops.kv_append(k, v, self.keys[layer], self.values[layer], slots, rows=path)
+
+    def commit(self, length: torch.Tensor) -> None:
+        """The prefixes grow by length[b] of the step's tokens."""
+        self.prefix += length

@@ -581,7 +581,9 @@ DFT_API int dft_kv_append(const dft_kv_append_args* args, void* stream);
  * a row does not see do not touch it, whatever they hold.
  * Types: q, k, v all bf16 or all fp16, head_dim 64, 128 or 256, unit stride
  * along it; 16-byte aligned q, k and v, their other strides multiples of 8
- * elements.  The outputs' strides are free. */
+ * elements.  The outputs' strides are free.  A request's rows times
+ * hq / hkv stay below 2^31 - 2^16.  The weights are rounded to the inputs'
+ * type for the product with v; scores, sums and outputs are held in fp32. */
 enum dft_attention_flags { DFT_ATTN_CAUSAL = 1 };
 
 /* Over a paged cache, which holds the new tokens already: request b's n_b
@@ -627,7 +629,8 @@ DFT_API int dft_paged_attention_workspace(const dft_paged_attention_args* args, 
 
 /* Over whole packed prompts: rows cu_seqlens[b] .. cu_seqlens[b+1] of q, k
  * and v are request b's tokens; row i sees key j <= i (DFT_ATTN_CAUSAL) or
- * every one.  A request of more than max_len tokens is cut to max_len. */
+ * every one.  A request of more than max_len tokens is cut to max_len.  Row
+ * strides of k and v from 0 to 2^24 - 8. */
 typedef struct dft_prompt_attention_args {
   int32_t batch, max_len;
   int32_t hq, hkv, head_dim;

@@ -212,3 +212,34 @@ def test_python_layer_takes_gpu_tensors_only():
               lambda: ops.page_plan(i, i, i.view(4, 1), i, i, i.long()[:2], page_size=4, rows=4)):
         with pytest.raises(ValueError, match="GPU tensors"):
             f()
+
+
+def test_attention_sizes_past_the_kernels_counters():
+    """Rows times the heads of a group are counted in 31 bits, a tile's rows reached by 32-bit offsets."""
+    from dforktree_amd import _lib
+    INVALID, UNSUPPORTED = _lib.DFT_ERR_INVALID, _lib.DFT_ERR_UNSUPPORTED
+    a = attention_args(_lib.PromptAttentionArgs)
+    a.max_len, a.k, a.v = 4, 16, 16
+    for want, bad in ((UNSUPPORTED, dict(max_len=1 << 30)), (UNSUPPORTED, dict(k_row_stride=1 << 24)),
+                      (UNSUPPORTED, dict(v_row_stride=1 << 24)), (INVALID, dict(k_row_stride=-8)),
+                      (INVALID, dict(v_row_stride=-8))):
+        assert call("dft_prompt_attention", a, **bad) == want, bad
+    p = attention_args(_lib.PagedAttentionArgs)
+    p.n_new, p.page_size, p.columns, p.num_pages = 1 << 30, 16, 4, 8
+    p.key_cache = p.value_cache = p.block_table = p.seq_len = 16
+    p.seq_len_dtype = _lib.DFT_I32
+    assert call("dft_paged_attention", p) == UNSUPPORTED
+
+
+def test_workspace_goes_with_the_sizes_alone():
+    """None where the block table is short; else a bound that the lengths do not move."""
+    from dforktree_amd import _lib
+    a = attention_args(_lib.PagedAttentionArgs)
+    a.page_size, a.num_pages = 16, 8
+    n = ctypes.c_int64(-1)
+    need = {}
+    for new, columns in ((1, 32), (1, 33), (1, 9000), (4, 33), (40, 33), (1000, 33)):
+        a.n_new, a.columns = new, columns
+        assert _lib.load().dft_paged_attention_workspace(ctypes.byref(a), ctypes.byref(n)) == _lib.DFT_OK
+        need[new, columns] = n.value
+    assert need[1, 32] == 0 < need[1, 33] == need[1, 9000] <= need[4, 33] < need[40, 33] == need[1000, 33]
