@@ -12,6 +12,69 @@ namespace {
 
 using namespace attend;
 
+struct Span {
+  int64_t r0;
+  int n, status;
+};
+__device__ __forceinline__ Span span_of(const dft_prompt_attention_args& a, int b) {
+  const int64_t r0 = a.cu_seqlens ? a.cu_seqlens[b] : (int64_t)b * a.max_len;
+  int64_t n = a.cu_seqlens ? (int64_t)a.cu_seqlens[b + 1] - r0 : a.max_len;
+  const bool cut = n < 0 || n > a.max_len || r0 < 0 || r0 + n > a.rows;
+  n = r0 < 0 ? 0 : min(min(n, (int64_t)a.max_len), a.rows - r0);
+  return {r0, (int)max(n, (int64_t)0), cut ? DFT_STATUS_SPAN : 0};
+}
+
+// Row tile `tile` of request b and kv head g.
+struct Item {
+  int b, g, tile;
+  Span span;
+};
+
+// Packed prompts of different lengths: the workgroup's item where those of
+// all requests stand by falling row tile, so that the first workgroups get
+// the most keys and none of them the tiles that a shorter prompt has not got
+// (six prompts of 257 to 2999 tokens, by request instead, nearly half of them
+// of that kind and spread over the grid: 228 us, so 197).  False past
+// the last one.  Each wave finds it for itself: a lane holds a request and
+// tries a tile, 64 at a time.  From 65 requests on that would cost more than
+// it gives.
+constexpr int kSorted = 64;
+template <int BM>
+__device__ __forceinline__ bool sorted_item(const dft_prompt_attention_args& a, int group, int most, Item& item) {
+  const int lane = threadIdx.x & 63;
+  Span span = span_of(a, min(lane, a.batch - 1));
+  if (a.status && blockIdx.x == 0 && threadIdx.x < a.batch) a.status[threadIdx.x] = span.status;
+  const uint32_t tiles = lane < a.batch ? (uint32_t)(span.n * group + BM - 1) / BM : 0;
+  auto from = [&](uint32_t tile) {  // items of row tile `tile` or later, of one kv head
+    uint32_t sum = 0;
+    for (int i = 0; i < a.batch; ++i) sum += __builtin_elementwise_sub_sat((uint32_t)__builtin_amdgcn_readlane(tiles, i), tile);
+    return sum;
+  };
+  uint32_t x = blockIdx.x / a.hkv, low = 0;
+  item.g = blockIdx.x - x * a.hkv;
+  const uint32_t first = __builtin_amdgcn_readlane(tiles, 0);
+  if (__ballot(lane < a.batch && tiles != first) == 0) {  // all alike
+    const uint32_t turn = x / a.batch;
+    if (turn >= first) return false;
+    item.b = x - turn * a.batch;
+    low = first - 1 - turn;
+  } else {
+    for (uint32_t width = most, step = 0; step != 1; width = step) {  // the last tile that more than x items come from
+      step = (width + 63) / 64;
+      const uint64_t more = __ballot(from(low + lane * step) > x);
+      if (!more) return false;
+      low += (__popcll(more) - 1) * step;
+    }
+    uint64_t has = __ballot(tiles > low);
+    for (x -= __builtin_amdgcn_readfirstlane(from(low + 1)); x; --x) has &= has - 1;
+    item.b = __ffsll((unsigned long long)has) - 1;
+  }
+  item.tile = (int)low;
+  item.span.n = __builtin_amdgcn_readlane(span.n, item.b);
+  item.span.r0 = __builtin_amdgcn_readlane((int)span.r0, item.b);
+  return true;
+}
+
 template <int D, int NW, class T>
 __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) prompt_kernel(dft_prompt_attention_args a, Scale sc, bool vec) {
   constexpr int kRow = 2 * D, kBytes = kTile * kRow;  // of a tile's keys, and of its values
@@ -22,18 +85,22 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) prompt_kernel(dft_p
   __shared__ int spoiled;  // the last tile found to hold a value that is not finite
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
   const int group = a.hq / a.hkv;
-  const int pairs = a.batch * a.hkv, turn = blockIdx.x / pairs, pair = blockIdx.x - turn * pairs;
-  const int b = pair / a.hkv, g = pair - b * a.hkv;
-
-  const int64_t r0 = a.cu_seqlens ? a.cu_seqlens[b] : (int64_t)b * a.max_len;
-  int64_t n64 = a.cu_seqlens ? (int64_t)a.cu_seqlens[b + 1] - r0 : a.max_len;
-  const bool cut = n64 < 0 || n64 > a.max_len || r0 < 0 || r0 + n64 > a.rows;
-  n64 = r0 < 0 ? 0 : min(min(n64, (int64_t)a.max_len), a.rows - r0);
-  const int n = (int)max(n64, (int64_t)0);
-  if (a.status && turn == 0 && g == 0 && threadIdx.x == 0) a.status[b] = cut ? DFT_STATUS_SPAN : 0;
-
-  // the longest rows first: they see the most keys
-  const int p0 = (int)(gridDim.x / pairs - 1 - turn) * 32 * NW, rows = n * group;
+  const int pairs = a.batch * a.hkv;
+  Item item;
+  if (a.cu_seqlens && a.batch > 1 && a.batch <= kSorted) {
+    if (!sorted_item<32 * NW>(a, group, gridDim.x / pairs, item)) return;
+  } else {
+    // the longest rows first: they see the most keys
+    const int turn = blockIdx.x / pairs, pair = blockIdx.x - turn * pairs;
+    item.b = pair / a.hkv;
+    item.g = pair - item.b * a.hkv;
+    item.tile = (int)(gridDim.x / pairs) - 1 - turn;
+    item.span = span_of(a, item.b);
+    if (a.status && turn == 0 && item.g == 0 && threadIdx.x == 0) a.status[item.b] = item.span.status;
+  }
+  const int g = item.g;
+  const int64_t r0 = item.span.r0;
+  const int n = item.span.n, p0 = item.tile * 32 * NW, rows = n * group;
   if (p0 >= rows) return;
   const bool causal = a.flags & DFT_ATTN_CAUSAL;
   const int last = (int)((uint32_t)(min(p0 + 32 * NW, rows) - 1) / (uint32_t)group);  // token of the workgroup's last row

@@ -904,7 +904,7 @@ def page_plan(prefix_len: torch.Tensor, new_len: torch.Tensor, block_table: torc
     except KeyError:
         raise TypeError(f"index_dtype must be int32 or int64, got {index_dtype}") from None
     words = torch.empty(4 * batch + 1, device=dev, dtype=torch.int32)
-    out["cu_seqlens"], out["seq_len"], out["held"], out["status"] = words.split([batch + 1, batch, batch, batch])
+    out["cu_seqlens"], out["seq_len"], out["held"], out["status"] = words.split_with_sizes([batch + 1, batch, batch, batch])
     out["free_pos"] = torch.empty(2, device=dev, dtype=torch.int64)
     a.batch, a.columns, a.page_size, a.trim = batch, block_table.shape[1], page_size, int(bool(trim))
     a.rows, a.capacity = rows, free_pages.numel()
