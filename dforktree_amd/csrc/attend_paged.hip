@@ -426,9 +426,13 @@ __device__ __forceinline__ uint64_t tree_bits(uint64_t bits, int before, int j0)
 
 // ---- up to 32 rows ---------------------------------------------------------
 // All four waves work on the same 32-key tiles: each forms the scores of all
-// rows and takes a quarter of the output's columns, so nothing is exchanged
-// between them.  Four tiles' room in the LDS keeps three on their way, 48 D x
-// 8 bytes a workgroup; page ids come three tiles ahead of their use.
+// rows (on 16 x 16 products, half the work of 32 x 32 ones for the 4 to 16
+// rows of a decode step) and takes a quarter of the output's columns, so
+// nothing is exchanged between them.  Four tiles' room in the LDS keeps three
+// on their way, 72 to 96 KB a CU: bound by HBM, and HBM by what is on its way.
+// 64 requests of 300 to 8191 keys (8 kv heads, d 128): 178 us, 6.2 TB/s; two
+// waves on halves of 64-key tiles two deep took 249, copies without the
+// read-once mark 218.
 constexpr int kFewTile = 32, kFewStages = 4;
 
 // V^T fragment: 16 columns, the tile's 32 keys in the order of the weights
@@ -660,7 +664,14 @@ __global__ void __launch_bounds__(256) few_kernel(dft_paged_attention_args a, Sc
 }
 
 // ---- more rows -------------------------------------------------------------
-// NW waves of 32 rows each.
+// NW waves of 32 rows each, on 64-key tiles two deep: 32-key tiles four deep
+// cost more per tile than their deeper pipeline gives (draft trees 156 us for
+// 148, chunks 740 for 516 on one build).  With 128 columns two workgroups
+// share a CU; with 256 the accumulators leave room for one wave a SIMD, whose
+// products and everything else then overlap within the wave only.  32-node
+// trees of 64 requests over 500 to 4000 keys (8 kv heads, d 128): 148 us,
+// 4.3 TB/s and 510 TFLOP/s, 16 more for the join; chunks of 777 and 1024 rows
+// over 9000 to 15001 keys (2 kv heads, d 256): 425 us, 840 TFLOP/s.
 template <int D, int NW, int KT, int STAGES, bool ONCE, class T>
 __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) many_kernel(dft_paged_attention_args a, Scale sc, Plan pl) {
   constexpr int BM = 32 * NW;
@@ -774,7 +785,9 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) many_kernel(dft_pag
 // ---- the join --------------------------------------------------------------
 // Joins the parts of the items that share boundaries cut.  The workgroups of
 // an item's boundaries deal its units out among them: as many workgroups as
-// there are parts to read.  With few parts a wave takes a unit, with many the
+// there are parts to read (5 to 6 us at 16 rows an item, 16 at 128 rows, where
+// it moves 100 MB; a workgroup per part and unit, most of them idle, took 13
+// and 31).  With few parts a wave takes a unit, with many the
 // waves divide a unit's parts.
 constexpr int kJoinWaves = 8;
 

@@ -4,7 +4,11 @@
 // of one kv head) of one prompt and walks over the keys they see in tiles of
 // 64, which its waves share.  A tile's scores are formed beside the tile
 // before's weights, so its keys come a tile earlier than its values; the LDS
-// holds two tiles of either, one in use, one on its way.
+// holds two tiles of either, one in use, one on its way.  With 128 columns two
+// workgroups of four waves share a CU; eight waves on one tile gave 524 us for
+// 513.  One prompt of 8192 (32 heads, 8 kv heads, d 128, causal): 506 us, 1.09
+// PFLOP/s, the matrix unit busy 63% of the time at the 1.8 GHz that the card's
+// power leaves.
 #include "attend.h"
 
 namespace dft {
