@@ -48,7 +48,8 @@ constexpr int part_floats() {
 
 struct Request {
   int64_t r0;
-  int n, keys, before;  // rows (times the group within 31 bits), keys, keys in front of the rows' own (negative: some rows have none)
+  int n, keys;  // rows (times the group within 31 bits), keys
+  int before;   // keys in front of the rows' own (negative: some rows have none)
   int status;
 };
 
@@ -176,6 +177,7 @@ struct Walk {
     int64_t mine = 0, total;
     for (int r = b0; r < b1; ++r) mine += weight(r);
     const int64_t ahead = scan<NT>(mine, red, total);
+    // (a share's tiles in 31 bits: 2^36 keys, some hours' work)
     const int64_t size = max((total + pl.shares - 1) / pl.shares, (int64_t)(kLeastKeys / KT)), pos = share * size;
     left = min(size, total - pos);
     if (pos >= ahead && pos < ahead + mine) {
@@ -237,8 +239,8 @@ struct Walk {
   }
 };
 
-// Where the value pieces lie: few_kernel reads them by 16 lanes of 4 consecutive rows each over
-// 2 pieces.
+// Where the value pieces lie: few_kernel reads them by 16 lanes of 4
+// consecutive rows each over 2 pieces.
 template <int D>
 __device__ __forceinline__ int few_value_swizzle(int row) {
   return D == 64 ? ((row >> 1) & 3) << 1 : (row & 7) << 1;
@@ -273,16 +275,16 @@ struct Feed {
   Room& room;
   Walk lead;      // the walk as far as the ids
   int group;
-  uint64_t id_at;  // the last ids fetched
+  uint64_t id_at;        // the last ids fetched
   int id_slot;
-  int ids, count, used;      // tiles whose ids are fetched; of the share; behind us
-  uint64_t base;             // of what the lane looks up: keys or values
+  int ids, count, used;  // tiles whose ids are fetched; of the share; behind us
+  uint64_t base;         // of what the lane looks up: keys or values
   int64_t page_stride, token_stride;
   int wave, lane;
 
   __device__ __forceinline__ Feed(const dft_paged_attention_args& a, const Plan& pl, Room& room, const Walk& walk, int group,
                                   int wave)
-      : a(a), pl(pl), room(room), lead(walk), group(group), id_at(0), id_slot(0), ids(0), count((int)min(walk.left, (int64_t)0x7fffffff)), used(0),
+      : a(a), pl(pl), room(room), lead(walk), group(group), id_at(0), id_slot(0), ids(0), count((int)walk.left), used(0),
         wave(wave), lane(threadIdx.x & 63) {
     const bool value = lane & kMine;
     base = value ? (uint64_t)(uintptr_t)a.value_cache + 2 * (walk.g * a.vc_h_stride)
@@ -377,15 +379,14 @@ struct Feed {
       copy(t);
     }
     if constexpr (kSkew) {  // the first tile's keys, for all waves
-      wait(min(kAhead, count));
+      wait(1);
       __syncthreads();
     }
   }
   // until this wave's copies are done, but for those of `behind` tiles
   __device__ __forceinline__ void wait(int behind) const {
-    if (kAhead == 3 && behind >= 3)
-      __builtin_amdgcn_s_waitcnt(wait_loads(3 * kLoads));
-    else if (kAhead == 3 && behind == 2)
+    static_assert(kAhead == (FEW ? 3 : 1));  // behind: at most 2, or 1
+    if (FEW && behind == 2)
       __builtin_amdgcn_s_waitcnt(wait_loads(2 * kLoads));
     else if (behind == 1)
       __builtin_amdgcn_s_waitcnt(wait_loads(kLoads));
@@ -394,7 +395,6 @@ struct Feed {
   }
   // the current tile, for all waves
   __device__ __forceinline__ void ready() {
-    static_assert(kAhead == 1 || kAhead == 3);
     wait(min(count - 1 - used, kAhead - 1));
     __syncthreads();
   }
