@@ -134,13 +134,35 @@ __device__ __forceinline__ Place place_of(const Request& q, int group, int g, in
   return {q.r0 + i, g * group + (r - i * group), p < rows};
 }
 
-// A workgroup's walk over its share.
+// A workgroup's walk over its share, from its last item back to its first.  A
+// share of a request with many row tiles mostly holds the end of one item and
+// the beginning of the next; taken in this order the shares beside it stand at
+// the same keys or one same distance further on, and find them in the L2.
 template <int BM, int KT, int NT>
 struct Walk {
-  int64_t left;  // tiles of the share not begun
+  int64_t left;  // tiles of the share that are not done
   int g, share;  // kv head, number of the share on its line
-  int b, tile, off, all;  // the item, the tiles of it that are done, all of them
+  int b, tile;   // the item
+  int off, stop, all;  // the share's tiles of it, how many it has
   Request q;
+
+  // An item's tile on the line, found by the thread whose requests hold it.
+  struct Found {
+    Request q;
+    int b, tile, off;
+  };
+  template <class Weight>
+  static __device__ __forceinline__ Found find(const dft_paged_attention_args& a, int group, int b, int64_t rest,
+                                               Weight weight) {
+    Found f;
+    for (int64_t w; rest >= (w = weight(b)); ++b) rest -= w;
+    f.q = request<ByLane>(a, b);
+    f.b = b;
+    f.tile = 0;
+    for (int n; rest >= (n = tiles_of<BM, KT>(a, f.q, group, f.tile)); ++f.tile) rest -= n;
+    f.off = (int)rest;
+    return f;
+  }
 
   __device__ __forceinline__ bool begin(const dft_paged_attention_args& a, const Plan& pl, int group) {
     __shared__ int64_t red[NT / 64];
@@ -156,7 +178,7 @@ struct Walk {
       q = request<ByWave>(a, b);
       if (a.status && tile == 0 && g == 0 && threadIdx.x == 0) a.status[b] = q.status;
       if (tile >= row_tiles_of<BM>(q, group)) return false;
-      left = all = tiles_of<BM, KT>(a, q, group, tile);
+      left = stop = all = tiles_of<BM, KT>(a, q, group, tile);
       return true;
     }
     // consecutive shares of a line on one XCD
@@ -180,56 +202,53 @@ struct Walk {
     // (a share's tiles in 31 bits: 2^36 keys, some hours' work)
     const int64_t size = max((total + pl.shares - 1) / pl.shares, (int64_t)(kLeastKeys / KT)), pos = share * size;
     left = min(size, total - pos);
-    if (pos >= ahead && pos < ahead + mine) {
-      int64_t rest = pos - ahead;
-      int r = b0;
-      for (int64_t w; rest >= (w = weight(r)); ++r) rest -= w;
-      const Request q = request<ByLane>(a, r);
-      int t = 0;
-      for (int n; rest >= (n = tiles_of<BM, KT>(a, q, group, t)); ++t) rest -= n;
-      at[0] = r, at[1] = t, at[2] = (int)rest;
+    Head* head = reinterpret_cast<Head*>(pl.heads) + x;
+    if (left > 0) {
+      const int64_t last = pos + left - 1;
+      if (pos >= ahead && pos < ahead + mine) {
+        const Found f = find(a, group, b0, pos - ahead, weight);
+        Head h;
+        h.first = pos - f.off;
+        h.last = h.first + tiles_of<BM, KT>(a, f.q, group, f.tile);
+        h.share = size;
+        h.b = f.b, h.tile = f.tile, h.inside = f.off > 0, h.pad = 0;
+        *head = h;
+      }
+      if (last >= ahead && last < ahead + mine) {
+        const Found f = find(a, group, b0, last - ahead, weight);
+        at[0] = f.b, at[1] = f.tile, at[2] = f.off;
+      }
+    } else if (threadIdx.x == 0) {
+      head->inside = 0;
     }
     __syncthreads();
-    Head* head = reinterpret_cast<Head*>(pl.heads) + x;
-    if (left <= 0) {
-      if (threadIdx.x == 0) head->inside = 0;
-      return false;
-    }
+    if (left <= 0) return false;
     b = __builtin_amdgcn_readfirstlane(at[0]);
     tile = __builtin_amdgcn_readfirstlane(at[1]);
-    off = __builtin_amdgcn_readfirstlane(at[2]);
+    stop = __builtin_amdgcn_readfirstlane(at[2]) + 1;
     left = uniform64(left);
+    off = (int)max(stop - left, (int64_t)0);
     q = request<ByWave>(a, b);
     all = tiles_of<BM, KT>(a, q, group, tile);
-    if (threadIdx.x == 0) {
-      Head h;
-      h.first = pos - off;
-      h.last = h.first + all;
-      h.share = size;
-      h.b = b, h.tile = tile, h.inside = off > 0, h.pad = 0;
-      *head = h;
-    }
     return true;
   }
 
-  // behind `done` tiles of the item; false past the share's end
-  __device__ __forceinline__ bool next(const dft_paged_attention_args& a, int group, int done) {
-    left -= done;
-    off += done;
+  // to the item in front; false past the share's first
+  __device__ __forceinline__ bool next(const dft_paged_attention_args& a, int group) {
+    left -= stop - off;
     if (left <= 0) return false;
-    if (off < all) return true;
-    off = 0;
-    if (++tile >= row_tiles_of<BM>(q, group)) {
-      tile = 0;
+    if (--tile < 0) {
       do {
-        if (++b >= a.batch) {
+        if (--b < 0) {
           left = 0;
           return false;
         }
         q = request<ByWave>(a, b);
       } while (q.n == 0);
+      tile = row_tiles_of<BM>(q, group) - 1;
     }
-    all = tiles_of<BM, KT>(a, q, group, tile);
+    stop = all = tiles_of<BM, KT>(a, q, group, tile);
+    off = (int)max(stop - left, (int64_t)0);
     return true;
   }
 
@@ -273,7 +292,8 @@ struct Feed {
   const dft_paged_attention_args& a;
   const Plan& pl;
   Room& room;
-  Walk lead;      // the walk as far as the ids
+  Walk lead;  // the walk as far as the ids
+  int ahead;  // and its tile of the item
   int group;
   uint64_t id_at;        // the last ids fetched
   int id_slot;
@@ -284,7 +304,7 @@ struct Feed {
 
   __device__ __forceinline__ Feed(const dft_paged_attention_args& a, const Plan& pl, Room& room, const Walk& walk, int group,
                                   int wave)
-      : a(a), pl(pl), room(room), lead(walk), group(group), id_at(0), id_slot(0), ids(0), count((int)walk.left), used(0),
+      : a(a), pl(pl), room(room), lead(walk), ahead(walk.off), group(group), id_at(0), id_slot(0), ids(0), count((int)walk.left), used(0),
         wave(wave), lane(threadIdx.x & 63) {
     const bool value = lane & kMine;
     base = value ? (uint64_t)(uintptr_t)a.value_cache + 2 * (walk.g * a.vc_h_stride)
@@ -305,12 +325,15 @@ struct Feed {
   __device__ __forceinline__ void fetch_ids() {
     if (ids < count) {
       id_slot = ids & (kSlots - 1);
-      const int j0 = lead.off * KT;
+      const int j0 = ahead * KT;
       const uint32_t j = (uint32_t)max(min(j0 + lane % KT, lead.q.keys - 1), 0);
       id_at = (uint64_t)(uintptr_t)(a.block_table + lead.b * a.table_row_stride + column(j));
       room.tile[id_slot] = int2{j0, lead.q.keys};
       ++ids;
-      lead.next(a, group, 1);
+      if (++ahead == lead.stop) {
+        lead.next(a, group);
+        ahead = lead.off;
+      }
     }
     dma4_at(id_at, lds_address(room.ids[id_slot]));
   }
@@ -562,7 +585,7 @@ __global__ void __launch_bounds__(256) few_kernel(dft_paged_attention_args a, Sc
   bool more = true;
   while (more) {
     const Request q = walk.q;
-    const int begin = walk.off, stop = (int)min((int64_t)walk.all, begin + walk.left);
+    const int begin = walk.off, stop = walk.stop;
     Place to[NQ];
     uint64_t bits[NQ];
     int limit[NQ], fewest = q.keys;
@@ -659,7 +682,7 @@ __global__ void __launch_bounds__(256) few_kernel(dft_paged_attention_args a, Sc
         a.lse[to[y].row * a.lse_row_stride + to[y].h] = lse_of(top[y], sum[y]);
       }
     }
-    more = walk.next(a, group, stop - begin);
+    more = walk.next(a, group);
   }
 }
 
@@ -697,7 +720,7 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) many_kernel(dft_pag
   bool more = true;
   while (more) {
     const Request q = walk.q;
-    const int begin = walk.off, stop = (int)min((int64_t)walk.all, begin + walk.left);
+    const int begin = walk.off, stop = walk.stop;
     const int rows = q.n * group, pw = walk.tile * BM + 32 * wave;
     const bool works = pw < rows;
     const Place to = place_of(q, group, walk.g, pw + (lane & 31));
@@ -778,7 +801,7 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) many_kernel(dft_pag
         }
       }
     }
-    more = walk.next(a, group, stop - begin);
+    more = walk.next(a, group);
   }
 }
 
