@@ -21,7 +21,11 @@ namespace {
 using namespace attend;
 
 constexpr int kCus = 256, kXcds = 8;
-constexpr int kLeastKeys = 256;  // of a share
+// Keys in a share at least.  With few rows a part costs little, and a short
+// cache is read sooner by more workgroups (one request of 1000 keys, 8 kv
+// heads, d 128: 16.7 us a step of 64, 21.9 of 256); with many its accumulators
+// cost more than that (a tree of 32 nodes over 8000 keys: 38.2 and 33.8 us).
+constexpr int kLeastFew = 64, kLeastMany = 256;
 constexpr int kUncutKeys = 512;  // an item of at most so many keys is never cut
 
 // What a share that begins inside an item leaves for the join.
@@ -202,7 +206,7 @@ struct Walk {
     for (int r = b0; r < b1; ++r) mine += weight(r);
     const int64_t ahead = scan<NT>(mine, red, total);
     // (a share's tiles in 31 bits: 2^36 keys, some hours' work)
-    const int64_t size = max((total + pl.shares - 1) / pl.shares, (int64_t)(kLeastKeys / KT)), pos = share * size;
+    const int64_t size = max((total + pl.shares - 1) / pl.shares, (int64_t)((BM <= 32 ? kLeastFew : kLeastMany) / KT)), pos = share * size;
     left = min(size, total - pos);
     Head* head = reinterpret_cast<Head*>(pl.heads) + x;
     if (left > 0) {
