@@ -814,9 +814,10 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) many_kernel(dft_pag
 // ---- the join --------------------------------------------------------------
 // Joins the parts of the items that share boundaries cut.  The workgroups of
 // an item's boundaries deal its units out among them: as many workgroups as
-// there are parts to read (5 to 6 us at 16 rows an item, 16 at 128 rows, where
-// it moves 100 MB; a workgroup per part and unit, most of them idle, took 13
-// and 31).  With few parts a wave takes a unit, with many the
+// there are parts to read, times four with many rows, whose parts have four
+// times a workgroup's units (5 to 6 us at 16 rows an item; at 128 rows 10 for
+// four trees, 15.6 for 64, where it moves 100 MB, 16.5 in both with one each;
+// a workgroup per part and unit, most of them idle, took 13 and 31).  With few parts a wave takes a unit, with many the
 // waves divide a unit's parts.
 constexpr int kJoinWaves = 8;
 
@@ -835,7 +836,8 @@ __global__ void __launch_bounds__(64 * kJoinWaves) join_kernel(dft_paged_attenti
   const int units = kJoinWaves / split, turn = wave % split;  // units at a time; which of the parts
   const float* first = pl.parts + ((int64_t)g * pl.shares + begin) * 2 * part_floats<D, BM>();
   const Request q = request<ByWave>(a, h.b);
-  for (int u0 = (share - 1 - (int)begin) * units; u0 < kUnits; u0 += (parts - 1) * units) {
+  const int step = (parts - 1) * (int)gridDim.y * units;
+  for (int u0 = ((share - 1 - (int)begin) * (int)gridDim.y + blockIdx.y) * units; u0 < kUnits; u0 += step) {
     const int unit = min(u0 + wave / split, kUnits - 1), block = unit / kOf, in = unit % kOf;
     const int row = block * kLane + lane % kLane;
     const int d = kLane == 16 ? 16 * in + 4 * (lane / 16) : 8 * in + 4 * (lane / 32);
@@ -923,7 +925,7 @@ int launch(const dft_paged_attention_args& a, const Shape& s, const Plan& pl, hi
   else if (s.rows == 32)
     join_kernel<D, 32><<<lines, 64 * kJoinWaves, 0, stream>>>(a, pl);
   else
-    join_kernel<D, 128><<<lines, 64 * kJoinWaves, 0, stream>>>(a, pl);
+    join_kernel<D, 128><<<dim3(lines, 4), 64 * kJoinWaves, 0, stream>>>(a, pl);
   return hipGetLastError() == hipSuccess ? DFT_OK : DFT_ERR_LAUNCH;
 }
 
