@@ -26,7 +26,11 @@ constexpr int kCus = 256, kXcds = 8;
 // heads, d 128: 16.7 us a step of 64, 21.9 of 256); with many its accumulators
 // cost more than that (a tree of 32 nodes over 8000 keys: 38.2 and 33.8 us).
 constexpr int kLeastFew = 64, kLeastMany = 256;
-constexpr int kUncutKeys = 512;  // an item of at most so many keys is never cut
+// An item of at most so many keys is never cut: no scan, no parts, no second
+// launch.  One token each over 470 keys, uncut, and over 500 in a wider table,
+// cut: 1 request 20.4 and 16.9 us, 64 requests 27.3 and 34.6; trees of 32
+// nodes, 1 request 20.3 and 24.4, 16 requests 22.5 and 42.6.
+constexpr int kUncutKeys = 512;
 
 // What a share that begins inside an item leaves for the join.
 struct Head {
@@ -890,6 +894,8 @@ struct Shape {
 Shape shape_of(const dft_paged_attention_args& a) {
   Shape s = {};
   const int64_t rows = (int64_t)a.n_new * (a.hq / a.hkv);
+  // trees of 4 and 8 nodes (16 and 32 rows, 64 requests over 500 to 4000 keys):
+  // 138 and 142 us with few_kernel, 158 and 152 with many_kernel
   s.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : 128;
   s.once = rows <= s.rows;  // a key is read for one item only
   s.uncut = (int64_t)a.columns * a.page_size <= kUncutKeys;
