@@ -12,9 +12,9 @@ on the device.  A step is
     kv.accept(layer, k, v, plan, path)            # each layer's accepted path, then
     kv.commit(path_len)
 
-The kernels run on the current stream and nothing here waits for the device,
-so a step of fixed sizes can be captured in a HIP graph (over ``held``,
-``free_pos`` and ``prefix``, which every step replaces or updates in place).
+The kernels run on the current stream, nothing here waits for the device, and
+``held``, ``free_pos`` and ``prefix`` are updated in place: a step of fixed
+sizes, captured in a HIP graph, goes on from where the replay before it ended.
 """
 from __future__ import annotations
 
@@ -50,7 +50,8 @@ class PagedKV:
         tree's (``ops.tree_struct``)."""
         p = ops.page_plan(self.prefix, new_len, self.block_table, self.held, self.free_pages, self.free_pos,
                           page_size=self.page_size, rows=rows, trim=trim, depth=depth)
-        self.held, self.free_pos = p["held"], p["free_pos"]
+        self.held.copy_(p["held"])
+        self.free_pos.copy_(p["free_pos"])
         return p | {"n_new": n_new, "anc_bits": anc_bits}
 
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, plan: dict) -> None:

@@ -97,3 +97,45 @@ def test_serving_loop(cuda, page_size, hq, hkv, d):
         history[layer][0] = history[layer][0][:0]
     step([0, 2, 1], trim=True)
     assert int(kv.held[0]) == 0 and kv.free_pos[1] - before[1] >= held
+
+
+def test_replayed_steps(cuda):
+    """A decode step captured once: every replay takes the next token, and pages when it needs one."""
+    from dforktree_amd.paged import PagedKV
+    announce("replayed steps")
+    B, hq, hkv, d, ps = 2, 4, 2, 64, 4
+    kv = PagedKV(1, B, 8, 16, ps, hkv, d, device=cuda)
+    g = torch.Generator().manual_seed(0)
+    x = torch.zeros(B, hq + 2 * hkv, d, dtype=BF16, device=cuda)
+    one = torch.ones(B, dtype=torch.int32, device=cuda)
+
+    def step():
+        plan = kv.plan(one, rows=B, n_new=1)
+        kv.append(0, x[:, hq:hq + hkv], x[:, hq + hkv:], plan)
+        o = kv.attend(0, x[:, :hq], plan)
+        kv.commit(one)
+        return o
+
+    seen = []
+    for replay in range(12):
+        host = torch.randn(B, hq + 2 * hkv, d, generator=g).to(BF16)
+        seen.append(host.double().numpy())
+        x.copy_(host)
+        if replay == 0:
+            o = step()  # eager
+        elif replay == 1:
+            torch.cuda.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                o = step()
+        if replay:
+            torch.cuda.synchronize()
+            graph.replay()
+        torch.cuda.synchronize()
+        assert kv.prefix.tolist() == [replay + 1] * B and kv.held.tolist() == [replay // ps + 1] * B
+        past = np.stack(seen, 1)  # [B, tokens, heads, d]
+        for b in range(B):
+            sees = np.ones((1, replay + 1), bool)
+            want = P.attend(past[b, -1:, :hq], past[b, :, hq:hq + hkv], past[b, :, hq + hkv:], sees, d ** -0.5)[0]
+            off = np.abs(o[b:b + 1].double().cpu().numpy() - want).max()
+            assert off <= 2 * 2.0 ** -8 * np.abs(past[b, :, hq + hkv:]).max()
