@@ -8,13 +8,21 @@ on the device.  A step is
     for layer ...:
         kv.append(layer, k, v, plan)              # before the attention
         o = kv.attend(layer, q, plan)
-    kv.commit(new_len)                            # all of them, or for a draft tree:
+    kv.commit(new_len)                            # all that have a place, or for a draft tree:
     kv.accept(layer, k, v, plan, path)            # each layer's accepted path, then
     kv.commit(path_len)
 
+A request that the plan refuses (plan["status"]: DFT_STATUS_PAGES when the
+pages ran out, DFT_STATUS_TABLE when its row of the block table is full) takes
+no part in the step: nothing of it is written, its rows see no key, and
+``commit`` adds nothing to its prefix, so the same tokens can be planned again
+once there are pages.  One whose rows were cut (DFT_STATUS_SPAN) commits what
+was left of them.
+
 The kernels run on the current stream, nothing here waits for the device, and
-``held``, ``free_pos`` and ``prefix`` are updated in place: a step of fixed
-sizes, captured in a HIP graph, goes on from where the replay before it ended.
+``held``, ``free_pos``, ``prefix`` and ``served`` are updated in place: a step
+of fixed sizes, captured in a HIP graph, goes on from where the replay before
+it ended.
 """
 from __future__ import annotations
 
@@ -38,6 +46,7 @@ class PagedKV:
         i32 = dict(dtype=torch.int32, device=device)
         self.block_table = torch.full((batch, columns), -1, **i32)
         self.held, self.prefix = torch.zeros(batch, **i32), torch.zeros(batch, **i32)
+        self.served = torch.zeros(batch, **i32)  # the last plan's tokens that have places and are not committed
         self.free_pages = torch.arange(pages, **i32)
         self.free_pos = torch.tensor([0, pages], dtype=torch.int64, device=device)
 
@@ -50,6 +59,7 @@ class PagedKV:
         tree's (``ops.tree_struct``)."""
         p = ops.page_plan(self.prefix, new_len, self.block_table, self.held, self.free_pages, self.free_pos,
                           page_size=self.page_size, rows=rows, trim=trim, depth=depth)
+        torch.sub(p["seq_len"], self.prefix, out=self.served).clamp_(min=0)  # a refused request's seq_len is 0
         self.held.copy_(p["held"])
         self.free_pos.copy_(p["free_pos"])
         return p | {"n_new": n_new, "anc_bits": anc_bits}
@@ -75,5 +85,8 @@ class PagedKV:
         ops.kv_append(k, v, self.keys[layer], self.values[layer], slots, rows=path)
 
     def commit(self, length: torch.Tensor) -> None:
-        """The prefixes grow by length[b] of the step's tokens."""
+        """The prefixes grow by length[b] of the step's tokens, as far as the
+        plan gave them places: none of a refused request's."""
+        length = torch.minimum(length, self.served)
         self.prefix += length
+        self.served -= length
