@@ -77,12 +77,12 @@ class PagedKV:
     def accept(self, layer: int, k: torch.Tensor, v: torch.Tensor, plan: dict, path: torch.Tensor) -> None:
         """The keys and values of an accepted path to the places right behind
         the prefix.  path [batch, columns]: rows of k and v (the step's), -1
-        past a request's last one; a request has at least as many rows as its
-        path columns that are not -1."""
-        batch, columns = path.shape
-        at = plan["cu_seqlens"][:-1, None].long() + torch.arange(columns, device=path.device)
+        past a request's last one; what is longer than the rows that the plan
+        has of a request is left out, as ``commit`` leaves it out."""
+        cu = plan["cu_seqlens"].long()
+        at = cu[:-1, None] + torch.arange(path.shape[1], device=path.device)
         slots = plan["slots"][at.clamp_max(plan["slots"].numel() - 1)]
-        ops.kv_append(k, v, self.keys[layer], self.values[layer], slots, rows=path)
+        ops.kv_append(k, v, self.keys[layer], self.values[layer], torch.where(at < cu[1:, None], slots, -1), rows=path)
 
     def commit(self, length: torch.Tensor) -> None:
         """The prefixes grow by length[b] of the step's tokens, as far as the

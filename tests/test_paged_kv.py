@@ -85,3 +85,21 @@ def test_a_plan_commits_no_more_than_it_placed(make):
     for length, prefix in ((ints(2), 2), (torch.tensor([2]), 4), (ints(2), 5), (ints(1), 5)):
         kv.commit(length)
         assert kv.prefix.tolist() == [prefix] and kv.prefix.dtype == torch.int32
+
+
+def test_a_cut_request_keeps_to_its_own_places(make):
+    """The rows end inside request 1's tree and before request 2's: what of their paths has no place is left out."""
+    kv = make(1, 3, 4, 9, 4)
+    plan = kv.plan(ints(2, 4, 3), rows=4, n_new=4)
+    assert plan["status"].tolist() == [0, P.STATUS_SPAN, P.STATUS_SPAN]
+    x = marks(10, 11, 20, 21, 22, 23, 30, 31, 32)
+    kv.accept(0, x, x, plan, torch.tensor([[0, 1, -1], [2, 3, 5], [6, 7, 8]]))
+    kv.commit(ints(2, 3, 3))
+    assert kv.prefix.tolist() == [2, 2, 0]
+    assert tokens(kv, 0) == [10, 11] and tokens(kv, 1) == [20, 21]
+    assert sorted(kv.keys[kv.keys != 0].tolist()) == [10, 11, 20, 21]
+    kv.prefix.zero_()
+    plan = kv.plan(ints(0, 4, 3), rows=4, n_new=4)  # request 2 follows a whole one
+    kv.keys.zero_()
+    kv.accept(0, x, x, plan, torch.tensor([[0, 1, -1], [2, 3, 5], [6, 7, 8]]))
+    assert sorted(kv.keys[kv.keys != 0].tolist()) == [20, 21, 23]
