@@ -79,6 +79,8 @@ class PagedKV:
         the prefix.  path [batch, columns]: rows of k and v (the step's), -1
         past a request's last one; what is longer than the rows that the plan
         has of a request is left out, as ``commit`` leaves it out."""
+        if not plan["slots"].numel():  # no row, so no place either
+            return
         cu = plan["cu_seqlens"].long()
         at = cu[:-1, None] + torch.arange(path.shape[1], device=path.device)
         slots = plan["slots"][at.clamp_max(plan["slots"].numel() - 1)]

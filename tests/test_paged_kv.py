@@ -103,3 +103,12 @@ def test_a_cut_request_keeps_to_its_own_places(make):
     kv.keys.zero_()
     kv.accept(0, x, x, plan, torch.tensor([[0, 1, -1], [2, 3, 5], [6, 7, 8]]))
     assert sorted(kv.keys[kv.keys != 0].tolist()) == [20, 21, 23]
+
+
+def test_a_step_without_rows(make):
+    """Every request waits: nothing is written, and no slot of none is looked up."""
+    kv = make(1, 2, 4, 9, 4)
+    plan = kv.plan(ints(0, 0), rows=0, n_new=0)
+    kv.accept(0, marks(), marks(), plan, torch.full((2, 3), -1))
+    kv.commit(ints(0, 0))
+    assert not kv.keys.any() and kv.prefix.tolist() == [0, 0]
