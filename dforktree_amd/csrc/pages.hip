@@ -89,13 +89,20 @@ __global__ void __launch_bounds__(THREADS) page_plan_kernel(dft_page_plan_args a
     return x <= 0x7fffffffll ? (int64_t)((uint64_t)(uint32_t)x * p.magic >> p.shift) : x / ps;
   };
 
+  // Lengths as far as they matter, so that no sum of them leaves 64 bits: a
+  // prefix past kFar needs more pages than a table has columns (2^31) even of
+  // the largest pages (2^31), more new tokens than `rows` are cut to it.
+  constexpr int64_t kFar = INT64_MAX - (1ll << 33);
+  auto prefix_of = [&](int b) { return min(max(ld_i(a.prefix_len, b, a.prefix_len_dtype), (int64_t)0), kFar); };
+  auto new_of = [&](int b) { return min(max(ld_i(a.new_len, b, a.new_len_dtype), (int64_t)0), a.rows + 1); };
+
   // rows
   if (threadIdx.x < 2) within[threadIdx.x] = 0;
   Sums s = {{0, 0}};
-  for (int b = b0; b < b1; ++b) s.v[0] += max(ld_i(a.new_len, b, a.new_len_dtype), (int64_t)0);
+  for (int b = b0; b < b1; ++b) s.v[0] += new_of(b);
   s = block_scan<THREADS>(s, red);
   for (int b = b0; b < b1; ++b) {
-    s.v[0] += max(ld_i(a.new_len, b, a.new_len_dtype), (int64_t)0);
+    s.v[0] += new_of(b);
     end[b] = (int32_t)min(s.v[0], a.rows);
   }
   __syncthreads();
@@ -103,7 +110,7 @@ __global__ void __launch_bounds__(THREADS) page_plan_kernel(dft_page_plan_args a
   auto pages = [&](int b, int& status, int64_t& prefix, int& n) -> int64_t {  // wanted - held
     const int64_t len = ld_i(a.new_len, b, a.new_len_dtype), pre = ld_i(a.prefix_len, b, a.prefix_len_dtype);
     n = end[b] - (b ? end[b - 1] : 0);
-    prefix = max(pre, (int64_t)0);
+    prefix = min(max(pre, (int64_t)0), kFar);
     status = n != len || pre < 0 ? DFT_STATUS_SPAN : 0;
     const int64_t want = over(prefix + n + ps - 1);
     if (want > a.columns) status |= DFT_STATUS_TABLE;
@@ -175,7 +182,7 @@ __global__ void __launch_bounds__(THREADS) page_plan_kernel(dft_page_plan_args a
   }
   for (int64_t x = turned; x < given; x += step) {
     const int b = find(give, B, x);
-    const int64_t want = over(max(ld_i(a.prefix_len, b, a.prefix_len_dtype), (int64_t)0) + end[b] - (b ? end[b - 1] : 0) + ps - 1);
+    const int64_t want = over(prefix_of(b) + end[b] - (b ? end[b - 1] : 0) + ps - 1);
     const int64_t col = want + x - (b ? give[b - 1] : 0);
     a.free_pages[wrap(back + x)] = a.block_table[b * a.table_row_stride + col];
   }
@@ -183,7 +190,7 @@ __global__ void __launch_bounds__(THREADS) page_plan_kernel(dft_page_plan_args a
     int64_t slot = -1, at = 0;
     if (r < rows) {
       const int b = find(end, B, r);
-      const int64_t pre = max(ld_i(a.prefix_len, b, a.prefix_len_dtype), (int64_t)0);
+      const int64_t pre = prefix_of(b);
       const int64_t place = pre + r - (b ? end[b - 1] : 0);
       at = a.depth ? pre + ld_i(a.depth, r, a.depth_dtype) : place;
       if (!(state[b] & (DFT_STATUS_TABLE | DFT_STATUS_PAGES))) {
