@@ -13,10 +13,16 @@
 // pieces are placed by an XOR of the row, which the copies' source addresses
 // carry, so that neither read has bank conflicts.
 //
-// The running maximum is only moved when a row's score exceeds it by 2^8: the
-// weights then stay below 2^8 times the number of keys, which fp32 sums and
-// bf16 / fp16 weights hold as well as weights up to 1, and the accumulators
-// are rescaled in a few tiles instead of in most.
+// A row's reference is only moved when a score exceeds the one that set it by
+// kSlack log2 units, to kBase below that score: the accumulators are rescaled
+// in a few tiles instead of in most, and the row's largest weight stands
+// between 2^kBase and 2^(kBase + kSlack).  Weights are rounded to the inputs'
+// type.  bf16 holds them as well as weights up to 1.  fp16 loses relative
+// precision below 2^-14: with kBase 7 a key's weight is off by at most
+// 2^-25 / 2^7 = 2^-32 of the row's sum where half a step is less than that.
+// (With 0, 500 keys around 2^-27 beside one of weight 1 came out a third off,
+// and weights below 2^-25 were lost.)  Its kSlack leaves 2^5 to fp16's end for
+// the rounding of scores up to 2^26.
 #pragma once
 
 #include <math.h>
@@ -35,6 +41,7 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 struct Bf16 {
   typedef bf16x8 x8;
   static constexpr uint32_t kExp = 0x7f80, kOne = 0x3f80;
+  static constexpr float kBase = 0, kSlack = 8;
   static __device__ __forceinline__ f32x16 mfma(x8 a, x8 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
@@ -45,6 +52,7 @@ struct Bf16 {
 struct F16 {
   typedef f16x8 x8;
   static constexpr uint32_t kExp = 0x7c00, kOne = 0x3c00;
+  static constexpr float kBase = 7, kSlack = 4;
   static __device__ __forceinline__ f32x16 mfma(x8 a, x8 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
   }
@@ -55,7 +63,6 @@ struct F16 {
 
 constexpr int kTile = 64;          // keys per tile
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr float kSlack = 8.f;      // log2 units a row's score may exceed its reference by
 constexpr int kWaitDma = 0x0f70;   // s_waitcnt vmcnt(0)
 
 #define DFT_LDS __attribute__((address_space(3)))
@@ -395,11 +402,12 @@ struct Rows {
   // Moves the reference of the rows whose scores (high: their maximum so far)
   // exceed it by too much.
   __device__ __forceinline__ void settle(float c) {
-    if (!__any(high * c > top + kSlack)) return;
+    constexpr float kMost = T::kBase + T::kSlack;
+    if (!__any(high * c - top > kMost)) return;
     // row by row: what a row gets does not depend on the others of the wave
     const float new_top = fmaxf(high, __shfl_xor(high, 32)) * c;
-    const bool move = new_top > top + kSlack;
-    const float next = move ? new_top : top, by = move ? __builtin_amdgcn_exp2f(top - next) : 1.f;
+    const bool move = new_top - top > kMost;
+    const float next = move ? new_top - T::kBase : top, by = move ? __builtin_amdgcn_exp2f(top - next) : 1.f;
     top = next;
     sum *= by;
 #pragma unroll

@@ -514,11 +514,12 @@ __device__ __forceinline__ void few_tile(uint32_t k, uint32_t v, int wave, const
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int r = 0; r < 4; ++r) high = fmaxf(high, s[y][t][r]);
-    if (__any(high * c > top[y] + kSlack)) {
+    constexpr float kMost = T::kBase + T::kSlack;
+    if (__any(high * c - top[y] > kMost)) {
       high = fmaxf(high, __shfl_xor(high, 16));
       const float new_top = fmaxf(high, __shfl_xor(high, 32)) * c;
-      const bool move = new_top > top[y] + kSlack;
-      const float next = move ? new_top : top[y], by = move ? __builtin_amdgcn_exp2f(top[y] - next) : 1.f;
+      const bool move = new_top - top[y] > kMost;
+      const float next = move ? new_top - T::kBase : top[y], by = move ? __builtin_amdgcn_exp2f(top[y] - next) : 1.f;
       top[y] = next;
       sum[y] *= by;
 #pragma unroll

@@ -583,7 +583,8 @@ DFT_API int dft_kv_append(const dft_kv_append_args* args, void* stream);
  * along it; 16-byte aligned q, k and v, their other strides multiples of 8
  * elements.  The outputs' strides are free.  A request's rows times
  * hq / hkv stay below 2^31 - 2^16.  The weights are rounded to the inputs'
- * type for the product with v; scores, sums and outputs are held in fp32. */
+ * type for the product with v (fp16's, where that is more than half a step,
+ * by 2^-32 of the row's sum); scores, sums and outputs are held in fp32. */
 enum dft_attention_flags { DFT_ATTN_CAUSAL = 1 };
 
 /* Over a paged cache, which holds the new tokens already: request b's n_b
