@@ -57,7 +57,7 @@ constexpr int part_floats() {
 struct Request {
   int64_t r0;
   int n, keys;  // rows (times the group within 31 bits), keys
-  int before;   // keys in front of the rows' own (negative: some rows have none)
+  int before;   // keys in front of the first row's own (negative: some rows have none)
   int status;
 };
 
@@ -84,12 +84,15 @@ __device__ __forceinline__ Request request(const dft_paged_attention_args& a, in
   q.r0 = a.cu_seqlens ? By::i32(a.cu_seqlens + b) : (int64_t)b * a.n_new;
   int64_t n = a.cu_seqlens ? (int64_t)By::i32(a.cu_seqlens + b + 1) - q.r0 : a.n_new;
   q.status = n < 0 || n > a.n_new || q.r0 < 0 || q.r0 + n > a.rows ? DFT_STATUS_SPAN : 0;
+  // a cut request's rows are its first ones: those cut off stand behind them
+  // (up to 2^31 - 2^16 of them, as many as rows can be)
+  const int given = (int)min(max(n, (int64_t)0), (int64_t)0x7fff0000);
   n = q.r0 < 0 ? 0 : min(min(n, (int64_t)a.n_new), a.rows - q.r0);
   q.n = (int)max(n, (int64_t)0);
   const int64_t top = 0x7fffffff - kTile, room = (int64_t)a.columns * a.page_size;
   const int64_t seq = max(By::index(a.seq_len, b, a.seq_len_dtype), (int64_t)0);
   if (seq > room) q.status |= DFT_STATUS_TABLE;
-  q.before = (int)(min(seq, top) - q.n);
+  q.before = (int)(min(seq, top) - given);
   q.keys = a.num_pages ? (int)min(min(seq, room), top) : 0;
   return q;
 }

@@ -588,7 +588,9 @@ DFT_API int dft_kv_append(const dft_kv_append_args* args, void* stream);
 enum dft_attention_flags { DFT_ATTN_CAUSAL = 1 };
 
 /* Over a paged cache, which holds the new tokens already: request b's n_b
- * rows (row0 as in dft_verify_args) are the last n_b of its seq_len[b] keys.
+ * rows (row0 as in dft_verify_args) are the last n_b of its seq_len[b] keys;
+ * where they are cut, the first ones are left, with the keys they have in the
+ * whole request.
  * Row i sees, with DFT_ATTN_CAUSAL, keys j <= seq_len - n_b + i; with
  * anc_bits (n_new <= 64) the keys before seq_len - n_b and new token j where
  * bit j of its word is set; with neither every key.  A page id outside

@@ -1,0 +1,41 @@
+"""Paged and prompt attention where a request is cut, no row is left, rows belong to nobody, or the launch's bounds are far
+above the work."""
+import pytest
+import torch
+
+from conftest import announce
+from oracle import paged as P
+from test_gpu_attention import BF16, Paged, ancestry, check, dense
+
+pytestmark = pytest.mark.gpu
+
+
+def ints(cuda, x):
+    return torch.tensor(x, dtype=torch.int32, device=cuda)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("kept", [2, 9])
+@pytest.mark.parametrize("tree", [False, True])
+@pytest.mark.parametrize("far", [90, 900])
+def test_a_cut_request_keeps_its_first_rows(cuda, d, kept, tree, far):
+    """They see what they see in the whole request: the rows that are left out still stand behind them."""
+    from dforktree_amd import _lib, ops
+    announce(f"cut to {kept} rows d={d} tree={tree} prefix={far}")
+    sizes = [2, 40, 1]
+    t = Paged(cuda, d, [30, far, 70], sizes, hq=8, hkv=2, d=d, ps=16)
+    bits = ancestry(sizes, 4) if tree else None
+    k, v = t.caches()
+    o = torch.full(t.q.shape, 7.0, dtype=BF16, device=cuda)
+    lse, status = torch.full(t.q.shape[:2], 7.0, device=cuda), ints(cuda, [9] * 3)
+    ops.paged_attention(t.gpu(t.q), k, v, t.gpu(t.table), ints(cuda, t.total), cu_seqlens=t.gpu(t.cu), n_new=kept, o=o, lse=lse,
+                        anc_bits=None if bits is None else t.gpu(bits), status=status)
+    torch.cuda.synchronize()
+    assert status.tolist() == [0, _lib.DFT_STATUS_SPAN, 0]
+    assert (o[2 + kept:42] == 7).all() and (lse[2 + kept:42] == 7).all()
+    for b, n in enumerate(sizes):
+        r0, L, m = int(t.cu[b]), t.total[b], min(n, kept)
+        sees = (P.sees_tree(bits[r0:r0 + n].numpy(), L) if tree else P.sees_causal(n, L))[:m]
+        keys, values = (torch.as_tensor(P.paged_keys(c.float().numpy(), t.table[b].numpy(), L)[0]).double() for c in (t.k, t.v))
+        r = slice(r0, r0 + m)
+        check(o[r], lse[r], dense(t.q[r].double(), keys, values, sees, d ** -0.5), L, BF16, 10.0, f"request {b}")
