@@ -889,6 +889,12 @@ __global__ void __launch_bounds__(64 * kJoinWaves) join_kernel(dft_paged_attenti
   }
 }
 
+// The status words of a launch without rows.
+__global__ void __launch_bounds__(256) status_kernel(dft_paged_attention_args a) {
+  const int b = blockIdx.x * 256 + threadIdx.x;
+  if (b < a.batch) a.status[b] = request<ByLane>(a, b).status;
+}
+
 // The launch's sizes.
 struct Shape {
   int rows;  // of an item: 16, 32 (few_kernel), 128 (many_kernel)
@@ -953,6 +959,11 @@ int launch_type(const dft_paged_attention_args& a, const Shape& s, const Plan& p
 int64_t paged_attention_workspace(const dft_paged_attention_args* a) {
   const Shape s = shape_of(*a);
   return s.heads_bytes + s.parts_bytes;
+}
+
+int launch_paged_status(const dft_paged_attention_args* a, hipStream_t stream) {
+  status_kernel<<<(a->batch + 255) / 256, 256, 0, stream>>>(*a);
+  return hipGetLastError() == hipSuccess ? DFT_OK : DFT_ERR_LAUNCH;
 }
 
 int launch_paged_attention(const dft_paged_attention_args* args, hipStream_t stream) {

@@ -193,6 +193,12 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) prompt_kernel(dft_p
   if (a.lse && half == 0) a.lse[(r0 + i) * a.lse_row_stride + h] = lse_of(w.top, sum);
 }
 
+// The status words of a launch without rows.
+__global__ void __launch_bounds__(256) status_kernel(dft_prompt_attention_args a) {
+  const int b = blockIdx.x * 256 + threadIdx.x;
+  if (b < a.batch) a.status[b] = span_of(a, b).status;
+}
+
 template <int D, class T>
 int launch(const dft_prompt_attention_args& a, hipStream_t stream) {
   const int64_t rows = (int64_t)a.max_len * (a.hq / a.hkv);
@@ -213,6 +219,11 @@ int launch_type(const dft_prompt_attention_args& a, hipStream_t stream) {
 }
 
 }  // namespace
+
+int launch_prompt_status(const dft_prompt_attention_args* a, hipStream_t stream) {
+  status_kernel<<<(a->batch + 255) / 256, 256, 0, stream>>>(*a);
+  return hipGetLastError() == hipSuccess ? DFT_OK : DFT_ERR_LAUNCH;
+}
 
 int launch_prompt_attention(const dft_prompt_attention_args* a, hipStream_t stream) {
   return a->dtype == DFT_BF16 ? launch_type<Bf16>(*a, stream) : launch_type<F16>(*a, stream);

@@ -19,7 +19,9 @@ int launch_page_plan(const dft_page_plan_args* a, hipStream_t stream);
 int launch_kv_append(const dft_kv_append_args* a, hipStream_t stream);
 int launch_paged_attention(const dft_paged_attention_args* a, hipStream_t stream);
 int64_t paged_attention_workspace(const dft_paged_attention_args* a);
+int launch_paged_status(const dft_paged_attention_args* a, hipStream_t stream);
 int launch_prompt_attention(const dft_prompt_attention_args* a, hipStream_t stream);
+int launch_prompt_status(const dft_prompt_attention_args* a, hipStream_t stream);
 }  // namespace dft
 
 namespace {
@@ -303,7 +305,13 @@ int dft_kv_append(const dft_kv_append_args* a, void* stream) {
 
 int dft_paged_attention(const dft_paged_attention_args* a, void* stream) {
   const int st = paged_attention_status(a);
-  if (st != DFT_OK) return st < 0 ? DFT_OK : st;
+  if (st > 0) return st;
+  if (st < 0) {  // no rows: only the status words are left to write
+    if (!a->status || !a->batch) return DFT_OK;
+    if (a->batch > 65535) return DFT_ERR_UNSUPPORTED;
+    if (!a->seq_len || !index_tag(a->seq_len_dtype)) return DFT_ERR_INVALID;
+    return dft::launch_paged_status(a, static_cast<hipStream_t>(stream));
+  }
   const int64_t need = dft::paged_attention_workspace(a);
   if (need > 0 && (!a->workspace || !aligned16(a->workspace) || a->workspace_bytes < need)) return DFT_ERR_INVALID;
   return dft::launch_paged_attention(a, static_cast<hipStream_t>(stream));
@@ -321,7 +329,12 @@ int dft_paged_attention_workspace(const dft_paged_attention_args* a, int64_t* by
 
 int dft_prompt_attention(const dft_prompt_attention_args* a, void* stream) {
   const int st = attention_status(a, a ? a->max_len : 0);
-  if (st != DFT_OK) return st < 0 ? DFT_OK : st;
+  if (st > 0) return st;
+  if (st < 0) {  // no rows: only the status words are left to write
+    if (!a->status || !a->batch) return DFT_OK;
+    if (a->batch > 65535) return DFT_ERR_UNSUPPORTED;
+    return dft::launch_prompt_status(a, static_cast<hipStream_t>(stream));
+  }
   if (!a->k || !a->v || !aligned16(a->k) || !aligned16(a->v)) return DFT_ERR_INVALID;
   if (a->k_row_stride % 8 || a->k_h_stride % 8 || a->v_row_stride % 8 || a->v_h_stride % 8) return DFT_ERR_INVALID;
   // a tile's 64 rows are reached by 32-bit byte offsets from its first

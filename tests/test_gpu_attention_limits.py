@@ -39,3 +39,29 @@ def test_a_cut_request_keeps_its_first_rows(cuda, d, kept, tree, far):
         keys, values = (torch.as_tensor(P.paged_keys(c.float().numpy(), t.table[b].numpy(), L)[0]).double() for c in (t.k, t.v))
         r = slice(r0, r0 + m)
         check(o[r], lse[r], dense(t.q[r].double(), keys, values, sees, d ** -0.5), L, BF16, 10.0, f"request {b}")
+
+
+def test_status_without_rows(cuda):
+    """The status words are written also where there is no row to write."""
+    from dforktree_amd import _lib, ops
+    announce("status without rows")
+    SPAN, TABLE = _lib.DFT_STATUS_SPAN, _lib.DFT_STATUS_TABLE
+    x = torch.zeros(4, 4, 64, dtype=BF16, device=cuda)
+    cache = torch.zeros(3, 16, 2, 64, dtype=BF16, device=cuda)
+    for rows, limit, cu, want in ((4, 0, [0, 0, 3], [0, SPAN]), (0, 3, [0, 0, 3], [0, SPAN]), (0, 0, [0, 0, 0], [0, 0]),
+                                  (4, 0, [2, 1, 1], [SPAN, 0])):
+        for columns, extra in ((2, TABLE), (40, 0)):
+            status = ints(cuda, [99, 99])
+            ops.paged_attention(x[:rows], cache, cache, torch.zeros(2, columns, dtype=torch.int32, device=cuda),
+                                ints(cuda, [5, 100]), cu_seqlens=ints(cuda, cu), n_new=limit, status=status)
+            torch.cuda.synchronize()
+            assert status.tolist() == [want[0], want[1] | extra], (rows, limit, cu, columns)
+        status = ints(cuda, [99, 99])
+        ops.prompt_attention(x[:rows], x[:rows, :2], x[:rows, :2], ints(cuda, cu), max_len=limit, status=status)
+        torch.cuda.synchronize()
+        assert status.tolist() == want, (rows, limit, cu)
+    status = ints(cuda, [99, 99])
+    ops.paged_attention(x[:0], cache, cache, torch.zeros(2, 2, dtype=torch.int32, device=cuda), ints(cuda, [5, 100]),
+                        status=status)  # without cu_seqlens
+    torch.cuda.synchronize()
+    assert status.tolist() == [0, TABLE]
