@@ -968,7 +968,7 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, key_cache: torch.Tensor, value_c
         raise ValueError(f"slots has {n} entries for {k.shape[0]} rows")
     if status is not None and (status.dtype != torch.int32 or status.numel() < 1):
         raise ValueError("status must be an int32 tensor of one entry")
-    if not k.numel() or not n:
+    if not n or not k.shape[1] * k.shape[2]:  # without rows in k and v every entry is one past them
         return
     a.heads, a.head_dim, a.page_size = k.shape[1], k.shape[2], key_cache.shape[1]
     a.src_dtype, a.cache_dtype = _ftag(k, "k"), _ftag(key_cache, "key_cache")
