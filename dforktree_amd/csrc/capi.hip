@@ -82,8 +82,7 @@ int tree_status(const dft_tree_args* a) {
   return DFT_OK;
 }
 
-// Checks that both attention entry points share: heads, types, the rows'
-// 16-byte pieces and the grid.
+// Checks of sizes and types that both attention entry points share; -1: no rows.
 template <class Args>
 int attention_status(const Args* a, int span) {
   if (!a) return DFT_ERR_INVALID;
@@ -96,9 +95,13 @@ int attention_status(const Args* a, int span) {
   if (a->batch > 65535 || a->hq > 65535) return DFT_ERR_UNSUPPORTED;
   // a request's rows times the heads of a group are counted in 31 bits
   if ((int64_t)span * (a->hq / a->hkv) > 0x7fff0000ll) return DFT_ERR_UNSUPPORTED;
-  if (!a->q || !a->o) return DFT_ERR_INVALID;
-  if (!aligned16(a->q) || a->q_row_stride % 8 || a->q_h_stride % 8) return DFT_ERR_INVALID;
   return DFT_OK;
+}
+
+// The rows, which are read in 16-byte pieces.
+template <class Args>
+bool attention_rows(const Args* a) {
+  return a->q && a->o && aligned16(a->q) && a->q_row_stride % 8 == 0 && a->q_h_stride % 8 == 0;
 }
 
 int paged_attention_status(const dft_paged_attention_args* a) {
@@ -109,6 +112,7 @@ int paged_attention_status(const dft_paged_attention_args* a) {
   if (a->anc_bits && a->n_new > 64) return DFT_ERR_UNSUPPORTED;
   if (a->anc_bits && (a->flags & DFT_ATTN_CAUSAL)) return DFT_ERR_INVALID;  // one mask or the other
   if (st < 0) return st;
+  if (!attention_rows(a)) return DFT_ERR_INVALID;
   if (!a->seq_len || !index_tag(a->seq_len_dtype)) return DFT_ERR_INVALID;
   if ((!a->block_table && a->columns) || ((!a->key_cache || !a->value_cache) && a->num_pages)) return DFT_ERR_INVALID;
   if (!aligned16(a->key_cache) || !aligned16(a->value_cache)) return DFT_ERR_INVALID;
@@ -320,7 +324,7 @@ int dft_paged_attention(const dft_paged_attention_args* a, void* stream) {
 int dft_paged_attention_workspace(const dft_paged_attention_args* a, int64_t* bytes) {
   if (!bytes) return DFT_ERR_INVALID;
   *bytes = 0;
-  // the sizes decide: what the pointers hold is not looked at
+  // the sizes decide: the pointers need not be there yet
   const int st = attention_status(a, a ? a->n_new : 0);
   if (st > DFT_OK) return st;
   if (st == DFT_OK) *bytes = dft::paged_attention_workspace(a);
@@ -335,6 +339,7 @@ int dft_prompt_attention(const dft_prompt_attention_args* a, void* stream) {
     if (a->batch > 65535) return DFT_ERR_UNSUPPORTED;
     return dft::launch_prompt_status(a, static_cast<hipStream_t>(stream));
   }
+  if (!attention_rows(a)) return DFT_ERR_INVALID;
   if (!a->k || !a->v || !aligned16(a->k) || !aligned16(a->v)) return DFT_ERR_INVALID;
   if (a->k_row_stride % 8 || a->k_h_stride % 8 || a->v_row_stride % 8 || a->v_h_stride % 8) return DFT_ERR_INVALID;
   // a tile's 64 rows are reached by 32-bit byte offsets from its first
