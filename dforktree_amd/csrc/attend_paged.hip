@@ -908,11 +908,11 @@ Shape shape_of(const dft_paged_attention_args& a) {
   // 138 and 142 us with few_kernel, 158 and 152 with many_kernel
   s.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : 128;
   s.once = rows <= s.rows;  // a key is read for one item only
-  s.uncut = (int64_t)a.columns * a.page_size <= kUncutKeys;
-  if (s.uncut) {
-    s.grid = (int64_t)a.batch * a.hkv * ((rows + s.rows - 1) / s.rows);
-    return s;
-  }
+  // a grid counts work-items, 256 a workgroup, in 32 bits: a large n_new over a
+  // large batch can ask for more, most of them for rows that there are not
+  s.grid = (int64_t)a.batch * a.hkv * ((rows + s.rows - 1) / s.rows);
+  s.uncut = (int64_t)a.columns * a.page_size <= kUncutKeys && s.grid <= 0xffffffffll / 256;
+  if (s.uncut) return s;
   // as many workgroups as the LDS holds: 512 D bytes of tiles each, and a little
   const int room = kCus * (a.head_dim == 256 ? 1 : a.head_dim == 128 ? 2 : 3);
   s.shares = a.hkv < room ? room / a.hkv : 1;
@@ -976,7 +976,6 @@ int launch_paged_attention(const dft_paged_attention_args* args, hipStream_t str
     a->kc_page_stride = a->kc_token_stride = a->kc_h_stride = a->vc_page_stride = a->vc_token_stride = a->vc_h_stride = 0;
   }
   const Shape s = shape_of(*a);
-  if (s.grid > 0xffffffffll / 512) return DFT_ERR_UNSUPPORTED;  // a grid counts work-items in 32 bits
   Plan pl = {};
   pl.heads = static_cast<char*>(a->workspace);
   pl.parts = reinterpret_cast<float*>(pl.heads + s.heads_bytes);

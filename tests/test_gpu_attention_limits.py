@@ -1,5 +1,6 @@
 """Paged and prompt attention where a request is cut, no row is left, rows belong to nobody, or the launch's bounds are far
 above the work."""
+import numpy as np
 import pytest
 import torch
 
@@ -65,3 +66,17 @@ def test_status_without_rows(cuda):
                         status=status)  # without cu_seqlens
     torch.cuda.synchronize()
     assert status.tolist() == [0, TABLE]
+
+
+def test_bounds_far_above_the_rows(cuda):
+    """n_new is a bound: short rows under a long one are served."""
+    from dforktree_amd import ops
+    announce("far bounds")
+    rng = np.random.default_rng(0)
+    prefix, new = [int(x) for x in rng.integers(0, 60, 300)], [int(x) for x in rng.integers(0, 4, 300)]
+    t = Paged(cuda, 0, prefix, new, hq=1, hkv=1, d=64, ps=16)
+    k, v = t.caches()
+    lse = torch.empty(t.rows, 1, device=cuda)
+    o = ops.paged_attention(t.gpu(t.q), k, v, t.gpu(t.table), ints(cuda, t.total), cu_seqlens=t.gpu(t.cu), n_new=1 << 23, lse=lse)
+    torch.cuda.synchronize()
+    t.check(o, lse, what="paged")
