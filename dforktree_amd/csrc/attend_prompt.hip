@@ -199,14 +199,30 @@ __global__ void __launch_bounds__(256) status_kernel(dft_prompt_attention_args a
   if (b < a.batch) a.status[b] = span_of(a, b).status;
 }
 
+// A grid has the row tiles of the longest prompt for every prompt and counts
+// work-items in 32 bits: packed batches that need more go in several launches.
 template <int D, class T>
-int launch(const dft_prompt_attention_args& a, hipStream_t stream) {
-  const int64_t rows = (int64_t)a.max_len * (a.hq / a.hkv);
+int launch(const dft_prompt_attention_args& args, hipStream_t stream) {
   constexpr int NW = 4;
-  const int64_t blocks = (rows + 32 * NW - 1) / (32 * NW) * a.batch * a.hkv;
-  if (blocks > 0xffffffffll / (64 * NW)) return DFT_ERR_UNSUPPORTED;  // a grid counts work-items in 32 bits
-  prompt_kernel<D, NW, T><<<(unsigned)blocks, 64 * NW, 0, stream>>>(a, split_scale(a.scale), vector_out(a));
-  return hipGetLastError() == hipSuccess ? DFT_OK : DFT_ERR_LAUNCH;
+  constexpr int64_t kMost = 0xffffffffll / (64 * NW);
+  dft_prompt_attention_args a = args;
+  if (a.cu_seqlens && a.max_len > a.rows) a.max_len = (int)a.rows;  // longer ones end past the rows and are cut to them
+  const int64_t rows = (int64_t)a.max_len * (a.hq / a.hkv);
+  const int64_t each = (rows + 32 * NW - 1) / (32 * NW) * a.hkv;
+  int64_t per = a.batch;
+  if (per * each > kMost) {
+    per = kMost / each;
+    if (!per || !a.cu_seqlens) return DFT_ERR_UNSUPPORTED;
+  }
+  const Scale scale = split_scale(a.scale);
+  for (int64_t b = 0; b < args.batch; b += per) {
+    a.batch = (int)(args.batch - b < per ? args.batch - b : per);
+    prompt_kernel<D, NW, T><<<(unsigned)(each * a.batch), 64 * NW, 0, stream>>>(a, scale, vector_out(a));
+    if (hipGetLastError() != hipSuccess) return DFT_ERR_LAUNCH;
+    if (a.cu_seqlens) a.cu_seqlens += a.batch;
+    if (a.status) a.status += a.batch;
+  }
+  return DFT_OK;
 }
 
 template <class T>

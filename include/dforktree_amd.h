@@ -633,7 +633,9 @@ DFT_API int dft_paged_attention_workspace(const dft_paged_attention_args* args, 
 /* Over whole packed prompts: rows cu_seqlens[b] .. cu_seqlens[b+1] of q, k
  * and v are request b's tokens; row i sees key j <= i (DFT_ATTN_CAUSAL) or
  * every one.  A request of more than max_len tokens is cut to max_len.  Row
- * strides of k and v from 0 to 2^24 - 8. */
+ * strides of k and v from 0 to 2^24 - 8.  ceil(max_len hq / hkv / 128) hkv
+ * workgroups a request, max_len at most `rows`: below 2^24 of them, without
+ * cu_seqlens below 2^24 for all requests. */
 typedef struct dft_prompt_attention_args {
   int32_t batch, max_len;
   int32_t hq, hkv, head_dim;

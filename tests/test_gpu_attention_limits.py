@@ -6,7 +6,7 @@ import torch
 
 from conftest import announce
 from oracle import paged as P
-from test_gpu_attention import BF16, Paged, ancestry, check, dense
+from test_gpu_attention import BF16, Paged, ancestry, check, check_prompt, dense, prompt
 
 pytestmark = pytest.mark.gpu
 
@@ -80,3 +80,38 @@ def test_bounds_far_above_the_rows(cuda):
     o = ops.paged_attention(t.gpu(t.q), k, v, t.gpu(t.table), ints(cuda, t.total), cu_seqlens=t.gpu(t.cu), n_new=1 << 23, lse=lse)
     torch.cuda.synchronize()
     t.check(o, lse, what="paged")
+
+
+def test_prompt_bounds_far_above_the_rows(cuda):
+    """max_len is a bound: short prompts under a long one are served."""
+    from dforktree_amd import ops
+    announce("far bounds of prompts")
+    rng = np.random.default_rng(0)
+    sizes = [int(x) for x in rng.integers(0, 60, 100)]
+    qkv, want, lse = prompt(cuda, sizes, 4, 4, 64, BF16)
+    check_prompt(qkv, want, lse, sizes, 4, 4, 64, BF16, what="prompts")
+    x = qkv.to(cuda)
+    o = ops.prompt_attention(x[:, :4], x[:, 4:8], x[:, 8:], ints(cuda, [0, *np.cumsum(sizes)]), max_len=1 << 24)
+    torch.cuda.synchronize()
+    assert torch.equal(o, want)
+
+
+def test_one_long_prompt_among_very_many(cuda):
+    """More row tiles (of the longest, for every prompt) than one launch can count."""
+    from dforktree_amd import ops
+    announce("one long prompt among 65535")
+    B, n, hq, hkv, d = 65535, 1100, 32, 8, 64
+    sizes = np.ones(B, int)
+    sizes[B - 3] = n
+    cu = ints(cuda, [0, *np.cumsum(sizes)])
+    g = torch.Generator(device=cuda).manual_seed(1)
+    q, k, v = (torch.randn(int(sizes.sum()), h, d, generator=g, device=cuda).to(BF16) for h in (hq, hkv, hkv))
+    status = torch.full((B,), 9, dtype=torch.int32, device=cuda)
+    o = ops.prompt_attention(q, k, v, cu, max_len=n, status=status)
+    torch.cuda.synchronize()
+    assert not status.any()
+    r = slice(B - 3, B - 3 + n)
+    assert torch.equal(o[r], ops.prompt_attention(q[r], k[r], v[r]))
+    alone = torch.ones(q.shape[0], dtype=torch.bool, device=cuda)
+    alone[r] = False
+    assert torch.equal(o[alone], v[alone].repeat_interleave(hq // hkv, 1))  # one token sees itself
