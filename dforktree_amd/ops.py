@@ -945,7 +945,8 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, key_cache: torch.Tensor, value_c
     rows[i], goes to slot slots[i] (``page_plan``'s), cast to the cache's
     type; a negative slot or row is skipped.  One past the cache or past T is
     skipped as well and sets ``status`` (int32, one entry, never cleared) to
-    1.  No slot may occur twice.  With ``rows`` = the nodes of the accepted
+    1.  No slot may occur twice, and with k and v in the caches' own memory no
+    entry may write what another reads.  With ``rows`` = the nodes of the accepted
     paths (-1 padded) and ``slots`` = the places after their prefixes this
     commits a draft tree's keys and values.
     """
@@ -1050,7 +1051,11 @@ def paged_attention(q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch
     gets o = 0 and lse = -inf.  ``scale`` defaults to d ** -0.5.  ``lse``
     (float32 [rows, hq]) receives the logarithm of each softmax's sum, with
     which outputs over parts of the keys are joined; ``status`` (int32
-    [batch]) DFT_STATUS_SPAN and DFT_STATUS_TABLE bits.  Returns o.
+    [batch]) DFT_STATUS_SPAN and DFT_STATUS_TABLE bits: a request of more than
+    n_new rows is cut to its first n_new, one of more keys than its table has
+    places sees those it has.  Returns o, where rows of no request (behind the
+    last one's, or cut off) keep what a given ``o`` holds and are otherwise
+    uninitialised, as in ``lse``.
     """
     dev = _device_of(q, key_cache, value_cache, block_table, seq_len, cu_seqlens, anc_bits, o, lse)
     _check_cache(key_cache, value_cache)
@@ -1115,8 +1120,8 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     unit-stride views (slices of one projection), hq a multiple of hkv.
     Request b's tokens are rows cu_seqlens[b] .. cu_seqlens[b + 1] (max_len:
     the longest's, on the host) or b * max_len ...; each sees the ones up to
-    itself (``causal``) or all.  ``scale``, ``o``, ``lse`` and ``status`` as in
-    ``paged_attention``.  Returns o.
+    itself (``causal``) or all.  ``scale``, ``o``, ``lse``, ``status`` and rows of
+    no request as in ``paged_attention``.  Returns o.
     """
     dev = _device_of(q, k, v, cu_seqlens, o, lse)
     q, k, v = _aligned_rows(q, "q"), _aligned_rows(k, "k"), _aligned_rows(v, "v")

@@ -70,7 +70,9 @@ class PagedKV:
 
     def attend(self, layer: int, q: torch.Tensor, plan: dict, **kw) -> torch.Tensor:
         """The new rows' attention over their request's tokens, the new ones
-        included: causal, or a tree's where the plan has its anc_bits."""
+        included: causal, or a tree's where the plan has its anc_bits.  Rows
+        past the plan's last (rows above the tokens' total) are uninitialised
+        unless ``o`` is given, a refused request's rows 0."""
         return ops.paged_attention(q, self.keys[layer], self.values[layer], self.block_table, plan["seq_len"],
                                    cu_seqlens=plan["cu_seqlens"], n_new=plan["n_new"], anc_bits=plan["anc_bits"], **kw)
 

@@ -58,8 +58,8 @@ enum dft_status {
 
 enum dft_dtype { DFT_F32 = 0, DFT_BF16 = 1, DFT_F16 = 2, DFT_I32 = 3, DFT_I64 = 4 };
 
-/* Per-request status words (the optional `status` arrays of dft_verify_args
- * and dft_commit_args): every launch writes status[b] for every request b
+/* Per-request status words (the optional `status` arrays of dft_verify_args,
+ * dft_commit_args and the attentions, dft_page_plan's): every launch writes status[b] for every request b
  * (no clearing needed), as a set of these bits; 0 = the request was taken
  * as given. */
 enum dft_request_status {
@@ -548,7 +548,9 @@ DFT_API int dft_page_plan(const dft_page_plan_args* args, void* stream);
 /* New K/V rows into their slots: row rows[i] (or i) of k and v to slot
  * slots[i], cast to the cache's type.  A negative slot or row is skipped; one
  * past the cache or past src_rows is skipped too and sets *status, when
- * given, to 1 (never cleared).  No two entries may name one slot.  The rows
+ * given, to 1 (never cleared).  No two entries may name one slot.  k and v may
+ * lie in the caches' memory (rows moved within a cache) as long as no entry
+ * writes what another reads: entries are taken in no order.  The rows
  * of an accepted path (rows = its nodes, slots = the places after the
  * prefix) make this the KV side of a commit. */
 typedef struct dft_kv_append_args {
@@ -581,7 +583,9 @@ DFT_API int dft_kv_append(const dft_kv_append_args* args, void* stream);
  * a row does not see do not touch it, whatever they hold.
  * Types: q, k, v all bf16 or all fp16, head_dim 64, 128 or 256, unit stride
  * along it; 16-byte aligned q, k and v, their other strides multiples of 8
- * elements.  The outputs' strides are free.  A request's rows times
+ * elements.  The outputs' strides are free; they must not overlap k, v or a
+ * cache.  Rows of o and lse that belong to no request (past the last one's, as
+ * a captured step's padding, or cut off) are not written.  A request's rows times
  * hq / hkv stay below 2^31 - 2^16.  The weights are rounded to the inputs'
  * type for the product with v (fp16's, where that is more than half a step,
  * by 2^-32 of the row's sum); scores, sums and outputs are held in fp32. */

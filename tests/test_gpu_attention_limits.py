@@ -115,3 +115,44 @@ def test_one_long_prompt_among_very_many(cuda):
     alone = torch.ones(q.shape[0], dtype=torch.bool, device=cuda)
     alone[r] = False
     assert torch.equal(o[alone], v[alone].repeat_interleave(hq // hkv, 1))  # one token sees itself
+
+
+def test_rows_of_no_request_are_not_written(cuda):
+    """Rows past the last request (a captured step's padding) keep what they hold."""
+    from dforktree_amd import ops
+    announce("padding rows")
+    t = Paged(cuda, 1, [20, 700], [3, 4], hq=8, hkv=2, d=64, ps=16)
+    q = torch.cat([t.q, torch.full((5, 8, 64), float("nan"), dtype=BF16)]).to(cuda)
+    k, v = t.caches()
+    for n_new, width in ((4, None), (40, None), (4, 32)):
+        o, lse = torch.full(q.shape, 7.0, dtype=BF16, device=cuda), torch.full(q.shape[:2], 7.0, device=cuda)
+        ops.paged_attention(q, k, v, t.gpu(t.table)[:, :width], ints(cuda, t.total), cu_seqlens=t.gpu(t.cu), n_new=n_new, o=o,
+                            lse=lse)
+        torch.cuda.synchronize()
+        assert (o[7:] == 7).all() and (lse[7:] == 7).all() and torch.isfinite(o).all()
+        if width is None:
+            t.check(o, lse, what=f"n_new={n_new}")
+    x = torch.randn(12, 8, 64, device=cuda).to(BF16)
+    o = torch.full((12, 4, 64), 7.0, dtype=BF16, device=cuda)
+    ops.prompt_attention(x[:, :4], x[:, 4:6], x[:, 6:], ints(cuda, [0, 3, 7]), max_len=6, o=o)
+    torch.cuda.synchronize()
+    assert (o[7:] == 7).all() and not (o[:7] == 7).all(-1).any()
+
+
+@pytest.mark.parametrize("new", [[1, 20], [1, 3]])
+def test_far_interleaved_caches(cuda, new):
+    """Keys and values as every other page of one buffer, with a page stride past 2^31 elements."""
+    from dforktree_amd import ops
+    announce(f"far interleaved caches {new}")
+    t = Paged(cuda, 14, [10, 15], new, hq=8, hkv=2, d=128, ps=16, poison=False)
+    pages, page = t.k.shape[0], 16 * 2 * 128
+    step = (1 << 31) + 4 * page
+    buffer = torch.empty((pages - 1) * step + 2 * page, dtype=BF16, device=cuda)
+    k, v = (torch.as_strided(buffer, (pages, 16, 2, 128), (step, 256, 128, 1), at) for at in (0, page))
+    k.copy_(t.gpu(t.k))
+    v.copy_(t.gpu(t.v))
+    lse = torch.empty(t.q.shape[:2], device=cuda)
+    o = ops.paged_attention(t.gpu(t.q), k, v, t.gpu(t.table), ints(cuda, t.total), cu_seqlens=t.gpu(t.cu), n_new=max(new), lse=lse)
+    t.check(o, lse, what="interleaved")
+    del buffer, k, v
+    torch.cuda.empty_cache()

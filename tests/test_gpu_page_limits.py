@@ -30,3 +30,19 @@ def test_lengths_of_any_size(cuda, ps, batch):
     new = [2, TOP, TOP, -TOP - 1, TOP]
     r = compare(cuda, [0, 1, 5, 2, 3], new, table[:5], [0] * 5, free, [9, 9 + len(free)], ps=max(ps, 16), rows=12, index=torch.int64)
     assert r["cu_seqlens"].tolist() == [0, 2, 12, 12, 12, 12] and r["status"].tolist() == [0, 1, 1, 1, 1]
+
+
+@pytest.mark.parametrize("batch", [4097, 8192])
+def test_largest_batches(cuda, batch):
+    """Running sums in more LDS than a launch has without asking, up to the limit."""
+    announce(f"plan of {batch} requests")
+    rng = np.random.default_rng(batch)
+    prefix, new = rng.integers(0, 60, batch), rng.integers(0, 9, batch)
+    held = -(-prefix // 4) + rng.integers(0, 3, batch)
+    table, free = tables(rng, held, 25, 2 * batch)
+    head = 11
+    ring = np.full(int(sum(held)) + len(free), -1, np.int32)
+    ring[(head + np.arange(len(free))) % len(ring)] = free
+    for trim in (False, True):
+        compare(cuda, prefix, new, table, held, ring, [head, head + len(free)], ps=4, rows=int(new.sum()), trim=trim,
+                depth=rng.integers(0, 9, int(new.sum())))
