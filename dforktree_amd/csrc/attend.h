@@ -403,7 +403,7 @@ struct Rows {
   // exceed it by too much.
   __device__ __forceinline__ void settle(float c) {
     constexpr float kMost = T::kBase + T::kSlack;
-    if (!__any(high * c - top > kMost)) return;
+    if (!__any(high * c > top + kMost)) return;
     // row by row: what a row gets does not depend on the others of the wave
     const float new_top = fmaxf(high, __shfl_xor(high, 32)) * c;
     const bool move = new_top - top > kMost;

@@ -82,13 +82,13 @@ template <class By>
 __device__ __forceinline__ Request request(const dft_paged_attention_args& a, int b) {
   Request q;
   q.r0 = a.cu_seqlens ? By::i32(a.cu_seqlens + b) : (int64_t)b * a.n_new;
-  int64_t n = a.cu_seqlens ? (int64_t)By::i32(a.cu_seqlens + b + 1) - q.r0 : a.n_new;
+  const int64_t n = a.cu_seqlens ? (int64_t)By::i32(a.cu_seqlens + b + 1) - q.r0 : a.n_new;
   q.status = n < 0 || n > a.n_new || q.r0 < 0 || q.r0 + n > a.rows ? DFT_STATUS_SPAN : 0;
   // a cut request's rows are its first ones: those cut off stand behind them
   // (up to 2^31 - 2^16 of them, as many as rows can be)
   const int given = (int)min(max(n, (int64_t)0), (int64_t)0x7fff0000);
-  n = q.r0 < 0 ? 0 : min(min(n, (int64_t)a.n_new), a.rows - q.r0);
-  q.n = (int)max(n, (int64_t)0);
+  const int64_t there = q.r0 < 0 ? 0 : max(a.rows - q.r0, (int64_t)0);
+  q.n = min(min(given, a.n_new), (int)min(there, (int64_t)0x7fffffff));
   const int64_t top = 0x7fffffff - kTile, room = (int64_t)a.columns * a.page_size;
   const int64_t seq = max(By::index(a.seq_len, b, a.seq_len_dtype), (int64_t)0);
   if (seq > room) q.status |= DFT_STATUS_TABLE;
@@ -518,7 +518,7 @@ __device__ __forceinline__ void few_tile(uint32_t k, uint32_t v, int wave, const
 #pragma unroll
       for (int r = 0; r < 4; ++r) high = fmaxf(high, s[y][t][r]);
     constexpr float kMost = T::kBase + T::kSlack;
-    if (__any(high * c - top[y] > kMost)) {
+    if (__any(high * c > top[y] + kMost)) {
       high = fmaxf(high, __shfl_xor(high, 16));
       const float new_top = fmaxf(high, __shfl_xor(high, 32)) * c;
       const bool move = new_top - top[y] > kMost;
