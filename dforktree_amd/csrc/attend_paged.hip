@@ -26,10 +26,12 @@ constexpr int kCus = 256, kXcds = 8;
 // heads, d 128: 16.7 us a step of 64, 21.9 of 256); with many its accumulators
 // cost more than that (a tree of 32 nodes over 8000 keys: 38.2 and 33.8 us).
 constexpr int kLeastFew = 64, kLeastMany = 256;
-// An item of at most so many keys is never cut: no scan, no parts, no second
-// launch.  One token each over 470 keys, uncut, and over 500 in a wider table,
-// cut: 1 request 20.4 and 16.9 us, 64 requests 27.3 and 34.6; trees of 32
-// nodes, 1 request 20.3 and 24.4, 16 requests 22.5 and 42.6.
+// Where the whole table holds at most so many keys no item is cut: no scan, no
+// parts, no second launch.  470 keys each in a table of 496, uncut, and in one
+// of 640, cut (8 kv heads, d 128), us a call: one token for 1, 4, 16 and 64
+// requests 18.1, 18.3, 18.6, 27.3 and 16.0, 18.8, 22.7, 30.5; trees of 32 nodes
+// 19.9, 19.9, 21.9, 41.7 and 27.3, 28.3, 32.4, 44.1.  (A single request's token
+// alone is read sooner by more workgroups.)
 constexpr int kUncutKeys = 512;
 
 // What a share that begins inside an item leaves for the join.
@@ -466,7 +468,7 @@ __device__ __forceinline__ uint64_t tree_bits(uint64_t bits, int before, int j0)
 // rows of a decode step) and takes a quarter of the output's columns, so
 // nothing is exchanged between them.  Four tiles' room in the LDS keeps three
 // on their way, 72 to 96 KB a CU: bound by HBM, and HBM by what is on its way.
-// 64 requests of 300 to 8191 keys (8 kv heads, d 128): 178 us, 6.2 TB/s; two
+// 64 requests of 300 to 8191 keys (8 kv heads, d 128): 184 us, 6.0 TB/s; two
 // waves on halves of 64-key tiles two deep took 249, copies without the
 // read-once mark 218.
 constexpr int kFewTile = 32, kFewStages = 4;
@@ -482,7 +484,7 @@ __device__ __forceinline__ typename T::x8 few_value(uint32_t v, int columns) {
 }
 
 // One tile for NQ x 16 rows (lane l: row l % 16) and the wave's DT x 16
-// columns.  As Rows::tile, on 16 x 16 products.
+// columns.  As Rows::scores and Rows::step, on 16 x 16 products.
 template <int D, int NQ, int DT, class T>
 __device__ __forceinline__ void few_tile(uint32_t k, uint32_t v, int wave, const typename T::x8 (&q)[NQ][D / 32],
                                          f32x4 (&o)[NQ][DT], float (&top)[NQ], float (&sum)[NQ], float c, bool partial,
@@ -708,7 +710,10 @@ __global__ void __launch_bounds__(256) few_kernel(dft_paged_attention_args a, Sc
 // products and everything else then overlap within the wave only.  32-node
 // trees of 64 requests over 500 to 4000 keys (8 kv heads, d 128): 148 us,
 // 4.3 TB/s and 510 TFLOP/s, 16 more for the join; chunks of 777 and 1024 rows
-// over 9000 to 15001 keys (2 kv heads, d 256): 410 us, 870 TFLOP/s.
+// over 9000 to 15001 keys (2 kv heads, d 256): 430 us with the join's 16, 820
+// TFLOP/s (the profiler makes it 444 to 462 and 16).  Some 50 of them pass
+// before the first key: one thread walks a request's row tiles (Walk::begin),
+// which takes 500 us of a chunk of 16384 tokens, 8 heads each, out of 3880.
 template <int D, int NW, int KT, int STAGES, bool ONCE, class T>
 __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) many_kernel(dft_paged_attention_args a, Scale sc, Plan pl) {
   constexpr int BM = 32 * NW;
@@ -913,7 +918,11 @@ Shape shape_of(const dft_paged_attention_args& a) {
   s.grid = (int64_t)a.batch * a.hkv * ((rows + s.rows - 1) / s.rows);
   s.uncut = (int64_t)a.columns * a.page_size <= kUncutKeys && s.grid <= 0xffffffffll / 256;
   if (s.uncut) return s;
-  // as many workgroups as the LDS holds: 512 D bytes of tiles each, and a little
+  // As many workgroups as a CU takes at once with 256 and 128 columns, whose
+  // tiles are 512 D bytes of the LDS each.  With 64 columns three, between two
+  // (as many as many_kernel's registers allow) and four (as the LDS does), for
+  // a token of 64 requests 137 us (153 and 128), one of 60000 keys 40 (45 and
+  // 45), 32-node trees 138 (115 and 131), 8-node ones 99 (102 and 108).
   const int room = kCus * (a.head_dim == 256 ? 1 : a.head_dim == 128 ? 2 : 3);
   s.shares = a.hkv < room ? room / a.hkv : 1;
   s.grid = (s.shares * a.hkv + kXcds - 1) / kXcds * kXcds;

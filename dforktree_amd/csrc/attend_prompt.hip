@@ -6,7 +6,7 @@
 // before's weights, so its keys come a tile earlier than its values; the LDS
 // holds two tiles of either, one in use, one on its way.  With 128 columns two
 // workgroups of four waves share a CU; eight waves on one tile gave 524 us for
-// 513.  One prompt of 8192 (32 heads, 8 kv heads, d 128, causal): 506 us, 1.09
+// 513.  One prompt of 8192 (32 heads, 8 kv heads, d 128, causal): 515 us, 1.07
 // PFLOP/s, the matrix unit busy 63% of the time at the 1.8 GHz that the card's
 // power leaves.
 #include "attend.h"

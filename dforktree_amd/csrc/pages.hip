@@ -3,9 +3,9 @@
 //                   lengths, pages taken from and returned to a ring
 //   dft_kv_append   new K/V rows (or an accepted path's) into their slots
 //
-// Neither computes: the plan is bound by the latency of its look-ups (6 us for
-// 64 requests, 7.2 for 4608 rows of 128, 12 for 256000 of 1000), the append by
-// HBM (16387 rows of 8 heads x 128: 21.8 us, 6.1 TB/s).
+// Neither computes: the plan is bound by the latency of its look-ups (5.6 us
+// for 64 requests, 7.1 for 4608 rows of 128, 11.9 for 256000 of 1000), the append
+// by HBM (16387 rows of 8 heads x 128: 21.6 us, 6.2 TB/s).
 #include <stdint.h>
 
 #include "dft_device.h"
