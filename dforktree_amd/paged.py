@@ -55,11 +55,13 @@ class PagedKV:
         """Room for new_len[b] tokens behind every request's prefix
         (``ops.page_plan``): rows, their total or more, and n_new, the most of
         one request, are known on the host.  ``trim`` first returns the pages
-        that a rejected draft left; ``depth`` and ``anc_bits`` are a draft
+        that a rejected draft left, and all of a request that has ended (its
+        prefix set to 0, nothing new); ``depth`` and ``anc_bits`` are a draft
         tree's (``ops.tree_struct``)."""
         p = ops.page_plan(self.prefix, new_len, self.block_table, self.held, self.free_pages, self.free_pos,
                           page_size=self.page_size, rows=rows, trim=trim, depth=depth)
-        torch.sub(p["seq_len"], self.prefix, out=self.served).clamp_(min=0)  # a refused request's seq_len is 0
+        p["served"] = (p["seq_len"] - self.prefix).clamp_(min=0)  # a refused request's seq_len is 0
+        self.served.copy_(p["served"])
         self.held.copy_(p["held"])
         self.free_pos.copy_(p["free_pos"])
         return p | {"n_new": n_new, "anc_bits": anc_bits}
@@ -88,9 +90,11 @@ class PagedKV:
         slots = plan["slots"][at.clamp_max(plan["slots"].numel() - 1)]
         ops.kv_append(k, v, self.keys[layer], self.values[layer], torch.where(at < cu[1:, None], slots, -1), rows=path)
 
-    def commit(self, length: torch.Tensor) -> None:
+    def commit(self, length: torch.Tensor, plan: Optional[dict] = None) -> None:
         """The prefixes grow by length[b] of the step's tokens, as far as the
-        plan gave them places: none of a refused request's."""
-        length = torch.minimum(length, self.served)
+        last plan gave them places: none of a refused request's.  With several
+        plans in a step every commit names its ``plan``."""
+        left = self.served if plan is None else plan["served"]
+        length = torch.minimum(length, left)
         self.prefix += length
-        self.served -= length
+        left -= length

@@ -112,3 +112,17 @@ def test_a_step_without_rows(make):
     kv.accept(0, marks(), marks(), plan, torch.full((2, 3), -1))
     kv.commit(ints(0, 0))
     assert not kv.keys.any() and kv.prefix.tolist() == [0, 0]
+
+
+def test_two_plans_of_one_step(make):
+    """A prompt and a single token planned apart: each plan says what is to be committed of it."""
+    kv = make(1, 2, 4, 9, 4)
+    prompt = kv.plan(ints(6, 0), rows=6, n_new=6)
+    token = kv.plan(ints(0, 1), rows=1, n_new=1)
+    kv.append(0, *[marks(10, 11, 12, 13, 14, 15)] * 2, prompt)
+    kv.append(0, *[marks(20)] * 2, token)
+    kv.commit(ints(6, 0), prompt)
+    kv.commit(ints(0, 1), token)
+    assert tokens(kv, 0) == [10, 11, 12, 13, 14, 15] and tokens(kv, 1) == [20]
+    kv.commit(ints(6, 0), prompt)
+    assert kv.prefix.tolist() == [6, 1]
