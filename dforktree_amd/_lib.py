@@ -16,6 +16,7 @@ DFT_F32, DFT_BF16, DFT_F16, DFT_I32, DFT_I64 = 0, 1, 2, 3, 4
 DFT_VERIFY_AUX_K_PER_KHEAD = 1
 DFT_COMMIT_KV, DFT_COMMIT_CHECK_ANC, DFT_COMMIT_LEN_IS_LAST = 1, 2, 4
 DFT_STATUS_SPAN, DFT_STATUS_PATH, DFT_STATUS_WALK, DFT_STATUS_PAGES, DFT_STATUS_TABLE = 1, 2, 4, 8, 16
+DFT_STATUS_SLOT, DFT_STATUS_WEIGHT = 32, 64
 DFT_ATTN_CAUSAL = 1
 ABI_VERSION = 5
 
@@ -206,13 +207,66 @@ class PromptAttentionArgs(C.Structure):
     ]
 
 
+class PromptConvArgs(C.Structure):
+    _fields_ = [
+        ("batch", i32), ("max_len", i32), ("channels", i32), ("width", i32), ("silu", i32),
+        ("rows", i64), ("slots", i64),
+        ("x", vp), ("x_row_stride", i64), ("x_dtype", i32),
+        ("cu_seqlens", vp),
+        ("conv_state", vp), ("cs_slot_stride", i64), ("cs_chan_stride", i64), ("cs_col_stride", i64),
+        ("cs_dtype", i32),
+        ("cs_indices", vp), ("cs_indices_dtype", i32),
+        ("initial", vp),
+        ("weight", vp), ("w_chan_stride", i64), ("w_tap_stride", i64), ("w_dtype", i32),
+        ("bias", vp), ("bias_dtype", i32),
+        ("y", vp), ("y_row_stride", i64), ("y_dtype", i32),
+        ("status", vp),
+    ]
+
+
+class PromptGdnArgs(C.Structure):
+    _fields_ = [
+        ("batch", i32), ("max_len", i32), ("hk", i32), ("hv", i32), ("dk", i32), ("dv", i32),
+        ("scale", f32),
+        ("rows", i64), ("slots", i64),
+        ("y", vp), ("y_row_stride", i64), ("cu_seqlens", vp),
+        ("a", vp), ("a_row_stride", i64), ("a_dtype", i32),
+        ("b", vp), ("b_row_stride", i64), ("b_dtype", i32),
+        ("A_log", vp), ("A_log_dtype", i32),
+        ("dt_bias", vp), ("dt_bias_dtype", i32),
+        ("neg_exp_A", vp),
+        ("state", vp), ("state_slot_stride", i64), ("state_h_stride", i64),
+        ("state_k_stride", i64), ("state_v_stride", i64),
+        ("state_indices", vp), ("state_indices_dtype", i32),
+        ("initial", vp),
+        ("o", vp), ("o_row_stride", i64), ("o_h_stride", i64), ("o_dtype", i32),
+        ("status", vp), ("workspace", vp), ("workspace_bytes", i64),
+    ]
+
+
+class TreeAcceptArgs(C.Structure):
+    _fields_ = [
+        ("batch", i32), ("n_nodes", i32), ("vocab", i32), ("path_cols", i32),
+        ("rows", i64),
+        ("cu_seqlens", vp),
+        ("tokens", vp), ("tokens_dtype", i32),
+        ("parent", vp), ("parent_dtype", i32),
+        ("probs", vp), ("probs_row_stride", i64), ("probs_dtype", i32),
+        ("draft_probs", vp), ("draft_row_stride", i64), ("draft_dtype", i32),
+        ("uniform", vp), ("last", vp),
+        ("path", vp), ("path_len", vp), ("path_rows", vp), ("token", vp),
+        ("status", vp), ("workspace", vp), ("workspace_bytes", i64),
+    ]
+
+
 DFT_BITS_LITTLE, DFT_BITS_BIG = 0, 1
 
 EXPORTS = ("dft_tree_verify", "dft_tree_commit_verify", "dft_tree_conv", "dft_tree_commit", "dft_tree_struct",
            "dft_tree_struct_filled",
            "dft_anc_pack", "dft_block_inverse", "dft_packbits", "dft_tree_mask_pack", "dft_size_order",
            "dft_page_plan", "dft_kv_append", "dft_paged_attention", "dft_paged_attention_workspace",
-           "dft_prompt_attention",
+           "dft_prompt_attention", "dft_prompt_conv", "dft_prompt_gdn", "dft_prompt_gdn_workspace",
+           "dft_tree_accept", "dft_tree_accept_workspace",
            "dft_error_string", "dft_abi_version")
 
 
@@ -252,6 +306,11 @@ def load() -> C.CDLL:
                        ("dft_paged_attention", [C.POINTER(PagedAttentionArgs), vp]),
                        ("dft_paged_attention_workspace", [C.POINTER(PagedAttentionArgs), C.POINTER(i64)]),
                        ("dft_prompt_attention", [C.POINTER(PromptAttentionArgs), vp]),
+                       ("dft_prompt_conv", [C.POINTER(PromptConvArgs), vp]),
+                       ("dft_prompt_gdn", [C.POINTER(PromptGdnArgs), vp]),
+                       ("dft_prompt_gdn_workspace", [C.POINTER(PromptGdnArgs), C.POINTER(i64)]),
+                       ("dft_tree_accept", [C.POINTER(TreeAcceptArgs), vp]),
+                       ("dft_tree_accept_workspace", [C.POINTER(TreeAcceptArgs), C.POINTER(i64)]),
                        ("dft_block_inverse", [vp, i32, i32, i64, vp]),
                        ("dft_size_order", [vp, i32, i32, vp, vp])):
         fn = getattr(lib, name)

@@ -22,6 +22,13 @@ int64_t paged_attention_workspace(const dft_paged_attention_args* a);
 int launch_paged_status(const dft_paged_attention_args* a, hipStream_t stream);
 int launch_prompt_attention(const dft_prompt_attention_args* a, hipStream_t stream);
 int launch_prompt_status(const dft_prompt_attention_args* a, hipStream_t stream);
+int launch_prompt_conv(const dft_prompt_conv_args* a, hipStream_t stream);
+int64_t prompt_conv_blocks(const dft_prompt_conv_args* a);
+int launch_prompt_gdn(const dft_prompt_gdn_args* a, hipStream_t stream);
+int64_t prompt_gdn_blocks(const dft_prompt_gdn_args* a);
+int64_t prompt_gdn_workspace(const dft_prompt_gdn_args* a);
+int launch_tree_accept(const dft_tree_accept_args* a, hipStream_t stream);
+int64_t tree_accept_workspace(const dft_tree_accept_args* a);
 }  // namespace dft
 
 namespace {
@@ -120,6 +127,26 @@ int paged_attention_status(const dft_paged_attention_args* a) {
       a->vc_token_stride % 8 || a->vc_h_stride % 8)
     return DFT_ERR_INVALID;
   return DFT_OK;
+}
+
+// Sizes and types of the packed entry points (as verify_status).
+int prompt_gdn_sizes(const dft_prompt_gdn_args* a) {
+  if (!a) return DFT_ERR_INVALID;
+  if (a->batch < 0 || a->max_len < 0 || a->rows < 0 || a->slots < 0) return DFT_ERR_INVALID;
+  if (a->hk <= 0 || a->hv <= 0 || a->hv % a->hk != 0) return DFT_ERR_INVALID;
+  if (a->dk != 128 || a->dv != 128) return DFT_ERR_UNSUPPORTED;
+  if (a->batch == 0) return -1;
+  // cu_seqlens counts rows in 32 bits
+  if (a->rows > 0x7fffffffll || dft::prompt_gdn_blocks(a) > max_blocks(256)) return DFT_ERR_UNSUPPORTED;
+  return DFT_OK;
+}
+
+int tree_accept_sizes(const dft_tree_accept_args* a) {
+  if (!a) return DFT_ERR_INVALID;
+  if (a->batch < 0 || a->n_nodes < 0 || a->vocab < 0 || a->rows < 0 || a->path_cols < 1) return DFT_ERR_INVALID;
+  if (a->n_nodes > 64 || a->path_cols > 64) return DFT_ERR_UNSUPPORTED;
+  if (a->batch > 65535 || a->rows > 0x7fffffffll) return DFT_ERR_UNSUPPORTED;
+  return a->batch == 0 ? -1 : DFT_OK;
 }
 
 }  // namespace
@@ -346,6 +373,66 @@ int dft_prompt_attention(const dft_prompt_attention_args* a, void* stream) {
   if (a->k_row_stride < 0 || a->v_row_stride < 0) return DFT_ERR_INVALID;
   if (a->k_row_stride >= 1 << 24 || a->v_row_stride >= 1 << 24) return DFT_ERR_UNSUPPORTED;
   return dft::launch_prompt_attention(a, static_cast<hipStream_t>(stream));
+}
+
+int dft_prompt_conv(const dft_prompt_conv_args* a, void* stream) {
+  if (!a) return DFT_ERR_INVALID;
+  if (a->batch < 0 || a->max_len < 0 || a->channels < 0 || a->rows < 0 || a->slots < 0) return DFT_ERR_INVALID;
+  if (a->width < 1 || a->width > 8) return DFT_ERR_UNSUPPORTED;
+  if (!float_tag(a->x_dtype) || !float_tag(a->cs_dtype) || !float_tag(a->w_dtype) || !float_tag(a->y_dtype))
+    return DFT_ERR_INVALID;
+  if (a->bias && !float_tag(a->bias_dtype)) return DFT_ERR_INVALID;
+  if (a->cs_indices && !index_tag(a->cs_indices_dtype)) return DFT_ERR_INVALID;
+  if (a->batch == 0 || a->channels == 0) return DFT_OK;
+  if (a->rows > 0x7fffffffll || dft::prompt_conv_blocks(a) > max_blocks(256)) return DFT_ERR_UNSUPPORTED;
+  if (!a->weight || (a->rows && (!a->x || !a->y)) || (a->slots && a->width > 1 && !a->conv_state)) return DFT_ERR_INVALID;
+  return dft::launch_prompt_conv(a, static_cast<hipStream_t>(stream));
+}
+
+int dft_prompt_gdn(const dft_prompt_gdn_args* a, void* stream) {
+  const int st = prompt_gdn_sizes(a);
+  if (st != DFT_OK) return st < 0 ? DFT_OK : st;
+  if (!float_tag(a->a_dtype) || !float_tag(a->b_dtype) || !float_tag(a->dt_bias_dtype) || !float_tag(a->o_dtype) ||
+      (!a->neg_exp_A && !float_tag(a->A_log_dtype)))
+    return DFT_ERR_INVALID;
+  if (a->state_indices && !index_tag(a->state_indices_dtype)) return DFT_ERR_INVALID;
+  if (a->rows && (!a->y || !a->a || !a->b || !a->o)) return DFT_ERR_INVALID;
+  if ((!a->neg_exp_A && !a->A_log) || !a->dt_bias || (a->slots && !a->state)) return DFT_ERR_INVALID;
+  // q/k/v rows are read as 16-byte pieces
+  if (!aligned16(a->y) || a->y_row_stride % 8 != 0) return DFT_ERR_INVALID;
+  const int64_t need = dft::prompt_gdn_workspace(a);
+  if (need > 0 && (!a->workspace || !aligned16(a->workspace) || a->workspace_bytes < need)) return DFT_ERR_INVALID;
+  return dft::launch_prompt_gdn(a, static_cast<hipStream_t>(stream));
+}
+
+int dft_prompt_gdn_workspace(const dft_prompt_gdn_args* a, int64_t* bytes) {
+  if (!bytes) return DFT_ERR_INVALID;
+  *bytes = 0;
+  const int st = prompt_gdn_sizes(a);
+  if (st > DFT_OK) return st;
+  if (st == DFT_OK) *bytes = dft::prompt_gdn_workspace(a);
+  return DFT_OK;
+}
+
+int dft_tree_accept(const dft_tree_accept_args* a, void* stream) {
+  const int st = tree_accept_sizes(a);
+  if (st != DFT_OK) return st < 0 ? DFT_OK : st;
+  if (!index_tag(a->tokens_dtype) || !index_tag(a->parent_dtype) || !float_tag(a->probs_dtype)) return DFT_ERR_INVALID;
+  if (a->draft_probs && !float_tag(a->draft_dtype)) return DFT_ERR_INVALID;
+  if (a->rows && (!a->tokens || !a->parent || !a->uniform || (a->vocab && !a->probs))) return DFT_ERR_INVALID;
+  if (!a->last || !a->path || !a->path_len || !a->path_rows || !a->token) return DFT_ERR_INVALID;
+  const int64_t need = dft::tree_accept_workspace(a);
+  if (need > 0 && (!a->workspace || !aligned16(a->workspace) || a->workspace_bytes < need)) return DFT_ERR_INVALID;
+  return dft::launch_tree_accept(a, static_cast<hipStream_t>(stream));
+}
+
+int dft_tree_accept_workspace(const dft_tree_accept_args* a, int64_t* bytes) {
+  if (!bytes) return DFT_ERR_INVALID;
+  *bytes = 0;
+  const int st = tree_accept_sizes(a);
+  if (st > DFT_OK) return st;
+  if (st == DFT_OK) *bytes = dft::tree_accept_workspace(a);
+  return DFT_OK;
 }
 
 }  // extern "C"

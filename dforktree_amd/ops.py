@@ -22,7 +22,8 @@ import torch
 from . import _lib
 from ._lib import (DFT_BF16, DFT_BITS_BIG, DFT_BITS_LITTLE, DFT_F16, DFT_F32, DFT_I32, DFT_I64, AncPackArgs,
                    CommitArgs, ConvArgs, KvAppendArgs, MaskArgs, PackbitsArgs, PagedAttentionArgs, PagePlanArgs,
-                   PendingArgs, PromptAttentionArgs, TreeArgs, VerifyArgs, check, load)
+                   PendingArgs, PromptAttentionArgs, PromptConvArgs, PromptGdnArgs, TreeAcceptArgs, TreeArgs,
+                   VerifyArgs, check, load)
 
 _FLOAT_TAG = {torch.float32: DFT_F32, torch.bfloat16: DFT_BF16, torch.float16: DFT_F16}
 _INDEX_TAG = {torch.int32: DFT_I32, torch.int64: DFT_I64}
@@ -1009,7 +1010,7 @@ def _attention_out(q, o, lse, dev):
     return o
 
 
-def _packed_rows(cu_seqlens, rows, limit, name, batch):
+def _packed_rows(cu_seqlens, rows, limit, name, batch, of="q"):
     """(cu_seqlens, batch, rows of the longest request) of packed or uniform rows."""
     if cu_seqlens is not None:
         if cu_seqlens.dtype != torch.int32:
@@ -1026,7 +1027,7 @@ def _packed_rows(cu_seqlens, rows, limit, name, batch):
     if limit is None:
         limit = rows // max(batch, 1)
     if batch * limit > rows:
-        raise ValueError(f"{batch} requests of {limit} rows exceed the {rows} rows of q")
+        raise ValueError(f"{batch} requests of {limit} rows exceed the {rows} rows of {of}")
     return None, batch, limit
 
 
@@ -1150,3 +1151,260 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     a.status = _status_ptr(status, batch, dev)
     check("dft_prompt_attention", load().dft_prompt_attention(C.byref(a), _stream(dev)))
     return o
+
+
+# ---------------------------------------------------------------------------
+# a GDN layer over prompts and single tokens
+# ---------------------------------------------------------------------------
+def _initial(initial, batch):
+    """The [batch] flags of the requests that go on from their slot, as bytes."""
+    if initial is None:
+        return None
+    if initial.dtype not in (torch.bool, torch.uint8):
+        raise TypeError(f"initial must be bool or uint8, got {initial.dtype}")
+    if initial.numel() != batch:
+        raise ValueError(f"initial has {initial.numel()} entries for {batch} requests")
+    return initial.contiguous()
+
+
+def _pool_slots(indices, name, batch, pool, pool_name):
+    """(indices, their tag) of a pool that every request's state is written back to."""
+    if any(n > 1 and s == 0 for n, s in zip(pool.shape, pool.stride())):
+        raise ValueError(f"{pool_name} must not be expanded (it is updated in place)")
+    at, tag = _idx_vec(indices, name)
+    if at is not None and at.numel() != batch:
+        raise ValueError(f"{name} has {at.numel()} entries for {batch} requests")
+    if at is None and pool.shape[0] < batch:
+        raise ValueError(f"{pool_name} has {pool.shape[0]} slots for {batch} requests")
+    return at, tag
+
+
+def prompt_conv(x: torch.Tensor, conv_state: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
+                cu_seqlens: Optional[torch.Tensor] = None, *, max_len: Optional[int] = None,
+                batch: Optional[int] = None, silu: bool = True, cs_indices: Optional[torch.Tensor] = None,
+                initial: Optional[torch.Tensor] = None, y: Optional[torch.Tensor] = None,
+                status: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Causal conv1d in front of a GDN layer, over packed prompts or single
+    tokens (``dft_prompt_conv``).
+
+    x [rows, C] pre-conv tokens, channel stride 1; weight [C, W], W 1 to 8;
+    bias [C] or None; conv_state [slots, C, >= W-1], any strides: its first
+    W-1 columns are the inputs in front of a request's first row, and are left
+    holding its last ones.  Request b's rows are cu_seqlens[b] ..
+    cu_seqlens[b + 1] (max_len: the longest's, on the host) or b * max_len ...
+    (one token each: max_len 1).  It goes on from slot cs_indices[b] (or b),
+    or where ``initial`` [batch] bool is given and False from zeros; a negative
+    slot (a padded request) starts from zeros and is not written.  No two
+    requests may have one slot.  Writes y [rows, C] (x.dtype by default), which
+    must not overlap x; rows of no request (behind the last one's, or cut off)
+    keep what a given ``y`` holds and are otherwise uninitialised.  ``status``
+    (int32 [batch]) receives DFT_STATUS_SPAN (cut to max_len or to the rows
+    there are) and DFT_STATUS_SLOT bits (a slot past the pool: taken as a
+    negative one).  Returns y.
+    """
+    dev = _device_of(x, conv_state, weight, bias, cu_seqlens, cs_indices, initial, y, status)
+    if x.dim() != 2 or (x.stride(1) != 1 and x.shape[1] > 1):
+        raise ValueError("x must be [rows, channels] with channel stride 1")
+    rows, Cn = x.shape
+    if weight.dim() != 2 or weight.shape[0] != Cn:
+        raise ValueError(f"weight must be [C, W] = [{Cn}, W]")
+    W = weight.shape[1]
+    if bias is not None and (bias.numel() != Cn or not bias.is_contiguous()):
+        raise ValueError(f"bias must be a contiguous [{Cn}]")
+    if conv_state.dim() != 3 or conv_state.shape[1] != Cn or conv_state.shape[2] < W - 1:
+        raise ValueError(f"conv_state must be [slots, {Cn}, >= {W - 1}], got {tuple(conv_state.shape)}")
+    cu, batch, max_len = _packed_rows(cu_seqlens, rows, max_len, "max_len", batch, "x")
+    at, at_tag = _pool_slots(cs_indices, "cs_indices", batch, conv_state, "conv_state")
+    initial = _initial(initial, batch)
+    if y is None:
+        y = torch.empty(rows, Cn, device=dev, dtype=x.dtype)
+    elif y.shape != x.shape or (y.stride(1) != 1 and Cn > 1):
+        raise ValueError(f"y must be {tuple(x.shape)} with channel stride 1")
+    elif rows and Cn and y.data_ptr() == x.data_ptr():
+        raise ValueError("y must not be x's memory")
+    a = PromptConvArgs()
+    a.batch, a.max_len, a.channels, a.width, a.silu = batch, max_len, Cn, W, int(bool(silu))
+    a.rows, a.slots = rows, conv_state.shape[0]
+    a.x, a.x_row_stride, a.x_dtype = x.data_ptr(), x.stride(0), _ftag(x, "x")
+    a.cu_seqlens = _ptr(cu)
+    a.conv_state, a.cs_slot_stride, a.cs_chan_stride, a.cs_col_stride = conv_state.data_ptr(), *conv_state.stride()
+    a.cs_dtype = _ftag(conv_state, "conv_state")
+    a.cs_indices, a.cs_indices_dtype = _ptr(at), at_tag
+    a.initial = _ptr(initial)
+    a.weight, a.w_chan_stride, a.w_tap_stride, a.w_dtype = weight.data_ptr(), *weight.stride(), _ftag(weight, "weight")
+    if bias is not None:
+        a.bias, a.bias_dtype = bias.data_ptr(), _ftag(bias, "bias")
+    a.y, a.y_row_stride, a.y_dtype = y.data_ptr(), y.stride(0), _ftag(y, "y")
+    a.status = _status_ptr(status, batch, dev)
+    check("dft_prompt_conv", load().dft_prompt_conv(C.byref(a), _stream(dev)))
+    return y
+
+
+def prompt_gdn(y: torch.Tensor, a: torch.Tensor, b: torch.Tensor, A_log: Optional[torch.Tensor],
+               dt_bias: torch.Tensor, state: torch.Tensor, cu_seqlens: Optional[torch.Tensor] = None, *, hk: int,
+               hv: int, max_len: Optional[int] = None, batch: Optional[int] = None, scale: Optional[float] = None,
+               neg_exp_A: Optional[torch.Tensor] = None, state_indices: Optional[torch.Tensor] = None,
+               initial: Optional[torch.Tensor] = None, o: Optional[torch.Tensor] = None,
+               o_dtype: Optional[torch.dtype] = None, status: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The gated delta rule over packed prompts (``dft_prompt_gdn``): what a
+    tree step verifies on, or a chunk of a long prompt.
+
+    y [rows, 2*hk*128 + hv*128] bf16 with channel stride 1 (``prompt_conv``'s);
+    a, b [rows, hv]; A_log (or neg_exp_A = -exp(A_log), float32), dt_bias [hv];
+    state float32 [slots, hv, dk, dv] (index k, v; any strides -- pass
+    ``pool.transpose(-1, -2)`` for a V-major pool), updated in place.  Rows of
+    request b, its slot state_indices[b] (or b), ``initial`` and ``status`` as in
+    ``prompt_conv``.  Returns o [rows, hv, 128], where rows of no request keep
+    what a given ``o`` holds and are otherwise uninitialised.
+    """
+    dev = _device_of(y, a, b, A_log, dt_bias, state, cu_seqlens, neg_exp_A, state_indices, initial, o, status)
+    if y.dim() != 2 or y.stride(1) != 1:
+        raise ValueError("y must be [rows, channels] with channel stride 1")
+    if y.dtype != torch.bfloat16:
+        raise TypeError("y must be bfloat16")
+    rows = y.shape[0]
+    if hk < 1 or hv < 1 or hv % hk:
+        raise ValueError(f"hv must be a multiple of hk, got {hv} and {hk}")
+    if y.shape[1] < (2 * hk + hv) * D_HEAD:
+        raise ValueError(f"y has {y.shape[1]} channels, need {(2 * hk + hv) * D_HEAD}")
+    if y.data_ptr() % 16 or y.stride(0) % 8:  # read as 16-byte pieces, as in _verify_args
+        pitch = -(-y.shape[1] // 8) * 8
+        y = torch.empty(rows, pitch, device=dev, dtype=y.dtype)[:, :y.shape[1]].copy_(y)
+    for t, nm in ((a, "a"), (b, "b")):
+        if t.dim() != 2 or t.shape[0] < rows or t.shape[1] < hv or (t.stride(1) != 1 and hv > 1):
+            raise ValueError(f"{nm} must be [{rows}, {hv}] with stride 1 along heads")
+    if A_log is None and neg_exp_A is None:
+        raise ValueError("give A_log or neg_exp_A")
+    for t, nm in ((A_log, "A_log"), (dt_bias, "dt_bias"), (neg_exp_A, "neg_exp_A")):
+        if t is not None and (t.numel() < hv or not t.is_contiguous()):
+            raise ValueError(f"{nm} must be a contiguous [{hv}]")
+    if neg_exp_A is not None and neg_exp_A.dtype != torch.float32:
+        raise TypeError("neg_exp_A must be float32")
+    if state.dtype != torch.float32:
+        raise TypeError("state must be float32")
+    if state.dim() != 4 or tuple(state.shape[1:]) != (hv, D_HEAD, D_HEAD):
+        raise ValueError(f"state must be [slots, {hv}, 128, 128], got {tuple(state.shape)}")
+    cu, batch, max_len = _packed_rows(cu_seqlens, rows, max_len, "max_len", batch, "y")
+    at, at_tag = _pool_slots(state_indices, "state_indices", batch, state, "state")
+    initial = _initial(initial, batch)
+    if o is None:
+        o = torch.empty(rows, hv, D_HEAD, device=dev, dtype=o_dtype or y.dtype)
+    elif tuple(o.shape) != (rows, hv, D_HEAD) or o.stride(2) != 1:
+        raise ValueError(f"o must be [{rows}, {hv}, 128] with stride 1 along dv")
+    args = PromptGdnArgs()
+    args.batch, args.max_len, args.hk, args.hv = batch, max_len, hk, hv
+    args.dk = args.dv = D_HEAD
+    args.scale = D_HEAD ** -0.5 if scale is None else float(scale)
+    args.rows, args.slots = rows, state.shape[0]
+    args.y, args.y_row_stride, args.cu_seqlens = y.data_ptr(), y.stride(0), _ptr(cu)
+    args.a, args.a_row_stride, args.a_dtype = a.data_ptr(), a.stride(0), _ftag(a, "a")
+    args.b, args.b_row_stride, args.b_dtype = b.data_ptr(), b.stride(0), _ftag(b, "b")
+    if A_log is not None:
+        args.A_log, args.A_log_dtype = A_log.data_ptr(), _ftag(A_log, "A_log")
+    args.dt_bias, args.dt_bias_dtype = dt_bias.data_ptr(), _ftag(dt_bias, "dt_bias")
+    args.neg_exp_A = _ptr(neg_exp_A)
+    args.state = state.data_ptr()
+    args.state_slot_stride, args.state_h_stride, args.state_k_stride, args.state_v_stride = state.stride()
+    args.state_indices, args.state_indices_dtype = _ptr(at), at_tag
+    args.initial = _ptr(initial)
+    args.o, args.o_row_stride, args.o_h_stride, args.o_dtype = o.data_ptr(), o.stride(0), o.stride(1), _ftag(o, "o")
+    args.status = _status_ptr(status, batch, dev)
+    lib = load()
+    need = C.c_int64()
+    check("dft_prompt_gdn_workspace", lib.dft_prompt_gdn_workspace(C.byref(args), C.byref(need)))
+    if need.value:
+        work = torch.empty(need.value, device=dev, dtype=torch.uint8)
+        args.workspace, args.workspace_bytes = work.data_ptr(), need.value
+    check("dft_prompt_gdn", lib.dft_prompt_gdn(C.byref(args), _stream(dev)))
+    return o
+
+
+def token_gdn(y: torch.Tensor, a: torch.Tensor, b: torch.Tensor, A_log: Optional[torch.Tensor], dt_bias: torch.Tensor,
+              state: torch.Tensor, *, hk: int, hv: int, **kw) -> torch.Tensor:
+    """``prompt_gdn`` over one token a request: row b of y [batch, channels],
+    a and b takes the state of slot state_indices[b] (or b) one token on.  The
+    other keywords and the result are ``prompt_gdn``'s."""
+    return prompt_gdn(y, a, b, A_log, dt_bias, state, hk=hk, hv=hv, max_len=1, batch=y.shape[0], **kw)
+
+
+# ---------------------------------------------------------------------------
+# the accepted path
+# ---------------------------------------------------------------------------
+def _vocab_rows(t, rows, vocab, name):
+    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != vocab:
+        raise ValueError(f"{name} must be [{rows}, {vocab}], got {tuple(t.shape)}")
+    if t.stride(1) != 1 and vocab > 1:
+        raise ValueError(f"{name} must have stride 1 along the vocabulary")
+    return t.data_ptr(), t.stride(0), _ftag(t, name)
+
+
+def tree_accept(tokens: torch.Tensor, parent: torch.Tensor, probs: torch.Tensor, uniform: torch.Tensor,
+                last: torch.Tensor, *, draft_probs: Optional[torch.Tensor] = None,
+                cu_seqlens: Optional[torch.Tensor] = None, n_nodes: Optional[int] = None,
+                batch: Optional[int] = None, path_cols: int = 16, status: Optional[torch.Tensor] = None) -> dict:
+    """Which drafted tokens stand, by the target's probabilities and given
+    random numbers, and the token behind them (``dft_tree_accept``): a path and
+    a next token distributed as the target alone would draw them.
+
+    tokens, parent [rows]: each request's draft tree (node 0 its root, the last
+    token that stands already; parents in front of their children, as in
+    ``tree_struct``; a chain is parent[i] = i - 1); probs [rows, vocab]: the
+    target's distribution behind each node; uniform float32 [rows] in [0, 1): a
+    node's random number; last float32 [batch]: the next token's.  draft_probs
+    [rows, vocab]: what each node's children were drawn from, one after the
+    other without repeats; None for a drafter that does not draw (the likeliest
+    tokens, an n-gram table).  A child joins the path where u q(t) < r(t), and
+    takes its share out of r where not; values that are not positive count as
+    0, and rows of probs and draft_probs are taken to sum to 1.  Request b's
+    nodes start at cu_seqlens[b] (then n_nodes is the most of one request) or
+    at b * n_nodes.
+
+    Returns path int32 [batch, path_cols] (nodes from the root on, -1 past
+    them: ``tree_commit``'s and ``tree_commit_verify``'s), path_len int32 [batch],
+    rows int64 [batch, path_cols] (the same as rows of the step, -1 past them:
+    ``PagedKV.accept``'s) and token int64 [batch], the next token (-1 without
+    rows or without weight).  A path ends at path_cols (1 to 64) nodes.
+    ``status`` (int32 [batch]): DFT_STATUS_SPAN, DFT_STATUS_WEIGHT bits.
+    """
+    dev = _device_of(tokens, parent, probs, uniform, last, draft_probs, cu_seqlens, status)
+    tok, tok_tag = _idx_vec(tokens, "tokens")
+    par, par_tag = _idx_vec(parent, "parent")
+    rows = tok.numel()
+    if par.numel() != rows:
+        raise ValueError(f"parent has {par.numel()} entries, tokens {rows}")
+    if probs.dim() != 2:
+        raise ValueError("probs must be [rows, vocab]")
+    cu, batch, n_nodes = _packed_rows(cu_seqlens, rows, n_nodes, "n_nodes", batch, "tokens")
+    if n_nodes > MAX_NODES:
+        raise ValueError(f"at most {MAX_NODES} nodes per request, got {n_nodes}")
+    if path_cols < 1 or path_cols > MAX_NODES:
+        raise ValueError(f"a path holds 1 to {MAX_NODES} nodes, got {path_cols}")
+    for t, n, nm in ((uniform, rows, "uniform"), (last, batch, "last")):
+        if t.dtype != torch.float32:
+            raise TypeError(f"{nm} must be float32")
+        if t.numel() != n:
+            raise ValueError(f"{nm} has {t.numel()} entries, need {n}")
+    uniform, last = uniform.contiguous(), last.contiguous()
+    a = TreeAcceptArgs()
+    a.batch, a.n_nodes, a.vocab, a.path_cols, a.rows = batch, n_nodes, probs.shape[1], path_cols, rows
+    a.cu_seqlens = _ptr(cu)
+    a.tokens, a.tokens_dtype, a.parent, a.parent_dtype = tok.data_ptr(), tok_tag, par.data_ptr(), par_tag
+    a.probs, a.probs_row_stride, a.probs_dtype = _vocab_rows(probs, rows, probs.shape[1], "probs")
+    if draft_probs is not None:
+        a.draft_probs, a.draft_row_stride, a.draft_dtype = _vocab_rows(draft_probs, rows, probs.shape[1], "draft_probs")
+    a.uniform, a.last = uniform.data_ptr(), last.data_ptr()
+    words = torch.empty(batch * (path_cols + 1), device=dev, dtype=torch.int32)
+    longs = torch.empty(batch * (path_cols + 1), device=dev, dtype=torch.int64)
+    out = {"path": words[:batch * path_cols].view(batch, path_cols), "path_len": words[batch * path_cols:],
+           "rows": longs[:batch * path_cols].view(batch, path_cols), "token": longs[batch * path_cols:]}
+    a.path, a.path_len = out["path"].data_ptr(), out["path_len"].data_ptr()
+    a.path_rows, a.token = out["rows"].data_ptr(), out["token"].data_ptr()
+    a.status = _status_ptr(status, batch, dev)
+    lib = load()
+    need = C.c_int64()
+    check("dft_tree_accept_workspace", lib.dft_tree_accept_workspace(C.byref(a), C.byref(need)))
+    if need.value:
+        work = torch.empty(need.value, device=dev, dtype=torch.uint8)
+        a.workspace, a.workspace_bytes = work.data_ptr(), need.value
+    check("dft_tree_accept", lib.dft_tree_accept(C.byref(a), _stream(dev)))
+    return out

@@ -83,7 +83,12 @@ enum dft_request_status {
   /* the request's tokens need more pages than its row of the block table has
    * columns: dft_page_plan gave it none, dft_paged_attention reads what the
    * row holds */
-  DFT_STATUS_TABLE = 16
+  DFT_STATUS_TABLE = 16,
+  /* (dft_prompt_conv, dft_prompt_gdn) the request's slot is past the pool's
+   * last one: it was taken as a negative one */
+  DFT_STATUS_SLOT = 32,
+  /* (dft_tree_accept) there is no weight to draw the next token from: it is -1 */
+  DFT_STATUS_WEIGHT = 64
 };
 
 /* ---------------------------------------------------------------------------
@@ -663,6 +668,154 @@ typedef struct dft_prompt_attention_args {
 } dft_prompt_attention_args;
 
 DFT_API int dft_prompt_attention(const dft_prompt_attention_args* args, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * A GDN layer over whole prompts and single tokens: what brings the states
+ * there that the tree entry points verify on.  No counterpart in the
+ * reference, which takes both from SGLang.
+ *
+ * Rows are packed: request b's are row0(b) = cu_seqlens[b] (non-decreasing)
+ * up to cu_seqlens[b+1], or b * max_len .. with NULL; one of more than
+ * max_len rows is cut to its first max_len, and rows behind `rows` are cut off
+ * (DFT_STATUS_SPAN).  A request without rows keeps its state as it is.  Rows
+ * of no request are neither read nor written.
+ * Each request goes on from the state of its slot, or where `initial` is given
+ * and 0 for it from zeros, and leaves its new state there.  Slot: of the
+ * indices, or b with NULL.  A negative one (a padded request) starts from
+ * zeros and leaves nothing.  No two requests of a launch may have one slot.
+ * ------------------------------------------------------------------------- */
+
+/* Causal convolution: y_t[c] = act(sum_j w[c][j] x_{t-width+1+j}[c] + bias[c]),
+ * where the width - 1 inputs in front of a request's first row are the columns
+ * 0 .. width - 2 of its conv state, which is left holding its last ones. */
+typedef struct dft_prompt_conv_args {
+  int32_t batch, max_len, channels, width; /* width = taps, 1 to 8 */
+  int32_t silu;                            /* 1: SiLU, 0: identity */
+  int64_t rows;  /* of x and y */
+  int64_t slots; /* of conv_state */
+  const void* x; /* [rows][channels], channel stride 1 */
+  int64_t x_row_stride;
+  int32_t x_dtype;
+  const int32_t* cu_seqlens; /* [batch + 1] or NULL */
+  void* conv_state;          /* [slot][c][col] */
+  int64_t cs_slot_stride, cs_chan_stride, cs_col_stride;
+  int32_t cs_dtype;
+  const void* cs_indices; /* [batch] or NULL */
+  int32_t cs_indices_dtype;
+  const uint8_t* initial; /* [batch] or NULL: all 1 */
+  const void* weight;     /* [c][tap] */
+  int64_t w_chan_stride, w_tap_stride;
+  int32_t w_dtype;
+  const void* bias; /* [c] or NULL */
+  int32_t bias_dtype;
+  void* y; /* [rows][channels], channel stride 1; not x's memory */
+  int64_t y_row_stride;
+  int32_t y_dtype;
+  int32_t* status; /* optional [batch] */
+} dft_prompt_conv_args;
+
+DFT_API int dft_prompt_conv(const dft_prompt_conv_args* args, void* stream);
+
+/* The gated delta rule.  Per v head h (q/k head h / (hv / hk)) and row t, with
+ * q, k normalised (x / sqrt(sum x^2 + 1e-6)), q scaled, beta = sigmoid(b) and
+ * g = neg_exp_A softplus(a + dt_bias):
+ *   S <- e^g S;  u = beta (v - S^T k);  S <- S + k u^T;  o = S^T q.
+ * States, sums, decays and outputs are held in fp32, factors of products as
+ * bf16 pairs (2^-17 relative).  What is not finite in a row reaches at most
+ * the rows of its request from the 64 in a row on that it is one of. */
+typedef struct dft_prompt_gdn_args {
+  int32_t batch, max_len;
+  int32_t hk, hv; /* hv % hk == 0 */
+  int32_t dk, dv; /* both 128 */
+  float scale;    /* of q */
+  int64_t rows;   /* of y, a, b and o */
+  int64_t slots;  /* of state */
+  const void* y;  /* [rows, 2*hk*dk + hv*dv] bf16 = [q | k | v], channel stride 1, 16-byte aligned rows */
+  int64_t y_row_stride;
+  const int32_t* cu_seqlens; /* [batch + 1] or NULL */
+  const void* a; /* [rows, hv] */
+  int64_t a_row_stride;
+  int32_t a_dtype;
+  const void* b; /* [rows, hv] */
+  int64_t b_row_stride;
+  int32_t b_dtype;
+  const void* A_log; /* [hv]; neg_exp_A = -exp(A_log) where that is NULL */
+  int32_t A_log_dtype;
+  const void* dt_bias; /* [hv] */
+  int32_t dt_bias_dtype;
+  const float* neg_exp_A; /* [hv] or NULL */
+  float* state; /* S(k, v) at slot*slot_stride + h*h_stride + k*k_stride + v*v_stride */
+  int64_t state_slot_stride, state_h_stride, state_k_stride, state_v_stride;
+  const void* state_indices; /* [batch] or NULL */
+  int32_t state_indices_dtype;
+  const uint8_t* initial; /* [batch] or NULL: all 1 */
+  void* o;                /* [rows][hv][dv], channel stride 1 */
+  int64_t o_row_stride, o_h_stride;
+  int32_t o_dtype;
+  int32_t* status; /* optional [batch] */
+  void* workspace; /* dft_prompt_gdn_workspace bytes, 16-byte aligned; used by this launch alone until it is done */
+  int64_t workspace_bytes;
+} dft_prompt_gdn_args;
+
+DFT_API int dft_prompt_gdn(const dft_prompt_gdn_args* args, void* stream);
+/* *bytes = what `workspace` must hold for these sizes (pointers are not read) */
+DFT_API int dft_prompt_gdn_workspace(const dft_prompt_gdn_args* args, int64_t* bytes);
+
+/* ---------------------------------------------------------------------------
+ * Which drafted tokens stand: verification against the target's probabilities
+ * from given random numbers, so that path and next token are distributed as
+ * the target alone would draw them.
+ *
+ * Request b's nodes are rows row0(b) .. of tokens, parent, uniform, probs and
+ * draft_probs (row0 as in dft_verify_args); node 0 is the root, the last token
+ * that stands already, and node i >= 1's parent is max(parent[i], 0) < i.  Row
+ * i of probs is the target's distribution behind node i, of draft_probs the
+ * one that node i's children were drawn from, one after the other without
+ * repeats.  Values that are not positive (NaN too) count as 0.
+ * From the root on, with r = probs of the node that the path stands at, its
+ * children in index order, t = a child's token and u its random number:
+ *   with draft_probs, q = the node's row of it: the child joins the path where
+ *     u q(t) < r(t); else r <- max(r - q, 0) / sum (r is kept where that sum is
+ *     0), and q <- q without t, over what the refused tokens leave of 1 (0
+ *     where they leave nothing);
+ *   without (a drafter that does not draw): where u (1 - sum of the refused
+ *     tokens' r) < r(t); else r(t) <- 0.
+ * A path of path_cols nodes ends.  The next token is the smallest index whose
+ * running sum of r exceeds last[b] times r's sum (without draft_probs: of the
+ * node's whole row where its refused children hold all of it).  A token
+ * outside [0, vocab) never stands and takes nothing from r.  Everything is
+ * computed in 64 bits.
+ * ------------------------------------------------------------------------- */
+typedef struct dft_tree_accept_args {
+  int32_t batch, n_nodes; /* n_nodes as in dft_verify_args, <= 64 */
+  int32_t vocab;
+  int32_t path_cols; /* 1 .. 64 */
+  int64_t rows;      /* of tokens, parent, uniform, probs and draft_probs */
+  const int32_t* cu_seqlens; /* [batch + 1] or NULL */
+  const void* tokens;        /* [rows]; a root's is not read */
+  int32_t tokens_dtype;
+  const void* parent; /* [rows] local parent index */
+  int32_t parent_dtype;
+  const void* probs; /* [rows][vocab], unit stride along vocab */
+  int64_t probs_row_stride;
+  int32_t probs_dtype;
+  const void* draft_probs; /* the same, or NULL */
+  int64_t draft_row_stride;
+  int32_t draft_dtype;
+  const float* uniform; /* [rows] in [0, 1); a root's is not read */
+  const float* last;    /* [batch] in [0, 1) */
+  int32_t* path;        /* [batch][path_cols] nodes from the root on, -1 past them */
+  int32_t* path_len;    /* [batch] (0: a request without rows) */
+  int64_t* path_rows;   /* [batch][path_cols] row0 + node, -1 past them */
+  int64_t* token;       /* [batch] the next token, -1 without rows or without weight (DFT_STATUS_WEIGHT) */
+  int32_t* status;      /* optional [batch] */
+  void* workspace; /* dft_tree_accept_workspace bytes, 16-byte aligned; used by this launch alone until it is done */
+  int64_t workspace_bytes;
+} dft_tree_accept_args;
+
+DFT_API int dft_tree_accept(const dft_tree_accept_args* args, void* stream);
+/* *bytes = what `workspace` must hold for these sizes (pointers are not read) */
+DFT_API int dft_tree_accept_workspace(const dft_tree_accept_args* args, int64_t* bytes);
 
 DFT_API const char* dft_error_string(int status);
 DFT_API int dft_abi_version(void);
