@@ -153,14 +153,19 @@ __global__ void __launch_bounds__(256) gdn_rows_kernel(const dft_prompt_gdn_args
 constexpr int kChunk = 64, kXcds = 8;
 constexpr int kFragment = 1024;  // bytes: 64 lanes x 16
 // Of X - I and P, whose upper halves are zero, the row tile m (of 16) has steps
-// 0 .. m / 2: six fragments, X's in three parts, P's in two.  The row tiles 0
-// and 1 have a fragment of zeros for their other step, so that all waves do the
-// same (loads whose use depends on the wave are waited for too early: 3.3 us a
-// chunk).
-constexpr int kParts = 5, kTriangle = 6 * kParts * kFragment;
-constexpr int kCoef = 5 * kChunk * 4;  // beta, e^G rk beta, e^(G_63 - G) rk, e^G rq, {e^G_63}
+// 0 .. m / 2: six fragments, X's in three parts, P's in two behind them.  P's row
+// tiles 0 and 1 have a fragment of zeros for their other step, so that all
+// waves do the same (loads whose use depends on the wave are waited for too early).
+constexpr int kTriangle = 6 * 5 * kFragment;
+constexpr int kCoef = 5 * kChunk * 4;  // of the rows: beta, e^G rk beta, e^(G_63 - G) rk, e^G_63 (of all), e^G rq
 constexpr int kHead = kTriangle + kCoef + kFragment, kKeys = 16 * kFragment;
-__device__ __forceinline__ int triangle_at(int m, int s) { return (m < 2 ? m : 2 * m - 2 + s) * kParts * kFragment; }
+__device__ __forceinline__ int x_at(int m, int s) { return (m < 2 ? m : 2 * m - 2 + s) * 3 * kFragment; }
+__device__ __forceinline__ int p_at(int m, int s) { return 18 * kFragment + (m < 2 ? m : 2 * m - 2 + s) * 2 * kFragment; }
+
+// Row i of K^T's row tile m: such that the lane that holds rows 4 g .. of the
+// results of tiles 2 w and 2 w + 1 has the keys 32 w + 8 g .., which are its
+// terms of step w.
+__device__ __forceinline__ int key_of(int m, int i) { return 32 * (m / 2) + 8 * (i / 4) + 4 * (m % 2) + i % 4; }
 
 struct Work {
   char* heads;  // [tile][hv][kHead]: X, P, the rows' factors
@@ -268,8 +273,8 @@ __global__ void __launch_bounds__(256) gdn_chunk_kernel(const dft_prompt_gdn_arg
     coef[lane] = gate.beta;
     coef[kChunk + lane] = lane < n ? e * rk * gate.beta : 0;
     coef[2 * kChunk + lane] = lane < n ? __builtin_amdgcn_exp2f(all - sum) * rk : 0;
-    coef[3 * kChunk + lane] = e * rqs[lane];
-    coef[4 * kChunk + lane] = __builtin_amdgcn_exp2f(all);
+    coef[3 * kChunk + lane] = __builtin_amdgcn_exp2f(all);
+    coef[4 * kChunk + lane] = e * rqs[lane];
     *reinterpret_cast<u32x4*>(out + kTriangle + kCoef + 16 * lane) = u32x4{};
   }
 
@@ -325,7 +330,7 @@ __global__ void __launch_bounds__(256) gdn_chunk_kernel(const dft_prompt_gdn_arg
 #pragma unroll
   for (int y = 0; y < 2; ++y) {
     if (y > w / 2) continue;
-    char* at = out + triangle_at(w, y) + 3 * kFragment + 16 * lane;
+    char* at = out + p_at(w, y) + 16 * lane;
 #pragma unroll
     for (int z = 0; z < 2; ++z) *reinterpret_cast<u64x2*>(at + z * kFragment) = u64x2{p[2 * y].p[z], p[2 * y + 1].p[z]};
   }
@@ -336,7 +341,7 @@ __global__ void __launch_bounds__(256) gdn_chunk_kernel(const dft_prompt_gdn_arg
       const int m = 2 * w + y / 2, step = y % 2;
       uint16_t e8[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) e8[e] = keys[32 * step + 16 * (e / 4) + 4 * g + e % 4][16 * m + l16];
+      for (int e = 0; e < 8; ++e) e8[e] = keys[32 * step + 16 * (e / 4) + 4 * g + e % 4][key_of(m, l16)];
       *reinterpret_cast<u32x4*>(kt + (2 * m + step) * kFragment + 16 * lane) = __builtin_bit_cast(u32x4, e8);
     }
   }
@@ -371,7 +376,7 @@ __global__ void __launch_bounds__(256) gdn_chunk_kernel(const dft_prompt_gdn_arg
 #pragma unroll
   for (int y = 0; y < 2; ++y) {
     if (y > w / 2) continue;
-    char* at = out + triangle_at(w, y) + 16 * lane;
+    char* at = out + x_at(w, y) + 16 * lane;
 #pragma unroll
     for (int z = 0; z < 3; ++z) *reinterpret_cast<u64x2*>(at + z * kFragment) = u64x2{px[2 * y].p[z], px[2 * y + 1].p[z]};
   }
@@ -380,21 +385,50 @@ __global__ void __launch_bounds__(256) gdn_chunk_kernel(const dft_prompt_gdn_arg
 // What of the outputs is known at compile time.
 enum { kAnyOut = 0, kBf16Out = 1 };
 
-// The states through the chunks: a workgroup for 16 NT value columns of a
-// head.  Four waves take the state on, each for 16 rows of the chunk and for 32
-// keys of the state, which stays in their accumulators; S, W and U pass between
-// them through the LDS as operands of the next product.  Four more form the
-// outputs from S and U beside them.  The slices of a head read the same X, P, K
-// and Q, the heads of a k head the same K and Q: they form a family, whose
-// workgroups stand on one XCD, behind one L2 (one prompt of 8192, 16 k and 32 v
-// heads: 2.1 GB read past the L2s with the slices dealt out, now KKK).
+// global -> LDS, 16 bytes a lane
+__device__ __forceinline__ void copy16(const void* from, void* to) {
+  __builtin_amdgcn_global_load_lds(from, (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+}
+// s_waitcnt: until at most n vector-memory operations are outstanding
+constexpr unsigned wait_loads(int n) { return (unsigned)((n & 15) | ((n >> 4) << 14) | (7 << 4) | (15 << 8)); }
+// a barrier that waits for no copy
+__device__ __forceinline__ void barrier_only() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+constexpr int kScanThreads = 64 * 12;
+
+// The states through the chunks: a workgroup for 16 NT value columns of a head.
+// What bounds it is the chain S -> W -> U -> S of one chunk after the other, so
+// its twelve waves divide the work such that nothing else stands in it:
+//   0-3  the chain: each 32 keys of S in its accumulators, as results of K^T U
+//        and as terms of K S (whose four partial sums pass through the LDS), and
+//        16 of the chunk's rows of W and U, which pass through the LDS as the
+//        next product's operand
+//   4-7  the outputs of 16 rows each, from S and U
+//   8-10 copy the chain's operands to the LDS, each group as soon as the last
+//        chunk's has been used (loads by the chain's waves hold them up: 64 bytes
+//        a cycle and CU, 0.6 us a chunk)
+//   11   reads what is needed three chunks on into the L2
+// Three barriers a chunk: 1 the partial sums, 2 W, 3 U.
+// The slices of a head read the same X, P, K and Q, the heads of a k head the
+// same K and Q: they form a family, whose workgroups stand on one XCD, behind
+// one L2 (one prompt of 8192, 16 k and 32 v heads: 2.1 GB read past the L2s with
+// the slices dealt out, 0.3 so).
 template <int NT, bool VEC, int OUT>
-__global__ void __launch_bounds__(512, 1) gdn_scan_kernel(const dft_prompt_gdn_args a, Work work, int families) {
+__global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_kernel(const dft_prompt_gdn_args a, Work work, int families) {
   constexpr int BN = 16 * NT, kSlices = kD / BN, kSRow = kD + 8, kRow = kChunk + 8;
-  __shared__ __attribute__((aligned(16))) uint16_t Sb[3][BN][kSRow];
+  __shared__ __attribute__((aligned(16))) char k_lds[16 * kFragment], kt_lds[16 * kFragment], x_lds[18 * kFragment];
+  __shared__ __attribute__((aligned(16))) uint16_t v_lds[kChunk][BN];
+  __shared__ __attribute__((aligned(16))) float coef_lds[2][4][kChunk];
+  __shared__ __attribute__((aligned(16))) f32x4 sums[NT][4][4][64];  // [t][of wave][row tile][lane]
+  __shared__ __attribute__((aligned(16))) uint16_t Sb[2][BN][kSRow];
   __shared__ __attribute__((aligned(16))) uint16_t Wb[3][BN][kRow], Ub[2][BN][kRow], Vb[3][BN][kRow];
+  __shared__ __attribute__((aligned(16))) char touched[kFragment];
   if (blockIdx.x == 0 && a.status)
-    for (int b = threadIdx.x; b < a.batch; b += 512)
+    for (int b = threadIdx.x; b < a.batch; b += kScanThreads)
       a.status[b] = span_of(a, b).status | slot_of(a.state_indices, a.state_indices_dtype, a.initial, a.slots, b).status;
   const int members = a.batch * a.hv / families * kSlices;  // of a family
   const int round = blockIdx.x / (kXcds * members), in = blockIdx.x - round * kXcds * members;
@@ -410,34 +444,134 @@ __global__ void __launch_bounds__(512, 1) gdn_scan_kernel(const dft_prompt_gdn_a
   const uint16_t* y = static_cast<const uint16_t*>(a.y);
   auto put = [&](uint16_t* to, uint64_t x) { *reinterpret_cast<uint64_t*>(to) = x; };
   auto get = [&](const uint16_t* from) { return *reinterpret_cast<const bf16x8*>(from); };
-  // The rows of a chunk's tile, row 0's address at hand: a row past the request's last is its last one.  What is at hand
-  // moves on by whole chunks, and is looked up anew for one that is not whole.
-  const int64_t row_step = (int64_t)kChunk * a.y_row_stride;
+  auto fragment = [&](const char* from) { return *reinterpret_cast<const bf16x8*>(from + 16 * lane); };
+  // a row past the request's last is its last one
   auto row_at = [&](int at, int i) { return y + (s.r0 + min(at * kChunk + i, s.n - 1)) * a.y_row_stride; };
-  const int whole = s.n / kChunk;
-  const int64_t head_step = (int64_t)a.hv * kHead;
-  const char* head = work.heads + (first * a.hv + h) * kHead;
+  auto head_at = [&](int at) { return work.heads + ((first + min(at, chunks - 1)) * a.hv + h) * kHead; };
+  auto keys_at = [&](int at) { return work.keys + ((first + min(at, chunks - 1)) * a.hk + kh) * kKeys; };
 
+  if (wave == 11) {
+    const int part = (member % kSlices) * 64 + lane, parts = kSlices * 64;
+    for (int at = 0; at < chunks; ++at) {
+      if (at) {
+        barrier_only();
+        barrier_only();
+      } else {
+        barrier_only();
+        barrier_only();
+        barrier_only();
+      }
+      // lines of 128 bytes: the head's block, K^T, the rows of Q, K and V
+      constexpr int kHeadLines = (kHead + 127) / 128, kKeyLines = kKeys / 128, kRowLines = 2 * kChunk;
+      const int to = at + 3;
+      if (to < chunks)
+        for (int line = part; line < kHeadLines + kKeyLines + 3 * kRowLines; line += parts) {
+          const char* from;
+          int x = line;
+          if (x < kHeadLines) {
+            from = head_at(to) + min(x * 128, kHead - 16);
+          } else if ((x -= kHeadLines) < kKeyLines) {
+            from = keys_at(to) + x * 128;
+          } else {
+            x -= kKeyLines;
+            const int which = x / kRowLines, row = x % kRowLines / 2;
+            const int head = which == 0 ? kh : which == 1 ? a.hk + kh : 2 * a.hk + h;
+            from = reinterpret_cast<const char*>(row_at(to, row) + head * kD) + x % 2 * 128;
+          }
+          copy16(from, touched);
+        }
+      barrier_only();
+    }
+    __builtin_amdgcn_s_waitcnt(wait_loads(0));
+    return;
+  }
+  if (wave == 8) {  // X; V and the rows' factors
+    auto copy_v = [&](int at) {
+#pragma unroll
+      for (int m = 0; m < 2 * NT; ++m)
+        copy16(row_at(at, (64 * m + lane) / (2 * NT)) + (2 * a.hk + h) * kD + c0 + (64 * m + lane) % (2 * NT) * 8,
+               reinterpret_cast<char*>(v_lds) + m * kFragment);
+      copy16(head_at(at) + kTriangle + 16 * lane, coef_lds[at & 1]);
+    };
+    auto copy_x = [&](const char* head) {
+#pragma unroll
+      for (int m = 0; m < 18; ++m) copy16(head + m * kFragment + 16 * lane, x_lds + m * kFragment);
+    };
+    copy_v(0);
+    copy_x(head_at(0));
+    barrier_only();
+    for (int at = 0; at < chunks; ++at) {
+      __builtin_amdgcn_s_waitcnt(wait_loads(18));  // V
+      barrier_only();                              // 1
+      __builtin_amdgcn_s_waitcnt(wait_loads(0));   // X
+      barrier_only();                              // 2: V has been used
+      copy_v(at + 1);
+      barrier_only();  // 3: X has been used
+      copy_x(head_at(at + 1));
+    }
+    __builtin_amdgcn_s_waitcnt(wait_loads(0));
+    return;
+  }
+  if (wave == 9) {  // K
+    const uint16_t* row[4];  // rows 16 m + l16
+    auto rows = [&](int at) {
+#pragma unroll
+      for (int m = 0; m < 4; ++m) row[m] = row_at(at, 16 * m + l16) + (a.hk + kh) * kD + 8 * g;
+    };
+    auto copy_k = [&]() {
+#pragma unroll
+      for (int m = 0; m < 4; ++m)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) copy16(row[m] + 32 * x, k_lds + (4 * x + m) * kFragment);
+    };
+    rows(0);
+    copy_k();
+    __builtin_amdgcn_s_waitcnt(wait_loads(0));
+    barrier_only();
+    for (int at = 0; at < chunks; ++at) {
+      rows(at + 1);
+      barrier_only();  // 1: K has been used
+      copy_k();
+      barrier_only();  // 2
+      __builtin_amdgcn_s_waitcnt(wait_loads(0));
+      barrier_only();  // 3
+    }
+    return;
+  }
+  if (wave == 10) {  // K^T
+    barrier_only();
+    for (int at = 0; at < chunks; ++at) {
+      const char* keys = keys_at(at) + 16 * lane;
+      barrier_only();  // 1: the last chunk's has been used
+#pragma unroll
+      for (int m = 0; m < 16; ++m) copy16(keys + m * kFragment, kt_lds + m * kFragment);
+      barrier_only();  // 2
+      __builtin_amdgcn_s_waitcnt(wait_loads(0));
+      barrier_only();  // 3
+    }
+    return;
+  }
   if (wave >= 4) {
     const bool vec = a.o_dtype == DFT_F32 && reinterpret_cast<uintptr_t>(a.o) % 16 == 0 && a.o_row_stride % 4 == 0 && a.o_h_stride % 4 == 0;
     bf16x8 q[4], p[2][2];  // the wave's rows of Q and P
     float rq;              // e^G rq of row l16
-    const int q_at = kh * kD + 8 * g;
-    const uint16_t* row = row_at(0, 16 * w + l16) + q_at;
-    auto load_q = [&]() {
+    auto load_q = [&](int at) {
+      const uint16_t* row = row_at(at, 16 * w + l16) + kh * kD + 8 * g;
 #pragma unroll
       for (int j = 0; j < 4; ++j) q[j] = *reinterpret_cast<const bf16x8*>(row + 32 * j);
-      rq = reinterpret_cast<const float*>(head + kTriangle)[3 * kChunk + 16 * w + l16];
+      rq = reinterpret_cast<const float*>(head_at(at) + kTriangle)[4 * kChunk + 16 * w + l16];
     };
-    auto load_p = [&]() {
+    auto load_p = [&](int at) {
+      const char* head = head_at(at) + 16 * lane;
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
         for (int z = 0; z < 2; ++z)
-          p[j][z] = *reinterpret_cast<const bf16x8*>(head + (j && w < 2 ? kTriangle + kCoef : triangle_at(w, j) + (3 + z) * kFragment) + 16 * lane);
+          p[j][z] = *reinterpret_cast<const bf16x8*>(head + (j && w < 2 ? kTriangle + kCoef : p_at(w, j) + z * kFragment));
     };
-    load_q();
-    load_p();
+    load_q(0);
+    load_p(0);
+    barrier_only();
     for (int at = 0; at < chunks; ++at) {
       f32x4 o[NT];
       __syncthreads();
@@ -451,10 +585,7 @@ __global__ void __launch_bounds__(512, 1) gdn_scan_kernel(const dft_prompt_gdn_a
         }
         o[t] = (q0 + q1) * rq;
       }
-      const bool more = at + 1 < chunks;
-      head += more ? head_step : 0;
-      row = at + 1 < whole ? row + row_step : row_at(at + 1, 16 * w + l16) + q_at;
-      load_q();
+      load_q(at + 1);
       __syncthreads();
       __syncthreads();
 #pragma unroll
@@ -470,7 +601,7 @@ __global__ void __launch_bounds__(512, 1) gdn_scan_kernel(const dft_prompt_gdn_a
         }
         o[t] += o1;
       }
-      load_p();
+      load_p(at + 1);
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         const int i = at * kChunk + 16 * w + l16;
@@ -492,10 +623,10 @@ __global__ void __launch_bounds__(512, 1) gdn_scan_kernel(const dft_prompt_gdn_a
   }
 
   const Slot slot = slot_of(a.state_indices, a.state_indices_dtype, a.initial, a.slots, b);
-  f32x4 S[2][NT];  // keys 32 w + 16 x + 4 g .., column 16 t + l16
+  f32x4 S[2][NT];  // keys 32 w + 8 g + 4 x .., column 16 t + l16
   float* state = a.state + slot.at * a.state_slot_stride + h * a.state_h_stride;
   auto key_at = [&](int x, int t) {
-    return (32 * w + 16 * x + 4 * g) * a.state_k_stride + (c0 + 16 * t + l16) * a.state_v_stride;
+    return (32 * w + 8 * g + 4 * x) * a.state_k_stride + (c0 + 16 * t + l16) * a.state_v_stride;
   };
 #pragma unroll
   for (int x = 0; x < 2; ++x)
@@ -509,112 +640,65 @@ __global__ void __launch_bounds__(512, 1) gdn_scan_kernel(const dft_prompt_gdn_a
 #pragma unroll
         for (int r = 0; r < 4; ++r) S[x][t][r] = state[key_at(x, t) + r * a.state_k_stride];
     }
-  bf16x8 k[4], kt[2][2], X[2][3];  // the wave's rows of K, its 32 keys of K^T, its rows of X - I
-  uint16_t v[NT][4];
-  f32x4 beta, decayed, out;        // of rows 4 g ..: beta, e^G rk beta, e^(G_63 - G) rk
-  float keep;                      // e^G_63
-  const int k_at = (a.hk + kh) * kD + 8 * g, v_at = (2 * a.hk + h) * kD + c0 + l16;
-  const uint16_t *k_row = row_at(0, 16 * w + l16) + k_at, *v_row[4];
-#pragma unroll
-  for (int r = 0; r < 4; ++r) v_row[r] = row_at(0, 16 * w + 4 * g + r) + v_at;
-  const char* keys = work.keys + (first * a.hk + kh) * kKeys;
-  auto load_k = [&]() {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) k[j] = *reinterpret_cast<const bf16x8*>(k_row + 32 * j);
-  };
-  auto load_v = [&]() {
-    const float* coef = reinterpret_cast<const float*>(head + kTriangle);
-    beta = *reinterpret_cast<const f32x4*>(coef + 16 * w + 4 * g);
-    decayed = *reinterpret_cast<const f32x4*>(coef + kChunk + 16 * w + 4 * g);
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-#pragma unroll
-      for (int t = 0; t < NT; ++t) v[t][r] = v_row[r][16 * t];
-  };
-  auto load_x = [&]() {
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int z = 0; z < 3; ++z)
-        X[j][z] = *reinterpret_cast<const bf16x8*>(head + (j && w < 2 ? kTriangle + kCoef : triangle_at(w, j) + z * kFragment) + 16 * lane);
-    const float* coef = reinterpret_cast<const float*>(head + kTriangle);
-    out = *reinterpret_cast<const f32x4*>(coef + 2 * kChunk + 16 * w + 4 * g);
-  };
-  auto load_kt = [&]() {
-    keep = reinterpret_cast<const float*>(head + kTriangle)[4 * kChunk];
-#pragma unroll
-    for (int x = 0; x < 2; ++x)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) kt[x][j] = *reinterpret_cast<const bf16x8*>(keys + (2 * (2 * w + x) + j) * kFragment + 16 * lane);
-  };
   const int place = 32 * (w / 2) + 8 * g + 4 * (w % 2);  // of the lane's rows 16 w + 4 g .. as terms
-  // S as the next chunk's operand
-  auto hand_on = [&]() {
-#pragma unroll
-    for (int x = 0; x < 2; ++x)
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const Parts4<3> p = split4<3>(S[x][t]);
-#pragma unroll
-        for (int z = 0; z < 3; ++z) put(&Sb[z][16 * t + l16][32 * w + 16 * x + 4 * g], p.p[z]);
-      }
-  };
-  load_k();
-  load_v();
-  load_x();
-  load_kt();
-  hand_on();
-  // The next chunk's operands are loaded where this one's have been used: two thirds of a chunk ahead, and never many at
-  // once (a burst holds up the waves that issue it: 64 bytes a cycle and CU).
+  __builtin_amdgcn_s_setprio(2);
+  __syncthreads();
   for (int at = 0; at < chunks; ++at) {
-    const bool more = at + 1 < chunks;
+    const float(*coef)[kChunk] = coef_lds[at & 1];
     f32x4 u[NT];
-    __syncthreads();
+    bf16x8 k[4];
+#pragma unroll
+    for (int m = 0; m < 4; ++m) k[m] = fragment(k_lds + (4 * w + m) * kFragment);
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      f32x4 k0 = {}, k1 = {}, k2 = {};
+      const Parts4<3> lo = split4<3>(S[0][t]), hi = split4<3>(S[1][t]);
+      bf16x8 p[3];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        k0 = mfma16(k[j], get(&Sb[0][16 * t + l16][32 * j + 8 * g]), k0);
-        k1 = mfma16(k[j], get(&Sb[1][16 * t + l16][32 * j + 8 * g]), k1);
-        k2 = mfma16(k[j], get(&Sb[2][16 * t + l16][32 * j + 8 * g]), k2);
-      }
-      f32x4 vf;
+      for (int z = 0; z < 3; ++z) p[z] = __builtin_bit_cast(bf16x8, u64x2{lo.p[z], hi.p[z]});
+      f32x4 sum[4] = {};
 #pragma unroll
-      for (int r = 0; r < 4; ++r) vf[r] = bf16_bits_to_f32(v[t][r]);
-      u[t] = beta * vf - decayed * (k0 + (k1 + k2));
+      for (int z = 2; z >= 0; --z)
+#pragma unroll
+        for (int m = 0; m < 4; ++m) sum[m] = mfma16(k[m], p[z], sum[m]);
+#pragma unroll
+      for (int z = 0; z < 2; ++z) *reinterpret_cast<bf16x8*>(&Sb[z][16 * t + l16][32 * w + 8 * g]) = p[z];
+#pragma unroll
+      for (int m = 0; m < 4; ++m) sums[t][w][m][lane] = sum[m];
+    }
+    __syncthreads();
+    const f32x4 beta = *reinterpret_cast<const f32x4*>(&coef[0][16 * w + 4 * g]);
+    const f32x4 decayed = *reinterpret_cast<const f32x4*>(&coef[1][16 * w + 4 * g]);
+    const f32x4 out = *reinterpret_cast<const f32x4*>(&coef[2][16 * w + 4 * g]);
+    const float keep = coef[3][0];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const f32x4 ks = (sums[t][0][w][lane] + sums[t][1][w][lane]) + (sums[t][2][w][lane] + sums[t][3][w][lane]);
+      f32x4 v;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v[r] = bf16_bits_to_f32(v_lds[16 * w + 4 * g + r][16 * t + l16]);
+      u[t] = beta * v - decayed * ks;
       const Parts4<3> p = split4<3>(u[t]);
 #pragma unroll
       for (int z = 0; z < 3; ++z) put(&Wb[z][16 * t + l16][place], p.p[z]);
     }
-    __builtin_amdgcn_sched_barrier(0);
-    if (at + 1 < whole) {
-      k_row += row_step;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) v_row[r] += row_step;
-    } else {
-      k_row = row_at(at + 1, 16 * w + l16) + k_at;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) v_row[r] = row_at(at + 1, 16 * w + 4 * g + r) + v_at;
-    }
-    head += more ? head_step : 0;
-    load_k();
-    load_v();
     __syncthreads();
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       f32x4 u1 = {}, u2 = {};
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
+        if (j > w / 2) continue;
         const bf16x8 w0 = get(&Wb[0][16 * t + l16][32 * j + 8 * g]);
         const bf16x8 w1 = get(&Wb[1][16 * t + l16][32 * j + 8 * g]);
         const bf16x8 w2 = get(&Wb[2][16 * t + l16][32 * j + 8 * g]);
-        u1 = mfma16(X[j][0], w0, u1);
-        u2 = mfma16(X[j][1], w0, u2);
-        u1 = mfma16(X[j][0], w1, u1);
-        u2 = mfma16(X[j][2], w0, u2);
-        u1 = mfma16(X[j][0], w2, u1);
-        u2 = mfma16(X[j][1], w1, u2);
+        const char* at = x_lds + x_at(w, j);
+        const bf16x8 x0 = fragment(at), x1 = fragment(at + kFragment), x2 = fragment(at + 2 * kFragment);
+        u1 = mfma16(x0, w0, u1);
+        u2 = mfma16(x1, w0, u2);
+        u1 = mfma16(x0, w1, u1);
+        u2 = mfma16(x2, w0, u2);
+        u1 = mfma16(x0, w2, u1);
+        u2 = mfma16(x1, w1, u2);
       }
       u[t] += u1 + u2;
       const Parts4<3> d = split4<3>(u[t] * out);
@@ -624,9 +708,12 @@ __global__ void __launch_bounds__(512, 1) gdn_scan_kernel(const dft_prompt_gdn_a
 #pragma unroll
       for (int z = 0; z < 2; ++z) put(&Ub[z][16 * t + l16][place], p.p[z]);
     }
-    __builtin_amdgcn_sched_barrier(0);
-    load_x();
     __syncthreads();
+    bf16x8 kt[2][2];
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) kt[x][j] = fragment(kt_lds + (2 * (2 * w + x) + j) * kFragment);
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       f32x4 add[2] = {};
@@ -647,9 +734,6 @@ __global__ void __launch_bounds__(512, 1) gdn_scan_kernel(const dft_prompt_gdn_a
 #pragma unroll
       for (int x = 0; x < 2; ++x) S[x][t] += add[x];
     }
-    keys += more ? (int64_t)a.hk * kKeys : 0;
-    load_kt();
-    hand_on();
   }
   if (slot.at < 0) return;
 #pragma unroll
@@ -680,11 +764,11 @@ int launch_scan(const dft_prompt_gdn_args& a, const Work& work, hipStream_t stre
   const unsigned blocks = (unsigned)((families + kXcds - 1) / kXcds * kXcds * (a.batch * a.hv / families * (8 / NT)));
   const bool bf16 = a.o_dtype == DFT_BF16 && reinterpret_cast<uintptr_t>(a.o) % 8 == 0 && a.o_row_stride % 4 == 0 && a.o_h_stride % 4 == 0;
   if (!vector_state(a))
-    gdn_scan_kernel<NT, false, kAnyOut><<<blocks, 512, 0, stream>>>(a, work, families);
+    gdn_scan_kernel<NT, false, kAnyOut><<<blocks, kScanThreads, 0, stream>>>(a, work, families);
   else if (bf16)
-    gdn_scan_kernel<NT, true, kBf16Out><<<blocks, 512, 0, stream>>>(a, work, families);
+    gdn_scan_kernel<NT, true, kBf16Out><<<blocks, kScanThreads, 0, stream>>>(a, work, families);
   else
-    gdn_scan_kernel<NT, true, kAnyOut><<<blocks, 512, 0, stream>>>(a, work, families);
+    gdn_scan_kernel<NT, true, kAnyOut><<<blocks, kScanThreads, 0, stream>>>(a, work, families);
   return hipGetLastError() == hipSuccess ? DFT_OK : DFT_ERR_LAUNCH;
 }
 
