@@ -6,17 +6,19 @@
 // for whose rows i and j, G the running sum of g within the chunk, K and Q the
 // raw rows, rk and rq what normalises (and scales) them:
 //   A_ij = beta_i rk_i rk_j (k_i . k_j) e^(G_i - G_j)  (j < i),  X = (I + A)^-1
-//   P_ij = rq_i rk_j (q_i . k_j) e^(G_i - G_j)         (j <= i)
-//   W = beta (V - e^G rk (K S)),  U = X W
-//   O = e^G rq (Q S) + P U
-//   S <- e^G_63 S + K^T (e^(G_63 - G) rk U)
+//   W = beta (V - e^G rk (K S)),  U = rk (X W)
+//   O = rq (e^G (Q S) + P U),  P_ij = (q_i . k_j) e^(G_i - G_j)  (j <= i)
+//   S <- e^G_63 S + K^T (e^(G_63 - G) U)
 // gdn_chunk_kernel forms what needs no state, X and P, for all chunks at once,
 // gdn_scan_kernel takes the states through the chunks.  The raw rows are bf16,
-// so that K, Q and K^T are exact operands of bf16 products; what is not (S, X,
-// P, W, U) goes in as a pair hi + lo, 2^-16 relative at most, a product of two
-// pairs without lo * lo.  (States are handed on in fp32 from chunk to chunk
-// and are held to it: one bf16 factor would leave 2^-9 in them.)
+// so that K, Q and K^T are exact operands of bf16 products.  What is not goes in
+// as a sum of bf16 parts.  States are handed on in fp32 from call to call: what
+// they pass through (S, X - I, W, U) has three parts, 2^-24 relative at most,
+// and products of two such factors the six of 2^-16 or more (with two parts, a
+// third less products, the states came out 4 10^-6 off, with three 2 to 5 10^-7).
+// What only an output of the row passes through (P, U in O, S in Q S) has two.
 #include <algorithm>
+#include <type_traits>
 
 #include "packed.h"
 
@@ -152,24 +154,21 @@ __global__ void __launch_bounds__(256) gdn_rows_kernel(const dft_prompt_gdn_args
 //   32 s + 16 h + 4 g + e  at place  32 s + 8 g + 4 h + e.
 constexpr int kChunk = 64, kXcds = 8;
 constexpr int kFragment = 1024;  // bytes: 64 lanes x 16
-// Of X - I and P, whose upper halves are zero, the row tile m (of 16) has steps
-// 0 .. m / 2: six fragments, X's in three parts, P's in two behind them.  P's row
-// tiles 0 and 1 have a fragment of zeros for their other step, so that all
-// waves do the same (loads whose use depends on the wave are waited for too early).
-constexpr int kTriangle = 6 * 5 * kFragment;
-constexpr int kCoef = 5 * kChunk * 4;  // of the rows: beta, e^G rk beta, e^(G_63 - G) rk, e^G_63 (of all), e^G rq
-constexpr int kHead = kTriangle + kCoef + kFragment, kKeys = 16 * kFragment;
-__device__ __forceinline__ int x_at(int m, int s) { return (m < 2 ? m : 2 * m - 2 + s) * 3 * kFragment; }
-__device__ __forceinline__ int p_at(int m, int s) { return 18 * kFragment + (m < 2 ? m : 2 * m - 2 + s) * 2 * kFragment; }
-
-// Row i of K^T's row tile m: such that the lane that holds rows 4 g .. of the
-// results of tiles 2 w and 2 w + 1 has the keys 32 w + 8 g .., which are its
-// terms of step w.
-__device__ __forceinline__ int key_of(int m, int i) { return 32 * (m / 2) + 8 * (i / 4) + 4 * (m % 2) + i % 4; }
+// X - I, whose upper half is zero, in fp32: its row tile m (of 16) has steps 0 ..
+// m / 2, six fragments of 8 elements a lane, the first four of every lane first.
+constexpr int kX = 6 * 2 * kFragment;
+__host__ __device__ constexpr int x_at(int m, int s) { return m < 2 ? m : 2 * m - 2 + s; }
+// P's six in two parts, and a fragment of zeros for the other step of the row
+// tiles 0 and 1, so that all waves do the same (loads whose use depends on the
+// wave are waited for too early).
+constexpr int kP = (6 * 2 + 1) * kFragment;
+__host__ __device__ constexpr int p_at(int m, int s) { return m < 2 && s ? 12 : 2 * x_at(m, s); }
+// Factors of the rows, 64 floats each: beta, e^G rk beta, rk, e^(G_63 - G), e^G_63 (of all); e^G, rq.
+enum { kBeta, kDecayed, kUnit, kOut, kKeep, kDecay, kRq, kCoefs = 8 };
+constexpr int kHead = kX + kP + kCoefs * kChunk * 4;
 
 struct Work {
-  char* heads;  // [tile][hv][kHead]: X, P, the rows' factors
-  char* keys;   // [tile][hk][kKeys]: K^T
+  char* heads;  // [tile][hv][kHead]: X - I in fp32, P, the rows' factors
 };
 
 __device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) {
@@ -178,6 +177,10 @@ __device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) {
 __device__ __forceinline__ f32x4 mfma16_f32(float a, float b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
 }
+// Until an fp32 product's result is whole.  The compiler waits 10 states for it,
+// after which its last register may still be on its way: read first of the
+// four, behind a branch, it held the sum without its last terms.
+__device__ __forceinline__ void settle(f32x4& x) { asm volatile("s_nop 15" : "+a"(x)); }
 // x = p[0] + p[1] + ..., each the bf16 nearest to what is left
 template <int N>
 struct Parts4 {
@@ -197,19 +200,18 @@ __device__ __forceinline__ Parts4<N> split4(f32x4 x) {
 }
 typedef uint64_t u64x2 __attribute__((ext_vector_type(2)));
 
-// The part of a chunk and v head that needs no state: a workgroup of four
-// waves, wave w for rows 16 w ...  X row block by row block from X (I + A) = I:
-// diagonal blocks by substitution (their powers would lose what equal keys
-// leave of 32 bits), then X_ij = -(sum_(j<m<=i) X_im A_mj) X_jj in fp32
-// products, transposed, so that each result is the next one's operand and the
-// last the fragment that is stored.
+// X and P of a chunk and v head: a workgroup of four waves, wave w for rows 16 w ...
+// Row block by row block from X (I + A) = I: diagonal blocks by substitution
+// (their powers would lose what equal keys leave of 32 bits), then X_ij =
+// -(sum_(j<m<=i) X_im A_mj) X_jj in fp32 products, transposed, so that each result
+// is the next one's operand and the last the fragment that is stored.
 __global__ void __launch_bounds__(256) gdn_chunk_kernel(const dft_prompt_gdn_args a, Work work) {
   constexpr int kKRow = kD + 8, kARow = kChunk + 4;
   __shared__ __attribute__((aligned(16))) uint16_t keys[kChunk][kKRow];
   __shared__ __attribute__((aligned(16))) float A[kChunk][kARow];
-  __shared__ __attribute__((aligned(16))) float G[kChunk], beta[kChunk], rks[kChunk], rqs[kChunk];
+  __shared__ __attribute__((aligned(16))) float G[kChunk], beta[kChunk], rks[kChunk];
   const int64_t tile = blockIdx.x / a.hv;
-  const int h = (int)(blockIdx.x - tile * a.hv), group = a.hv / a.hk, kh = h / group;
+  const int h = (int)(blockIdx.x - tile * a.hv), kh = h / (a.hv / a.hk);
   const int b = find_tile<256>(a, tile, kChunk);
   if (b < 0) return;
   const Span s = span_of(a, b);
@@ -218,16 +220,13 @@ __global__ void __launch_bounds__(256) gdn_chunk_kernel(const dft_prompt_gdn_arg
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, g = lane >> 4;
 
   // rows past the request's last: zeros
-  bf16x8 q[4], k[4];
-  float qq = 0, kk = 0;
   const int mine = 16 * w + l16;
-  const uint16_t* row = static_cast<const uint16_t*>(a.y) + (r0 + min(mine, n - 1)) * a.y_row_stride + kh * kD + 8 * g;
-  u32x4 qw[4], kw[4];
+  const uint16_t* row = static_cast<const uint16_t*>(a.y) + (r0 + min(mine, n - 1)) * a.y_row_stride + (a.hk + kh) * kD + 8 * g;
+  u32x4 kw[4], qw[4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    qw[j] = *reinterpret_cast<const u32x4*>(row + 32 * j);
-    kw[j] = *reinterpret_cast<const u32x4*>(row + a.hk * kD + 32 * j);
-  }
+  for (int j = 0; j < 4; ++j) kw[j] = *reinterpret_cast<const u32x4*>(row + 32 * j);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) qw[j] = *reinterpret_cast<const u32x4*>(row - a.hk * kD + 32 * j);
   Gate gate = {};
   float sum = 0, all = 0;
   if (w == 0) {  // the gates, a row a lane, G in log2 units
@@ -243,72 +242,72 @@ __global__ void __launch_bounds__(256) gdn_chunk_kernel(const dft_prompt_gdn_arg
     G[lane] = sum;
     beta[lane] = gate.beta;
   }
+  bf16x8 k[4], q[4];
+  float kk = 0, qq = 0;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    if (mine >= n) qw[j] = kw[j] = u32x4{};
-    q[j] = __builtin_bit_cast(bf16x8, qw[j]);
+    if (mine >= n) kw[j] = qw[j] = u32x4{};
     k[j] = __builtin_bit_cast(bf16x8, kw[j]);
+    q[j] = __builtin_bit_cast(bf16x8, qw[j]);
     *reinterpret_cast<u32x4*>(&keys[mine][32 * j + 8 * g]) = kw[j];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      qq = fmaf((float)q[j][e], (float)q[j][e], qq);
       kk = fmaf((float)k[j][e], (float)k[j][e], kk);
+      qq = fmaf((float)q[j][e], (float)q[j][e], qq);
     }
   }
-  qq += __shfl_xor(qq, 16);
   kk += __shfl_xor(kk, 16);
-  qq += __shfl_xor(qq, 32);
+  qq += __shfl_xor(qq, 16);
   kk += __shfl_xor(kk, 32);
-  const float rq = a.scale / sqrtf(qq + 1e-6f);
+  qq += __shfl_xor(qq, 32);
+  char* out = work.heads + (tile * a.hv + h) * kHead;
   if (g == 0) {
     rks[mine] = 1.f / sqrtf(kk + 1e-6f);
-    rqs[mine] = rq;
+    reinterpret_cast<float*>(out + kX + kP)[kRq * kChunk + mine] = a.scale / sqrtf(qq + 1e-6f);
   }
   __syncthreads();
 
-  char* out = work.heads + (tile * a.hv + h) * kHead;
   if (w == 0) {
-    float* coef = reinterpret_cast<float*>(out + kTriangle);
-    const float e = __builtin_amdgcn_exp2f(sum), rk = rks[lane];
-    coef[lane] = gate.beta;
-    coef[kChunk + lane] = lane < n ? e * rk * gate.beta : 0;
-    coef[2 * kChunk + lane] = lane < n ? __builtin_amdgcn_exp2f(all - sum) * rk : 0;
-    coef[3 * kChunk + lane] = __builtin_amdgcn_exp2f(all);
-    coef[4 * kChunk + lane] = e * rqs[lane];
-    *reinterpret_cast<u32x4*>(out + kTriangle + kCoef + 16 * lane) = u32x4{};
+    float* coef = reinterpret_cast<float*>(out + kX + kP) + lane;
+    const float rk = rks[lane];
+    coef[kBeta * kChunk] = gate.beta;
+    coef[kDecayed * kChunk] = lane < n ? __builtin_amdgcn_exp2f(sum) * rk * gate.beta : 0;
+    coef[kUnit * kChunk] = lane < n ? rk : 0;
+    coef[kOut * kChunk] = lane < n ? __builtin_amdgcn_exp2f(all - sum) : 0;
+    coef[kKeep * kChunk] = __builtin_amdgcn_exp2f(all);
+    coef[kDecay * kChunk] = __builtin_amdgcn_exp2f(sum);
+    *reinterpret_cast<u32x4*>(out + kX + 12 * kFragment + 16 * lane) = u32x4{};
   }
 
   // A into the LDS, P to its place: Gram tiles of the wave's rows with those of tiles j <= w, K K^T and (Q K^T)^T
-  const f32x4 Gi = *reinterpret_cast<const f32x4*>(&G[16 * w + 4 * g]);
-  const f32x4 bi = *reinterpret_cast<const f32x4*>(&beta[16 * w + 4 * g]) * *reinterpret_cast<const f32x4*>(&rks[16 * w + 4 * g]);
   const float Gq = G[mine];
   Parts4<2> p[4];
+  const f32x4 Gi = *reinterpret_cast<const f32x4*>(&G[16 * w + 4 * g]);
+  const f32x4 bi = *reinterpret_cast<const f32x4*>(&beta[16 * w + 4 * g]) * *reinterpret_cast<const f32x4*>(&rks[16 * w + 4 * g]);
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     p[j] = {};
     if (j > w) continue;
-    f32x4 kj_t = {}, qj_t = {};
+    f32x4 dot = {}, qk = {};
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
       const bf16x8 kj = *reinterpret_cast<const bf16x8*>(&keys[16 * j + l16][32 * x + 8 * g]);
-      kj_t = mfma16(k[x], kj, kj_t);
-      qj_t = mfma16(kj, q[x], qj_t);
+      dot = mfma16(k[x], kj, dot);
+      qk = mfma16(kj, q[x], qk);
     }
     const float Gj = G[16 * j + l16], rj = rks[16 * j + l16];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const bool below = j < w || 4 * g + r > l16;
-      const float x = kj_t[r] * (bi[r] * rj) * __builtin_amdgcn_exp2f(Gi[r] - Gj);
+      const float x = dot[r] * (bi[r] * rj) * __builtin_amdgcn_exp2f(Gi[r] - Gj);
       A[16 * w + 4 * g + r][16 * j + l16] = below ? x : 0.f;
     }
     const f32x4 Gk = *reinterpret_cast<const f32x4*>(&G[16 * j + 4 * g]);
-    const f32x4 rk = *reinterpret_cast<const f32x4*>(&rks[16 * j + 4 * g]);
     f32x4 y;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const bool seen = j < w || 4 * g + r <= l16;
-      const float x = qj_t[r] * (rq * rk[r]) * __builtin_amdgcn_exp2f(Gq - Gk[r]);
-      y[r] = seen ? x : 0.f;
+      y[r] = seen ? qk[r] * __builtin_amdgcn_exp2f(Gq - Gk[r]) : 0.f;
     }
     p[j] = split4<2>(y);
   }
@@ -328,57 +327,44 @@ __global__ void __launch_bounds__(256) gdn_chunk_kernel(const dft_prompt_gdn_arg
     if (i / 4 == g) A[16 * w + i][16 * w + l16] = x[i];
   __syncthreads();
 #pragma unroll
-  for (int y = 0; y < 2; ++y) {
-    if (y > w / 2) continue;
-    char* at = out + p_at(w, y) + 16 * lane;
+  for (int j = 0; j < 2; ++j) {
+    if (j > w / 2) continue;
 #pragma unroll
-    for (int z = 0; z < 2; ++z) *reinterpret_cast<u64x2*>(at + z * kFragment) = u64x2{p[2 * y].p[z], p[2 * y + 1].p[z]};
-  }
-  if (h == kh * group) {  // K^T: row tiles 2 w and 2 w + 1, both steps
-    char* kt = work.keys + (tile * a.hk + kh) * kKeys;
-#pragma unroll
-    for (int y = 0; y < 4; ++y) {
-      const int m = 2 * w + y / 2, step = y % 2;
-      uint16_t e8[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) e8[e] = keys[32 * step + 16 * (e / 4) + 4 * g + e % 4][key_of(m, l16)];
-      *reinterpret_cast<u32x4*>(kt + (2 * m + step) * kFragment + 16 * lane) = __builtin_bit_cast(u32x4, e8);
-    }
+    for (int z = 0; z < 2; ++z)
+      *reinterpret_cast<u64x2*>(out + kX + (p_at(w, j) + z) * kFragment + 16 * lane) = u64x2{p[2 * j].p[z], p[2 * j + 1].p[z]};
   }
   // the row block, transposed: xt[j] is X_wj^T, lane: row l16 of X_wj, columns 4 g ..
-  f32x4 xt[4];
-  Parts4<3> px[4];
+  auto row_block = [&](auto which) {
+    constexpr int W = decltype(which)::value;
+    f32x4 xt[4] = {};
+    xt[W] = *reinterpret_cast<const f32x4*>(&A[16 * W + l16][16 * W + 4 * g]);
 #pragma unroll
-  for (int j = 3; j >= 0; --j) {
-    px[j] = {};
-    xt[j] = f32x4{};
-    if (j > w) continue;
-    if (j == w) {
-      xt[j] = *reinterpret_cast<const f32x4*>(&A[16 * w + l16][16 * w + 4 * g]);
-      f32x4 less = xt[j];  // the unit diagonal stays out
+    for (int j = W - 1; j >= 0; --j) {
+      f32x4 to[3] = {}, all = {};
 #pragma unroll
-      for (int r = 0; r < 4; ++r) less[r] = 4 * g + r == l16 ? 0.f : less[r];
-      px[j] = split4<3>(less);
-      continue;
+      for (int m = W; m > j; --m)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) to[m - 1] = mfma16_f32(A[16 * m + 4 * g + r][16 * j + l16], xt[m][r], to[m - 1]);
+#pragma unroll
+      for (int m = W; m > j; --m) {
+        settle(to[m - 1]);
+        all += to[m - 1];
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) xt[j] = mfma16_f32(-A[16 * j + 4 * g + r][16 * j + l16], all[r], xt[j]);
+      settle(xt[j]);
     }
-    f32x4 to[3] = {};
 #pragma unroll
-    for (int m = 3; m > 0; --m) {
-      if (m > w || m <= j) continue;
+    for (int r = 0; r < 4; ++r) xt[W][r] = 4 * g + r == l16 ? 0.f : xt[W][r];  // the unit diagonal stays out
 #pragma unroll
-      for (int r = 0; r < 4; ++r) to[m - 1] = mfma16_f32(A[16 * m + 4 * g + r][16 * j + l16], xt[m][r], to[m - 1]);
-    }
-    const f32x4 all = to[0] + to[1] + to[2];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) xt[j] = mfma16_f32(-A[16 * j + 4 * g + r][16 * j + l16], all[r], xt[j]);
-    px[j] = split4<3>(xt[j]);
-  }
-#pragma unroll
-  for (int y = 0; y < 2; ++y) {
-    if (y > w / 2) continue;
-    char* at = out + x_at(w, y) + 16 * lane;
-#pragma unroll
-    for (int z = 0; z < 3; ++z) *reinterpret_cast<u64x2*>(at + z * kFragment) = u64x2{px[2 * y].p[z], px[2 * y + 1].p[z]};
+    for (int j = 0; j < 2 * (W / 2) + 2; ++j)
+      *reinterpret_cast<f32x4*>(out + (2 * x_at(W, j / 2) + j % 2) * kFragment + 16 * lane) = xt[j];
+  };
+  switch (w) {
+    case 0: return row_block(std::integral_constant<int, 0>());
+    case 1: return row_block(std::integral_constant<int, 1>());
+    case 2: return row_block(std::integral_constant<int, 2>());
+    default: return row_block(std::integral_constant<int, 3>());
   }
 }
 
@@ -401,32 +387,33 @@ __device__ __forceinline__ void barrier_only() {
 constexpr int kScanThreads = 64 * 12;
 
 // The states through the chunks: a workgroup for 16 NT value columns of a head.
-// What bounds it is the chain S -> W -> U -> S of one chunk after the other, so
-// its twelve waves divide the work such that nothing else stands in it:
-//   0-3  the chain: each 32 keys of S in its accumulators, as results of K^T U
-//        and as terms of K S (whose four partial sums pass through the LDS), and
-//        16 of the chunk's rows of W and U, which pass through the LDS as the
-//        next product's operand
-//   4-7  the outputs of 16 rows each, from S and U
-//   8-10 copy the chain's operands to the LDS, each group as soon as the last
-//        chunk's has been used (loads by the chain's waves hold them up: 64 bytes
-//        a cycle and CU, 0.6 us a chunk)
-//   11   reads what is needed three chunks on into the L2
+// What bounds it is the chain S -> W -> U -> S of one chunk after the other, and
+// beside it the bytes that a CU gets from its L2 (some 23 a cycle).  So its
+// twelve waves divide the work such that nothing else stands in the chain, and
+// K is read once for K S and K^T U:
+//   0-3   the chain: each 32 keys of S in its accumulators, as results of K^T U
+//         and as terms of K S (whose four partial sums pass through the LDS), and
+//         16 of the chunk's rows of W and U, which pass through the LDS as the
+//         next product's operand
+//   4-7   the outputs of 16 rows each, from S and U
+//   8     copies K, V and the rows' factors to the LDS (loads by the chain's
+//         waves would hold them up)
+//   9-11  split X
 // Three barriers a chunk: 1 the partial sums, 2 W, 3 U.
-// The slices of a head read the same X, P, K and Q, the heads of a k head the
-// same K and Q: they form a family, whose workgroups stand on one XCD, behind
-// one L2 (one prompt of 8192, 16 k and 32 v heads: 2.1 GB read past the L2s with
-// the slices dealt out, 0.3 so).
+// The slices of a head read the same X, K and Q, the heads of a k head the same
+// K and Q: they form a family, whose workgroups stand on one XCD, behind one L2
+// (the same prompt, 16 k and 32 v heads: 2.1 GB read past the L2s with the slices
+// dealt out, 0.3 so).
 template <int NT, bool VEC, int OUT>
 __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_kernel(const dft_prompt_gdn_args a, Work work, int families) {
   constexpr int BN = 16 * NT, kSlices = kD / BN, kSRow = kD + 8, kRow = kChunk + 8;
-  __shared__ __attribute__((aligned(16))) char k_lds[16 * kFragment], kt_lds[16 * kFragment], x_lds[18 * kFragment];
+  // K's fragments (step x, row tile m) at 4 x + m; what lane (row l16, terms 8 g ..) takes lies in its place key_place
+  __shared__ __attribute__((aligned(16))) char k_lds[2][16 * kFragment], x_lds[18 * kFragment];
   __shared__ __attribute__((aligned(16))) uint16_t v_lds[kChunk][BN];
-  __shared__ __attribute__((aligned(16))) float coef_lds[2][4][kChunk];
+  __shared__ __attribute__((aligned(16))) float coef_lds[2][kCoefs][kChunk];
   __shared__ __attribute__((aligned(16))) f32x4 sums[NT][4][4][64];  // [t][of wave][row tile][lane]
   __shared__ __attribute__((aligned(16))) uint16_t Sb[2][BN][kSRow];
   __shared__ __attribute__((aligned(16))) uint16_t Wb[3][BN][kRow], Ub[2][BN][kRow], Vb[3][BN][kRow];
-  __shared__ __attribute__((aligned(16))) char touched[kFragment];
   if (blockIdx.x == 0 && a.status)
     for (int b = threadIdx.x; b < a.batch; b += kScanThreads)
       a.status[b] = span_of(a, b).status | slot_of(a.state_indices, a.state_indices_dtype, a.initial, a.slots, b).status;
@@ -444,169 +431,137 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_kernel(const dft_pro
   const uint16_t* y = static_cast<const uint16_t*>(a.y);
   auto put = [&](uint16_t* to, uint64_t x) { *reinterpret_cast<uint64_t*>(to) = x; };
   auto get = [&](const uint16_t* from) { return *reinterpret_cast<const bf16x8*>(from); };
-  auto fragment = [&](const char* from) { return *reinterpret_cast<const bf16x8*>(from + 16 * lane); };
+  // where row i of a row tile has its terms 8 c ..: no two of 16 lanes that read side by side share a bank
+  auto key_place = [](int i, int c) { return 64 * i + 16 * (c ^ (i >> 2 & 3)); };
   // a row past the request's last is its last one
   auto row_at = [&](int at, int i) { return y + (s.r0 + min(at * kChunk + i, s.n - 1)) * a.y_row_stride; };
   auto head_at = [&](int at) { return work.heads + ((first + min(at, chunks - 1)) * a.hv + h) * kHead; };
-  auto keys_at = [&](int at) { return work.keys + ((first + min(at, chunks - 1)) * a.hk + kh) * kKeys; };
 
-  if (wave == 11) {
-    const int part = (member % kSlices) * 64 + lane, parts = kSlices * 64;
-    for (int at = 0; at < chunks; ++at) {
-      if (at) {
-        barrier_only();
-        barrier_only();
-      } else {
-        barrier_only();
-        barrier_only();
-        barrier_only();
-      }
-      // lines of 128 bytes: the head's block, K^T, the rows of Q, K and V
-      constexpr int kHeadLines = (kHead + 127) / 128, kKeyLines = kKeys / 128, kRowLines = 2 * kChunk;
-      const int to = at + 3;
-      if (to < chunks)
-        for (int line = part; line < kHeadLines + kKeyLines + 3 * kRowLines; line += parts) {
-          const char* from;
-          int x = line;
-          if (x < kHeadLines) {
-            from = head_at(to) + min(x * 128, kHead - 16);
-          } else if ((x -= kHeadLines) < kKeyLines) {
-            from = keys_at(to) + x * 128;
-          } else {
-            x -= kKeyLines;
-            const int which = x / kRowLines, row = x % kRowLines / 2;
-            const int head = which == 0 ? kh : which == 1 ? a.hk + kh : 2 * a.hk + h;
-            from = reinterpret_cast<const char*>(row_at(to, row) + head * kD) + x % 2 * 128;
-          }
-          copy16(from, touched);
+  if (wave >= 9) {
+    const int x0 = 2 * (wave - 9);  // the wave's two fragments
+    f32x4 from[2][2];
+    auto load_x = [&](int at) {
+      const char* head = head_at(at) + 16 * lane;
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) from[x][j] = *reinterpret_cast<const f32x4*>(head + (2 * (x0 + x) + j) * kFragment);
+    };
+    u64x2 to[2][3];
+    auto split = [&]() {
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const Parts4<3> lo = split4<3>(from[x][0]), hi = split4<3>(from[x][1]);
+#pragma unroll
+        for (int z = 0; z < 3; ++z) {
+          to[x][z] = u64x2{lo.p[z], hi.p[z]};
+          asm volatile("" : "+v"(to[x][z]));  // here, not behind the barrier
         }
-      barrier_only();
-    }
-    __builtin_amdgcn_s_waitcnt(wait_loads(0));
-    return;
-  }
-  if (wave == 8) {  // X; V and the rows' factors
-    auto copy_v = [&](int at) {
-#pragma unroll
-      for (int m = 0; m < 2 * NT; ++m)
-        copy16(row_at(at, (64 * m + lane) / (2 * NT)) + (2 * a.hk + h) * kD + c0 + (64 * m + lane) % (2 * NT) * 8,
-               reinterpret_cast<char*>(v_lds) + m * kFragment);
-      copy16(head_at(at) + kTriangle + 16 * lane, coef_lds[at & 1]);
+      }
     };
-    auto copy_x = [&](const char* head) {
+    auto write = [&]() {
 #pragma unroll
-      for (int m = 0; m < 18; ++m) copy16(head + m * kFragment + 16 * lane, x_lds + m * kFragment);
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int z = 0; z < 3; ++z) *reinterpret_cast<u64x2*>(x_lds + (3 * (x0 + x) + z) * kFragment + 16 * lane) = to[x][z];
     };
-    copy_v(0);
-    copy_x(head_at(0));
+    load_x(0);
+    split();
+    write();
+    load_x(1);
     barrier_only();
     for (int at = 0; at < chunks; ++at) {
-      __builtin_amdgcn_s_waitcnt(wait_loads(18));  // V
-      barrier_only();                              // 1
-      __builtin_amdgcn_s_waitcnt(wait_loads(0));   // X
-      barrier_only();                              // 2: V has been used
-      copy_v(at + 1);
-      barrier_only();  // 3: X has been used
-      copy_x(head_at(at + 1));
+      __syncthreads();  // 1
+      split();
+      barrier_only();  // 2: X has been read
+      write();
+      load_x(at + 2);
+      barrier_only();  // 3
     }
-    __builtin_amdgcn_s_waitcnt(wait_loads(0));
     return;
   }
-  if (wave == 9) {  // K
-    const uint16_t* row[4];  // rows 16 m + l16
-    auto rows = [&](int at) {
+  if (wave == 8) {
+    const int i = lane >> 2, c = (lane & 3) ^ (i >> 2 & 3);  // key_place
+    const uint16_t *k_row[4], *v_row[2 * NT];
+    const char* coef;
+    auto find_k = [&](int at) {
 #pragma unroll
-      for (int m = 0; m < 4; ++m) row[m] = row_at(at, 16 * m + l16) + (a.hk + kh) * kD + 8 * g;
+      for (int m = 0; m < 4; ++m) k_row[m] = row_at(at, 16 * m + i) + (a.hk + kh) * kD + 8 * c;
     };
-    auto copy_k = [&]() {
+    auto find_v = [&](int at) {
+#pragma unroll
+      for (int m = 0; m < 2 * NT; ++m)
+        v_row[m] = row_at(at, (64 * m + lane) / (2 * NT)) + (2 * a.hk + h) * kD + c0 + (64 * m + lane) % (2 * NT) * 8;
+      coef = head_at(at) + kX + kP + 16 * lane;
+    };
+    auto copy_k = [&](int at) {
 #pragma unroll
       for (int m = 0; m < 4; ++m)
 #pragma unroll
-        for (int x = 0; x < 4; ++x) copy16(row[m] + 32 * x, k_lds + (4 * x + m) * kFragment);
+        for (int x = 0; x < 4; ++x) copy16(k_row[m] + 32 * x, k_lds[at & 1] + (4 * x + m) * kFragment);
     };
-    rows(0);
-    copy_k();
-    __builtin_amdgcn_s_waitcnt(wait_loads(0));
-    barrier_only();
-    for (int at = 0; at < chunks; ++at) {
-      rows(at + 1);
-      barrier_only();  // 1: K has been used
-      copy_k();
-      barrier_only();  // 2
-      __builtin_amdgcn_s_waitcnt(wait_loads(0));
-      barrier_only();  // 3
-    }
-    return;
-  }
-  if (wave == 10) {  // K^T
-    barrier_only();
-    for (int at = 0; at < chunks; ++at) {
-      const char* keys = keys_at(at) + 16 * lane;
-      barrier_only();  // 1: the last chunk's has been used
+    auto copy_v = [&](int at) {
 #pragma unroll
-      for (int m = 0; m < 16; ++m) copy16(keys + m * kFragment, kt_lds + m * kFragment);
-      barrier_only();  // 2
-      __builtin_amdgcn_s_waitcnt(wait_loads(0));
-      barrier_only();  // 3
+      for (int m = 0; m < 2 * NT; ++m) copy16(v_row[m], reinterpret_cast<char*>(v_lds) + m * kFragment);
+#pragma unroll
+      for (int m = 0; m < 2; ++m) copy16(coef + m * kFragment, reinterpret_cast<char*>(coef_lds[at & 1]) + m * kFragment);
+    };
+    find_k(0);
+    find_v(0);
+    copy_k(0);
+    copy_v(0);
+    find_k(1);
+    copy_k(1);
+    __builtin_amdgcn_s_waitcnt(wait_loads(16));
+    barrier_only();
+    for (int at = 0; at < chunks; ++at) {
+      __builtin_amdgcn_s_waitcnt(wait_loads(16));  // V
+      barrier_only();                              // 1
+      find_v(at + 1);
+      find_k(at + 2);
+#pragma unroll
+      for (int m = 0; m < 4; ++m) asm volatile("" : "+v"(k_row[m]));  // here, not behind the barriers
+#pragma unroll
+      for (int m = 0; m < 2 * NT; ++m) asm volatile("" : "+v"(v_row[m]));
+      barrier_only();  // 2: V has been read
+      copy_v(at + 1);
+      __builtin_amdgcn_s_waitcnt(wait_loads(2 * NT + 2));  // the next K
+      barrier_only();                                      // 3: K has been read
+      copy_k(at + 2);
     }
+    __builtin_amdgcn_s_waitcnt(wait_loads(0));
     return;
   }
   if (wave >= 4) {
     const bool vec = a.o_dtype == DFT_F32 && reinterpret_cast<uintptr_t>(a.o) % 16 == 0 && a.o_row_stride % 4 == 0 && a.o_h_stride % 4 == 0;
     bf16x8 q[4], p[2][2];  // the wave's rows of Q and P
-    float rq;              // e^G rq of row l16
+    float decay, rq;       // of row l16
     auto load_q = [&](int at) {
       const uint16_t* row = row_at(at, 16 * w + l16) + kh * kD + 8 * g;
 #pragma unroll
       for (int j = 0; j < 4; ++j) q[j] = *reinterpret_cast<const bf16x8*>(row + 32 * j);
-      rq = reinterpret_cast<const float*>(head_at(at) + kTriangle)[4 * kChunk + 16 * w + l16];
     };
     auto load_p = [&](int at) {
-      const char* head = head_at(at) + 16 * lane;
+      const char* head = head_at(at) + kX;
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
         for (int z = 0; z < 2; ++z)
-          p[j][z] = *reinterpret_cast<const bf16x8*>(head + (j && w < 2 ? kTriangle + kCoef : p_at(w, j) + z * kFragment));
+          p[j][z] = *reinterpret_cast<const bf16x8*>(head + (p_at(w, j) + (j && w < 2 ? 0 : z)) * kFragment + 16 * lane);
+      const float* coef = reinterpret_cast<const float*>(head + kP) + 16 * w + l16;
+      decay = coef[kDecay * kChunk];
+      rq = coef[kRq * kChunk];
     };
+    int64_t o_at = (s.r0 + 16 * w + l16) * a.o_row_stride + h * a.o_h_stride + c0 + 4 * g;
     load_q(0);
     load_p(0);
     barrier_only();
-    for (int at = 0; at < chunks; ++at) {
-      f32x4 o[NT];
-      __syncthreads();
+    f32x4 o[NT];
+    auto store_rows = [&](int at) {
+      if (at * kChunk + 16 * w + l16 < s.n) {
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        f32x4 q0 = {}, q1 = {};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          q0 = mfma16(get(&Sb[0][16 * t + l16][32 * j + 8 * g]), q[j], q0);
-          q1 = mfma16(get(&Sb[1][16 * t + l16][32 * j + 8 * g]), q[j], q1);
-        }
-        o[t] = (q0 + q1) * rq;
-      }
-      load_q(at + 1);
-      __syncthreads();
-      __syncthreads();
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        f32x4 o1 = {};
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const bf16x8 u0 = get(&Ub[0][16 * t + l16][32 * j + 8 * g]);
-          const bf16x8 u1 = get(&Ub[1][16 * t + l16][32 * j + 8 * g]);
-          o[t] = mfma16(u0, p[j][0], o[t]);
-          o1 = mfma16(u1, p[j][0], o1);
-          o1 = mfma16(u0, p[j][1], o1);
-        }
-        o[t] += o1;
-      }
-      load_p(at + 1);
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const int i = at * kChunk + 16 * w + l16;
-        if (i < s.n) {
-          const int64_t to = (s.r0 + i) * a.o_row_stride + h * a.o_h_stride + c0 + 16 * t + 4 * g;
+        for (int t = 0; t < NT; ++t) {
+          const int64_t to = o_at + 16 * t;
           if constexpr (OUT == kBf16Out) {
             typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
             *reinterpret_cast<bf16x4*>(static_cast<uint16_t*>(a.o) + to) = __builtin_convertvector(o[t], bf16x4);
@@ -618,7 +573,43 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_kernel(const dft_pro
           }
         }
       }
+      o_at += kChunk * a.o_row_stride;
+    };
+    // between barriers 3 and 1, which the chain passes fastest, only the products
+    for (int at = 0; at < chunks; ++at) {
+      __syncthreads();  // 1: S is there
+      if (at) {
+        store_rows(at - 1);
+        load_p(at);
+      }
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        f32x4 q0 = {}, q1 = {};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          q0 = mfma16(get(&Sb[0][16 * t + l16][32 * j + 8 * g]), q[j], q0);
+          q1 = mfma16(get(&Sb[1][16 * t + l16][32 * j + 8 * g]), q[j], q1);
+        }
+        o[t] = (q0 + q1) * decay;
+      }
+      load_q(at + 1);
+      __syncthreads();  // 2
+      __syncthreads();  // 3: U is there
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        f32x4 o0 = o[t], o1 = {};
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const bf16x8 u0 = get(&Ub[0][16 * t + l16][32 * j + 8 * g]);
+          const bf16x8 u1 = get(&Ub[1][16 * t + l16][32 * j + 8 * g]);
+          o0 = mfma16(u0, p[j][0], o0);
+          o1 = mfma16(u1, p[j][0], o1);
+          o1 = mfma16(u0, p[j][1], o1);
+        }
+        o[t] = (o0 + o1) * rq;
+      }
     }
+    store_rows(chunks - 1);
     return;
   }
 
@@ -641,14 +632,25 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_kernel(const dft_pro
         for (int r = 0; r < 4; ++r) S[x][t][r] = state[key_at(x, t) + r * a.state_k_stride];
     }
   const int place = 32 * (w / 2) + 8 * g + 4 * (w % 2);  // of the lane's rows 16 w + 4 g .. as terms
+  // K^T: row tile x of the wave's keys, terms of step j.  A transposing read hands 16 lanes' pieces of 4 keys (piece lane %
+  // 4) in 4 rows (lane / 4 % 4) out by the keys: lane l16 gets key 32 w + 8 (l16 / 4) + 4 x + l16 % 4.
+  auto transposed = [&](const char* keys, int x, int j) {
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) s16x4* Lds;
+    const int at = key_place(4 * g + (l16 >> 2), lane & 3) + 8 * x;
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(keys + 2 * j * kFragment + at));
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(keys + (2 * j + 1) * kFragment + at));
+    return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+  };
   __builtin_amdgcn_s_setprio(2);
   __syncthreads();
   for (int at = 0; at < chunks; ++at) {
     const float(*coef)[kChunk] = coef_lds[at & 1];
+    const char* keys = k_lds[at & 1] + 4 * w * kFragment;
     f32x4 u[NT];
     bf16x8 k[4];
 #pragma unroll
-    for (int m = 0; m < 4; ++m) k[m] = fragment(k_lds + (4 * w + m) * kFragment);
+    for (int m = 0; m < 4; ++m) k[m] = *reinterpret_cast<const bf16x8*>(keys + m * kFragment + key_place(l16, g));
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       const Parts4<3> lo = split4<3>(S[0][t]), hi = split4<3>(S[1][t]);
@@ -665,11 +667,9 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_kernel(const dft_pro
 #pragma unroll
       for (int m = 0; m < 4; ++m) sums[t][w][m][lane] = sum[m];
     }
-    __syncthreads();
-    const f32x4 beta = *reinterpret_cast<const f32x4*>(&coef[0][16 * w + 4 * g]);
-    const f32x4 decayed = *reinterpret_cast<const f32x4*>(&coef[1][16 * w + 4 * g]);
-    const f32x4 out = *reinterpret_cast<const f32x4*>(&coef[2][16 * w + 4 * g]);
-    const float keep = coef[3][0];
+    __syncthreads();  // 1
+    const f32x4 beta = *reinterpret_cast<const f32x4*>(&coef[kBeta][16 * w + 4 * g]);
+    const f32x4 decayed = *reinterpret_cast<const f32x4*>(&coef[kDecayed][16 * w + 4 * g]);
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       const f32x4 ks = (sums[t][0][w][lane] + sums[t][1][w][lane]) + (sums[t][2][w][lane] + sums[t][3][w][lane]);
@@ -681,7 +681,21 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_kernel(const dft_pro
 #pragma unroll
       for (int z = 0; z < 3; ++z) put(&Wb[z][16 * t + l16][place], p.p[z]);
     }
-    __syncthreads();
+    // what the next products take beside W and U
+    bf16x8 X[2][3], kt[2][2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int z = 0; z < 3; ++z)
+        X[j][z] = *reinterpret_cast<const bf16x8*>(x_lds + (3 * x_at(w, min(j, w / 2)) + z) * kFragment + 16 * lane);
+    const f32x4 unit = *reinterpret_cast<const f32x4*>(&coef[kUnit][16 * w + 4 * g]);
+    const f32x4 out = *reinterpret_cast<const f32x4*>(&coef[kOut][16 * w + 4 * g]);
+    const float keep = coef[kKeep][0];
+    __syncthreads();  // 2
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) kt[x][j] = transposed(keys, x, j);
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       f32x4 u1 = {}, u2 = {};
@@ -691,16 +705,14 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_kernel(const dft_pro
         const bf16x8 w0 = get(&Wb[0][16 * t + l16][32 * j + 8 * g]);
         const bf16x8 w1 = get(&Wb[1][16 * t + l16][32 * j + 8 * g]);
         const bf16x8 w2 = get(&Wb[2][16 * t + l16][32 * j + 8 * g]);
-        const char* at = x_lds + x_at(w, j);
-        const bf16x8 x0 = fragment(at), x1 = fragment(at + kFragment), x2 = fragment(at + 2 * kFragment);
-        u1 = mfma16(x0, w0, u1);
-        u2 = mfma16(x1, w0, u2);
-        u1 = mfma16(x0, w1, u1);
-        u2 = mfma16(x2, w0, u2);
-        u1 = mfma16(x0, w2, u1);
-        u2 = mfma16(x1, w1, u2);
+        u1 = mfma16(X[j][0], w0, u1);
+        u2 = mfma16(X[j][1], w0, u2);
+        u1 = mfma16(X[j][0], w1, u1);
+        u2 = mfma16(X[j][2], w0, u2);
+        u1 = mfma16(X[j][0], w2, u1);
+        u2 = mfma16(X[j][1], w1, u2);
       }
-      u[t] += u1 + u2;
+      u[t] = (u[t] + (u1 + u2)) * unit;
       const Parts4<3> d = split4<3>(u[t] * out);
 #pragma unroll
       for (int z = 0; z < 3; ++z) put(&Vb[z][16 * t + l16][place], d.p[z]);
@@ -708,12 +720,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_kernel(const dft_pro
 #pragma unroll
       for (int z = 0; z < 2; ++z) put(&Ub[z][16 * t + l16][place], p.p[z]);
     }
-    __syncthreads();
-    bf16x8 kt[2][2];
-#pragma unroll
-    for (int x = 0; x < 2; ++x)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) kt[x][j] = fragment(kt_lds + (2 * (2 * w + x) + j) * kFragment);
+    __syncthreads();  // 3
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       f32x4 add[2] = {};
@@ -779,7 +786,7 @@ int64_t prompt_gdn_blocks(const dft_prompt_gdn_args* a) {
   return std::max(((int64_t)a->batch * a->hv + kXcds * a->hv) * 8 * 2, by_rows(*a) ? 0 : tiles_of(*a) * a->hv);
 }
 int64_t prompt_gdn_workspace(const dft_prompt_gdn_args* a) {
-  return by_rows(*a) ? 0 : tiles_of(*a) * ((int64_t)a->hv * kHead + (int64_t)a->hk * kKeys);
+  return by_rows(*a) ? 0 : tiles_of(*a) * a->hv * kHead;
 }
 
 int launch_prompt_gdn(const dft_prompt_gdn_args* a, hipStream_t stream) {
@@ -793,10 +800,12 @@ int launch_prompt_gdn(const dft_prompt_gdn_args* a, hipStream_t stream) {
   }
   Work work;
   work.heads = static_cast<char*>(a->workspace);
-  work.keys = work.heads + tiles_of(*a) * a->hv * kHead;
   gdn_chunk_kernel<<<(unsigned)(tiles_of(*a) * a->hv), 256, 0, stream>>>(*a, work);
   if (hipGetLastError() != hipSuccess) return DFT_ERR_LAUNCH;
-  return launch_scan<1>(*a, work, stream);
+  // 16 value columns a workgroup, or 32 at 1.4 times the time a chunk: the longest request's chunks one after the other,
+  // or all of them over the CUs (us: one prompt of 8192, 32 heads, 275 and 384; six of 257 to 2999 361 and 317)
+  const double longest = std::min(a->rows, (int64_t)a->max_len) / 64.0, all = (a->rows / 64.0 + a->batch / 2.0) * a->hv / 256;
+  return std::max(longest, 8 * all) <= 1.4 * std::max(longest, 4 * all) ? launch_scan<1>(*a, work, stream) : launch_scan<2>(*a, work, stream);
 }
 
 }  // namespace dft
