@@ -28,24 +28,31 @@ namespace {
 using namespace packed;
 
 constexpr int kD = 128;
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 // g and beta of one row and head
 struct Gate {
   float g, beta;
 };
-__device__ __forceinline__ Gate gate_of(const dft_prompt_gdn_args& a, int64_t row, int h) {
-  const float rate = a.neg_exp_A ? a.neg_exp_A[h] : -expf(ld_f(a.A_log, h, a.A_log_dtype));
-  const float x = ld_f(a.a, row * a.a_row_stride + h, a.a_dtype) + ld_f(a.dt_bias, h, a.dt_bias_dtype);
-  const float soft = x > 20.f ? x : log1pf(expf(x));
-  return {rate * soft, 1.f / (1.f + expf(-ld_f(a.b, row * a.b_row_stride + h, a.b_dtype)))};
-}
+struct GateOf {  // of a head
+  float rate, bias;
+  __device__ __forceinline__ GateOf(const dft_prompt_gdn_args& a, int h)
+      : rate(a.neg_exp_A ? a.neg_exp_A[h] : -expf(ld_f(a.A_log, h, a.A_log_dtype))), bias(ld_f(a.dt_bias, h, a.dt_bias_dtype)) {}
+  __device__ __forceinline__ Gate operator()(float a, float b) const {
+    const float x = a + bias, soft = x > 20.f ? x : log1pf(expf(x));
+    return {rate * soft, 1.f / (1.f + expf(-b))};
+  }
+};
+__device__ __forceinline__ float gate_a(const dft_prompt_gdn_args& a, int64_t row, int h) { return ld_f(a.a, row * a.a_row_stride + h, a.a_dtype); }
+__device__ __forceinline__ float gate_b(const dft_prompt_gdn_args& a, int64_t row, int h) { return ld_f(a.b, row * a.b_row_stride + h, a.b_dtype); }
 
-// The sum over a row of 16 lanes, in all of them.
+// The sum over a row of 16 lanes, in all of them: rotations by 8, 4, 2 and 1
+// within the row.
 __device__ __forceinline__ float sum16(float x) {
-  x += __shfl_xor(x, 1);
-  x += __shfl_xor(x, 2);
-  x += __shfl_xor(x, 4);
-  x += __shfl_xor(x, 8);
+  x += __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(x), 0x128, 0xf, 0xf, true));
+  x += __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(x), 0x124, 0xf, 0xf, true));
+  x += __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(x), 0x122, 0xf, 0xf, true));
+  x += __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(x), 0x121, 0xf, 0xf, true));
   return x;
 }
 
@@ -55,16 +62,16 @@ __device__ __forceinline__ float sum16(float x) {
 // a wave's access covers whole columns and both sums over the keys stay within
 // 16 lanes.
 template <int V, bool VEC>
-__global__ void __launch_bounds__(256) gdn_rows_kernel(const dft_prompt_gdn_args a) {
+__global__ void __launch_bounds__(256) gdn_rows_kernel(const dft_prompt_gdn_args a, int most) {
   constexpr int kSplit = kD / V, kPass = V / 16;
   const int64_t x = blockIdx.x;
   if (x == 0 && a.status)
     for (int b = threadIdx.x; b < a.batch; b += 256)
       a.status[b] = span_of(a, b).status | slot_of(a.state_indices, a.state_indices_dtype, a.initial, a.slots, b).status;
   const int per = a.hv * kSplit;
-  const int b = (int)(x / per), r = (int)(x - (int64_t)b * per), h = r / kSplit, part = r - h * kSplit;
+  const int b = (int)(x / per), in = (int)(x - (int64_t)b * per), h = in / kSplit, part = in - h * kSplit;
   const Span s = span_of(a, b);
-  if (s.n <= 0) return;
+  if (s.n <= 0 || s.n > most) return;
   const Slot slot = slot_of(a.state_indices, a.state_indices_dtype, a.initial, a.slots, b);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, quad = lane >> 4;
   const int kh = h / (a.hv / a.hk), v0 = part * V + wave * (V / 4) + quad;  // + 4 pass: the lane's value columns
@@ -89,16 +96,36 @@ __global__ void __launch_bounds__(256) gdn_rows_kernel(const dft_prompt_gdn_args
       for (int e = 0; e < 8; ++e) S[p][e] = state[at(p, e)];
     }
   }
-  const uint16_t* y = static_cast<const uint16_t*>(a.y);
+  // a row's inputs, fetched a row ahead
+  struct Row {
+    u32x2 q[2], k[2];
+    uint16_t v[kPass];
+    float a, b;
+  };
+  const uint16_t* y = static_cast<const uint16_t*>(a.y) + s.r0 * a.y_row_stride;
+  auto fetch = [&](Row& r, int t) {
+    const uint16_t* yr = y + t * a.y_row_stride;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      r.q[x] = *reinterpret_cast<const u32x2*>(yr + kh * kD + 4 * i + 64 * x);
+      r.k[x] = *reinterpret_cast<const u32x2*>(yr + (a.hk + kh) * kD + 4 * i + 64 * x);
+    }
+#pragma unroll
+    for (int p = 0; p < kPass; ++p) r.v[p] = yr[(2 * a.hk + h) * kD + v0 + 4 * p];
+    r.a = gate_a(a, s.r0 + t, h);
+    r.b = gate_b(a, s.r0 + t, h);
+  };
+  const GateOf gate(a, h);
+  Row r;
+  fetch(r, 0);
   for (int t = 0; t < s.n; ++t) {
-    const int64_t row = s.r0 + t;
-    const uint16_t* yr = y + row * a.y_row_stride;
+    Row next;
+    fetch(next, min(t + 1, s.n - 1));
     float q[8], k[8], qq = 0, kk = 0, qk = 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const int c = kh * kD + 4 * i + (e & 3) + (e >> 2) * 64;
-      q[e] = bf16_bits_to_f32(yr[c]);
-      k[e] = bf16_bits_to_f32(yr[a.hk * kD + c]);
+      q[e] = bf16_bits_to_f32(r.q[e >> 2][e >> 1 & 1] >> (e & 1) * 16);
+      k[e] = bf16_bits_to_f32(r.k[e >> 2][e >> 1 & 1] >> (e & 1) * 16);
       qq = fmaf(q[e], q[e], qq);
       kk = fmaf(k[e], k[e], kk);
     }
@@ -110,8 +137,9 @@ __global__ void __launch_bounds__(256) gdn_rows_kernel(const dft_prompt_gdn_args
       qk = fmaf(q[e], k[e], qk);
     }
     qk = sum16(qk);
-    const Gate g = gate_of(a, row, h);
+    const Gate g = gate(r.a, r.b);
     const float decay = expf(g.g);
+    float out = 0;
 #pragma unroll
     for (int p = 0; p < kPass; ++p) {
       float kS = 0, qS = 0;
@@ -123,12 +151,13 @@ __global__ void __launch_bounds__(256) gdn_rows_kernel(const dft_prompt_gdn_args
       }
       kS = sum16(kS);
       qS = sum16(qS);
-      const int v = v0 + 4 * p;
-      const float u = g.beta * (bf16_bits_to_f32(yr[2 * a.hk * kD + h * kD + v]) - kS);
+      const float u = g.beta * (bf16_bits_to_f32(r.v[p]) - kS);
 #pragma unroll
       for (int e = 0; e < 8; ++e) S[p][e] = fmaf(k[e], u, S[p][e]);
-      if (i == p) store(a.o, row * a.o_row_stride + h * a.o_h_stride + v, a.o_dtype, fmaf(qk, u, qS));
+      if (i == p) out = fmaf(qk, u, qS);
     }
+    if (i < kPass) store(a.o, (s.r0 + t) * a.o_row_stride + h * a.o_h_stride + v0 + 4 * i, a.o_dtype, out);
+    r = next;
   }
   if (slot.at < 0) return;
 #pragma unroll
@@ -152,7 +181,7 @@ __global__ void __launch_bounds__(256) gdn_rows_kernel(const dft_prompt_gdn_args
 // product's operand without an exchange wherever both operands agree on it:
 // terms that are chunk rows stand in the order
 //   32 s + 16 h + 4 g + e  at place  32 s + 8 g + 4 h + e.
-constexpr int kChunk = 64, kXcds = 8;
+constexpr int kChunk = 64, kXcds = 8, kCus = 256;
 constexpr int kFragment = 1024;  // bytes: 64 lanes x 16
 // X - I, whose upper half is zero, in fp32: its row tile m (of 16) has steps 0 ..
 // m / 2, six fragments of 8 elements a lane, the first four of every lane first.
@@ -205,7 +234,7 @@ typedef uint64_t u64x2 __attribute__((ext_vector_type(2)));
 // (their powers would lose what equal keys leave of 32 bits), then X_ij =
 // -(sum_(j<m<=i) X_im A_mj) X_jj in fp32 products, transposed, so that each result
 // is the next one's operand and the last the fragment that is stored.
-__global__ void __launch_bounds__(256) gdn_chunk_kernel(const dft_prompt_gdn_args a, Work work) {
+__global__ void __launch_bounds__(256) gdn_chunk_kernel(const dft_prompt_gdn_args a, Work work, int past) {
   constexpr int kKRow = kD + 8, kARow = kChunk + 4;
   __shared__ __attribute__((aligned(16))) uint16_t keys[kChunk][kKRow];
   __shared__ __attribute__((aligned(16))) float A[kChunk][kARow];
@@ -215,6 +244,7 @@ __global__ void __launch_bounds__(256) gdn_chunk_kernel(const dft_prompt_gdn_arg
   const int b = find_tile<256>(a, tile, kChunk);
   if (b < 0) return;
   const Span s = span_of(a, b);
+  if (s.n <= past) return;
   const int t0 = (int)(tile - first_tile(s.r0, b, kChunk)) * kChunk, n = min(s.n - t0, kChunk);
   const int64_t r0 = s.r0 + t0;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, g = lane >> 4;
@@ -230,7 +260,8 @@ __global__ void __launch_bounds__(256) gdn_chunk_kernel(const dft_prompt_gdn_arg
   Gate gate = {};
   float sum = 0, all = 0;
   if (w == 0) {  // the gates, a row a lane, G in log2 units
-    gate = gate_of(a, r0 + min(lane, n - 1), h);
+    const int64_t r = r0 + min(lane, n - 1);
+    gate = GateOf(a, h)(gate_a(a, r, h), gate_b(a, r, h));
     if (lane >= n) gate.g = gate.beta = 0;
     sum = gate.g * 1.4426950408889634f;
 #pragma unroll
@@ -405,7 +436,7 @@ constexpr int kScanThreads = 64 * 12;
 // (the same prompt, 16 k and 32 v heads: 2.1 GB read past the L2s with the slices
 // dealt out, 0.3 so).
 template <int NT, bool VEC, int OUT>
-__global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_kernel(const dft_prompt_gdn_args a, Work work, int families) {
+__global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_kernel(const dft_prompt_gdn_args a, Work work, int families, int past) {
   constexpr int BN = 16 * NT, kSlices = kD / BN, kSRow = kD + 8, kRow = kChunk + 8;
   // K's fragments (step x, row tile m) at 4 x + m; what lane (row l16, terms 8 g ..) takes lies in its place key_place
   __shared__ __attribute__((aligned(16))) char k_lds[2][16 * kFragment], x_lds[18 * kFragment];
@@ -423,7 +454,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_kernel(const dft_pro
   if (family >= families) return;
   const int unit = family * (members / kSlices) + member / kSlices, slice = member % kSlices, b = unit / a.hv, h = unit - b * a.hv;
   const Span s = span_of(a, b);
-  if (s.n <= 0) return;
+  if (s.n <= past) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, g = lane >> 4;
   const int w = wave & 3, kh = h / (a.hv / a.hk), c0 = slice * BN;
   const int64_t first = first_tile(s.r0, b, kChunk);
@@ -761,51 +792,78 @@ bool vector_state(const dft_prompt_gdn_args& a) {
          a.state_h_stride % 4 == 0 && a.state_slot_stride % 4 == 0;
 }
 
-bool by_rows(const dft_prompt_gdn_args& a) { return a.max_len <= 2; }
+// Up to so many rows a request is taken row by row, by a launch of its own where
+// others are longer.  us for one request of 32 heads: 6.5, 11.8 and 19.1 for 1, 4
+// and 8 rows, 14.7 as a chunk of any length; 16 requests 12.4, 22.6, 35.2 and 61
+// as chunks; 64 requests 49, 68, 106 and 205.  With few of them the second launch
+// (2) costs more than the chunks of short requests, which run beside the others.
+struct Split {
+  int rows;
+  bool both;
+};
+Split split_of(const dft_prompt_gdn_args& a) {
+  const bool many = (int64_t)a.batch * a.hv >= 512;
+  const int rows = many ? 16 : 4;
+  if (a.max_len <= rows) return {rows, false};
+  return many && a.cu_seqlens ? Split{rows, true} : Split{0, false};
+}
+bool all_by_rows(const dft_prompt_gdn_args& a) { return a.max_len <= split_of(a).rows; }
 int64_t tiles_of(const dft_prompt_gdn_args& a) { return line_tiles(a.rows, a.batch, kChunk); }
 
+int launch_rows(const dft_prompt_gdn_args& a, int most, hipStream_t stream) {
+  // With few heads a fourth of the columns each (one request: 5.4 us, 6.5 whole; 64 requests: 57 and 49)
+  const int64_t heads = (int64_t)a.batch * a.hv;
+  const bool few = heads <= 128, vec = vector_state(a);
+  const unsigned blocks = (unsigned)(few ? 4 * heads : heads);
+  if (few && vec)
+    gdn_rows_kernel<32, true><<<blocks, 256, 0, stream>>>(a, most);
+  else if (few)
+    gdn_rows_kernel<32, false><<<blocks, 256, 0, stream>>>(a, most);
+  else if (vec)
+    gdn_rows_kernel<128, true><<<blocks, 256, 0, stream>>>(a, most);
+  else
+    gdn_rows_kernel<128, false><<<blocks, 256, 0, stream>>>(a, most);
+  return hipGetLastError() == hipSuccess ? DFT_OK : DFT_ERR_LAUNCH;
+}
+
 template <int NT>
-int launch_scan(const dft_prompt_gdn_args& a, const Work& work, hipStream_t stream) {
+int launch_scan(const dft_prompt_gdn_args& a, const Work& work, int past, hipStream_t stream) {
   // by k heads where there is one for every XCD, else by v heads
   const int families = a.batch * (a.batch * a.hk >= kXcds ? a.hk : a.hv);
   const unsigned blocks = (unsigned)((families + kXcds - 1) / kXcds * kXcds * (a.batch * a.hv / families * (8 / NT)));
   const bool bf16 = a.o_dtype == DFT_BF16 && reinterpret_cast<uintptr_t>(a.o) % 8 == 0 && a.o_row_stride % 4 == 0 && a.o_h_stride % 4 == 0;
   if (!vector_state(a))
-    gdn_scan_kernel<NT, false, kAnyOut><<<blocks, kScanThreads, 0, stream>>>(a, work, families);
+    gdn_scan_kernel<NT, false, kAnyOut><<<blocks, kScanThreads, 0, stream>>>(a, work, families, past);
   else if (bf16)
-    gdn_scan_kernel<NT, true, kBf16Out><<<blocks, kScanThreads, 0, stream>>>(a, work, families);
+    gdn_scan_kernel<NT, true, kBf16Out><<<blocks, kScanThreads, 0, stream>>>(a, work, families, past);
   else
-    gdn_scan_kernel<NT, true, kAnyOut><<<blocks, kScanThreads, 0, stream>>>(a, work, families);
+    gdn_scan_kernel<NT, true, kAnyOut><<<blocks, kScanThreads, 0, stream>>>(a, work, families, past);
   return hipGetLastError() == hipSuccess ? DFT_OK : DFT_ERR_LAUNCH;
 }
 
 }  // namespace
 
-// the most workgroups of a launch
+// the most workgroups of a launch, in units of 256 threads
 int64_t prompt_gdn_blocks(const dft_prompt_gdn_args* a) {
-  return std::max(((int64_t)a->batch * a->hv + kXcds * a->hv) * 8 * 2, by_rows(*a) ? 0 : tiles_of(*a) * a->hv);
+  // the scan's are three such, and padded to a multiple of the XCDs
+  return std::max(((int64_t)a->batch * a->hv + kXcds * a->hv) * 8 * (kScanThreads / 256), all_by_rows(*a) ? 0 : tiles_of(*a) * a->hv);
 }
-int64_t prompt_gdn_workspace(const dft_prompt_gdn_args* a) {
-  return by_rows(*a) ? 0 : tiles_of(*a) * a->hv * kHead;
-}
+int64_t prompt_gdn_workspace(const dft_prompt_gdn_args* a) { return all_by_rows(*a) ? 0 : tiles_of(*a) * a->hv * kHead; }
 
 int launch_prompt_gdn(const dft_prompt_gdn_args* a, hipStream_t stream) {
-  if (by_rows(*a)) {
-    const unsigned blocks = (unsigned)((int64_t)a->batch * a->hv);
-    if (vector_state(*a))
-      gdn_rows_kernel<128, true><<<blocks, 256, 0, stream>>>(*a);
-    else
-      gdn_rows_kernel<128, false><<<blocks, 256, 0, stream>>>(*a);
-    return hipGetLastError() == hipSuccess ? DFT_OK : DFT_ERR_LAUNCH;
+  const Split split = split_of(*a);
+  if (all_by_rows(*a) || split.both) {
+    const int st = launch_rows(*a, split.rows, stream);
+    if (st != DFT_OK || !split.both) return st;
   }
-  Work work;
-  work.heads = static_cast<char*>(a->workspace);
-  gdn_chunk_kernel<<<(unsigned)(tiles_of(*a) * a->hv), 256, 0, stream>>>(*a, work);
+  const Work work = {static_cast<char*>(a->workspace)};
+  gdn_chunk_kernel<<<(unsigned)(tiles_of(*a) * a->hv), 256, 0, stream>>>(*a, work, split.rows);
   if (hipGetLastError() != hipSuccess) return DFT_ERR_LAUNCH;
   // 16 value columns a workgroup, or 32 at 1.4 times the time a chunk: the longest request's chunks one after the other,
   // or all of them over the CUs (us: one prompt of 8192, 32 heads, 275 and 384; six of 257 to 2999 361 and 317)
-  const double longest = std::min(a->rows, (int64_t)a->max_len) / 64.0, all = (a->rows / 64.0 + a->batch / 2.0) * a->hv / 256;
-  return std::max(longest, 8 * all) <= 1.4 * std::max(longest, 4 * all) ? launch_scan<1>(*a, work, stream) : launch_scan<2>(*a, work, stream);
+  const double longest = std::min(a->rows, (int64_t)a->max_len) / 64.0, all = (a->rows / 64.0 + a->batch / 2.0) * a->hv / kCus;
+  return std::max(longest, 8 * all) <= 1.4 * std::max(longest, 4 * all) ? launch_scan<1>(*a, work, split.rows, stream)
+                                                                        : launch_scan<2>(*a, work, split.rows, stream);
 }
 
 }  // namespace dft

@@ -89,6 +89,23 @@ def test_packed(cuda, sizes, hk, hv):
     c.check(cu, batch=B, limit=max(sizes), cu_host=host, indices=slots_of(B, B + 2, cuda), initial=init, label=str(sizes))
 
 
+@pytest.mark.parametrize("sizes", [[1] * 200 + [300, 2, 16, 17, 15, 0, 64], [16] * 40 + [17] * 40, [5] * 140])
+def test_many_requests_short_and_long(cuda, sizes):
+    """From 512 heads on short requests go row by row beside long ones' chunks."""
+    host, cu = cu_of(sizes, cuda)
+    B = len(sizes)
+    c = Case(sum(sizes), 2, 8, B + 2, cuda, seed=B)
+    init = torch.tensor([i % 3 != 1 for i in range(B)], device=cuda)
+    c.check(cu, batch=B, limit=max(sizes), cu_host=host, indices=slots_of(B, B + 2, cuda), initial=init, label="mixed")
+
+
+def test_a_long_prompt(cuda):
+    """Errors do not grow from chunk to chunk: 2500 rows, and states that keep them all."""
+    for decay in (1e-3, 1.0):
+        c = Case(2500, 1, 1, 1, cuda, seed=20, decay=decay)
+        c.check(batch=1, limit=2500, o_dtype=F32, label=f"2500 rows, decay {decay}")
+
+
 @pytest.mark.parametrize("hk,hv,batch", [(1, 1, 1), (1, 3, 2), (2, 8, 5), (16, 32, 3), (4, 4, 300)])
 def test_tokens(cuda, hk, hv, batch):
     from dforktree_amd import ops

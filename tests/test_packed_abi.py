@@ -103,6 +103,35 @@ def test_refused_before_any_launch(name, make, status, cases):
     assert fn(ctypes.byref(a), None) == _lib.DFT_OK
 
 
+@pytest.mark.parametrize("name,make,bad", [("dft_prompt_gdn", gdn_args, dict(hv=3, hk=2))])
+def test_workspace_is_asked_for_and_checked(name, make, bad):
+    """Its size is known before there are buffers; a launch with less of it, or an unaligned one, is refused."""
+    from dforktree_amd import _lib
+    lib = _lib.load()
+    n, a = ctypes.c_int64(-1), make()
+    if name == "dft_prompt_gdn":
+        a.max_len, a.rows = 300, 600
+    size = getattr(lib, name + "_workspace")
+    assert size(ctypes.byref(a), None) == _lib.DFT_ERR_INVALID
+    blank = type(a)()
+    for f, t in a._fields_:
+        if t is not ctypes.c_void_p:
+            setattr(blank, f, getattr(a, f))
+    assert size(ctypes.byref(blank), ctypes.byref(n)) == _lib.DFT_OK and n.value > 0
+    for k, v in bad.items():
+        setattr(blank, k, v)
+    want = n.value
+    assert size(ctypes.byref(blank), ctypes.byref(n)) == _lib.DFT_ERR_INVALID and n.value == 0
+    for change in (dict(workspace=None), dict(workspace=24), dict(workspace_bytes=want - 1)):
+        b = make()
+        b.rows = a.rows
+        if name == "dft_prompt_gdn":
+            b.max_len = a.max_len
+        for k, v in change.items():
+            setattr(b, k, v)
+        assert getattr(lib, name)(ctypes.byref(b), None) == _lib.DFT_ERR_INVALID, change
+
+
 def test_operators_take_gpu_tensors():
     import torch
     from dforktree_amd import ops
