@@ -103,7 +103,8 @@ def test_refused_before_any_launch(name, make, status, cases):
     assert fn(ctypes.byref(a), None) == _lib.DFT_OK
 
 
-@pytest.mark.parametrize("name,make,bad", [("dft_prompt_gdn", gdn_args, dict(hv=3, hk=2))])
+@pytest.mark.parametrize("name,make,bad", [("dft_prompt_gdn", gdn_args, dict(hv=3, hk=2)),
+                                           ("dft_tree_accept", accept_args, dict(path_cols=0))])
 def test_workspace_is_asked_for_and_checked(name, make, bad):
     """Its size is known before there are buffers; a launch with less of it, or an unaligned one, is refused."""
     from dforktree_amd import _lib
