@@ -6,10 +6,20 @@
 // max(r - q, 0) where a refused child has another sibling, and r's running sum
 // at the end.  Such a pass over a row is cut into slices, a workgroup each.  A
 // launch does one pass for every request, whatever it is of that request's; the
-// next one walks again, with the sums there are, to the next pass.  Without the
-// drafter's probabilities the first pass is the last; with them kRounds launches
-// are made, and what is still open is done by the request's workgroup alone in
-// the last launch, which finds the token.
+// next one walks again, with the sums there are, to the next pass, until a walk's
+// last.  Without the drafter's probabilities the first pass is the last; with
+// them kRounds launches are made, and what is still open is done by the request's
+// workgroup alone in the last launch, which finds the token from the sums of its
+// slice: a slice's tokens side by side, added up over the workgroup.
+//
+// Bound by launches and by the walk's dependent fetches where passes are few: 23
+// us for one request of 16 nodes over 131072 tokens, 34 for 64 drawn chains, 22
+// for 64 trees of 32 nodes without a drafter's rows; of these the last launch is 8
+// to 12, and a launch that finds nothing to do costs 1.6.  48 drawn trees of 8 to
+// 40 nodes over 100003 tokens take 69: with two rounds, and a request's further
+// passes by its workgroup alone, 180.  Their passes are bound by the 64-bit units:
+// a reduction divides by two numbers that are the same for the whole row, so it
+// multiplies by their reciprocals.
 //
 // Sums are held in 64 bits: a sum of 10^5 probabilities in 32 bits moves one
 // drawn token in some hundred over a border.  They are added up in one order.
@@ -20,8 +30,8 @@
 namespace dft {
 namespace {
 
-constexpr int kNodes = 64, kSlices = 64, kRounds = 3;
-constexpr int kPass = 256, kLast = 1024, kWaves = kLast / 64;  // threads of a pass and of the last launch
+constexpr int kNodes = 64, kSlices = 64, kRounds = 4;
+constexpr int kPass = 256, kLast = 512, kWaves = kLast / 64;  // threads of a pass and of the last launch
 
 template <class T>
 __device__ __forceinline__ double weight(const void* p, int64_t at, int dt) {
@@ -40,6 +50,7 @@ struct Refused {
   int token[kNodes];
   double off[kNodes + 1];  // mass of the tokens in front of this one
   double sum[kNodes];      // of the weights left behind it (drafter's distribution given)
+  double by_off[kNodes], by_sum[kNodes];  // 1 / (1 - off), 1 / sum; 0 for what counts as none
 };
 
 // r at token x behind `count` refused ones; `open`: the last one's sum is not
@@ -77,8 +88,10 @@ __device__ __forceinline__ int wave_max(int x) {
 }
 
 struct Work {
-  double* sums;  // [round][batch][kSlices]
-  int* tops;     // the same: the last token of any weight, -1 for none
+  double* sums;        // [round][batch][kSlices]
+  int* tops;           // the same: the last token of any weight, -1 for none
+  int* done;           // [round][batch] whether the walk's last pass is made by then
+  struct Walk* walks;  // [batch] of those whose is
   int slices, length;  // of a pass; tokens of a slice
 };
 
@@ -144,6 +157,7 @@ __device__ __forceinline__ void walk(const dft_tree_accept_args& a, const packed
       kids = __ballot(parent == c);
       continue;
     }
+    w.f.by_off[count] = off >= 1 ? 0 : 1 / (1 - off);
     w.f.token[count++] = t;
     off += take;
     w.f.off[count] = off;
@@ -151,7 +165,9 @@ __device__ __forceinline__ void walk(const dft_tree_accept_args& a, const packed
       open = true;
       if (kids) {  // its sum decides about the next sibling
         if (pass == have) break;
-        w.f.sum[count - 1] = sum(pass++);
+        const double left = sum(pass++);
+        w.f.sum[count - 1] = left;
+        w.f.by_sum[count - 1] = left > 0 ? 1 / left : 0;
         open = false;
       }
     }
@@ -164,31 +180,96 @@ __device__ __forceinline__ void walk(const dft_tree_accept_args& a, const packed
   w.last = last;
 }
 
-// r's sum over [from, to) and its last token of any weight, by `threads` threads:
-// this thread's part.
+// Four tokens of a row, from x on, of which those in [from, to) are there.
+template <class T>
+__device__ __forceinline__ f32x4 four(const void* p, int64_t at, int dt, int x, int from, int to, bool whole) {
+  if constexpr (sizeof(T) > 1) {
+    if (whole && x >= from && x + 4 <= to) {
+      typedef T T4 __attribute__((ext_vector_type(4)));
+      return __builtin_convertvector(*reinterpret_cast<const T4*>(static_cast<const T*>(p) + at + x), f32x4);
+    }
+  }
+  f32x4 r = {};
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if (x + e < from || x + e >= to) continue;
+    if constexpr (sizeof(T) > 1)
+      r[e] = (float)static_cast<const T*>(p)[at + x + e];
+    else
+      r[e] = ld_f(p, at + x + e, dt);
+  }
+  return r;
+}
+// How far in front of a piece of four element `at` is; -1 where pieces are of no use.
+template <class T>
+__device__ __forceinline__ int in_piece(const void* p, int64_t at) {
+  if constexpr (sizeof(T) == 1) return -1;
+  return (int)((reinterpret_cast<uintptr_t>(static_cast<const T*>(p) + at) / sizeof(T)) & 3);
+}
+
+// This thread's part of a pass over tokens [from, to) of a row by `threads`
+// threads: the tokens x(0) .. x(15) and what is left of each, handed to `take` in
+// turn, sixteen at a time.  The reductions are products with 1 / (1 - off) and 1
+// / sum, two roundings of 2^-53 beside the quotients of the walk.
+template <bool DRAFT, class T, class Take>
+__device__ __forceinline__ void pass_over(const dft_tree_accept_args& a, int64_t row, const Refused& f, int count, bool open, int from,
+                                          int to, int thread, int threads, Take take) {
+  const int64_t p_at = row * a.probs_row_stride, q_at = row * a.draft_row_stride;
+  const bool drawn = DRAFT && count;
+  int lead = in_piece<T>(a.probs, p_at + from);
+  bool whole = lead >= 0;
+  if (drawn) whole &= lead == in_piece<T>(a.draft_probs, q_at + from);
+  lead = max(lead, 0);
+  for (int x0 = from - lead + 4 * thread; x0 < to; x0 += 16 * threads) {
+    f32x4 p[4], q[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int x = x0 + 4 * i * threads;
+      p[i] = four<T>(a.probs, p_at, a.probs_dtype, x, from, to, whole);
+      q[i] = drawn ? four<T>(a.draft_probs, q_at, a.draft_dtype, x, from, to, whole) : f32x4{};
+    }
+    double r[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) r[i] = p[i / 4][i % 4] > 0 ? (double)p[i / 4][i % 4] : 0.0;
+    uint32_t gone = 0;
+    for (int j = 0; j < count; ++j) {
+      const int t = f.token[j];
+      if constexpr (DRAFT) {
+        const bool raw = j == count - 1 && open;
+        const double by_off = f.by_off[j], by_sum = raw ? 1 : f.by_sum[j];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float q0 = q[i / 4][i % 4];
+          const double at = q0 > 0 && !(gone >> i & 1) ? (double)q0 * by_off : 0;
+          const double rest = fmax(r[i] - at, 0.0) * by_sum;
+          r[i] = by_sum > 0 ? rest : r[i];
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const bool is = x0 + 4 * (i / 4) * threads + i % 4 == t;
+        if constexpr (DRAFT)
+          gone |= (uint32_t)is << i;
+        else
+          r[i] = is ? 0 : r[i];
+      }
+    }
+    take(r, [&](int i) { return x0 + 4 * (i / 4) * threads + i % 4; });
+  }
+}
+// r's sum and its last token of any weight
 template <bool DRAFT, class T>
 __device__ __forceinline__ void add_up(const dft_tree_accept_args& a, int64_t row, const Refused& f, int count, bool open, int from,
                                        int to, int thread, int threads, double& sum, int& top) {
-  constexpr int kAhead = 8;
   sum = 0;
   top = -1;
-  const int64_t p_at = row * a.probs_row_stride, q_at = row * a.draft_row_stride;
-  for (int x = from + thread; x < to; x += kAhead * threads) {
-    double p[kAhead], q[kAhead];
+  pass_over<DRAFT, T>(a, row, f, count, open, from, to, thread, threads, [&](const double(&r)[16], auto x) {
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      const int at = min(x + i * threads, to - 1);
-      p[i] = weight<T>(a.probs, p_at + at, a.probs_dtype);
-      q[i] = DRAFT && count ? weight<T>(a.draft_probs, q_at + at, a.draft_dtype) : 0;
+    for (int i = 0; i < 16; ++i) {
+      sum += r[i];
+      if (r[i] > 0) top = x(i);
     }
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      const int at = x + i * threads;
-      const double r = at < to ? left_at<DRAFT>(p[i], q[i], at, f, count, open) : 0;
-      sum += r;
-      if (r > 0) top = at;
-    }
-  }
+  });
 }
 
 // One pass of every request's, in slices.
@@ -200,12 +281,16 @@ __global__ void __launch_bounds__(kPass) pass_kernel(const dft_tree_accept_args 
   const int b = blockIdx.x / work.slices, slice = blockIdx.x - b * work.slices, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const packed::Span s = packed::span_of(a.cu_seqlens, a.rows, a.n_nodes, b);
   if (s.n <= 0) return;
+  // (each round's words are read by the next one: this one's slices start at any time)
+  if (round && work.done[(round - 1) * a.batch + b]) {
+    if (slice == 0 && tid == 0) work.done[round * a.batch + b] = 1;
+    return;
+  }
   auto sum_of = [&](int pass) {
     return wave_sum(lane < work.slices ? work.sums[((int64_t)pass * a.batch + b) * kSlices + lane] : 0.0);
   };
   if (wave == 0) walk<DRAFT, T>(a, s, w, round, sum_of);
   __syncthreads();
-  if (w.pass != round) return;  // its last pass has been made
   const int from = min(slice * work.length, a.vocab), to = min(from + work.length, a.vocab);
   double sum;
   int top;
@@ -220,15 +305,37 @@ __global__ void __launch_bounds__(kPass) pass_kernel(const dft_tree_accept_args 
     work.sums[at] = sum;
     work.tops[at] = top;
   }
+  if (slice == 0) {
+    if (tid == 0) work.done[round * a.batch + b] = w.last;
+    const uint32_t* from = reinterpret_cast<const uint32_t*>(&w);
+    uint32_t* to = reinterpret_cast<uint32_t*>(work.walks + b);
+    for (int i = tid; i < (int)(sizeof(Walk) / 4); i += kPass) to[i] = from[i];
+  }
+}
+
+// The sum of the threads' values up to this one's, in thread order.
+__device__ __forceinline__ double scan(double x, double* waves) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const double up = __shfl_up(x, o);
+    if (lane >= o) x += up;
+  }
+  __syncthreads();
+  if (lane == 63) waves[wave] = x;
+  __syncthreads();
+  double ahead = 0;
+  for (int i = 0; i < wave; ++i) ahead += waves[i];
+  return ahead + x;
 }
 
 // The next token and the path, a workgroup a request.
 template <bool DRAFT, class T>
 __global__ void __launch_bounds__(kLast) last_kernel(const dft_tree_accept_args a, Work work, int rounds) {
   __shared__ Walk w;
-  __shared__ double sums[kSlices], extra[kRounds > kNodes ? kRounds : kNodes];
+  __shared__ double sums[kSlices], extra[kNodes], waves[kWaves], upto_all;
   __shared__ int tops[kSlices];
-  __shared__ double r_of[kLast];
+  __shared__ int found;
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const packed::Span s = packed::span_of(a.cu_seqlens, a.rows, a.n_nodes, b);
   int* path = a.path + (int64_t)b * a.path_cols;
@@ -238,7 +345,7 @@ __global__ void __launch_bounds__(kLast) last_kernel(const dft_tree_accept_args 
   if (s.n > 0) {
     const int V = a.vocab;
     auto part_of = [&](int from, int to, int i) { return from + (int)((int64_t)(to - from) * i / kWaves); };
-    // the sums of [from, to)'s sixteenths, a wave each
+    // the sums of [from, to)'s equal parts, a wave each
     auto sum_up = [&](int from, int to, int count, bool open) {
       double sum;
       int top;
@@ -249,25 +356,26 @@ __global__ void __launch_bounds__(kLast) last_kernel(const dft_tree_accept_args 
       if (lane == 0) sums[wave] = sum, tops[wave] = top;
       __syncthreads();
     };
-    auto total_of = [&](int parts) {
-      double total = 0;
-      for (int i = 0; i < parts; ++i) total += sums[i];
-      return total;
-    };
-    auto sum_of = [&](int pass) {
-      if (pass >= rounds) return extra[pass];
-      return wave_sum(lane < work.slices ? work.sums[((int64_t)pass * a.batch + b) * kSlices + lane] : 0.0);
-    };
-    // passes that no round was left for are made here
-    for (int have = rounds;; ++have) {
+    auto total_of = [&](int parts) { return wave_sum(lane < parts ? sums[lane] : 0.0); };
+    if (work.done[(rounds - 1) * a.batch + b]) {
+      const uint32_t* from = reinterpret_cast<const uint32_t*>(work.walks + b);
+      for (int i = tid; i < (int)(sizeof(Walk) / 4); i += kLast) reinterpret_cast<uint32_t*>(&w)[i] = from[i];
       __syncthreads();
-      if (wave == 0) walk<DRAFT, T>(a, s, w, have, sum_of);
-      __syncthreads();
-      if (w.last) break;
-      sum_up(0, V, w.f.count, w.open);
-      const double sum = total_of(kWaves);
-      __syncthreads();
-      if (tid == 0) extra[have] = sum;
+    } else {
+      auto sum_of = [&](int pass) {
+        if (pass >= rounds) return extra[pass];
+        return wave_sum(lane < work.slices ? work.sums[((int64_t)pass * a.batch + b) * kSlices + lane] : 0.0);
+      };
+      // passes that no round was left for are made here
+      for (int have = rounds;; ++have) {
+        __syncthreads();
+        if (wave == 0) walk<DRAFT, T>(a, s, w, have, sum_of);
+        __syncthreads();
+        if (w.last) break;
+        sum_up(0, V, w.f.count, w.open);
+        const double sum = total_of(kWaves);
+        if (tid == 0) extra[have] = sum;
+      }
     }
     length = w.length;
     // the parts that the running sum is cut into, and whose sums are at hand
@@ -297,41 +405,80 @@ __global__ void __launch_bounds__(kLast) last_kernel(const dft_tree_accept_args 
       const double target = (double)a.last[b] * total;
       double before = 0;
       int from = 0, to = V;
-      while (true) {
+      while (token < 0) {
         // the part where the running sum passes the target, else the last of any weight
-        int part = -1, last = 0;
-        double ahead = before, start = before;
-        for (int i = 0; i < parts; ++i) {
-          if (tops[i] >= 0) last = i;
-          if (part < 0 && ahead + sums[i] > target) part = i, start = ahead;
-          ahead += sums[i];
+        double up = lane < parts ? sums[lane] : 0;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+          const double x = __shfl_up(up, o);
+          if (lane >= o) up += x;
         }
-        if (part < 0) {
-          token = tops[last];
+        const uint64_t past = __ballot(lane < parts && before + up > target);
+        if (!past) {
+          token = wave_max(lane < parts ? tops[lane] : -1);
           break;
         }
+        const int part = __ffsll((unsigned long long)past) - 1;
+        const double ahead = part ? __shfl(up, part - 1) : 0;
         const int first = sliced ? min(part * work.length, V) : part_of(from, to, part);
         to = sliced ? min(first + work.length, V) : part_of(from, to, part + 1);
         from = first;
-        before = start;
+        before += ahead;
         sliced = false;
         parts = kWaves;
-        if (to - from <= 64) break;
-        sum_up(from, to, count, open);
-      }
-      if (token < 0) {  // 64 of them at most: by one wave
-        double r = 0;
-        if (lane < to - from) {
-          int top;
-          add_up<DRAFT, T>(a, s.r0 + w.node, w.f, count, open, from + lane, from + lane + 1, 0, 1, r, top);
+        const int lead = max(in_piece<T>(a.probs, (s.r0 + w.node) * a.probs_row_stride + from), 0);
+        if (lead + to - from > 16 * kLast) {
+          sum_up(from, to, count, open);
+          continue;
         }
-        double c = before;
-        for (int x = 0; x < to - from; ++x) {  // in order
-          const double rx = __shfl(r, x);
-          c += rx;
-          if (rx > 0) token = from + x;
-          if (c > target) break;
+        // few enough for one step: a piece of 4 tokens a thread, four times over, in order
+        double part_sum[4] = {}, r4[16] = {};
+        int x4 = 0;
+        pass_over<DRAFT, T>(a, s.r0 + w.node, w.f, count, open, from, to, tid, kLast, [&](const double(&r)[16], auto x) {
+          x4 = x(0);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            r4[i] = r[i];
+            part_sum[i / 4] += r[i];
+          }
+        });
+        if (tid == 0) found = V;
+        int last_top = -1;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const double upto = scan(part_sum[k], waves);
+          // the first piece of any weight whose sum passes the target, and in it the token that does
+          const uint64_t past = __ballot(before + upto > target && part_sum[k] > 0);
+          if (past && lane == __ffsll((unsigned long long)past) - 1) {
+            double c = before + (upto - part_sum[k]);
+            int at = V;
+            bool over = false;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const bool some = r4[4 * k + e] > 0;
+              if (!over && some) at = x4 + 4 * k * kLast + e;
+              c += r4[4 * k + e];
+              over |= some && c > target;
+            }
+            atomicMin(&found, at);
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (r4[4 * k + e] > 0) last_top = x4 + 4 * k * kLast + e;
+          if (tid == kLast - 1) upto_all = upto;
+          __syncthreads();
+          before += upto_all;
+          if (found < V) break;
         }
+        __syncthreads();
+        token = found;
+        if (token == V) {  // rounding: the last of any weight here
+          last_top = wave_max(last_top);
+          if (lane == 0) tops[wave] = last_top;
+          __syncthreads();
+          token = wave_max(lane < kWaves ? tops[lane] : -1);
+        }
+        break;
       }
     }
   }
@@ -352,7 +499,7 @@ int rounds_of(const dft_tree_accept_args& a) { return a.draft_probs ? kRounds : 
 Work work_of(const dft_tree_accept_args& a) {
   Work w = {};
   const int most = std::min(kSlices, std::max(1, 1024 / a.batch));
-  w.length = std::max(1024, (a.vocab + most - 1) / most);
+  w.length = std::max(1024, ((a.vocab + most - 1) / most + 1023) / 1024 * 1024);
   w.slices = std::max(1, (a.vocab + w.length - 1) / w.length);
   return w;
 }
@@ -373,13 +520,17 @@ int launch_type(const dft_tree_accept_args& a, const Work& work, hipStream_t str
 
 // (for either form: whether there is a drafter's distribution need not be known yet)
 int64_t tree_accept_workspace(const dft_tree_accept_args* a) {
-  return (int64_t)kRounds * a->batch * kSlices * (int64_t)(sizeof(double) + sizeof(int));
+  return (int64_t)a->batch * (sizeof(Walk) + kRounds * (kSlices * (sizeof(double) + sizeof(int)) + sizeof(int)));
 }
 
 int launch_tree_accept(const dft_tree_accept_args* a, hipStream_t stream) {
+  static_assert(sizeof(Walk) % 8 == 0);
   Work work = work_of(*a);
-  work.sums = static_cast<double*>(a->workspace);
-  work.tops = reinterpret_cast<int*>(work.sums + (int64_t)kRounds * a->batch * kSlices);
+  const int64_t passes = (int64_t)kRounds * a->batch;
+  work.walks = static_cast<Walk*>(a->workspace);
+  work.sums = reinterpret_cast<double*>(work.walks + a->batch);
+  work.tops = reinterpret_cast<int*>(work.sums + passes * kSlices);
+  work.done = work.tops + passes * kSlices;
   if (a->draft_probs && a->draft_dtype != a->probs_dtype) return launch_type<uint8_t>(*a, work, stream);
   switch (a->probs_dtype) {
     case DFT_BF16: return launch_type<__bf16>(*a, work, stream);
