@@ -145,7 +145,8 @@ int tree_accept_sizes(const dft_tree_accept_args* a) {
   if (!a) return DFT_ERR_INVALID;
   if (a->batch < 0 || a->n_nodes < 0 || a->vocab < 0 || a->rows < 0 || a->path_cols < 1) return DFT_ERR_INVALID;
   if (a->n_nodes > 64 || a->path_cols > 64) return DFT_ERR_UNSUPPORTED;
-  if (a->batch > 65535 || a->rows > 0x7fffffffll) return DFT_ERR_UNSUPPORTED;
+  // a token's index, and one some thousand past it, are counted in 31 bits
+  if (a->batch > 65535 || a->rows > 0x7fffffffll || a->vocab > 1 << 30) return DFT_ERR_UNSUPPORTED;
   return a->batch == 0 ? -1 : DFT_OK;
 }
 

@@ -71,6 +71,16 @@ def _stream(dev: torch.device) -> int:
     return torch._C._cuda_getCurrentRawStream(dev.index)
 
 
+def _launch(entry: str, args, dev: torch.device) -> None:
+    """One entry's launch on dev's current stream, with dev current: the default
+    stream's handle is the same on every device."""
+    if dev.index == torch.cuda.current_device():
+        check(entry, getattr(load(), entry)(C.byref(args), _stream(dev)))
+        return
+    with torch.cuda.device(dev):
+        check(entry, getattr(load(), entry)(C.byref(args), _stream(dev)))
+
+
 def _idx_vec(t: Optional[torch.Tensor], name: str):
     if t is None:
         return None, DFT_I32
@@ -1169,7 +1179,7 @@ def _initial(initial, batch):
 
 def _pool_slots(indices, name, batch, pool, pool_name):
     """(indices, their tag) of a pool that every request's state is written back to."""
-    if any(n > 1 and s == 0 for n, s in zip(pool.shape, pool.stride())):
+    if 0 in pool.stride() and any(n > 1 and s == 0 for n, s in zip(pool.shape, pool.stride())):
         raise ValueError(f"{pool_name} must not be expanded (it is updated in place)")
     at, tag = _idx_vec(indices, name)
     if at is not None and at.numel() != batch:
@@ -1236,7 +1246,7 @@ def prompt_conv(x: torch.Tensor, conv_state: torch.Tensor, weight: torch.Tensor,
         a.bias, a.bias_dtype = bias.data_ptr(), _ftag(bias, "bias")
     a.y, a.y_row_stride, a.y_dtype = y.data_ptr(), y.stride(0), _ftag(y, "y")
     a.status = _status_ptr(status, batch, dev)
-    check("dft_prompt_conv", load().dft_prompt_conv(C.byref(a), _stream(dev)))
+    _launch("dft_prompt_conv", a, dev)
     return y
 
 
@@ -1309,13 +1319,12 @@ def prompt_gdn(y: torch.Tensor, a: torch.Tensor, b: torch.Tensor, A_log: Optiona
     args.initial = _ptr(initial)
     args.o, args.o_row_stride, args.o_h_stride, args.o_dtype = o.data_ptr(), o.stride(0), o.stride(1), _ftag(o, "o")
     args.status = _status_ptr(status, batch, dev)
-    lib = load()
     need = C.c_int64()
-    check("dft_prompt_gdn_workspace", lib.dft_prompt_gdn_workspace(C.byref(args), C.byref(need)))
+    check("dft_prompt_gdn_workspace", load().dft_prompt_gdn_workspace(C.byref(args), C.byref(need)))
     if need.value:
         work = torch.empty(need.value, device=dev, dtype=torch.uint8)
         args.workspace, args.workspace_bytes = work.data_ptr(), need.value
-    check("dft_prompt_gdn", lib.dft_prompt_gdn(C.byref(args), _stream(dev)))
+    _launch("dft_prompt_gdn", args, dev)
     return o
 
 
@@ -1393,18 +1402,17 @@ def tree_accept(tokens: torch.Tensor, parent: torch.Tensor, probs: torch.Tensor,
     if draft_probs is not None:
         a.draft_probs, a.draft_row_stride, a.draft_dtype = _vocab_rows(draft_probs, rows, probs.shape[1], "draft_probs")
     a.uniform, a.last = uniform.data_ptr(), last.data_ptr()
-    words = torch.empty(batch * (path_cols + 1), device=dev, dtype=torch.int32)
-    longs = torch.empty(batch * (path_cols + 1), device=dev, dtype=torch.int64)
-    out = {"path": words[:batch * path_cols].view(batch, path_cols), "path_len": words[batch * path_cols:],
-           "rows": longs[:batch * path_cols].view(batch, path_cols), "token": longs[batch * path_cols:]}
+    out = {"path": torch.empty(batch, path_cols, device=dev, dtype=torch.int32),
+           "path_len": torch.empty(batch, device=dev, dtype=torch.int32),
+           "rows": torch.empty(batch, path_cols, device=dev, dtype=torch.int64),
+           "token": torch.empty(batch, device=dev, dtype=torch.int64)}
     a.path, a.path_len = out["path"].data_ptr(), out["path_len"].data_ptr()
     a.path_rows, a.token = out["rows"].data_ptr(), out["token"].data_ptr()
     a.status = _status_ptr(status, batch, dev)
-    lib = load()
     need = C.c_int64()
-    check("dft_tree_accept_workspace", lib.dft_tree_accept_workspace(C.byref(a), C.byref(need)))
+    check("dft_tree_accept_workspace", load().dft_tree_accept_workspace(C.byref(a), C.byref(need)))
     if need.value:
         work = torch.empty(need.value, device=dev, dtype=torch.uint8)
         a.workspace, a.workspace_bytes = work.data_ptr(), need.value
-    check("dft_tree_accept", lib.dft_tree_accept(C.byref(a), _stream(dev)))
+    _launch("dft_tree_accept", a, dev)
     return out

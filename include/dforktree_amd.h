@@ -720,8 +720,9 @@ DFT_API int dft_prompt_conv(const dft_prompt_conv_args* args, void* stream);
  * q, k normalised (x / sqrt(sum x^2 + 1e-6)), q scaled, beta = sigmoid(b) and
  * g = neg_exp_A softplus(a + dt_bias):
  *   S <- e^g S;  u = beta (v - S^T k);  S <- S + k u^T;  o = S^T q.
- * States, sums, decays and outputs are held in fp32, factors of products as
- * bf16 pairs (2^-17 relative).  What is not finite in a row reaches at most
+ * States, sums and decays are held in fp32; factors of the chunks' products
+ * are sums of bf16 parts, three where a state passes through (2^-24 relative),
+ * two where only outputs do (2^-17).  What is not finite in a row reaches at most
  * the rows of its request from the 64 in a row on that it is one of. */
 typedef struct dft_prompt_gdn_args {
   int32_t batch, max_len;
@@ -788,7 +789,7 @@ DFT_API int dft_prompt_gdn_workspace(const dft_prompt_gdn_args* args, int64_t* b
  * ------------------------------------------------------------------------- */
 typedef struct dft_tree_accept_args {
   int32_t batch, n_nodes; /* n_nodes as in dft_verify_args, <= 64 */
-  int32_t vocab;
+  int32_t vocab;     /* <= 2^30 */
   int32_t path_cols; /* 1 .. 64 */
   int64_t rows;      /* of tokens, parent, uniform, probs and draft_probs */
   const int32_t* cu_seqlens; /* [batch + 1] or NULL */

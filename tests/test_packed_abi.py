@@ -84,7 +84,7 @@ REFUSED = [
         dict(path_rows=None), dict(token=None), dict(tokens_dtype=0), dict(parent_dtype=2), dict(probs_dtype=3),
         dict(draft_probs=16, draft_dtype=4)]),
     ("dft_tree_accept", accept_args, UNSUPPORTED, [
-        dict(n_nodes=65), dict(path_cols=65), dict(batch=65536), dict(rows=1 << 31)]),
+        dict(n_nodes=65), dict(path_cols=65), dict(batch=65536), dict(rows=1 << 31), dict(vocab=(1 << 30) + 1)]),
 ]
 
 
@@ -146,3 +146,31 @@ def test_operators_take_gpu_tensors():
         ops.token_gdn(y, g, g, f(2), f(2), f(4, 2, 128, 128), hk=1, hv=2)
     with pytest.raises(ValueError, match="GPU"):
         ops.tree_accept(i, i, f(4, 10), f(4), f(1))
+
+
+@pytest.mark.parametrize("current", [0, 1])
+def test_launched_with_the_tensors_device_current(monkeypatch, current):
+    """The default stream's handle is 0 on every device: it names the current one's."""
+    import contextlib
+    from types import SimpleNamespace
+
+    import torch
+    from dforktree_amd import _lib, ops
+    seen, at = [], [current]
+
+    @contextlib.contextmanager
+    def device(dev):
+        was, at[0] = at[0], dev.index
+        yield
+        at[0] = was
+
+    def entry(args, stream):
+        seen.append((at[0], stream))
+        return _lib.DFT_OK
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: at[0])
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(ops, "_stream", lambda dev: 0)
+    monkeypatch.setattr(ops, "load", lambda: SimpleNamespace(dft_prompt_conv=entry))
+    ops._launch("dft_prompt_conv", _lib.PromptConvArgs(), torch.device("cuda", 1))
+    assert seen == [(1, 0)] and at == [current]
