@@ -212,7 +212,7 @@ __device__ __forceinline__ f32x4 mfma16_f32(float a, float b, f32x4 c) {
 // Until an fp32 product's result is whole.  The compiler waits 10 states for it,
 // after which its last register may still be on its way: read first of the
 // four, behind a branch, it held the sum without its last terms.
-__device__ __forceinline__ void settle(f32x4& x) { asm volatile("s_nop 15" : "+a"(x)); }
+__device__ __forceinline__ void settle(f32x4& x) { asm volatile("s_nop 15" : "+v"(x)); }
 // x = p[0] + p[1] + ..., each the bf16 nearest to what is left
 template <int N>
 struct Parts4 {
@@ -237,7 +237,10 @@ typedef uint64_t u64x2 __attribute__((ext_vector_type(2)));
 // (their powers would lose what equal keys leave of 32 bits), then X_ij =
 // -(sum_(j<m<=i) X_im A_mj) X_jj in fp32 products, transposed, so that each result
 // is the next one's operand and the last the fragment that is stored.
-__global__ void __launch_bounds__(256) gdn_chunk_kernel(const dft_prompt_gdn_args a, Work work, int past) {
+// Bound by the instructions that its waves issue, so by what of them stand ready:
+// 128 registers, four workgroups a CU.  A prompt of 8192 rows and 32 heads KKK us; two
+// workgroups a CU 78.
+__global__ void __launch_bounds__(256, 4) gdn_chunk_kernel(const dft_prompt_gdn_args a, Work work, int past) {
   constexpr int kKRow = kD + 8, kARow = kChunk + 4;
   __shared__ __attribute__((aligned(16))) uint16_t keys[kChunk][kKRow];
   __shared__ __attribute__((aligned(16))) float A[kChunk][kARow];
@@ -276,28 +279,23 @@ __global__ void __launch_bounds__(256) gdn_chunk_kernel(const dft_prompt_gdn_arg
     G[lane] = sum;
     beta[lane] = gate.beta;
   }
+  // the norms stand on the diagonals of the wave's own Gram tiles: row l16's in lane (l16, l16 / 4), register l16 % 4
   bf16x8 k[4], q[4];
-  float kk = 0, qq = 0;
+  f32x4 kk = {}, qq = {};
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     if (mine >= n) kw[j] = qw[j] = u32x4{};
     k[j] = __builtin_bit_cast(bf16x8, kw[j]);
     q[j] = __builtin_bit_cast(bf16x8, qw[j]);
     *reinterpret_cast<u32x4*>(&keys[mine][32 * j + 8 * g]) = kw[j];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      kk = fmaf((float)k[j][e], (float)k[j][e], kk);
-      qq = fmaf((float)q[j][e], (float)q[j][e], qq);
-    }
+    kk = mfma16(k[j], k[j], kk);
+    qq = mfma16(q[j], q[j], qq);
   }
-  kk += __shfl_xor(kk, 16);
-  qq += __shfl_xor(qq, 16);
-  kk += __shfl_xor(kk, 32);
-  qq += __shfl_xor(qq, 32);
   char* out = work.heads + (tile * a.hv + h) * kHead;
-  if (g == 0) {
-    rks[mine] = 1.f / sqrtf(kk + 1e-6f);
-    reinterpret_cast<float*>(out + kX + kP)[kRq * kChunk + mine] = a.scale / sqrtf(qq + 1e-6f);
+  if (l16 / 4 == g) {
+    auto own = [&](f32x4 x) { return l16 & 2 ? (l16 & 1 ? x[3] : x[2]) : (l16 & 1 ? x[1] : x[0]); };
+    rks[mine] = 1.f / sqrtf(own(kk) + 1e-6f);
+    reinterpret_cast<float*>(out + kX + kP)[kRq * kChunk + mine] = a.scale / sqrtf(own(qq) + 1e-6f);
   }
   __syncthreads();
 
@@ -313,11 +311,9 @@ __global__ void __launch_bounds__(256) gdn_chunk_kernel(const dft_prompt_gdn_arg
     *reinterpret_cast<u32x4*>(out + kX + 12 * kFragment + 16 * lane) = u32x4{};
   }
 
-  // A into the LDS, P to its place: Gram tiles of the wave's rows with those of tiles j <= w, K K^T and (Q K^T)^T
-  const float Gq = G[mine];
+  // A into the LDS, P to its place, transposed: Gram tiles K K^T and K Q^T of the keys of tiles j <= w with the wave's rows
+  const float Gq = G[mine], bk = beta[mine] * rks[mine];
   Parts4<2> p[4];
-  const f32x4 Gi = *reinterpret_cast<const f32x4*>(&G[16 * w + 4 * g]);
-  const f32x4 bi = *reinterpret_cast<const f32x4*>(&beta[16 * w + 4 * g]) * *reinterpret_cast<const f32x4*>(&rks[16 * w + 4 * g]);
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     p[j] = {};
@@ -326,40 +322,22 @@ __global__ void __launch_bounds__(256) gdn_chunk_kernel(const dft_prompt_gdn_arg
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
       const bf16x8 kj = *reinterpret_cast<const bf16x8*>(&keys[16 * j + l16][32 * x + 8 * g]);
-      dot = mfma16(k[x], kj, dot);
+      dot = mfma16(kj, k[x], dot);
       qk = mfma16(kj, q[x], qk);
     }
-    const float Gj = G[16 * j + l16], rj = rks[16 * j + l16];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const bool below = j < w || 4 * g + r > l16;
-      const float x = dot[r] * (bi[r] * rj) * __builtin_amdgcn_exp2f(Gi[r] - Gj);
-      A[16 * w + 4 * g + r][16 * j + l16] = below ? x : 0.f;
-    }
     const f32x4 Gk = *reinterpret_cast<const f32x4*>(&G[16 * j + 4 * g]);
-    f32x4 y;
+    const f32x4 rk = *reinterpret_cast<const f32x4*>(&rks[16 * j + 4 * g]);
+    f32x4 x, y;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const bool seen = j < w || 4 * g + r <= l16;
-      y[r] = seen ? qk[r] * __builtin_amdgcn_exp2f(Gq - Gk[r]) : 0.f;
+      const int ahead = j < w ? 1 : l16 - (4 * g + r);  // of the key the row is
+      const float decay = __builtin_amdgcn_exp2f(Gq - Gk[r]);
+      x[r] = ahead > 0 ? dot[r] * (bk * rk[r]) * decay : 0.f;
+      y[r] = ahead >= 0 ? qk[r] * decay : 0.f;
     }
+    *reinterpret_cast<f32x4*>(&A[mine][16 * j + 4 * g]) = x;
     p[j] = split4<2>(y);
   }
-  // the wave's diagonal block, a column a lane (four times over), in its place
-  __builtin_amdgcn_wave_barrier();
-  float x[16];
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    float y = i == l16 ? 1.f : 0.f;
-#pragma unroll
-    for (int m = 0; m < i; ++m) y = fmaf(-A[16 * w + i][16 * w + m], x[m], y);
-    x[i] = y;
-  }
-  __builtin_amdgcn_wave_barrier();
-#pragma unroll
-  for (int i = 0; i < 16; ++i)
-    if (i / 4 == g) A[16 * w + i][16 * w + l16] = x[i];
-  __syncthreads();
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     if (j > w / 2) continue;
@@ -367,11 +345,49 @@ __global__ void __launch_bounds__(256) gdn_chunk_kernel(const dft_prompt_gdn_arg
     for (int z = 0; z < 2; ++z)
       *reinterpret_cast<u64x2*>(out + kX + (p_at(w, j) + z) * kFragment + 16 * lane) = u64x2{p[2 * j].p[z], p[2 * j + 1].p[z]};
   }
+  // the wave's diagonal block: its two halves' inverses D by substitution, a column a lane (four times over), and with L
+  // what is below them X = D - D L D
+  __builtin_amdgcn_wave_barrier();
+  f32x4 diagonal;
+  {
+    const int at = 16 * w + (l16 & 8);
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float y = i == (l16 & 7) ? 1.f : 0.f;
+#pragma unroll
+      for (int m = 0; m < i; ++m) y = fmaf(-A[at + i][at + m], x[m], y);
+      x[i] = y;
+    }
+    __builtin_amdgcn_wave_barrier();
+    if (g == 0)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) A[at + i][16 * w + l16] = x[i];
+    __builtin_amdgcn_wave_barrier();
+    diagonal = *reinterpret_cast<const f32x4*>(&A[mine][16 * w + 4 * g]);
+    if (l16 >= 8 && g < 2) diagonal = f32x4{};
+    const bool below = g >= 2 && l16 < 8;
+    float D[4];
+    f32x4 DL = {};
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const float y = A[16 * w + 4 * g + r][16 * w + l16];
+      D[r] = below ? 0.f : -y;
+      DL = mfma16_f32(below ? y : 0.f, diagonal[r], DL);
+    }
+    settle(DL);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) diagonal = mfma16_f32(D[r], DL[r], diagonal);
+    settle(diagonal);
+    __builtin_amdgcn_wave_barrier();
+    *reinterpret_cast<f32x4*>(&A[mine][16 * w + 4 * g]) = diagonal;
+  }
+  __syncthreads();
   // the row block, transposed: xt[j] is X_wj^T, lane: row l16 of X_wj, columns 4 g ..
   auto row_block = [&](auto which) {
     constexpr int W = decltype(which)::value;
     f32x4 xt[4] = {};
-    xt[W] = *reinterpret_cast<const f32x4*>(&A[16 * W + l16][16 * W + 4 * g]);
+    xt[W] = diagonal;
 #pragma unroll
     for (int j = W - 1; j >= 0; --j) {
       f32x4 to[3] = {}, all = {};
