@@ -245,8 +245,10 @@ __global__ void __launch_bounds__(256, 4) gdn_chunk_kernel(const dft_prompt_gdn_
   __shared__ __attribute__((aligned(16))) uint16_t keys[kChunk][kKRow];
   __shared__ __attribute__((aligned(16))) float A[kChunk][kARow];
   __shared__ __attribute__((aligned(16))) float G[kChunk], beta[kChunk], rks[kChunk];
-  const int64_t tile = blockIdx.x / a.hv;
-  const int h = (int)(blockIdx.x - tile * a.hv), kh = h / (a.hv / a.hk);
+  // the v heads of a k head read the same rows: one after the other on one XCD
+  const int share = a.hv / a.hk, in = blockIdx.x / kXcds;
+  const int64_t unit = (int64_t)(in / share) * kXcds + blockIdx.x % kXcds, tile = unit / a.hk;
+  const int kh = (int)(unit - tile * a.hk), h = kh * share + in % share;
   const int b = find_tile<256>(a, tile, kChunk);
   if (b < 0) return;
   const Span s = span_of(a, b);
@@ -829,6 +831,8 @@ Split split_of(const dft_prompt_gdn_args& a) {
 bool all_by_rows(const dft_prompt_gdn_args& a) { return a.max_len <= split_of(a).rows; }
 int64_t tiles_of(const dft_prompt_gdn_args& a) { return line_tiles(a.rows, a.batch, kChunk); }
 
+int64_t chunk_blocks(const dft_prompt_gdn_args& a) { return (tiles_of(a) * a.hk + kXcds - 1) / kXcds * kXcds * (a.hv / a.hk); }
+
 int launch_rows(const dft_prompt_gdn_args& a, int most, hipStream_t stream) {
   // With few heads a fourth of the columns each (one request: 5.4 us, 6.5 whole; 64 requests: 57 and 49)
   const int64_t heads = (int64_t)a.batch * a.hv;
@@ -865,7 +869,7 @@ int launch_scan(const dft_prompt_gdn_args& a, const Work& work, int past, hipStr
 // the most workgroups of a launch, in units of 256 threads
 int64_t prompt_gdn_blocks(const dft_prompt_gdn_args* a) {
   // the scan's are three such, and padded to a multiple of the XCDs
-  return std::max(((int64_t)a->batch * a->hv + kXcds * a->hv) * 8 * (kScanThreads / 256), all_by_rows(*a) ? 0 : tiles_of(*a) * a->hv);
+  return std::max(((int64_t)a->batch * a->hv + kXcds * a->hv) * 8 * (kScanThreads / 256), all_by_rows(*a) ? 0 : chunk_blocks(*a));
 }
 int64_t prompt_gdn_workspace(const dft_prompt_gdn_args* a) { return all_by_rows(*a) ? 0 : tiles_of(*a) * a->hv * kHead; }
 
@@ -876,7 +880,7 @@ int launch_prompt_gdn(const dft_prompt_gdn_args* a, hipStream_t stream) {
     if (st != DFT_OK || !split.both) return st;
   }
   const Work work = {static_cast<char*>(a->workspace)};
-  gdn_chunk_kernel<<<(unsigned)(tiles_of(*a) * a->hv), 256, 0, stream>>>(*a, work, split.rows);
+  gdn_chunk_kernel<<<(unsigned)chunk_blocks(*a), 256, 0, stream>>>(*a, work, split.rows);
   if (hipGetLastError() != hipSuccess) return DFT_ERR_LAUNCH;
   // 16 value columns a workgroup, or 32 at 1.4 times the time a chunk: the longest request's chunks one after the other,
   // or all of them over the CUs (us: one prompt of 8192, 32 heads, 275 and 384; six of 257 to 2999 361 and 317)
