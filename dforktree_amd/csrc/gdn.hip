@@ -238,8 +238,8 @@ typedef uint64_t u64x2 __attribute__((ext_vector_type(2)));
 // -(sum_(j<m<=i) X_im A_mj) X_jj in fp32 products, transposed, so that each result
 // is the next one's operand and the last the fragment that is stored.
 // Bound by the instructions that its waves issue, so by what of them stand ready:
-// 128 registers, four workgroups a CU.  A prompt of 8192 rows and 32 heads KKK us; two
-// workgroups a CU 78.
+// 128 registers, four workgroups a CU.  A prompt of 8192 rows and 32 heads 52 us,
+// 4.5 TB/s; with two workgroups a CU 78.
 __global__ void __launch_bounds__(256, 4) gdn_chunk_kernel(const dft_prompt_gdn_args a, Work work, int past) {
   constexpr int kKRow = kD + 8, kARow = kChunk + 4;
   __shared__ __attribute__((aligned(16))) uint16_t keys[kChunk][kKRow];
@@ -438,6 +438,20 @@ __device__ __forceinline__ void barrier_only() {
 
 constexpr int kScanThreads = 64 * 12;
 
+// The request at this place in the order of falling lengths, of at most 64: the
+// others as they come.  (20 prompts of 500 rows and one of 8192 behind them: 550
+// us, as they come 663; six of 257 to 2999 no better for it.)
+__device__ __forceinline__ int nth_longest(const dft_prompt_gdn_args& a, int place) {
+  if (!a.cu_seqlens || a.batch == 1 || a.batch > 64) return place;
+  const int lane = threadIdx.x & 63, n = lane < a.batch ? span_of(a, lane).n : 0;
+  int longer = 0;
+  for (int i = 0; i < a.batch; ++i) {
+    const int other = __builtin_amdgcn_readlane(n, i);
+    longer += other > n || (other == n && i < lane);
+  }
+  return __ffsll((unsigned long long)__ballot(lane < a.batch && longer == place)) - 1;
+}
+
 // The states through the chunks: a workgroup for 16 NT value columns of a head.
 // What bounds it is the chain S -> W -> U -> S of one chunk after the other, and
 // beside it the bytes that a CU gets from its L2 (some 23 a cycle).  So its
@@ -473,7 +487,8 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_kernel(const dft_pro
   const int round = blockIdx.x / (kXcds * members), in = blockIdx.x - round * kXcds * members;
   const int family = round * kXcds + in % kXcds, member = in / kXcds;
   if (family >= families) return;
-  const int unit = family * (members / kSlices) + member / kSlices, slice = member % kSlices, b = unit / a.hv, h = unit - b * a.hv;
+  const int unit = family * (members / kSlices) + member / kSlices, slice = member % kSlices;
+  const int turn = unit / a.hv, h = unit - turn * a.hv, b = nth_longest(a, turn);
   const Span s = span_of(a, b);
   if (s.n <= past) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, g = lane >> 4;
@@ -814,17 +829,18 @@ bool vector_state(const dft_prompt_gdn_args& a) {
 }
 
 // Up to so many rows a request is taken row by row, by a launch of its own where
-// others are longer.  us for one request of 32 heads: 6.5, 11.8 and 19.1 for 1, 4
-// and 8 rows, 14.7 as a chunk of any length; 16 requests 12.4, 22.6, 35.2 and 61
-// as chunks; 64 requests 49, 68, 106 and 205.  With few of them the second launch
-// (2) costs more than the chunks of short requests, which run beside the others.
+// others are longer.  us for one request of 32 heads: 5.3, 9.0, 14.2 and 25 for 1,
+// 4, 8 and 16 rows, 14.1 as a chunk; 16 requests 11.9, 22, 35 and 60, 60 to 62 as
+// chunks; 64 requests 48, 70, 102 and 182, 197 to 204 as chunks.  With few of them
+// the second launch (2) costs more than the chunks of short requests, which run
+// beside the others.
 struct Split {
   int rows;
   bool both;
 };
 Split split_of(const dft_prompt_gdn_args& a) {
   const bool many = (int64_t)a.batch * a.hv >= 512;
-  const int rows = many ? 16 : 4;
+  const int rows = many ? 16 : 7;
   if (a.max_len <= rows) return {rows, false};
   return many && a.cu_seqlens ? Split{rows, true} : Split{0, false};
 }
@@ -882,10 +898,10 @@ int launch_prompt_gdn(const dft_prompt_gdn_args* a, hipStream_t stream) {
   const Work work = {static_cast<char*>(a->workspace)};
   gdn_chunk_kernel<<<(unsigned)chunk_blocks(*a), 256, 0, stream>>>(*a, work, split.rows);
   if (hipGetLastError() != hipSuccess) return DFT_ERR_LAUNCH;
-  // 16 value columns a workgroup, or 32 at 1.4 times the time a chunk: the longest request's chunks one after the other,
-  // or all of them over the CUs (us: one prompt of 8192, 32 heads, 275 and 384; six of 257 to 2999 361 and 317)
+  // 16 value columns a workgroup, or 32 at 1.6 times the time a chunk: the longest request's chunks one after the other,
+  // or all of them over the CUs (us: one prompt of 8192, 32 heads, 245 and 358; six of 257 to 2999 333 and 272)
   const double longest = std::min(a->rows, (int64_t)a->max_len) / 64.0, all = (a->rows / 64.0 + a->batch / 2.0) * a->hv / kCus;
-  return std::max(longest, 8 * all) <= 1.4 * std::max(longest, 4 * all) ? launch_scan<1>(*a, work, split.rows, stream)
+  return std::max(longest, 8 * all) <= 1.6 * std::max(longest, 4 * all) ? launch_scan<1>(*a, work, split.rows, stream)
                                                                         : launch_scan<2>(*a, work, split.rows, stream);
 }
 
