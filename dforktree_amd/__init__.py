@@ -4,7 +4,8 @@ Public pieces:
 
 * ``dforktree_amd.ops``        batched / packed operators over the HIP C ABI
   (tree_verify, tree_conv, tree_commit, tree_struct, block_inverse_, and
-  page_plan, kv_append, paged_attention, prompt_attention);
+  page_plan, kv_append, paged_attention, prompt_attention, and prompt_conv,
+  prompt_gdn, token_gdn, tree_accept);
 * ``dforktree_amd.paged``      ``PagedKV``: a serving loop's KV cache over the
   last four, for the full-attention layers;
 * ``dforktree_amd.plugin``     the reference-named drop-in modules
