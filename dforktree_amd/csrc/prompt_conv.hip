@@ -90,7 +90,7 @@ __global__ void __launch_bounds__(256) prompt_conv4_kernel(const dft_prompt_conv
   // the weights do not wait for the search
   u32x4 wv[4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) wv[j] = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(p.weight) + 4 * cc + 8 * j);
+  for (int j = 0; j < 4; ++j) wv[j] = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(p.weight) + (int64_t)4 * cc + 8 * j);
   const int b = find_tile<256>(p, x, kTile);
   if (b < 0 || !works) return;
   const Span s = span_of(p, b);

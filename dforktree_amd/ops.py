@@ -1264,8 +1264,9 @@ def prompt_gdn(y: torch.Tensor, a: torch.Tensor, b: torch.Tensor, A_log: Optiona
     state float32 [slots, hv, dk, dv] (index k, v; any strides -- pass
     ``pool.transpose(-1, -2)`` for a V-major pool), updated in place.  Rows of
     request b, its slot state_indices[b] (or b), ``initial`` and ``status`` as in
-    ``prompt_conv``.  Returns o [rows, hv, 128], where rows of no request keep
-    what a given ``o`` holds and are otherwise uninitialised.
+    ``prompt_conv``.  Returns o [rows, hv, 128], which must not overlap y, and
+    where rows of no request keep what a given ``o`` holds and are otherwise
+    uninitialised.
     """
     dev = _device_of(y, a, b, A_log, dt_bias, state, cu_seqlens, neg_exp_A, state_indices, initial, o, status)
     if y.dim() != 2 or y.stride(1) != 1:

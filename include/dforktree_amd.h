@@ -750,7 +750,7 @@ typedef struct dft_prompt_gdn_args {
   const void* state_indices; /* [batch] or NULL */
   int32_t state_indices_dtype;
   const uint8_t* initial; /* [batch] or NULL: all 1 */
-  void* o;                /* [rows][hv][dv], channel stride 1 */
+  void* o;                /* [rows][hv][dv], channel stride 1; not y's memory */
   int64_t o_row_stride, o_h_stride;
   int32_t o_dtype;
   int32_t* status; /* optional [batch] */

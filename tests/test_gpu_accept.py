@@ -199,6 +199,50 @@ def test_strides(cuda):
         c.check(cuda, label="strided")
 
 
+@pytest.mark.parametrize("V", [3, 1001, 20000])
+def test_rows_of_unlike_alignment(cuda, V):
+    """The drafter's rows start elsewhere in a piece of four than the target's."""
+    c = Case([9, 30, 4], V, "star", True, seed=16)
+    c.u.fill_(1 - 2.0 ** -24)
+    for name, at, width in (("probs", 3, V + 6), ("draft", 5, V + 9)):
+        wide = torch.full((43, width), float("nan"), device=cuda)
+        wide[:, at:at + V] = getattr(c, name)
+        setattr(c, name, wide[:, at:at + V])
+    c.check(cuda, label="unlike alignment")
+
+
+def test_no_vocabulary(cuda):
+    from dforktree_amd import ops
+    announce("tree_accept without tokens")
+    i, p, u = torch.zeros(5, dtype=torch.int32, device=cuda), torch.ones(5, 0, device=cuda), torch.rand(5, device=cuda)
+    for draft in (None, p):
+        status = torch.zeros(1, dtype=torch.int32, device=cuda)
+        got = ops.tree_accept(i, i, p, u, u[:1], draft_probs=draft, status=status)
+        assert got["token"].tolist() == [-1] and got["path_len"].tolist() == [1]
+        assert got["path"][0].tolist() == [0] + [-1] * 15 and status.tolist() == [P.STATUS_WEIGHT]
+
+
+def test_two_at_once(cuda):
+    """Two calls on streams of their own."""
+    from dforktree_amd import ops
+    announce("tree_accept on two streams")
+    cases = [Case([33, 64, 20], 20001, "tree", True, seed=s) for s in (17, 18)]
+    args = [([x.to(cuda) for x in (c.tokens, c.parent, c.probs, c.u, c.last)],
+             dict(draft_probs=c.draft.to(cuda), cu_seqlens=torch.tensor(c.cu, dtype=torch.int32, device=cuda), n_nodes=64))
+            for c in cases]
+    want = [ops.tree_accept(*t, **kw) for t, kw in args]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    for _ in range(8):
+        for k in (0, 1):
+            with torch.cuda.stream(streams[k]):
+                got[k].append(ops.tree_accept(*args[k][0], **args[k][1]))
+    torch.cuda.synchronize()
+    for k in (0, 1):
+        for g in got[k]:
+            assert all(torch.equal(g[n], want[k][n]) for n in g)
+
+
 def test_offsets_past_32_bits(cuda):
     c = Case([9, 30, 4], 1001, "tree", True, seed=13)
     for name in ("probs", "draft"):

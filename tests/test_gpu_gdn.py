@@ -325,6 +325,31 @@ def test_captured_and_on_another_stream(cuda, sizes):
         torch.cuda.synchronize()
 
 
+def test_two_at_once(cuda):
+    """Two calls on streams of their own, each with chunks and its own workspace."""
+    from dforktree_amd import ops
+    announce("prompt_gdn on two streams")
+    cases = [Case(200, 2, 4, 3, cuda, seed=s) for s in (31, 32)]
+    cu = torch.tensor([0, 70, 71, 200], dtype=torch.int32, device=cuda)
+    run = lambda c, pool: ops.prompt_gdn(c.y, c.a, c.b, c.A_log, c.dt_bias, pool.transpose(-1, -2), cu, hk=2, hv=4,  # noqa: E731
+                                         max_len=129)
+    want = []
+    for c in cases:
+        pool = c.pool.clone()
+        want.append((run(c, pool), pool))
+    pools = [[c.pool.clone() for _ in range(6)] for c in cases]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    for i in range(6):
+        for k in (0, 1):
+            with torch.cuda.stream(streams[k]):
+                got[k].append(run(cases[k], pools[k][i]))
+    torch.cuda.synchronize()
+    for k in (0, 1):
+        for o, pool in zip(got[k], pools[k]):
+            assert torch.equal(o, want[k][0]) and torch.equal(pool, want[k][1])
+
+
 def test_same_on_every_run(cuda):
     """No sum depends on the order in which workgroups finish, or on the requests beside one."""
     from dforktree_amd import ops
