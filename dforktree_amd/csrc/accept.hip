@@ -8,9 +8,9 @@
 // launch does one pass for every request, whatever it is of that request's; the
 // next one walks again, with the sums there are, to the next pass, until a walk's
 // last.  Without the drafter's probabilities the first pass is the last; with
-// them kRounds launches are made, and what is still open is done by the request's
-// workgroup alone in the last launch, which finds the token from the sums of its
-// slice: a slice's tokens side by side, added up over the workgroup.
+// them up to kRounds launches are made, and what is still open is done by the
+// request's workgroup alone in the last launch, which finds the token from the
+// sums of its slice: a slice's tokens side by side, added up over the workgroup.
 //
 // Bound by launches and by the walk's dependent fetches where passes are few: 23
 // us for one request of 16 nodes over 131072 tokens, 34 for 64 drawn chains, 22
@@ -494,7 +494,8 @@ __global__ void __launch_bounds__(kLast) last_kernel(const dft_tree_accept_args 
   }
 }
 
-int rounds_of(const dft_tree_accept_args& a) { return a.draft_probs ? kRounds : 1; }
+// A pass for every refused child with a sibling behind it, and the last one: no more than there are children.
+int rounds_of(const dft_tree_accept_args& a) { return a.draft_probs ? std::min(kRounds, std::max(a.n_nodes - 1, 1)) : 1; }
 // Slices such that a pass has some thousand workgroups, of no less than 1024 tokens.
 Work work_of(const dft_tree_accept_args& a) {
   Work w = {};
