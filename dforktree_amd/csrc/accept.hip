@@ -12,11 +12,11 @@
 // request's workgroup alone in the last launch, which finds the token from the
 // sums of its slice: a slice's tokens side by side, added up over the workgroup.
 //
-// Bound by launches and by the walk's dependent fetches where passes are few: 23
-// us for one request of 16 nodes over 131072 tokens, 34 for 64 drawn chains, 22
+// Bound by launches and by the walk's dependent fetches where passes are few: 22
+// us for one request of 16 nodes over 131072 tokens, 33 for 64 drawn chains, 22
 // for 64 trees of 32 nodes without a drafter's rows; of these the last launch is 8
-// to 12, and a launch that finds nothing to do costs 1.6.  48 drawn trees of 8 to
-// 40 nodes over 100003 tokens take 69: with two rounds, and a request's further
+// to 11, and a launch that finds nothing to do costs 1.6.  48 drawn trees of 8 to
+// 40 nodes over 100003 tokens take 66: with two rounds, and a request's further
 // passes by its workgroup alone, 180.  Their passes are bound by the 64-bit units:
 // a reduction divides by two numbers that are the same for the whole row, so it
 // multiplies by their reciprocals.
@@ -30,7 +30,7 @@
 namespace dft {
 namespace {
 
-constexpr int kNodes = 64, kSlices = 64, kRounds = 4;
+constexpr int kNodes = 64, kSlices = 64, kRounds = 4, kShort = 16384;
 constexpr int kPass = 256, kLast = 512, kWaves = kLast / 64;  // threads of a pass and of the last launch
 
 template <class T>
@@ -48,35 +48,10 @@ __device__ __forceinline__ double weight(const void* p, int64_t at, int dt) {
 struct Refused {
   int count;
   int token[kNodes];
-  double off[kNodes + 1];  // mass of the tokens in front of this one
-  double sum[kNodes];      // of the weights left behind it (drafter's distribution given)
-  double by_off[kNodes], by_sum[kNodes];  // 1 / (1 - off), 1 / sum; 0 for what counts as none
+  // 1 over 1 less the drafter's mass of the tokens in front of this one, and over the sum of the weights left behind it; 0
+  // for what counts as none
+  double by_off[kNodes], by_sum[kNodes];
 };
-
-// r at token x behind `count` refused ones; `open`: the last one's sum is not
-// known, and not divided by.
-template <bool DRAFT>
-__device__ __forceinline__ double left_at(double p, double q0, int x, const Refused& f, int count, bool open) {
-  if constexpr (!DRAFT) {
-    for (int j = 0; j < count; ++j)
-      if (f.token[j] == x) return 0;
-    return p;
-  } else {
-    double r = p;
-    bool gone = false;
-    for (int j = 0; j < count; ++j) {
-      const double off = f.off[j];
-      const double q = gone || off >= 1 ? 0 : off > 0 ? q0 / (1 - off) : q0;
-      const double rest = fmax(r - q, 0.0);
-      if (j == count - 1 && open)
-        r = rest;
-      else if (f.sum[j] > 0)
-        r = rest / f.sum[j];
-      gone |= f.token[j] == x;
-    }
-    return r;
-  }
-}
 
 __device__ __forceinline__ double wave_sum(double x) {
   for (int o = 32; o; o >>= 1) x += __shfl_xor(x, o);
@@ -103,82 +78,103 @@ struct Walk {
   bool open, last;         // whether that is of the last refusal, and the walk's last
 };
 
-// By the first wave, a node a lane.  sum(pass): an earlier round's, `have` of them.
-template <bool DRAFT, class T, class Sum>
-__device__ __forceinline__ void walk(const dft_tree_accept_args& a, const packed::Span& s, Walk& w, int have, Sum sum) {
-  const int lane = threadIdx.x & 63;
+// Lane c's value, c the same for all.
+__device__ __forceinline__ double of_lane(double x, int c) {
+  const uint64_t bits = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)bits, c), hi = __builtin_amdgcn_readlane((uint32_t)(bits >> 32), c);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+
+// The walk, by one wave, a node a lane: every lane holds what is left of r and q
+// at its own token, so that a refusal costs the same however many there were.
+template <bool DRAFT, class T>
+struct Walker {
   int parent = -1, token = 0;
   double u = 0, p = 0, q = 0;
-  if (lane > 0 && lane < s.n) {
-    const int64_t row = s.r0 + lane, up = max(ld_i(a.parent, row, a.parent_dtype), (int64_t)0);
-    const int64_t t = ld_i(a.tokens, row, a.tokens_dtype);
-    if (up < lane && t >= 0 && t < a.vocab) {
-      parent = (int)up;
-      token = (int)t;
-      u = a.uniform[row];
-      p = weight<T>(a.probs, (s.r0 + up) * a.probs_row_stride + t, a.probs_dtype);
-      if (DRAFT) q = weight<T>(a.draft_probs, (s.r0 + up) * a.draft_row_stride + t, a.draft_dtype);
-    }
-  }
-  // every lane keeps the same state, and writes the same to the LDS
-  int node = 0, length = s.n > 0, count = 0, pass = 0;
-  bool open = false, last = false;
+  // at the node where the path stands: r at the lane's token, before and after it is divided by the sum, and whether the
+  // token has been refused
+  double r, rest = 0;
+  bool gone = false;
+  int node = 0, length, count = 0, pass = 0;
+  bool open = false, waits = false;  // (every lane keeps the same of these)
   double off = 0;
-  w.path[0] = 0;
-  w.f.off[0] = 0;
-  uint64_t kids = __ballot(parent == 0);
-  while (true) {
-    if (!kids || length >= a.path_cols) {
-      last = true;
-      break;
-    }
-    const int c = __ffsll((unsigned long long)kids) - 1;
-    kids &= kids - 1;
-    const int t = __shfl(token, c);
-    const double uc = __shfl(u, c), pc = __shfl(p, c), qc = __shfl(q, c);
-    bool gone = false;
-    for (int j = 0; j < count; ++j) gone |= w.f.token[j] == t;
-    const double r = left_at<DRAFT>(pc, qc, t, w.f, count, false);
-    bool stands;
-    double take;  // what a refusal takes: of q, without a drafter's of r
-    if constexpr (DRAFT) {
-      stands = uc * (gone || off >= 1 ? 0 : off > 0 ? qc / (1 - off) : qc) < r;
-      take = gone ? 0 : qc;
-    } else {
-      stands = uc * (1 - off) < r;
-      take = r;
-    }
-    if (stands) {
-      node = c;
-      w.path[length++] = c;
-      count = 0;
-      off = 0;
-      open = false;
-      kids = __ballot(parent == c);
-      continue;
-    }
-    w.f.by_off[count] = off >= 1 ? 0 : 1 / (1 - off);
-    w.f.token[count++] = t;
-    off += take;
-    w.f.off[count] = off;
-    if constexpr (DRAFT) {
-      open = true;
-      if (kids) {  // its sum decides about the next sibling
-        if (pass == have) break;
-        const double left = sum(pass++);
-        w.f.sum[count - 1] = left;
-        w.f.by_sum[count - 1] = left > 0 ? 1 / left : 0;
-        open = false;
+  uint64_t kids;
+
+  __device__ __forceinline__ Walker(const dft_tree_accept_args& a, const packed::Span& s, Walk& w) : length(s.n > 0) {
+    const int lane = threadIdx.x & 63;
+    if (lane > 0 && lane < s.n) {
+      const int64_t row = s.r0 + lane, up = max(ld_i(a.parent, row, a.parent_dtype), (int64_t)0);
+      const int64_t t = ld_i(a.tokens, row, a.tokens_dtype);
+      if (up < lane && t >= 0 && t < a.vocab) {
+        parent = (int)up;
+        token = (int)t;
+        u = a.uniform[row];
+        p = weight<T>(a.probs, (s.r0 + up) * a.probs_row_stride + t, a.probs_dtype);
+        if (DRAFT) q = weight<T>(a.draft_probs, (s.r0 + up) * a.draft_row_stride + t, a.draft_dtype);
       }
     }
+    r = p;
+    kids = __ballot(parent == 0);
+    w.path[0] = 0;
   }
-  w.f.count = count;
-  w.node = node;
-  w.length = length;
-  w.pass = pass;
-  w.open = open;
-  w.last = last;
-}
+
+  // On to the pass that comes next, with sum(pass) of the `have` ones made.
+  template <class Sum>
+  __device__ __forceinline__ void operator()(const dft_tree_accept_args& a, Walk& w, int have, Sum sum) {
+    bool last = false;
+    while (true) {
+      if (waits) {
+        if (pass == have) break;
+        const double left = sum(pass++);
+        w.f.by_sum[count - 1] = left > 0 ? 1 / left : 0;
+        if (left > 0) r = rest / left;
+        open = waits = false;
+      }
+      if (!kids || length >= a.path_cols) {
+        last = true;
+        break;
+      }
+      const int c = __ffsll((unsigned long long)kids) - 1;
+      kids &= kids - 1;
+      const int t = __builtin_amdgcn_readlane(token, c);
+      bool stands;
+      double take;  // what a refusal takes: of q, without a drafter's of r
+      if constexpr (DRAFT) {
+        const double now = gone || off >= 1 ? 0 : off > 0 ? q / (1 - off) : q;
+        stands = of_lane(u, c) * of_lane(now, c) < of_lane(r, c);
+        take = of_lane(gone ? 0 : q, c);
+        rest = fmax(r - now, 0.0);
+      } else {
+        take = of_lane(gone ? 0 : p, c);
+        stands = of_lane(u, c) * (1 - off) < take;
+      }
+      if (stands) {
+        node = c;
+        w.path[length++] = c;
+        count = 0;
+        off = 0;
+        open = gone = false;
+        r = p;
+        kids = __ballot(parent == c);
+        continue;
+      }
+      gone |= token == t;
+      w.f.by_off[count] = off >= 1 ? 0 : 1 / (1 - off);
+      w.f.token[count++] = t;
+      off += take;
+      if constexpr (DRAFT) {
+        open = true;
+        waits = kids;  // its sum decides about the next sibling
+      }
+    }
+    w.f.count = count;
+    w.node = node;
+    w.length = length;
+    w.pass = pass;
+    w.open = open;
+    w.last = last;
+  }
+};
 
 // Four tokens of a row, from x on, of which those in [from, to) are there.
 template <class T>
@@ -289,7 +285,7 @@ __global__ void __launch_bounds__(kPass) pass_kernel(const dft_tree_accept_args 
   auto sum_of = [&](int pass) {
     return wave_sum(lane < work.slices ? work.sums[((int64_t)pass * a.batch + b) * kSlices + lane] : 0.0);
   };
-  if (wave == 0) walk<DRAFT, T>(a, s, w, round, sum_of);
+  if (wave == 0) Walker<DRAFT, T>(a, s, w)(a, w, round, sum_of);
   __syncthreads();
   const int from = min(slice * work.length, a.vocab), to = min(from + work.length, a.vocab);
   double sum;
@@ -337,6 +333,22 @@ __global__ void __launch_bounds__(kLast) last_kernel(const dft_tree_accept_args 
   __shared__ int tops[kSlices];
   __shared__ int found;
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  // fetched side by side, whether there is a use for it or not: the walk, every round's sums, the random number
+  constexpr int kWords = sizeof(Walk) / 4;
+  static_assert(kWords <= kLast && kRounds * kSlices <= kLast);
+  const double last = a.last[b];
+  double slice_sum = 0;
+  int slice_top = -1, done = 0;
+  uint32_t word = 0;
+  if (rounds) {
+    done = work.done[(rounds - 1) * a.batch + b];
+    if (tid < kWords) word = reinterpret_cast<const uint32_t*>(work.walks + b)[tid];
+    if (tid < rounds * kSlices && lane < work.slices) {
+      const int64_t at = ((int64_t)wave * a.batch + b) * kSlices + lane;
+      slice_sum = work.sums[at];
+      slice_top = work.tops[at];
+    }
+  }
   const packed::Span s = packed::span_of(a.cu_seqlens, a.rows, a.n_nodes, b);
   int* path = a.path + (int64_t)b * a.path_cols;
   int64_t* path_rows = a.path_rows + (int64_t)b * a.path_cols;
@@ -357,9 +369,8 @@ __global__ void __launch_bounds__(kLast) last_kernel(const dft_tree_accept_args 
       __syncthreads();
     };
     auto total_of = [&](int parts) { return wave_sum(lane < parts ? sums[lane] : 0.0); };
-    if (work.done[(rounds - 1) * a.batch + b]) {
-      const uint32_t* from = reinterpret_cast<const uint32_t*>(work.walks + b);
-      for (int i = tid; i < (int)(sizeof(Walk) / 4); i += kLast) reinterpret_cast<uint32_t*>(&w)[i] = from[i];
+    if (done) {
+      if (tid < kWords) reinterpret_cast<uint32_t*>(&w)[tid] = word;
       __syncthreads();
     } else {
       auto sum_of = [&](int pass) {
@@ -367,9 +378,10 @@ __global__ void __launch_bounds__(kLast) last_kernel(const dft_tree_accept_args 
         return wave_sum(lane < work.slices ? work.sums[((int64_t)pass * a.batch + b) * kSlices + lane] : 0.0);
       };
       // passes that no round was left for are made here
+      Walker<DRAFT, T> walker(a, s, w);
       for (int have = rounds;; ++have) {
         __syncthreads();
-        if (wave == 0) walk<DRAFT, T>(a, s, w, have, sum_of);
+        if (wave == 0) walker(a, w, have, sum_of);
         __syncthreads();
         if (w.last) break;
         sum_up(0, V, w.f.count, w.open);
@@ -383,11 +395,7 @@ __global__ void __launch_bounds__(kLast) last_kernel(const dft_tree_accept_args 
     bool open = w.open, sliced = w.pass < rounds;
     if (sliced) {
       parts = work.slices;
-      if (tid < parts) {
-        const int64_t at = ((int64_t)w.pass * a.batch + b) * kSlices + tid;
-        sums[tid] = work.sums[at];
-        tops[tid] = work.tops[at];
-      }
+      if (wave == w.pass) sums[lane] = slice_sum, tops[lane] = slice_top;
       __syncthreads();
     } else {
       sum_up(0, V, count, open);
@@ -402,7 +410,7 @@ __global__ void __launch_bounds__(kLast) last_kernel(const dft_tree_accept_args 
       total = total_of(parts);
     }
     if (total > 0) {
-      const double target = (double)a.last[b] * total;
+      const double target = last * total;
       double before = 0;
       int from = 0, to = V;
       while (token < 0) {
@@ -494,8 +502,14 @@ __global__ void __launch_bounds__(kLast) last_kernel(const dft_tree_accept_args 
   }
 }
 
-// A pass for every refused child with a sibling behind it, and the last one: no more than there are children.
-int rounds_of(const dft_tree_accept_args& a) { return a.draft_probs ? std::min(kRounds, std::max(a.n_nodes - 1, 1)) : 1; }
+// A pass for every refused child with a sibling behind it, and the last one: no
+// more than there are children.  None over short rows, which a request's workgroup
+// passes over as fast (64 trees of 16 nodes, us in a captured graph: over 2000 tokens
+// 11 and 13, drawn 26 and 37; 16000 13 and 15, 39 and 51; 32000 17 and 16, 65 and 49).
+int rounds_of(const dft_tree_accept_args& a) {
+  if (a.vocab <= kShort) return 0;
+  return a.draft_probs ? std::min(kRounds, std::max(a.n_nodes - 1, 1)) : 1;
+}
 // Slices such that a pass has some thousand workgroups, of no less than 1024 tokens.
 Work work_of(const dft_tree_accept_args& a) {
   Work w = {};

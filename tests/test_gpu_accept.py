@@ -211,6 +211,40 @@ def test_rows_of_unlike_alignment(cuda, V):
     c.check(cuda, label="unlike alignment")
 
 
+@pytest.mark.parametrize("seed", range(3))
+def test_many_refusals_over_long_rows(cuda, seed):
+    """More passes over whole rows than launches make, beside requests of few."""
+    c = Case([40, 3, 64, 1, 9], 20001 + seed, "star" if seed else "tree", True, seed=40 + seed, sharp=0.3)
+    c.u.fill_(1 - 2.0 ** -24)
+    c.check(cuda, label="refused over long rows")
+
+
+def test_captured_over_long_rows(cuda):
+    from dforktree_amd import ops
+    announce("tree_accept over long rows in a graph")
+    c = Case([30, 9, 20], 30001, "tree", True, seed=19)
+    t = [x.to(cuda) for x in (c.tokens, c.parent, c.probs, c.u, c.last, c.draft)]
+    cu = torch.tensor(c.cu, dtype=torch.int32, device=cuda)
+    run = lambda: ops.tree_accept(*t[:5], draft_probs=t[5], cu_seqlens=cu, n_nodes=30)  # noqa: E731
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run()
+    for step in range(4):
+        g = torch.Generator().manual_seed(step)
+        t[3].copy_(torch.rand(59, generator=g) ** (0.2 if step % 2 else 1))
+        t[4].copy_(torch.rand(3, generator=g))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = run()
+        for k in out:
+            assert torch.equal(out[k], want[k]), (step, k)
+
+
 def test_no_vocabulary(cuda):
     from dforktree_amd import ops
     announce("tree_accept without tokens")
