@@ -226,26 +226,23 @@ __device__ __forceinline__ void pass_over(const dft_tree_accept_args& a, int64_t
     }
     double r[16];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) r[i] = p[i / 4][i % 4] > 0 ? (double)p[i / 4][i % 4] : 0.0;
-    uint32_t gone = 0;
+    for (int i = 0; i < 16; ++i) {
+      r[i] = p[i / 4][i % 4] > 0 ? (double)p[i / 4][i % 4] : 0.0;
+      if (DRAFT) q[i / 4][i % 4] = q[i / 4][i % 4] > 0 ? q[i / 4][i % 4] : 0.f;
+    }
     for (int j = 0; j < count; ++j) {
-      const int t = f.token[j];
-      if constexpr (DRAFT) {
-        const bool raw = j == count - 1 && open;
-        const double by_off = f.by_off[j], by_sum = raw ? 1 : f.by_sum[j];
+      const double by_sum = !DRAFT || (j == count - 1 && open) ? 1 : f.by_sum[j];
+      if (DRAFT && by_sum > 0) {
+        const double by_off = f.by_off[j];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float q0 = q[i / 4][i % 4];
-          const double at = q0 > 0 && !(gone >> i & 1) ? (double)q0 * by_off : 0;
-          const double rest = fmax(r[i] - at, 0.0) * by_sum;
-          r[i] = by_sum > 0 ? rest : r[i];
-        }
+        for (int i = 0; i < 16; ++i) r[i] = fmax(r[i] - (double)q[i / 4][i % 4] * by_off, 0.0) * by_sum;
       }
+      const int at = f.token[j] - x0;  // the refused one: out of q, or without a drafter's out of r
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const bool is = x0 + 4 * (i / 4) * threads + i % 4 == t;
+        const bool is = at == 4 * (i / 4) * threads + i % 4;
         if constexpr (DRAFT)
-          gone |= (uint32_t)is << i;
+          q[i / 4][i % 4] = is ? 0.f : q[i / 4][i % 4];
         else
           r[i] = is ? 0 : r[i];
       }
