@@ -12,14 +12,14 @@
 // request's workgroup alone in the last launch, which finds the token from the
 // sums of its slice: a slice's tokens side by side, added up over the workgroup.
 //
-// Bound by launches and by the walk's dependent fetches where passes are few: 22
-// us for one request of 16 nodes over 131072 tokens, 33 for 64 drawn chains, 22
-// for 64 trees of 32 nodes without a drafter's rows; of these the last launch is 8
-// to 11, and a launch that finds nothing to do costs 1.6.  48 drawn trees of 8 to
-// 40 nodes over 100003 tokens take 66: with two rounds, and a request's further
-// passes by its workgroup alone, 180.  Their passes are bound by the 64-bit units:
-// a reduction divides by two numbers that are the same for the whole row, so it
-// multiplies by their reciprocals.
+// Bound by launches and by the walk's dependent fetches where passes are few: 21
+// us for one request of 16 nodes over 131072 tokens, 32 for 64 drawn chains, 21
+// for 64 trees of 32 nodes without a drafter's rows; of these the last launch is 7
+// to 10, and a launch that finds nothing to do costs 1.6.  48 drawn trees of 8 to
+// 40 nodes over 100003 tokens take 49; with two rounds only, and a request's
+// further passes by its workgroup alone, three times as much.  Their passes are
+// bound by the 64-bit units: a reduction divides by two numbers that are the same
+// for the whole row, so it multiplies by their reciprocals.
 //
 // Sums are held in 64 bits: a sum of 10^5 probabilities in 32 bits moves one
 // drawn token in some hundred over a border.  They are added up in one order.
@@ -507,10 +507,12 @@ int rounds_of(const dft_tree_accept_args& a) {
   if (a.vocab <= kShort) return 0;
   return a.draft_probs ? std::min(kRounds, std::max(a.n_nodes - 1, 1)) : 1;
 }
-// Slices such that a pass has some thousand workgroups, of no less than 1024 tokens.
+// Slices such that a pass has some two thousand workgroups, of no less than 1024
+// tokens.  (With one thousand 48 drawn trees take 56 us instead of 49, 64 chains
+// 30 instead of 32.)
 Work work_of(const dft_tree_accept_args& a) {
   Work w = {};
-  const int most = std::min(kSlices, std::max(1, 1024 / a.batch));
+  const int most = std::min(kSlices, std::max(1, 2048 / a.batch));
   w.length = std::max(1024, ((a.vocab + most - 1) / most + 1023) / 1024 * 1024);
   w.slices = std::max(1, (a.vocab + w.length - 1) / w.length);
   return w;
