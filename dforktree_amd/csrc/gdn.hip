@@ -12,11 +12,9 @@
 // gdn_chunk_kernel forms what needs no state, X and P, for all chunks at once,
 // gdn_scan_kernel takes the states through the chunks.  The raw rows are bf16,
 // so that K, Q and K^T are exact operands of bf16 products.  What is not goes in
-// as a sum of bf16 parts.  States are handed on in fp32 from call to call: what
-// they pass through (S, X - I, W, U) has three parts, 2^-24 relative at most,
-// and products of two such factors the six of 2^-16 or more (with two parts, a
-// third less products, the states came out 4 10^-6 off, with three 2 to 5 10^-7).
-// What only an output of the row passes through (P, U in O, S in Q S) has two.
+// as a sum of three bf16 parts, 2^-24 relative at most, and a product of two such
+// factors as its six of 2^-16 or more.  (With two parts states and fp32 outputs
+// come out 4 10^-6 off.  Two where only outputs pass through: 8 to 10% less time.)
 #include <algorithm>
 #include <type_traits>
 
@@ -190,11 +188,11 @@ constexpr int kFragment = 1024;  // bytes: 64 lanes x 16
 // m / 2, six fragments of 8 elements a lane, the first four of every lane first.
 constexpr int kX = 6 * 2 * kFragment;
 __host__ __device__ constexpr int x_at(int m, int s) { return m < 2 ? m : 2 * m - 2 + s; }
-// P's six in two parts, and a fragment of zeros for the other step of the row
+// P's six in three parts, and a fragment of zeros for the other step of the row
 // tiles 0 and 1, so that all waves do the same (loads whose use depends on the
 // wave are waited for too early).
-constexpr int kP = (6 * 2 + 1) * kFragment;
-__host__ __device__ constexpr int p_at(int m, int s) { return m < 2 && s ? 12 : 2 * x_at(m, s); }
+constexpr int kP = (6 * 3 + 1) * kFragment;
+__host__ __device__ constexpr int p_at(int m, int s) { return m < 2 && s ? 18 : 3 * x_at(m, s); }
 // Factors of the rows, 64 floats each: beta, e^G rk beta, rk, e^(G_63 - G), e^G_63 (of all); e^G, rq.
 enum { kBeta, kDecayed, kUnit, kOut, kKeep, kDecay, kRq, kCoefs = 8 };
 constexpr int kHead = kX + kP + kCoefs * kChunk * 4;
@@ -310,12 +308,12 @@ __global__ void __launch_bounds__(256, 4) gdn_chunk_kernel(const dft_prompt_gdn_
     coef[kOut * kChunk] = lane < n ? __builtin_amdgcn_exp2f(all - sum) : 0;
     coef[kKeep * kChunk] = __builtin_amdgcn_exp2f(all);
     coef[kDecay * kChunk] = __builtin_amdgcn_exp2f(sum);
-    *reinterpret_cast<u32x4*>(out + kX + 12 * kFragment + 16 * lane) = u32x4{};
+    *reinterpret_cast<u32x4*>(out + kX + 18 * kFragment + 16 * lane) = u32x4{};
   }
 
   // A into the LDS, P to its place, transposed: Gram tiles K K^T and K Q^T of the keys of tiles j <= w with the wave's rows
   const float Gq = G[mine], bk = beta[mine] * rks[mine];
-  Parts4<2> p[4];
+  Parts4<3> p[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     p[j] = {};
@@ -338,13 +336,13 @@ __global__ void __launch_bounds__(256, 4) gdn_chunk_kernel(const dft_prompt_gdn_
       y[r] = ahead >= 0 ? qk[r] * decay : 0.f;
     }
     *reinterpret_cast<f32x4*>(&A[mine][16 * j + 4 * g]) = x;
-    p[j] = split4<2>(y);
+    p[j] = split4<3>(y);
   }
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     if (j > w / 2) continue;
 #pragma unroll
-    for (int z = 0; z < 2; ++z)
+    for (int z = 0; z < 3; ++z)
       *reinterpret_cast<u64x2*>(out + kX + (p_at(w, j) + z) * kFragment + 16 * lane) = u64x2{p[2 * j].p[z], p[2 * j + 1].p[z]};
   }
   // the wave's diagonal block: its two halves' inverses D by substitution, a column a lane (four times over), and with L
@@ -479,8 +477,8 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_kernel(const dft_pro
   __shared__ __attribute__((aligned(16))) uint16_t v_lds[kChunk][BN];
   __shared__ __attribute__((aligned(16))) float coef_lds[2][kCoefs][kChunk];
   __shared__ __attribute__((aligned(16))) f32x4 sums[NT][4][4][64];  // [t][of wave][row tile][lane]
-  __shared__ __attribute__((aligned(16))) uint16_t Sb[2][BN][kSRow];
-  __shared__ __attribute__((aligned(16))) uint16_t Wb[3][BN][kRow], Ub[2][BN][kRow], Vb[3][BN][kRow];
+  __shared__ __attribute__((aligned(16))) uint16_t Sb[3][BN][kSRow];
+  __shared__ __attribute__((aligned(16))) uint16_t Wb[3][BN][kRow], Ub[3][BN][kRow], Vb[3][BN][kRow];
   if (blockIdx.x == 0 && a.status)
     for (int b = threadIdx.x; b < a.batch; b += kScanThreads)
       a.status[b] = span_of(a, b).status | slot_of(a.state_indices, a.state_indices_dtype, a.initial, a.slots, b).status;
@@ -602,7 +600,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_kernel(const dft_pro
   }
   if (wave >= 4) {
     const bool vec = a.o_dtype == DFT_F32 && reinterpret_cast<uintptr_t>(a.o) % 16 == 0 && a.o_row_stride % 4 == 0 && a.o_h_stride % 4 == 0;
-    bf16x8 q[4], p[2][2];  // the wave's rows of Q and P
+    bf16x8 q[4], p[2][3];  // the wave's rows of Q and P
     float decay, rq;       // of row l16
     auto load_q = [&](int at) {
       const uint16_t* row = row_at(at, 16 * w + l16) + kh * kD + 8 * g;
@@ -614,7 +612,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_kernel(const dft_pro
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int z = 0; z < 2; ++z)
+        for (int z = 0; z < 3; ++z)
           p[j][z] = *reinterpret_cast<const bf16x8*>(head + (p_at(w, j) + (j && w < 2 ? 0 : z)) * kFragment + 16 * lane);
       const float* coef = reinterpret_cast<const float*>(head + kP) + 16 * w + l16;
       decay = coef[kDecay * kChunk];
@@ -652,29 +650,32 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_kernel(const dft_pro
       }
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        f32x4 q0 = {}, q1 = {};
+        f32x4 sum[3] = {};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          q0 = mfma16(get(&Sb[0][16 * t + l16][32 * j + 8 * g]), q[j], q0);
-          q1 = mfma16(get(&Sb[1][16 * t + l16][32 * j + 8 * g]), q[j], q1);
-        }
-        o[t] = (q0 + q1) * decay;
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int z = 0; z < 3; ++z) sum[z] = mfma16(get(&Sb[z][16 * t + l16][32 * j + 8 * g]), q[j], sum[z]);
+        o[t] = (sum[0] + (sum[1] + sum[2])) * decay;
       }
       load_q(at + 1);
       __syncthreads();  // 2
       __syncthreads();  // 3: U is there
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        f32x4 o0 = o[t], o1 = {};
+        f32x4 o0 = o[t], o1 = {}, o2 = {}, o3 = {};
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          const bf16x8 u0 = get(&Ub[0][16 * t + l16][32 * j + 8 * g]);
-          const bf16x8 u1 = get(&Ub[1][16 * t + l16][32 * j + 8 * g]);
-          o0 = mfma16(u0, p[j][0], o0);
-          o1 = mfma16(u1, p[j][0], o1);
-          o1 = mfma16(u0, p[j][1], o1);
+          bf16x8 u[3];
+#pragma unroll
+          for (int z = 0; z < 3; ++z) u[z] = get(&Ub[z][16 * t + l16][32 * j + 8 * g]);
+          o0 = mfma16(u[0], p[j][0], o0);
+          o1 = mfma16(u[1], p[j][0], o1);
+          o2 = mfma16(u[0], p[j][1], o2);
+          o3 = mfma16(u[1], p[j][1], o3);
+          o1 = mfma16(u[2], p[j][0], o1);
+          o2 = mfma16(u[0], p[j][2], o2);
         }
-        o[t] = (o0 + o1) * rq;
+        o[t] = (o0 + ((o1 + o2) + o3)) * rq;
       }
     }
     store_rows(chunks - 1);
@@ -731,7 +732,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_kernel(const dft_pro
 #pragma unroll
         for (int m = 0; m < 4; ++m) sum[m] = mfma16(k[m], p[z], sum[m]);
 #pragma unroll
-      for (int z = 0; z < 2; ++z) *reinterpret_cast<bf16x8*>(&Sb[z][16 * t + l16][32 * w + 8 * g]) = p[z];
+      for (int z = 0; z < 3; ++z) *reinterpret_cast<bf16x8*>(&Sb[z][16 * t + l16][32 * w + 8 * g]) = p[z];
 #pragma unroll
       for (int m = 0; m < 4; ++m) sums[t][w][m][lane] = sum[m];
     }
@@ -784,9 +785,9 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_kernel(const dft_pro
       const Parts4<3> d = split4<3>(u[t] * out);
 #pragma unroll
       for (int z = 0; z < 3; ++z) put(&Vb[z][16 * t + l16][place], d.p[z]);
-      const Parts4<2> p = split4<2>(u[t]);
+      const Parts4<3> p = split4<3>(u[t]);
 #pragma unroll
-      for (int z = 0; z < 2; ++z) put(&Ub[z][16 * t + l16][place], p.p[z]);
+      for (int z = 0; z < 3; ++z) put(&Ub[z][16 * t + l16][place], p.p[z]);
     }
     __syncthreads();  // 3
 #pragma unroll

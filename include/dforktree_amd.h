@@ -721,8 +721,7 @@ DFT_API int dft_prompt_conv(const dft_prompt_conv_args* args, void* stream);
  * g = neg_exp_A softplus(a + dt_bias):
  *   S <- e^g S;  u = beta (v - S^T k);  S <- S + k u^T;  o = S^T q.
  * States, sums and decays are held in fp32; factors of the chunks' products
- * are sums of bf16 parts, three where a state passes through (2^-24 relative),
- * two where only outputs do (2^-17).  What is not finite in a row reaches at most
+ * are sums of three bf16 parts (2^-24 relative).  What is not finite in a row reaches at most
  * the rows of its request from the 64 in a row on that it is one of. */
 typedef struct dft_prompt_gdn_args {
   int32_t batch, max_len;
