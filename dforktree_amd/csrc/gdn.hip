@@ -230,11 +230,20 @@ __device__ __forceinline__ Parts4<N> split4(f32x4 x) {
 }
 typedef uint64_t u64x2 __attribute__((ext_vector_type(2)));
 
+// A row's decay, in log2 units, down to which it matters: 2^-512 is zero in fp32
+// already, for this row and for every span of rows that it is one of, and sums
+// stay finite.
+constexpr double kLeast = -512;
+
 // X and P of a chunk and v head: a workgroup of four waves, wave w for rows 16 w ...
 // Row block by row block from X (I + A) = I: diagonal blocks by substitution
 // (their powers would lose what equal keys leave of 32 bits), then X_ij =
 // -(sum_(j<m<=i) X_im A_mj) X_jj in fp32 products, transposed, so that each result
 // is the next one's operand and the last the fragment that is stored.
+// A decay between two rows is the difference of two running sums: they are added
+// up in 64 bits and kept in two floats, or a few rows that leave nothing of the
+// state would leave the weak gates behind them a sum of thousands, in steps of
+// 10^-3 (24 rows of g = -300 among weak ones: states 4 10^-4 off, so 1 10^-7).
 // Bound by the instructions that its waves issue, so by what of them stand ready:
 // 128 registers, four workgroups a CU.  A prompt of 8192 rows and 32 heads 52 us,
 // 4.5 TB/s; with two workgroups a CU 78.
@@ -242,7 +251,7 @@ __global__ void __launch_bounds__(256, 4) gdn_chunk_kernel(const dft_prompt_gdn_
   constexpr int kKRow = kD + 8, kARow = kChunk + 4;
   __shared__ __attribute__((aligned(16))) uint16_t keys[kChunk][kKRow];
   __shared__ __attribute__((aligned(16))) float A[kChunk][kARow];
-  __shared__ __attribute__((aligned(16))) float G[kChunk], beta[kChunk], rks[kChunk];
+  __shared__ __attribute__((aligned(16))) float G[2][kChunk], beta[kChunk], rks[kChunk];
   // the v heads of a k head read the same rows: one after the other on one XCD
   const int share = a.hv / a.hk, in = blockIdx.x / kXcds;
   const int64_t unit = (int64_t)(in / share) * kXcds + blockIdx.x % kXcds, tile = unit / a.hk;
@@ -264,19 +273,21 @@ __global__ void __launch_bounds__(256, 4) gdn_chunk_kernel(const dft_prompt_gdn_
 #pragma unroll
   for (int j = 0; j < 4; ++j) qw[j] = *reinterpret_cast<const u32x4*>(row - a.hk * kD + 32 * j);
   Gate gate = {};
-  float sum = 0, all = 0;
+  double sum = 0, all = 0;
   if (w == 0) {  // the gates, a row a lane, G in log2 units
     const int64_t r = r0 + min(lane, n - 1);
     gate = GateOf(a, h)(gate_a(a, r, h), gate_b(a, r, h));
     if (lane >= n) gate.g = gate.beta = 0;
-    sum = gate.g * 1.4426950408889634f;
+    sum = gate.g * 1.4426950408889634;
+    if (sum < kLeast) sum = kLeast;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
-      const float up = __shfl_up(sum, o);
+      const double up = __shfl_up(sum, o);
       if (lane >= o) sum += up;
     }
     all = __shfl(sum, 63);
-    G[lane] = sum;
+    G[0][lane] = (float)sum;
+    G[1][lane] = (float)(sum - (float)sum);
     beta[lane] = gate.beta;
   }
   // the norms stand on the diagonals of the wave's own Gram tiles: row l16's in lane (l16, l16 / 4), register l16 % 4
@@ -303,16 +314,17 @@ __global__ void __launch_bounds__(256, 4) gdn_chunk_kernel(const dft_prompt_gdn_
     float* coef = reinterpret_cast<float*>(out + kX + kP) + lane;
     const float rk = rks[lane];
     coef[kBeta * kChunk] = gate.beta;
-    coef[kDecayed * kChunk] = lane < n ? __builtin_amdgcn_exp2f(sum) * rk * gate.beta : 0;
+    const float decay = __builtin_amdgcn_exp2f((float)sum);
+    coef[kDecayed * kChunk] = lane < n ? decay * rk * gate.beta : 0;
     coef[kUnit * kChunk] = lane < n ? rk : 0;
-    coef[kOut * kChunk] = lane < n ? __builtin_amdgcn_exp2f(all - sum) : 0;
-    coef[kKeep * kChunk] = __builtin_amdgcn_exp2f(all);
-    coef[kDecay * kChunk] = __builtin_amdgcn_exp2f(sum);
+    coef[kOut * kChunk] = lane < n ? __builtin_amdgcn_exp2f((float)(all - sum)) : 0;
+    coef[kKeep * kChunk] = __builtin_amdgcn_exp2f((float)all);
+    coef[kDecay * kChunk] = decay;
     *reinterpret_cast<u32x4*>(out + kX + 18 * kFragment + 16 * lane) = u32x4{};
   }
 
   // A into the LDS, P to its place, transposed: Gram tiles K K^T and K Q^T of the keys of tiles j <= w with the wave's rows
-  const float Gq = G[mine], bk = beta[mine] * rks[mine];
+  const float Gq = G[0][mine], Gq_low = G[1][mine], bk = beta[mine] * rks[mine];
   Parts4<3> p[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
@@ -325,13 +337,14 @@ __global__ void __launch_bounds__(256, 4) gdn_chunk_kernel(const dft_prompt_gdn_
       dot = mfma16(kj, k[x], dot);
       qk = mfma16(kj, q[x], qk);
     }
-    const f32x4 Gk = *reinterpret_cast<const f32x4*>(&G[16 * j + 4 * g]);
+    const f32x4 Gk = *reinterpret_cast<const f32x4*>(&G[0][16 * j + 4 * g]);
+    const f32x4 Gk_low = *reinterpret_cast<const f32x4*>(&G[1][16 * j + 4 * g]);
     const f32x4 rk = *reinterpret_cast<const f32x4*>(&rks[16 * j + 4 * g]);
     f32x4 x, y;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int ahead = j < w ? 1 : l16 - (4 * g + r);  // of the key the row is
-      const float decay = __builtin_amdgcn_exp2f(Gq - Gk[r]);
+      const float decay = __builtin_amdgcn_exp2f((Gq - Gk[r]) + (Gq_low - Gk_low[r]));
       x[r] = ahead > 0 ? dot[r] * (bk * rk[r]) * decay : 0.f;
       y[r] = ahead >= 0 ? qk[r] * decay : 0.f;
     }

@@ -53,3 +53,33 @@ def test_weak_gates(cuda, sizes, hk, hv):
     """Chunks with 16 and with 32 value columns a workgroup."""
     c = Case(sum(sizes), hk, hv, len(sizes), cuda, seed=sum(sizes), gates=F32, decay=0.02)
     check(c, sizes, cuda, label="weak gates")
+
+
+def strong(c, at, g):
+    """Rows `at` with the log decay g among weak ones, through softplus's inverse."""
+    gen = torch.Generator().manual_seed(len(at))
+    weak = 1e-3 + 0.02 * torch.rand(c.a.shape, generator=gen, dtype=torch.float64)
+    a = torch.log(torch.expm1(weak))
+    a[at] = -g
+    c.a = a.float().to(c.y.device)
+    c.A_log, c.dt_bias = torch.zeros(c.hv, device=c.y.device), torch.zeros(c.hv, device=c.y.device)
+
+
+@pytest.mark.parametrize("sizes", [[64], [200], [30, 100, 64]])
+@pytest.mark.parametrize("g", [-30.0, -100.0, -300.0, -4000.0, float("-inf")])
+@pytest.mark.parametrize("share", [0.0, 0.1, 0.4, 0.75])
+def test_resets_among_weak_gates(cuda, sizes, g, share):
+    """Rows that leave nothing of the state, one of them or some of every chunk: what the weak gates behind them keep is as
+    exact as without them."""
+    n = sum(sizes)
+    c = Case(n, 1, 2, len(sizes), cuda, seed=n, gates=F32)
+    at = torch.randperm(n, generator=torch.Generator().manual_seed(n))[:max(1, int(share * n))]
+    strong(c, at, g)
+    check(c, sizes, cuda, label=f"{len(at)} rows of g={g}")
+
+
+@pytest.mark.parametrize("sizes", [[64], [130], [20, 300, 65], [1000], [100] * 40])
+@pytest.mark.parametrize("decay", [0.3, 1.0, 30.0, 1000.0])
+def test_ordinary_and_strong_gates(cuda, sizes, decay):
+    c = Case(sum(sizes), 2, 8, len(sizes), cuda, seed=sum(sizes) + 1, gates=F32, decay=decay)
+    check(c, sizes, cuda, label=f"decay {decay}")
