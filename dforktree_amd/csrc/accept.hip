@@ -411,14 +411,15 @@ __global__ void __launch_bounds__(kLast) last_kernel(const dft_tree_accept_args 
       double before = 0;
       int from = 0, to = V;
       while (token < 0) {
-        // the part where the running sum passes the target, else the last of any weight
+        // the part where the running sum passes the target, else the last of any weight (one of none has a sum that is
+        // added up in another order, which may pass it first)
         double up = lane < parts ? sums[lane] : 0;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
           const double x = __shfl_up(up, o);
           if (lane >= o) up += x;
         }
-        const uint64_t past = __ballot(lane < parts && before + up > target);
+        const uint64_t past = __ballot(lane < parts && sums[lane] > 0 && before + up > target);
         if (!past) {
           token = wave_max(lane < parts ? tops[lane] : -1);
           break;
