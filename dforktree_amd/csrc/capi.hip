@@ -384,9 +384,12 @@ int dft_prompt_conv(const dft_prompt_conv_args* a, void* stream) {
     return DFT_ERR_INVALID;
   if (a->bias && !float_tag(a->bias_dtype)) return DFT_ERR_INVALID;
   if (a->cs_indices && !index_tag(a->cs_indices_dtype)) return DFT_ERR_INVALID;
-  if (a->batch == 0 || a->channels == 0) return DFT_OK;
+  if (a->batch == 0) return DFT_OK;
+  if (a->channels == 0 && !a->status) return DFT_OK;
   if (a->rows > 0x7fffffffll || dft::prompt_conv_blocks(a) > max_blocks(256)) return DFT_ERR_UNSUPPORTED;
-  if (!a->weight || (a->rows && (!a->x || !a->y)) || (a->slots && a->width > 1 && !a->conv_state)) return DFT_ERR_INVALID;
+  if (a->channels &&
+      (!a->weight || (a->rows && (!a->x || !a->y)) || (a->slots && a->width > 1 && !a->conv_state)))
+    return DFT_ERR_INVALID;
   return dft::launch_prompt_conv(a, static_cast<hipStream_t>(stream));
 }
 

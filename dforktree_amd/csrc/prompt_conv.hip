@@ -18,9 +18,12 @@ using namespace packed;
 constexpr int kMaxTaps = 8;
 constexpr int kRows = 16, kTileRows = 64;  // of a tile, here and in prompt_conv4_kernel
 
+// Workgroups beside each other over the channels (of none: one, for the status).
+__host__ __device__ inline int channel_blocks(const dft_prompt_conv_args& p) { return p.channels ? (p.channels + 255) / 256 : 1; }
+
 // The types and strides as they come, a thread a channel.
 __global__ void __launch_bounds__(256) prompt_conv_kernel(const dft_prompt_conv_args p) {
-  const int blocks = (p.channels + 255) / 256;
+  const int blocks = channel_blocks(p);
   const int64_t x = blockIdx.x / blocks;
   if (blockIdx.x == 0 && p.status)
     for (int b = threadIdx.x; b < p.batch; b += 256)
@@ -206,7 +209,7 @@ __global__ void __launch_bounds__(256) prompt_conv4_kernel(const dft_prompt_conv
 bool aligned16(const void* x) { return reinterpret_cast<uintptr_t>(x) % 16 == 0; }
 // The types and layouts of prompt_conv4_kernel: a layer's own.
 bool by_pieces(const dft_prompt_conv_args& a) {
-  return a.width == 4 && a.channels % 8 == 0 && a.x_dtype == DFT_BF16 && a.y_dtype == DFT_BF16 && a.w_dtype == DFT_BF16 &&
+  return a.width == 4 && a.channels && a.channels % 8 == 0 && a.x_dtype == DFT_BF16 && a.y_dtype == DFT_BF16 && a.w_dtype == DFT_BF16 &&
          a.w_tap_stride == 1 && a.w_chan_stride == 4 && aligned16(a.x) && aligned16(a.y) && aligned16(a.weight) &&
          a.x_row_stride % 8 == 0 && a.y_row_stride % 8 == 0;
 }
@@ -217,7 +220,7 @@ bool window_pieces(const dft_prompt_conv_args& a) {
 }  // namespace
 
 int64_t prompt_conv_blocks(const dft_prompt_conv_args* a) {
-  return line_tiles(a->rows, a->batch, kRows) * ((a->channels + 255) / 256);
+  return line_tiles(a->rows, a->batch, kRows) * channel_blocks(*a);
 }
 
 int launch_prompt_conv(const dft_prompt_conv_args* a, hipStream_t stream) {
