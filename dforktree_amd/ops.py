@@ -1189,6 +1189,39 @@ def _pool_slots(indices, name, batch, pool, pool_name):
     return at, tag
 
 
+def _end(t):
+    """The address behind t's last element."""
+    return t.data_ptr() + (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size()
+
+
+def _pieces(t):
+    """(address, pitch, bytes, how many) of the pieces with unit stride of t [rows, width] or [rows, heads, width]."""
+    n, width = t.element_size(), t.shape[-1] * t.element_size()
+    heads = range(t.shape[1]) if t.dim() == 3 else range(1)
+    return [(t.data_ptr() + h * t.stride(1) * n, t.stride(0) * n, width, t.shape[0]) for h in heads]
+
+
+def _own_memory(out, name, x, x_name):
+    """Refuses an output whose rows lie over each other, or surely over those of an input."""
+    if not out.numel() or not x.numel():
+        return
+    if any(n > 1 and s < out.shape[-1] for n, s in zip(out.shape[:-1], out.stride()[:-1])):
+        raise ValueError(f"{name}'s rows must not lie over each other")
+    if _end(out) <= x.data_ptr() or _end(x) <= out.data_ptr():
+        return
+    (x_at, x_pitch, x_width, x_rows), = _pieces(x)
+    for at, pitch, width, rows in _pieces(out):
+        if at + (rows - 1) * pitch + width <= x_at or x_at + (x_rows - 1) * x_pitch + x_width <= at:
+            continue
+        apart = at - x_at
+        if pitch == x_pitch and pitch > 0:  # rows side by side in a wider buffer are as good as any
+            if x_width <= apart % pitch <= pitch - width:
+                continue
+        elif not -width < apart < x_width:  # where the first rows do not meet it is not looked into further
+            continue
+        raise ValueError(f"{name} must not lie over {x_name}'s memory")
+
+
 def prompt_conv(x: torch.Tensor, conv_state: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
                 cu_seqlens: Optional[torch.Tensor] = None, *, max_len: Optional[int] = None,
                 batch: Optional[int] = None, silu: bool = True, cs_indices: Optional[torch.Tensor] = None,
@@ -1206,7 +1239,7 @@ def prompt_conv(x: torch.Tensor, conv_state: torch.Tensor, weight: torch.Tensor,
     or where ``initial`` [batch] bool is given and False from zeros; a negative
     slot (a padded request) starts from zeros and is not written.  No two
     requests may have one slot.  Writes y [rows, C] (x.dtype by default), which
-    must not overlap x; rows of no request (behind the last one's, or cut off)
+    must not overlap x or itself; rows of no request (behind the last one's, or cut off)
     keep what a given ``y`` holds and are otherwise uninitialised.  ``status``
     (int32 [batch]) receives DFT_STATUS_SPAN (cut to max_len or to the rows
     there are) and DFT_STATUS_SLOT bits (a slot past the pool: taken as a
@@ -1230,8 +1263,8 @@ def prompt_conv(x: torch.Tensor, conv_state: torch.Tensor, weight: torch.Tensor,
         y = torch.empty(rows, Cn, device=dev, dtype=x.dtype)
     elif y.shape != x.shape or (y.stride(1) != 1 and Cn > 1):
         raise ValueError(f"y must be {tuple(x.shape)} with channel stride 1")
-    elif rows and Cn and y.data_ptr() == x.data_ptr():
-        raise ValueError("y must not be x's memory")
+    else:
+        _own_memory(y, "y", x, "x")
     a = PromptConvArgs()
     a.batch, a.max_len, a.channels, a.width, a.silu = batch, max_len, Cn, W, int(bool(silu))
     a.rows, a.slots = rows, conv_state.shape[0]
@@ -1264,9 +1297,9 @@ def prompt_gdn(y: torch.Tensor, a: torch.Tensor, b: torch.Tensor, A_log: Optiona
     state float32 [slots, hv, dk, dv] (index k, v; any strides -- pass
     ``pool.transpose(-1, -2)`` for a V-major pool), updated in place.  Rows of
     request b, its slot state_indices[b] (or b), ``initial`` and ``status`` as in
-    ``prompt_conv``.  Returns o [rows, hv, 128], which must not overlap y, and
-    where rows of no request keep what a given ``o`` holds and are otherwise
-    uninitialised.
+    ``prompt_conv``.  Returns o [rows, hv, 128], which must not overlap y or
+    itself, and where rows of no request keep what a given ``o`` holds and are
+    otherwise uninitialised.
     """
     dev = _device_of(y, a, b, A_log, dt_bias, state, cu_seqlens, neg_exp_A, state_indices, initial, o, status)
     if y.dim() != 2 or y.stride(1) != 1:
@@ -1278,6 +1311,7 @@ def prompt_gdn(y: torch.Tensor, a: torch.Tensor, b: torch.Tensor, A_log: Optiona
         raise ValueError(f"hv must be a multiple of hk, got {hv} and {hk}")
     if y.shape[1] < (2 * hk + hv) * D_HEAD:
         raise ValueError(f"y has {y.shape[1]} channels, need {(2 * hk + hv) * D_HEAD}")
+    given = y
     if y.data_ptr() % 16 or y.stride(0) % 8:  # read as 16-byte pieces, as in _verify_args
         pitch = -(-y.shape[1] // 8) * 8
         y = torch.empty(rows, pitch, device=dev, dtype=y.dtype)[:, :y.shape[1]].copy_(y)
@@ -1302,6 +1336,8 @@ def prompt_gdn(y: torch.Tensor, a: torch.Tensor, b: torch.Tensor, A_log: Optiona
         o = torch.empty(rows, hv, D_HEAD, device=dev, dtype=o_dtype or y.dtype)
     elif tuple(o.shape) != (rows, hv, D_HEAD) or o.stride(2) != 1:
         raise ValueError(f"o must be [{rows}, {hv}, 128] with stride 1 along dv")
+    else:
+        _own_memory(o, "o", given[:, :(2 * hk + hv) * D_HEAD], "y")
     args = PromptGdnArgs()
     args.batch, args.max_len, args.hk, args.hv = batch, max_len, hk, hv
     args.dk = args.dv = D_HEAD
