@@ -546,7 +546,7 @@ int launch_tree_accept(const dft_tree_accept_args* a, hipStream_t stream) {
   work.sums = reinterpret_cast<double*>(work.walks + a->batch);
   work.tops = reinterpret_cast<int*>(work.sums + passes * kSlices);
   work.done = work.tops + passes * kSlices;
-  if (a->draft_probs && a->draft_dtype != a->probs_dtype) return launch_type<uint8_t>(*a, work, stream);
+  if (a->draft_probs && a->draft_dtype != a->probs_dtype) return launch<true, uint8_t>(*a, work, stream);
   switch (a->probs_dtype) {
     case DFT_BF16: return launch_type<__bf16>(*a, work, stream);
     case DFT_F16: return launch_type<_Float16>(*a, work, stream);
