@@ -15,7 +15,7 @@ import torch
 
 from conftest import announce, rel_l2
 from oracle import packed as P
-from test_gpu_gdn import BF16, F32, Case, cu_of, slots_of  # noqa: F401
+from test_gpu_gdn import F32, Case, cu_of
 
 pytestmark = pytest.mark.gpu
 
