@@ -207,10 +207,6 @@ __device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) {
 __device__ __forceinline__ f32x4 mfma16_f32(float a, float b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
 }
-// Until an fp32 product's result is whole.  The compiler waits 10 states for it,
-// after which its last register may still be on its way: read first of the
-// four, behind a branch, it held the sum without its last terms.
-__device__ __forceinline__ void settle(f32x4& x) { asm volatile("s_nop 15" : "+v"(x)); }
 // x = p[0] + p[1] + ..., each the bf16 nearest to what is left
 template <int N>
 struct Parts4 {
@@ -388,10 +384,8 @@ __global__ void __launch_bounds__(256, 4) gdn_chunk_kernel(const dft_prompt_gdn_
       D[r] = below ? 0.f : -y;
       DL = mfma16_f32(below ? y : 0.f, diagonal[r], DL);
     }
-    settle(DL);
 #pragma unroll
     for (int r = 0; r < 4; ++r) diagonal = mfma16_f32(D[r], DL[r], diagonal);
-    settle(diagonal);
     __builtin_amdgcn_wave_barrier();
     *reinterpret_cast<f32x4*>(&A[mine][16 * w + 4 * g]) = diagonal;
   }
@@ -409,13 +403,9 @@ __global__ void __launch_bounds__(256, 4) gdn_chunk_kernel(const dft_prompt_gdn_
 #pragma unroll
         for (int r = 0; r < 4; ++r) to[m - 1] = mfma16_f32(A[16 * m + 4 * g + r][16 * j + l16], xt[m][r], to[m - 1]);
 #pragma unroll
-      for (int m = W; m > j; --m) {
-        settle(to[m - 1]);
-        all += to[m - 1];
-      }
+      for (int m = W; m > j; --m) all += to[m - 1];
 #pragma unroll
       for (int r = 0; r < 4; ++r) xt[j] = mfma16_f32(-A[16 * j + 4 * g + r][16 * j + l16], all[r], xt[j]);
-      settle(xt[j]);
     }
 #pragma unroll
     for (int r = 0; r < 4; ++r) xt[W][r] = 4 * g + r == l16 ? 0.f : xt[W][r];  // the unit diagonal stays out
