@@ -12,14 +12,17 @@
 // request's workgroup alone in the last launch, which finds the token from the
 // sums of its slice: a slice's tokens side by side, added up over the workgroup.
 //
-// Bound by launches and by the walk's dependent fetches where passes are few: 21
-// us for one request of 16 nodes over 131072 tokens, 32 for 64 drawn chains, 21
-// for 64 trees of 32 nodes without a drafter's rows; of these the last launch is 7
-// to 10, and a launch that finds nothing to do costs 1.6.  48 drawn trees of 8 to
-// 40 nodes over 100003 tokens take 49; with two rounds only, and a request's
-// further passes by its workgroup alone, three times as much.  Their passes are
-// bound by the 64-bit units: a reduction divides by two numbers that are the same
-// for the whole row, so it multiplies by their reciprocals.
+// Bound by launches and by the walk's dependent fetches where passes are few: 17
+// to 22 us for one request of 16 nodes over 131072 tokens, 31 for 64 drawn chains,
+// 20 for 64 trees of 32 nodes without a drafter's rows; of these the last launch
+// is 5 to 9, and a launch that finds nothing to do costs 1.4 to 3.  48 drawn trees
+// of 8 to 40 nodes over 100003 tokens take 39 to 49, by how many children their
+// random numbers refuse.  Their passes are bound by the 64-bit units: a reduction
+// divides by two numbers that are the same for the whole row, so it multiplies by
+// their reciprocals.
+// The passes of a request past the fourth are its one workgroup's, and every pass
+// repeats the reductions in front of it: a node over 131072 tokens with 5, 7, 15,
+// 39 and 63 refused children takes 99 us, 223 us, 1.0, 6.0 and 15 ms.
 //
 // Sums are held in 64 bits: a sum of 10^5 probabilities in 32 bits moves one
 // drawn token in some hundred over a border.  They are added up in one order.
@@ -502,15 +505,18 @@ __global__ void __launch_bounds__(kLast) last_kernel(const dft_tree_accept_args 
 
 // A pass for every refused child with a sibling behind it, and the last one: no
 // more than there are children.  None over short rows, which a request's workgroup
-// passes over as fast (64 trees of 16 nodes, us in a captured graph: over 2000 tokens
-// 11 and 13, drawn 26 and 37; 16000 13 and 15, 39 and 51; 32000 17 and 16, 65 and 49).
+// passes over as fast.  Trees of 16 nodes, us in a captured graph, without rounds
+// and with: one request over 2000 tokens 10 and 11, drawn 9 and 15, 16000 11.5 and
+// 11, 10 and 16, 64000 19 and 11, 55 and 29; 64 requests 11 and 12, 22 and 30,
+// then 12 and 13, 26 and 34, then 24 and 18, 65 and 50; 500 requests 14 and 15, 35
+// and 54, then 18 and 23, 49 and 74, then 37 and 45, 124 and 145.
 int rounds_of(const dft_tree_accept_args& a) {
   if (a.vocab <= kShort) return 0;
   return a.draft_probs ? std::min(kRounds, std::max(a.n_nodes - 1, 1)) : 1;
 }
 // Slices such that a pass has some two thousand workgroups, of no less than 1024
-// tokens.  (With one thousand 48 drawn trees take 56 us instead of 49, 64 chains
-// 30 instead of 32.)
+// tokens.  (With one thousand the same 48 drawn trees took 56 us instead of 49, 64
+// chains 30 instead of 32.)
 Work work_of(const dft_tree_accept_args& a) {
   Work w = {};
   const int most = std::min(kSlices, std::max(1, 2048 / a.batch));

@@ -14,7 +14,7 @@
 // so that K, Q and K^T are exact operands of bf16 products.  What is not goes in
 // as a sum of three bf16 parts, 2^-24 relative at most, and a product of two such
 // factors as its six of 2^-16 or more.  (With two parts states and fp32 outputs
-// come out 4 10^-6 off.  Two where only outputs pass through: 8 to 10% less time.)
+// come out 4 10^-6 off.  Two where only outputs pass through: 6 to 10% less time.)
 #include <algorithm>
 #include <type_traits>
 
@@ -60,7 +60,8 @@ __device__ __forceinline__ float sum16(float x) {
 // a wave's access covers whole columns and both sums over the keys stay within
 // 16 lanes.  Bound by the states' bytes: 64 requests of 32 heads 50.8 us, 5.3
 // TB/s (written past the caches; through them 62.5.  Half the columns a
-// workgroup 60.7, a quarter 68).
+// workgroup 60.7, a quarter 68).  A pool whose values lie side by side is read and
+// written by elements: 143.
 template <int V, bool VEC>
 __global__ void __launch_bounds__(256) gdn_rows_kernel(const dft_prompt_gdn_args a, int most) {
   constexpr int kSplit = kD / V, kPass = V / 16;
@@ -241,8 +242,9 @@ constexpr double kLeast = -512;
 // state would leave the weak gates behind them a sum of thousands, in steps of
 // 10^-3 (24 rows of g = -300 among weak ones: states 4 10^-4 off, so 1 10^-7).
 // Bound by the instructions that its waves issue, so by what of them stand ready:
-// 128 registers, four workgroups a CU.  A prompt of 8192 rows and 32 heads 52 us,
-// 4.5 TB/s; with two workgroups a CU 78.
+// 128 registers, four workgroups a CU.  A prompt of 8192 rows and 32 heads 54 us
+// for 213 MB read and written, 4.0 TB/s; with two workgroups a CU, and two parts
+// of P, 78 where it took 52.
 __global__ void __launch_bounds__(256, 4) gdn_chunk_kernel(const dft_prompt_gdn_args a, Work work, int past) {
   constexpr int kKRow = kD + 8, kARow = kChunk + 4;
   __shared__ __attribute__((aligned(16))) uint16_t keys[kChunk][kKRow];
@@ -440,8 +442,8 @@ __device__ __forceinline__ void barrier_only() {
 constexpr int kScanThreads = 64 * 12;
 
 // The request at this place in the order of falling lengths, of at most 64: the
-// others as they come.  (20 prompts of 500 rows and one of 8192 behind them: 550
-// us, as they come 663; six of 257 to 2999 no better for it.)
+// others as they come.  (20 prompts of 500 rows and one of 8192 behind them: 600
+// us, as they come 733; six of 257 to 2999 no better for it.)
 __device__ __forceinline__ int nth_longest(const dft_prompt_gdn_args& a, int place) {
   if (!a.cu_seqlens || a.batch == 1 || a.batch > 64) return place;
   const int lane = threadIdx.x & 63, n = lane < a.batch ? span_of(a, lane).n : 0;
@@ -470,8 +472,8 @@ __device__ __forceinline__ int nth_longest(const dft_prompt_gdn_args& a, int pla
 // The slices of a head read the same X, K and Q, the heads of a k head the same
 // K and Q: they form a family, whose workgroups stand on one XCD, behind one L2
 // (a prompt of 8192 rows, 16 k and 32 v heads: 2.1 GB read past the L2s with the
-// slices dealt out, 0.3 so).  That prompt's states take 190 us, 1.5 a chunk (224
-// under the profiler): the matrix unit is busy 21% of it and the LDS 53, the waves wait 57%.
+// slices dealt out, 0.3 so).  That prompt's states take 217 us, 1.7 a chunk (237
+// under the profiler): the matrix unit is busy 24% of it and the LDS 56, the waves wait 55%.
 template <int NT, bool VEC, int OUT>
 __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_kernel(const dft_prompt_gdn_args a, Work work, int families, int past) {
   constexpr int BN = 16 * NT, kSlices = kD / BN, kSRow = kD + 8, kRow = kChunk + 8;
@@ -834,9 +836,9 @@ bool vector_state(const dft_prompt_gdn_args& a) {
 }
 
 // Up to so many rows a request is taken row by row, by a launch of its own where
-// others are longer.  us for one request of 32 heads: 5.3, 9.0, 14.2 and 25 for 1,
-// 4, 8 and 16 rows, 14.1 as a chunk; 16 requests 11.9, 22, 35 and 60, 60 to 62 as
-// chunks; 64 requests 48, 70, 102 and 182, 197 to 204 as chunks.  With few of them
+// others are longer.  us for one request of 32 heads: 6.1, 9.9, 15.1 and 25.5 for 1,
+// 4, 8 and 16 rows, 15.5 as a chunk; 16 requests 14, 23, 34 and 57, 73 to 75 as
+// chunks; 64 requests 48, 66, 97 and 173, 310 to 316 as chunks.  With few of them
 // the second launch (2) costs more than the chunks of short requests, which run
 // beside the others.
 struct Split {
@@ -904,7 +906,7 @@ int launch_prompt_gdn(const dft_prompt_gdn_args* a, hipStream_t stream) {
   gdn_chunk_kernel<<<(unsigned)chunk_blocks(*a), 256, 0, stream>>>(*a, work, split.rows);
   if (hipGetLastError() != hipSuccess) return DFT_ERR_LAUNCH;
   // 16 value columns a workgroup, or 32 at 1.6 times the time a chunk: the longest request's chunks one after the other,
-  // or all of them over the CUs (us: one prompt of 8192, 32 heads, 245 and 358; six of 257 to 2999 333 and 272)
+  // or all of them over the CUs (us: one prompt of 8192, 32 heads, 282 and 402; six of 257 to 2999 354 and 302)
   const double longest = std::min(a->rows, (int64_t)a->max_len) / 64.0, all = (a->rows / 64.0 + a->batch / 2.0) * a->hv / kCus;
   return std::max(longest, 8 * all) <= 1.6 * std::max(longest, 4 * all) ? launch_scan<1>(*a, work, split.rows, stream)
                                                                         : launch_scan<2>(*a, work, split.rows, stream);
