@@ -16,7 +16,7 @@
 // to 22 us for one request of 16 nodes over 131072 tokens, 31 for 64 drawn chains,
 // 20 for 64 trees of 32 nodes without a drafter's rows; of these the last launch
 // is 5 to 9, and a launch that finds nothing to do costs 1.4 to 3.  48 drawn trees
-// of 8 to 40 nodes over 100003 tokens take 39 to 49, by how many children their
+// of 8 to 40 nodes over 100003 tokens take 39 to 70, by how many children their
 // random numbers refuse.  Their passes are bound by the 64-bit units: a reduction
 // divides by two numbers that are the same for the whole row, so it multiplies by
 // their reciprocals.
