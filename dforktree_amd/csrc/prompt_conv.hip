@@ -79,8 +79,8 @@ __global__ void __launch_bounds__(256) prompt_conv_kernel(const dft_prompt_conv_
 // The exponential's argument is rounded once, |z| 2^-24 of the value: nothing
 // beside the output's 2^-8 (with expf 102 us where it took 82).  Bound by HBM: six
 // prompts of 257 to 2999 rows, 8192 channels, 65 us, 4.9 TB/s, 72 over three such
-// batches in turn (tiles of 16, 32, 64
-// and 128 rows 75, 82, 70 and 77; rows read as data read once 66).
+// batches in turn (tiles of 16, 32, 64 and 128 rows 75, 82, 70 and 77; rows read as
+// data read once 66).
 template <bool STATE>
 __global__ void __launch_bounds__(256) prompt_conv4_kernel(const dft_prompt_conv_args p) {
   constexpr int kTile = kTileRows, kAhead = 4;
